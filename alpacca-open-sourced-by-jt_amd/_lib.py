@@ -30,6 +30,32 @@ SIGNATURES = {
     "alpx_host_device_pointer": (_c_int, [_c_ptr, ctypes.POINTER(_c_ptr)]),
     "alpx_kv_append": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_i64, _c_int, _c_int,
                                 _c_int, _c_int, _c_int, _c_i64, _c_ptr, _c_ptr]),
+    "alpx_tree_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+                                            _c_int, _c_int]),
+    "alpx_tree_attention": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_int, _c_ptr,
+                                     _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_size, _c_int,
+                                     _c_int, _c_int, _c_int, _c_int, _c_int, _c_i64, _c_i64,
+                                     _c_i64, _c_i64, _c_i64, _c_i64, _c_float, _c_int, _c_int,
+                                     _c_ptr]),
+    "alpx_tree_attention_paged": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int,
+                                           _c_int, _c_ptr, _c_i64, _c_int, _c_ptr, _c_ptr,
+                                           _c_int, _c_ptr, _c_ptr, _c_ptr, _c_size, _c_int,
+                                           _c_int, _c_int, _c_int, _c_int, _c_int, _c_float,
+                                           _c_int, _c_int, _c_ptr]),
+    "alpx_tree_masks": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int,
+                                 _c_int, _c_ptr]),
+    "alpx_tree_commit": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_i64,
+                                  _c_int, _c_int, _c_int, _c_int, _c_int, _c_ptr]),
+    "alpx_tree_commit_paged": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_ptr,
+                                        _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int,
+                                        _c_int, _c_ptr]),
+    "alpx_paged_resize": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int,
+                                   _c_int, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
+                                   _c_ptr, _c_ptr]),
+    "alpx_attention_prologue_rows": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
+                                              _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_ptr, _c_ptr,
+                                              _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+                                              _c_ptr, ctypes.c_double, _c_float, _c_ptr]),
     "alpx_kv_append_paged": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int,
                                       _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
                                       _c_i64, _c_ptr, _c_ptr]),

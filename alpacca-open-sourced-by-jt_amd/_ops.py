@@ -926,3 +926,135 @@ def prepare_recurrent_step(*args, **kwargs):
     """``recurrent_step`` as a PreparedCall (same arguments)."""
     fn, call_args, device, out, buffers = _recurrent_step_call(*args, **kwargs)
     return PreparedCall(fn, call_args, device, buffers + (out,), out)
+
+
+# ------------------------------------------------------- drafted tokens
+
+
+def _enqueue(fn, device, *args):
+    """One C-ABI call (arguments without the stream) on torch's current stream
+    of ``device``, which need not be the current device."""
+    torch = _torch()
+    if device.index == torch.cuda.current_device():
+        _lib.check(fn(*args, _lib.current_stream(device.index)))
+        return
+    with torch.cuda.device(device):
+        _lib.check(fn(*args, _lib.current_stream(device.index)))
+
+
+def _address(tensor):
+    return None if tensor is None else tensor.data_ptr()
+
+
+@functools.lru_cache(maxsize=1024)
+def _tree_bytes(*sizes):
+    """``alpx_tree_workspace_bytes``, a pure function of the sizes."""
+    return _lib.lib().alpx_tree_workspace_bytes(*sizes)
+
+
+def tree_attention(q, key_cache, value_cache, masks, *, length, prefix_lens, counts, scale,
+                   block_table=None, gate=None, out_dtype=None, out=None):
+    """Drafts ``q [B, N, Hq, D]`` over caches ``[C, B, Hkv, D|Dv]``, or over
+    pages ``[P, page_size, Hkv, D|Dv]`` through ``block_table``; returns
+    ``[B, N, Hq, Dv]``.  The workspace is the call's own, from torch's
+    stream-ordered allocator, so calls on different streams and captured
+    graphs share nothing."""
+    torch = _torch()
+    batch, nodes, q_heads, key_dim = q.shape
+    kv_heads, value_dim = value_cache.shape[2:]
+    if out is None:
+        out = torch.empty((batch, nodes, q_heads, value_dim),
+                          dtype=q.dtype if out_dtype is None else out_dtype, device=q.device)
+    code = _lib.dtype_code(torch, q.dtype)
+    nbytes = _tree_bytes(batch, nodes, q_heads, kv_heads, key_dim, value_dim, length, code)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    shared = (masks.data_ptr(), 0 if masks.shape[0] == 1 else nodes * masks.shape[2],
+              masks.shape[2], prefix_lens.data_ptr(), _address(counts), length, _address(gate),
+              out.data_ptr(), _address(ws), nbytes, batch, nodes, q_heads, kv_heads, key_dim,
+              value_dim)
+    tail = (float(scale), code, _lib.dtype_code(torch, out.dtype))
+    caches = (q.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr())
+    L = _lib.lib()
+    if block_table is None:
+        row, value_row = kv_heads * key_dim, kv_heads * value_dim
+        _enqueue(L.alpx_tree_attention, q.device, *caches, *shared, batch * row, row, key_dim,
+                 batch * value_row, value_row, value_dim, *tail)
+    else:
+        _enqueue(L.alpx_tree_attention_paged, q.device, *caches, block_table.data_ptr(),
+                 block_table.shape[1], key_cache.shape[1], key_cache.shape[0], *shared, *tail)
+    return out
+
+
+def tree_masks(parents, *, lengths=None, counts=None):
+    """``(masks [B, N, ceil(N / 64)] int64, depths [B, N] int32, position lanes
+    [B, N, 4] int64 or None)`` of ``parents [B, N]``."""
+    torch = _torch()
+    batch, nodes = parents.shape
+    words = (nodes + 63) // 64
+    device = parents.device
+    masks = torch.empty((batch, nodes, words), dtype=torch.int64, device=device)
+    depths = torch.empty((batch, nodes), dtype=torch.int32, device=device)
+    lanes = None
+    if lengths is not None:
+        lanes = torch.empty((batch, nodes, 4), dtype=torch.int64, device=device)
+    _enqueue(_lib.lib().alpx_tree_masks, device, parents.data_ptr(), _address(counts),
+             _address(lengths), masks.data_ptr(), depths.data_ptr(), _address(lanes), batch, nodes,
+             words)
+    return masks, depths, lanes
+
+
+def tree_commit(key_cache, value_cache, paths, *, prefix_lens, accepted, block_table=None):
+    """Moves row ``prefix + paths[b, i]`` of each sequence to row
+    ``prefix + i`` for ``i < accepted[b]``."""
+    torch = _torch()
+    batch, path_max = paths.shape
+    outer, inner, kv_heads, key_dim = key_cache.shape
+    value_dim = value_cache.shape[3]
+    code = _lib.dtype_code(torch, key_cache.dtype)
+    caches = (key_cache.data_ptr(), value_cache.data_ptr())
+    rows = (paths.data_ptr(), accepted.data_ptr(), prefix_lens.data_ptr(), code)
+    sizes = (batch, kv_heads, key_dim, value_dim, path_max)
+    L = _lib.lib()
+    if block_table is None:
+        _enqueue(L.alpx_tree_commit, key_cache.device, *caches, *rows, outer, *sizes)
+    else:
+        _enqueue(L.alpx_tree_commit_paged, key_cache.device, *caches, block_table.data_ptr(),
+                 block_table.shape[1], inner, outer, *rows, *sizes)
+
+
+def paged_resize(block_table, lengths, free_pages, free_count, targets, *, page_size, tokens):
+    """Takes every sequence from ``lengths[b]`` to ``targets[b]`` rows (in
+    place); returns ``(starts, slots, positions, sequences, granted)``."""
+    torch = _torch()
+    batch, max_pages = block_table.shape
+    device = block_table.device
+    # one buffer: three rows of `tokens`, then starts and grants
+    buf = torch.empty(3 * tokens + 2 * batch + 1, dtype=torch.int32, device=device)
+    slots, positions, sequences = (buf[i * tokens:(i + 1) * tokens] for i in range(3))
+    starts = buf[3 * tokens:3 * tokens + batch + 1]
+    granted = buf[3 * tokens + batch + 1:]
+    _enqueue(_lib.lib().alpx_paged_resize, device, block_table.data_ptr(), lengths.data_ptr(),
+             free_pages.data_ptr(), free_count.data_ptr(), targets.data_ptr(), batch, max_pages,
+             page_size, free_pages.shape[0], tokens, starts.data_ptr(), slots.data_ptr(),
+             positions.data_ptr(), sequences.data_ptr(), granted.data_ptr())
+    return starts, slots, positions, sequences, granted
+
+
+def attention_prologue_rows(query_gate, key, value, q_norm, k_norm, key_pages, value_pages, slots,
+                            position_lanes, *, sections, frequency_base, eps):
+    """Prologue of packed tokens ``query_gate [T, Hq, 2D]``, ``key [T, Hkv *
+    D]``, ``value [T, Hkv * Dv]`` into pool rows ``slots``; returns
+    ``(query, gate)``, each ``[T, Hq, D]``."""
+    torch = _torch()
+    tokens, q_heads, joint = query_gate.shape
+    pages, page_size, kv_heads, dim = key_pages.shape
+    value_dim = value_pages.shape[3]
+    query, gate = torch.empty((2, tokens, q_heads, dim), dtype=query_gate.dtype,
+                              device=query_gate.device)
+    _enqueue(_lib.lib().alpx_attention_prologue_rows, query_gate.device, query_gate.data_ptr(),
+             key.data_ptr(), value.data_ptr(), q_norm.data_ptr(), k_norm.data_ptr(),
+             query.data_ptr(), gate.data_ptr(), key_pages.data_ptr(), value_pages.data_ptr(),
+             pages * page_size, slots.data_ptr(), position_lanes.data_ptr(),
+             _lib.dtype_code(torch, query_gate.dtype), tokens, q_heads, kv_heads, dim, value_dim,
+             _sections(sections), float(frequency_base), float(eps))
+    return query, gate

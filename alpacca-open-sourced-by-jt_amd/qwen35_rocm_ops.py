@@ -167,6 +167,32 @@ class RocmPagedAttentionWorkspace:
         }
 
 
+@dataclass(frozen=True)
+class RocmTreeMasks:
+    """Draft trees (extension): visibility words ``masks [batch, nodes,
+    ceil(nodes / 64)]`` (int64, bit j % 64 of word j / 64 is draft j),
+    ``depths [batch, nodes]`` (int32, -1 past a sequence's drafts) and, where
+    lengths were given, ``position_lanes [batch, nodes, 4]`` (int64)."""
+
+    masks: Any
+    depths: Any
+    position_lanes: Any
+
+
+@dataclass(frozen=True)
+class RocmPagedRows:
+    """New rows of a page pool (extension), packed in the order of sequences:
+    ``starts [batch + 1]``; per row, -1 past the last, its pool row
+    ``slots``, its position in its sequence ``positions`` and that sequence
+    ``sequences``; ``granted [batch]`` (1 or 0).  All int32."""
+
+    starts: Any
+    slots: Any
+    positions: Any
+    sequences: Any
+    granted: Any
+
+
 class Qwen35RocmOps:
     """gfx950 implementation of the Qwen35 attention/recurrence boundaries."""
 
@@ -1166,6 +1192,254 @@ class Qwen35RocmOps:
         return _ops.prefill_paged(query, key_pages, value_pages, block_table,
                                   batch_index=batch_index, pos0=position,
                                   kv_tokens=position + tokens, scale=scale_value, gate=gate)
+
+    # ------------------------------------------------------ drafted tokens
+
+    def _device_ints(self, value, name, shape, *, low=None, high=None):
+        """An int32 device tensor of ``shape``; a host sequence (one axis) is
+        checked against ``[low, high]`` and uploaded."""
+        torch = self.torch
+        if not torch.is_tensor(value) or value.device.type != "cuda":
+            host = [int(v) for v in value]
+            if (len(host),) != tuple(shape) or any(
+                    (low is not None and v < low) or (high is not None and v > high)
+                    for v in host):
+                bounds = "" if high is None else f" in [{low}, {high}]"
+                raise ValueError(f"{name} must hold one entry{bounds} per sequence")
+            return torch.tensor(host, dtype=torch.int32, device=self.device)
+        if value.dtype != torch.int32:
+            raise TypeError(f"{name} must use int32")
+        if value.get_device() != self.device_index:
+            raise ValueError(
+                f"{name} is on device {value.get_device()}, expected {self.device_index}")
+        if tuple(value.shape) != tuple(shape):
+            raise ValueError(f"{name} has {_shape(value)}, expected {tuple(shape)}")
+        if not value.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+        return value
+
+    def tree_masks(self, parents: Any, *, lengths: Any = None,
+                   counts: Any = None) -> RocmTreeMasks:
+        """Visibility masks of draft trees (extension): draft i of a sequence,
+        child of draft ``parents[b, i]`` (device int32 ``[B, N]``; outside
+        ``[0, i)``: a root), sees itself and its ancestors.  Drafts at or
+        past ``counts[b]`` see nothing.  With ``lengths [B]``, the rows each
+        sequence holds, also their rotary position lanes, the text lanes of
+        ``lengths[b] + depth``: drafts of one depth share a position."""
+        if not self.torch.is_tensor(parents) or parents.dim() != 2:
+            raise ValueError("draft parents must be a [batch, nodes] tensor")
+        batch, nodes = _shape(parents)
+        if batch <= 0 or not 0 < nodes <= 1024:
+            raise ValueError("draft trees hold 1 to 1024 drafts")
+        parents = self._device_ints(parents, "draft parents", (batch, nodes))
+        if counts is not None:
+            counts = self._device_ints(counts, "draft counts", (batch,), low=0, high=nodes)
+        if lengths is not None:
+            lengths = self._device_ints(lengths, "lengths", (batch,), low=0, high=2 ** 31 - 1)
+        return RocmTreeMasks(*_ops.tree_masks(parents, lengths=lengths, counts=counts))
+
+    def _tree_args(self, query, key_cache, value_cache, masks, batch, capacity, length,
+                   prefix_lens, counts, scale, gate, out_dtype, out):
+        torch = self.torch
+        query = self._tensor(query, "draft query", dimensions=4)
+        length = _positive_integer("attention cache length", length)
+        query_batch, nodes, query_heads, width = _shape(query)
+        kv_heads, key_width = _shape(key_cache)[2:]
+        value_width = int(value_cache.shape[3])
+        if length > capacity:
+            raise ValueError("attention cache length exceeds capacity")
+        if query_batch != batch or width != key_width:
+            raise ValueError("attention query does not match K cache batch/head width")
+        if nodes <= 0:
+            raise ValueError("draft query must hold at least one draft")
+        if kv_heads <= 0 or query_heads % kv_heads:
+            raise ValueError("attention query heads must be a multiple of KV heads")
+        self._same_dtype("attention", query, key_cache, value_cache)
+        if not torch.is_tensor(masks) or masks.dtype != torch.int64:
+            raise TypeError("draft masks must be an int64 tensor")
+        if masks.device != query.device or not masks.is_contiguous():
+            raise ValueError("draft masks must be a contiguous tensor on the cache device")
+        if masks.dim() != 3 or masks.shape[0] not in (1, batch) or masks.shape[1] != nodes \
+                or 64 * masks.shape[2] < nodes:
+            raise ValueError("draft masks must be [batch or 1, nodes, words] with 64 drafts a word")
+        if gate is not None:
+            gate = self._tensor(gate, "sigmoid-gate logits", dimensions=4)
+            if _shape(gate) != (batch, nodes, query_heads, value_width):
+                raise ValueError("sigmoid-gate logits must match the attention output")
+            self._same_dtype("attention gate", query, gate)
+        prefix_lens = self._device_ints(prefix_lens, "prefix_lens", (batch,), low=0, high=length)
+        if counts is not None:
+            counts = self._device_ints(counts, "draft counts", (batch,), low=0, high=nodes)
+        if out is not None:
+            self._out_buffer(out, (batch, nodes, query_heads, value_width),
+                             query.dtype if out_dtype is None else out_dtype, "attention output")
+        scale_value = (1.0 / math.sqrt(key_width) if scale is None
+                       else _positive_finite("attention scale", scale))
+        return dict(length=length, prefix_lens=prefix_lens, counts=counts, scale=scale_value,
+                    gate=gate, out_dtype=out_dtype, out=out)
+
+    def tree_attention(self, query: Any, key_cache: Any, value_cache: Any, masks: Any, *,
+                       length: int, prefix_lens: Any, counts: Any = None,
+                       scale: float | None = None, gate: Any = None, out_dtype: Any = None,
+                       out: Any = None) -> Any:
+        """``online_attention`` for a tree of drafts per sequence (extension):
+        draft i of ``query [B, N, Hq, D]`` attends to rows ``0 ..
+        prefix_lens[b] - 1`` of its sequence and to those draft rows
+        ``prefix_lens[b] + j`` (already in the cache) whose bit j is set in
+        ``masks [B or 1, N, words]`` (``tree_masks``).  Drafts at or past
+        ``counts[b]``, and drafts that see no row, give zeros.  ``length``
+        bounds every sequence's rows, drafts included; device lengths past it
+        are clamped.  Returns ``[B, N, Hq, Dv]``."""
+        key_cache = self._tensor(key_cache, "attention key cache", dimensions=4)
+        value_cache = self._tensor(value_cache, "attention value cache", dimensions=4)
+        capacity, batch, kv_heads, _ = _shape(key_cache)
+        if _shape(value_cache)[:3] != (capacity, batch, kv_heads):
+            raise ValueError("attention K/V cache capacity, batch, or heads differ")
+        return _ops.tree_attention(query, key_cache, value_cache, masks,
+                                   **self._tree_args(query, key_cache, value_cache, masks, batch,
+                                                     capacity, length, prefix_lens, counts, scale,
+                                                     gate, out_dtype, out))
+
+    def paged_tree_attention(self, query: Any, key_pages: Any, value_pages: Any, block_table: Any,
+                             masks: Any, *, length: int, prefix_lens: Any, counts: Any = None,
+                             scale: float | None = None, gate: Any = None, out_dtype: Any = None,
+                             out: Any = None) -> Any:
+        """``tree_attention`` over a page pool: the same rows give the same
+        bits."""
+        key_pages, value_pages = self._paged(key_pages, value_pages, block_table)
+        batch, max_pages = _shape(block_table)
+        return _ops.tree_attention(query, key_pages, value_pages, masks, block_table=block_table,
+                                   **self._tree_args(query, key_pages, value_pages, masks, batch,
+                                                     max_pages * int(key_pages.shape[1]), length,
+                                                     prefix_lens, counts, scale, gate, out_dtype,
+                                                     out))
+
+    def _commit_args(self, paths, batch, prefix_lens, accepted):
+        if not self.torch.is_tensor(paths) or paths.dim() != 2 or paths.shape[1] <= 0:
+            raise ValueError("accepted paths must be a [batch, steps] tensor")
+        paths = self._device_ints(paths, "accepted paths", (batch, int(paths.shape[1])))
+        return dict(
+            paths=paths,
+            prefix_lens=self._device_ints(prefix_lens, "prefix_lens", (batch,), low=0,
+                                          high=2 ** 31 - 1),
+            accepted=self._device_ints(accepted, "accepted counts", (batch,), low=0,
+                                       high=int(paths.shape[1])))
+
+    def tree_commit_(self, key_cache: Any, value_cache: Any, paths: Any, *, prefix_lens: Any,
+                     accepted: Any) -> None:
+        """Moves the K/V rows of the accepted drafts up behind the prefix
+        (extension): row ``prefix_lens[b] + paths[b, i]`` becomes row
+        ``prefix_lens[b] + i`` for ``i < accepted[b]``, bit for bit.
+        ``paths [B, steps]`` (device int32) names drafts in rising order and
+        ends where it stops rising.  The sequence then holds
+        ``prefix_lens[b] + accepted[b]`` rows."""
+        key_cache = self._tensor(key_cache, "attention key cache", dimensions=4)
+        value_cache = self._tensor(value_cache, "attention value cache", dimensions=4)
+        if _shape(value_cache)[:3] != _shape(key_cache)[:3]:
+            raise ValueError("attention K/V cache capacity, batch, or heads differ")
+        self._same_dtype("tree commit", key_cache, value_cache)
+        _ops.tree_commit(key_cache, value_cache,
+                         **self._commit_args(paths, int(key_cache.shape[1]), prefix_lens,
+                                             accepted))
+
+    def paged_tree_commit_(self, key_pages: Any, value_pages: Any, block_table: Any, paths: Any,
+                           *, prefix_lens: Any, accepted: Any) -> None:
+        """``tree_commit_`` over a page pool; a row whose table entry lies
+        outside the pool is not moved."""
+        key_pages, value_pages = self._paged(key_pages, value_pages, block_table)
+        _ops.tree_commit(key_pages, value_pages, block_table=block_table,
+                         **self._commit_args(paths, int(block_table.shape[0]), prefix_lens,
+                                             accepted))
+
+    def paged_resize_(self, block_table: Any, lengths: Any, free_pages: Any, free_count: Any,
+                      targets: Any, *, page_size: int, tokens: int) -> RocmPagedRows:
+        """Block tables and slots from request lengths, on the device
+        (extension): takes every sequence of a page pool from ``lengths[b]``
+        to ``targets[b]`` rows, without a copy to the host.  Pages that
+        shrinking sequences give up go onto the stack ``free_pages
+        [num_pages]``, of which ``free_count [1]`` are in use; growing ones
+        then take theirs from its top, in the order of sequences.  A request
+        is granted while the pages needed up to and with it are there and its
+        new rows end within ``tokens``; a refused one keeps its length and
+        pages.  ``block_table [B, max_pages]`` (-1 past a sequence's pages),
+        ``lengths``, ``free_pages`` and ``free_count`` (all int32) are
+        updated in place.  Returns where the new rows lie: ``slots`` go to
+        ``paged_attention_prologue_rows_``."""
+        torch = self.torch
+        if not torch.is_tensor(block_table) or block_table.dim() != 2:
+            raise TypeError("block table must be a [batch, max_pages] int32 tensor")
+        batch, max_pages = _shape(block_table)
+        if batch <= 0 or max_pages <= 0:
+            raise ValueError("block table cannot be empty")
+        block_table = self._device_ints(block_table, "block table", (batch, max_pages))
+        for name, value in (("lengths", lengths), ("free_pages", free_pages),
+                            ("free_count", free_count)):
+            if not torch.is_tensor(value) or value.device.type != "cuda" or value.dim() != 1:
+                raise TypeError(f"{name} must be a one-dimensional device tensor")
+        lengths = self._device_ints(lengths, "lengths", (batch,))
+        free_pages = self._device_ints(free_pages, "free_pages", _shape(free_pages))
+        if not free_pages.numel():
+            raise ValueError("free_pages cannot be empty")
+        free_count = self._device_ints(free_count, "free_count", (1,))
+        size = _positive_integer("page_size", page_size)
+        if size & (size - 1):
+            raise ValueError("page_size must be a power of two")
+        targets = self._device_ints(targets, "targets", (batch,), low=0, high=max_pages * size)
+        return RocmPagedRows(*_ops.paged_resize(block_table, lengths, free_pages, free_count,
+                                                targets, page_size=size,
+                                                tokens=_nonnegative_integer("tokens", tokens)))
+
+    def paged_attention_prologue_rows_(self, query_gate: Any, key: Any, value: Any,
+                                       query_norm: Any, key_norm: Any, key_pages: Any,
+                                       value_pages: Any, slots: Any, position_lanes: Any, *,
+                                       sections: Sequence[int], frequency_base: float,
+                                       epsilon: float) -> tuple[Any, Any]:
+        """``attention_prologue_`` for packed tokens of any sequences and
+        positions (extension): token t of ``query_gate [T, Hq * 2 D]``, ``key
+        [T, Hkv * D]`` and ``value [T, Hkv * Dv]`` is rotated by its own
+        ``position_lanes [T, 4]`` (int64: time, height, width, extra, as
+        ``imrope``), and its key and value are written to pool row
+        ``slots[t]`` (int32, page * page_size + row; one outside the pool
+        writes neither; no two tokens may share one).  Serves draft trees
+        (``tree_masks``) and image or video prompts.  Returns ``(query
+        [T, Hq, D], gate [T, Hq, D])``."""
+        key_pages = self._tensor(key_pages, "attention key pages", dimensions=4)
+        value_pages = self._tensor(value_pages, "attention value pages", dimensions=4)
+        pages, size, kv_heads, width = _shape(key_pages)
+        if _shape(value_pages)[:3] != (pages, size, kv_heads):
+            raise ValueError("attention K/V pages differ in count, size or heads")
+        value_width = int(value_pages.shape[3])
+        query_gate = self._tensor(query_gate, "joint Q/gate projection", dimensions=2)
+        key = self._tensor(key, "attention key", dimensions=2)
+        value = self._tensor(value, "attention value", dimensions=2)
+        query_norm = self._fp32(query_norm, "query RMSNorm weight", dimensions=1)
+        key_norm = self._fp32(key_norm, "key RMSNorm weight", dimensions=1)
+        tokens = int(query_gate.shape[0])
+        if tokens <= 0:
+            raise ValueError("the prologue needs at least one token")
+        if int(query_gate.shape[1]) % (2 * width) or not query_gate.shape[1]:
+            raise ValueError("joint Q/gate projection does not match the page head width")
+        query_heads = int(query_gate.shape[1]) // (2 * width)
+        if query_heads % kv_heads:
+            raise ValueError("attention query heads must be a multiple of KV heads")
+        if _shape(key) != (tokens, kv_heads * width) or _shape(value) != (tokens,
+                                                                          kv_heads * value_width):
+            raise ValueError("attention key/value do not match the page token shape")
+        if _shape(query_norm) != (width,) or _shape(key_norm) != (width,):
+            raise ValueError("RMSNorm weight must match the head dimension")
+        self._same_dtype("attention prologue", query_gate, key, value, key_pages, value_pages)
+        slots = self._device_ints(slots, "slots", (tokens,), low=-1, high=pages * size - 1)
+        position_lanes = self._tensor(position_lanes, "IMRoPE position lanes", allow_integer=True)
+        if position_lanes.dtype != self.torch.int64 or _shape(position_lanes) != (tokens, 4):
+            raise ValueError("IMRoPE position lanes must be int64 shape (tokens, 4)")
+        if len(sections) != 4:
+            raise ValueError("IMRoPE requires four sections")
+        section = tuple(_nonnegative_integer("IMRoPE section", item) for item in sections)
+        return _ops.attention_prologue_rows(
+            query_gate.reshape(tokens, query_heads, 2 * width), key, value, query_norm, key_norm,
+            key_pages, value_pages, slots, position_lanes, sections=section,
+            frequency_base=_positive_finite("frequency_base", frequency_base),
+            eps=_positive_finite("epsilon", epsilon))
 
     # ------------------------------------------------------ chunked prefill
 

@@ -674,6 +674,122 @@ int alpx_recurrent_prefill_prep(const float* current, const float* conv_weight,
                                 int out_dtype, void* stream);
 
 /*
+ * Trees of drafted tokens (extensions: the reference decodes one token per
+ * sequence).  Sequence b of a cache holds prefix_lens[b] rows and behind
+ * them one row per draft, draft j at row prefix_lens[b] + j.
+ *
+ * alpx_tree_attention: draft i of sequence b attends the sequence's prefix
+ * rows and those draft rows whose bit is set in its mask,
+ *   out[b, i, h, :] = softmax_j(scale * q[b, i, h] . K[j, b, h // G]) . V[j, b, h // G]
+ *                     (* sigmoid(gate[b, i, h, :]) when gate != NULL),
+ * as alpx_decode_gqa does for one token.  q [batch, nodes, q_heads, key_dim]
+ * and gate / out [batch, nodes, q_heads, value_dim] are contiguous; caches
+ * with the strides of alpx_decode_gqa, or, for the paged form, pages and a
+ * block table as alpx_decode_gqa_paged (page_size a power of two of at least
+ * 32).  masks [batch, nodes, mask_words] (64-bit words, bit j % 64 of word
+ * j / 64 is draft row j; mask_batch_stride words between sequences, 0: all
+ * share one tree).  prefix_lens and counts (null: `nodes` drafts each) are
+ * device int32 [batch]; the sequence's rows are clamped to [0, length], and
+ * nothing behind them is read.  A draft at or past counts[b], and one that
+ * sees no row, yields zeros.  Infinities and NaN in rows that a draft does
+ * not see stay out of its result.  Head widths up to 256 of any dtype,
+ * stride and alignment; rows of 16-byte multiples run fastest.  Arithmetic
+ * is fp32 (fp16 / bf16: the probabilities are rounded to the cache's type
+ * for their product, the sums are not).
+ * workspace: alpx_tree_workspace_bytes bytes (0: none is needed); scratch,
+ * which calls that may overlap must not share.
+ */
+size_t alpx_tree_workspace_bytes(int batch, int nodes, int q_heads, int kv_heads, int key_dim,
+                                 int value_dim, int length, int dtype);
+int alpx_tree_attention(const void* q, const void* key_cache, const void* value_cache,
+                        const uint64_t* masks, int64_t mask_batch_stride, int mask_words,
+                        const int32_t* prefix_lens, const int32_t* counts, int length,
+                        const void* gate, void* out, void* workspace, size_t workspace_bytes,
+                        int batch, int nodes, int q_heads, int kv_heads, int key_dim,
+                        int value_dim, int64_t k_pos_stride, int64_t k_batch_stride,
+                        int64_t k_head_stride, int64_t v_pos_stride, int64_t v_batch_stride,
+                        int64_t v_head_stride, float scale, int dtype, int out_dtype,
+                        void* stream);
+int alpx_tree_attention_paged(const void* q, const void* key_pages, const void* value_pages,
+                              const int32_t* block_table, int max_pages, int page_size,
+                              int num_pages, const uint64_t* masks, int64_t mask_batch_stride,
+                              int mask_words, const int32_t* prefix_lens, const int32_t* counts,
+                              int length, const void* gate, void* out, void* workspace,
+                              size_t workspace_bytes, int batch, int nodes, int q_heads,
+                              int kv_heads, int key_dim, int value_dim, float scale, int dtype,
+                              int out_dtype, void* stream);
+
+/* Masks, depths and positions of draft trees from parents [batch, nodes]
+ * (device int32): draft i sees itself and its ancestors.  A parent outside
+ * [0, i) makes draft i a root.  masks [batch, nodes, mask_words] with
+ * mask_words = ceil(nodes / 64); depths [batch, nodes] (roots 0);
+ * position_lanes [batch, nodes, 4] int64 (null: not wanted), the text lanes
+ * (p, p, p, 0) of p = lengths[b] + depth.  Drafts at or past counts[b]
+ * (null: all count) get empty masks, depth -1 and lanes of 0.  Up to 1024
+ * drafts.  One launch. */
+int alpx_tree_masks(const int32_t* parents, const int32_t* counts, const int32_t* lengths,
+                    uint64_t* masks, int32_t* depths, int64_t* position_lanes, int batch,
+                    int nodes, int mask_words, void* stream);
+
+/* Moves the K / V rows of an accepted path up behind the prefix: row
+ * prefix_lens[b] + paths[b, i] of sequence b becomes row prefix_lens[b] + i,
+ * for i < accepted[b] (bit-exact).  paths [batch, path_max] names drafts in
+ * rising order; a path ends at the first entry that does not rise.  Rows at
+ * or past the capacity, and rows whose table entry lies outside the pool,
+ * are neither read nor written; rows behind the accepted ones stay as they
+ * are.  Caches [capacity, batch, kv_heads, dim] or pages and a block table.
+ * One launch. */
+int alpx_tree_commit(void* key_cache, void* value_cache, const int32_t* paths,
+                     const int32_t* accepted, const int32_t* prefix_lens, int dtype,
+                     int64_t capacity, int batch, int kv_heads, int key_dim, int value_dim,
+                     int path_max, void* stream);
+int alpx_tree_commit_paged(void* key_pages, void* value_pages, const int32_t* block_table,
+                           int max_pages, int page_size, int num_pages, const int32_t* paths,
+                           const int32_t* accepted, const int32_t* prefix_lens, int dtype,
+                           int batch, int kv_heads, int key_dim, int value_dim, int path_max,
+                           void* stream);
+
+/* Block tables from request lengths: sequence b of a page pool goes from
+ * lengths[b] to targets[b] rows (device int32).  Pages that a shrinking
+ * sequence no longer needs leave its row of block_table [batch, max_pages]
+ * (entries become -1) for the stack free_pages [num_pages], of which
+ * free_count[0] are in use; then growing sequences take their pages from its
+ * top, in the order of sequences.  A request is granted while the pages
+ * needed up to and with it are at most what the stack then holds, and its
+ * new rows end within `tokens`; one that needs no page is not held up by a
+ * lack of them.  A target (or length) outside [0, max_pages * page_size] is
+ * refused.  block_table, lengths, free_pages and free_count are updated in
+ * place; granted [batch] holds 1 or 0, and a refused sequence keeps its
+ * length and pages.  The new rows of all sequences are packed in order:
+ * sequence b's are starts[b] .. starts[b + 1] - 1 (starts [batch + 1]), and
+ * new row t has pool row slots[t] (page * page_size + row in page), position
+ * positions[t] in its sequence sequences[t]; all three are [tokens], -1 past
+ * the last new row.  Cutting sequences back by the rows of the last call
+ * restores the stack.  page_size a power of two; pool and sequences of less
+ * than 2^31 rows.  One launch, two for more than 4096 tokens. */
+int alpx_paged_resize(int32_t* block_table, int32_t* lengths, int32_t* free_pages,
+                      int32_t* free_count, const int32_t* targets, int batch, int max_pages,
+                      int page_size, int num_pages, int tokens, int32_t* starts, int32_t* slots,
+                      int32_t* positions, int32_t* sequences, int32_t* granted, void* stream);
+
+/* alpx_attention_prologue for packed tokens of any sequences and positions
+ * (an extension): token t of query_gate [T, Hq, 2D], key [T, Hkv, D] and
+ * value [T, Hkv, Dv] is rotated by its own position lanes (time, height,
+ * width, extra: position_lanes [T, 4] int64, as alpx_imrope), and its key
+ * and value go to row slots[t] of key_rows [pool_rows, Hkv, D] and
+ * value_rows [pool_rows, Hkv, Dv] (a page pool, page after page); a slot
+ * outside [0, pool_rows) writes neither.  Two tokens must not share a slot.
+ * query_out [T, Hq, D], gate_out [T, Hq, D].  head dims up to 512. */
+int alpx_attention_prologue_rows(const void* query_gate, const void* key, const void* value,
+                                 const float* q_norm, const float* k_norm, void* query_out,
+                                 void* gate_out, void* key_rows, void* value_rows,
+                                 int64_t pool_rows, const int32_t* slots,
+                                 const int64_t* position_lanes, int dtype, int tokens,
+                                 int q_heads, int kv_heads, int head_dim, int value_dim,
+                                 const int* sections, double frequency_base, float eps,
+                                 void* stream);
+
+/*
  * Kernel timing (measurement support, no reference counterpart: it serves
  * the roofline measurement of bench.py).  While enabled, each entry point
  * records a pair of HIP events on its launch stream around the kernel named

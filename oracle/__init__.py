@@ -12,6 +12,9 @@ library replaces (alpaccaroo, mounted read-only as the reference tree):
   kernels: causal convolution step, SiLU, L2 / RMS / gated RMS norms, the
   recurrent parameters, IMROPE, the query/gate split, and the composed
   attention prologue and recurrent-layer step.
+* ``oracle.drafts`` -- trees of drafted tokens: what a draft sees, its
+  attention, the page pool's bookkeeping and the accepted path's rows (no
+  counterpart in the reference).
 * ``oracle.rope`` -- the llama "norm" (adjacent-pair) rotary embedding used
   to build prefill inputs.
 * ``oracle.inputs`` -- seeded synthetic inputs for the five benchmark
@@ -29,6 +32,6 @@ the mistake it would catch).  No function of this package is left
 "parity unpinned".
 """
 
-from . import attention, gdn, inputs, layer, rope  # noqa: F401
+from . import attention, drafts, gdn, inputs, layer, rope  # noqa: F401
 
-__all__ = ["attention", "gdn", "inputs", "layer", "rope"]
+__all__ = ["attention", "drafts", "gdn", "inputs", "layer", "rope"]
