@@ -45,9 +45,13 @@ struct TreeArgs {
   int words;
   int length, batch, nodes, q_heads, kv_heads, group, key_dim, value_dim;
   int col_tiles;      // column tiles per (sequence, kv head)
+  int slots;          // shares of the rows per (kv head, column tile)
+  float* part_o;      // partial states, see `segment_of`
+  float2* part_st;
   float scale_log2;
   int out_dtype;
-  int vec_q;          // q rows may be read, and out rows written, in vectors
+  int vec_q, vec_o;   // q rows may be read, out rows written in vectors
+  int direct;         // vec_o, value_dim = DP: a slot writes its whole sequences
 };
 
 // Loads that may come through the scalar cache: what they read is written
@@ -58,11 +62,83 @@ __device__ __forceinline__ int load_const(const int32_t* p) {
 }
 
 // Rows of sequence b: its prefix [0, P), its drafts [P, end).
-__device__ __forceinline__ void tree_rows(const TreeArgs& a, int b, int& P, int& end) {
-  P = min(max(load_const(a.prefix + b), 0), a.length);
-  int n = a.counts != nullptr ? load_const(a.counts + b) : a.nodes;
+__device__ __forceinline__ void lane_rows(const TreeArgs& a, int b, int& P, int& end) {
+  P = min(max(a.prefix[b], 0), a.length);
+  int n = a.counts != nullptr ? a.counts[b] : a.nodes;
   n = min(max(n, 0), a.nodes);
   end = min(P + n, a.length);
+}
+
+// Shares of the rows.  The sequences' tiles of BK rows, one sequence after
+// the other, are dealt out in runs of `per` to the slots, so that every slot
+// gets the same number whatever the lengths; a run may end one sequence and
+// begin another.  Slot s leaves the partial state of its tiles of sequence b
+// in segment s + b: both rise along the list, so no two segments share a
+// number, and there are at most slots + batch.  A run that holds a whole
+// sequence writes its output and leaves no partial state, only a mark
+// whether that output is finite.
+struct Share {
+  int per;    // tiles per slot
+  int first;  // tiles before the sequence
+  int b;      // the sequence, -1: none
+  int tiles;  // its tiles
+  int P, end; // its rows
+};
+
+// One wave's sum over its lanes, and inclusive sums.
+__device__ __forceinline__ int wave_sums(int x, int lane, int& total) {
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int y = __shfl_up(x, off);
+    if (lane >= off) x += y;
+  }
+  total = __shfl(x, 63);
+  return x;
+}
+
+// The share of the tile list that holds tile `want` (of sequence want_b if
+// that is >= 0).  Every lane of a wave calls this, and gets the same.
+template <int BK>
+__device__ __forceinline__ Share find_share(const TreeArgs& a, int per, int want, int want_b) {
+  const int lane = threadIdx.x & 63;
+  Share r = {per, 0, -1, 0, 0, 0};
+  int before = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 64) {
+    int P = 0, end = 0;
+    const int b = b0 + lane;
+    if (b < a.batch) lane_rows(a, b, P, end);
+    const int nt = (end + BK - 1) / BK;
+    int total;
+    const int incl = before + wave_sums(nt, lane, total);
+    const bool mine = want_b >= 0 ? b == want_b : (want >= incl - nt && want < incl);
+    const unsigned long long hit = __ballot(mine);
+    if (hit != 0) {
+      const int src = __ffsll((long long)hit) - 1;
+      r.b = b0 + src;
+      r.tiles = __builtin_amdgcn_readlane(nt, src);
+      r.first = __builtin_amdgcn_readlane(incl, src) - r.tiles;
+      r.P = __builtin_amdgcn_readlane(P, src);
+      r.end = __builtin_amdgcn_readlane(end, src);
+      return r;
+    }
+    before += total;
+  }
+  return r;
+}
+
+// Tiles per slot.
+template <int BK>
+__device__ __forceinline__ int tiles_per_slot(const TreeArgs& a, int& all) {
+  const int lane = threadIdx.x & 63;
+  int sum = 0;
+  for (int b = lane; b < a.batch; b += 64) {
+    int P, end;
+    lane_rows(a, b, P, end);
+    sum += (end + BK - 1) / BK;
+  }
+  (void)wave_sums(sum, lane, all);
+  all = __builtin_amdgcn_readfirstlane(all);
+  return max(1, (all + a.slots - 1) / a.slots);
 }
 
 __device__ __forceinline__ f32x16 mfma32x32x16(f16x8 a, f16x8 b, f32x16 c) {
@@ -90,6 +166,11 @@ struct Shape {
   static constexpr int kTileB = BK * kRowB;
   static constexpr int kIW = kTileB / 4096;      // direct loads per wave and tile
   static constexpr int MB = DP / 32;             // 32-channel blocks of O^T
+  // O and the sums of the waves that share keys are joined in LDS.
+  static constexpr int kMergeB = (WK - 1) * WQ * (MB * 16 + 2) * 256;
+  static constexpr int kLds = 4 * kTileB > kMergeB ? 4 * kTileB : kMergeB;
+  // Blocks per CU (160 KiB of LDS, a little of it the compiler's).
+  static constexpr int kPerCu = kLds > 80 * 1024 ? 1 : kLds > 40 * 1024 ? 2 : 4;
   static_assert(BK % (32 * WK) == 0 && kIW >= 1, "tiles split evenly over the waves");
   // The rows a wave loads lie in one 32-row group of the tile, so a page of
   // 32 rows or more is looked up once per wave and tile.
@@ -131,6 +212,13 @@ __device__ __forceinline__ bool finite(T x) {
   return fabsf(to_f32(x)) < INFINITY;
 }
 
+// Weight of a part whose reference is m in a sum whose reference is M.  A
+// part that saw no row has sums of 0 (and one whose every score was a NaN
+// keeps its NaN).
+__device__ __forceinline__ float weight(float m, float M) {
+  return m == -INFINITY ? 1.f : fast_exp2(m - M);
+}
+
 template <typename TO>
 __device__ __forceinline__ void store4(void* out, int64_t at, const float (&r)[4], int n,
                                        bool vec) {
@@ -158,75 +246,38 @@ __device__ __forceinline__ void write4(const TreeArgs& a, int64_t row, int d0, f
       if (i < n) r[i] *= stable_sigmoid(to_f32(((const T*)a.gate)[at + i]));
   }
   switch (a.out_dtype) {
-    case ALPX_F32: store4<float>(a.out, at, r, n, a.vec_q); break;
-    case ALPX_F16: store4<f16_t>(a.out, at, r, n, a.vec_q); break;
-    default: store4<bf16_t>(a.out, at, r, n, a.vec_q); break;
+    case ALPX_F32: store4<float>(a.out, at, r, n, a.vec_o); break;
+    case ALPX_F16: store4<f16_t>(a.out, at, r, n, a.vec_o); break;
+    default: store4<bf16_t>(a.out, at, r, n, a.vec_o); break;
   }
 }
 
-// One block: column tile `ct` of (sequence b, kv head).
-template <typename T, int DP, int WK, int BK, bool DMA>
-__global__ void __launch_bounds__(256, 1) tree_kernel(TreeArgs a) {
-  typedef Shape<T, DP, WK, BK> S;
+// One block: slot `s`, kv head and column tile; it walks its run of tiles,
+// sequence by sequence.
+template <typename T, typename S, bool DMA>
+__global__ void __launch_bounds__(256, S::kPerCu) tree_kernel(TreeArgs a) {
+  constexpr int DP = S::DP, WK = S::WK, BK = S::BK;
   constexpr bool F32 = sizeof(T) == 4;
   constexpr int MB = S::MB, KR = S::KR, EPU = S::EPU, U = S::U, kRowB = S::kRowB;
   constexpr int kTileB = S::kTileB;
   typedef T Unit __attribute__((ext_vector_type(EPU)));
   constexpr int NQ = DP / (2 * EPU);  // units of a query row per lane (half of them)
-  constexpr int kMergeB = (WK - 1) * S::WQ * (MB * 16 + 2) * 256;
-  constexpr int kLds = 4 * kTileB > kMergeB ? 4 * kTileB : kMergeB;
-  __shared__ __attribute__((aligned(1024))) char smem[kLds];  // K 0, V 0, K 1, V 1
+  __shared__ __attribute__((aligned(1024))) char smem[S::kLds];  // K 0, V 0, K 1, V 1
 
-  const int tid = threadIdx.x, lane = tid & 63;
+  const int tid = threadIdx.x, thread_lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wq = wave % S::WQ, wk = wave / S::WQ;
-  const int hl = lane & 31, half = lane >> 5;
+  const int G = a.group;
 
+  // The column tiles of one (slot, kv head) run next to each other on one
+  // XCD, whose L2 then holds the tiles that they all read.
   const int xcd = blockIdx.x % kXcds, at = blockIdx.x / kXcds;
   const int ct = at % a.col_tiles;
   const int unit = (at / a.col_tiles) * kXcds + xcd;
-  if (unit >= a.batch * a.kv_heads) return;
-  const int b = unit / a.kv_heads, kvh = unit % a.kv_heads;
-  int P, end;
-  tree_rows(a, b, P, end);
-  const int count = end - P;
-
-  const int G = a.group;
-  const int col = ct * S::kCols + 32 * wq + hl;
-  const int node = col / G;
-  const bool in_range = node < a.nodes, live = node < count;
-  const int64_t qrow = ((int64_t)b * a.nodes + (in_range ? node : 0)) * a.q_heads +
-                       kvh * G + (col - node * G);
-  const uint32_t* mask = a.masks + b * a.mask_b + (int64_t)(in_range ? node : 0) * a.words;
-
-  // B operand of S^T: this lane's units of its column's query row (unit
-  // 2 j + half of every pair j), zero past the head width.
-  Unit qv[NQ];
-  {
-    const T* qp = (const T*)a.q + qrow * a.key_dim;
-#pragma unroll
-    for (int j = 0; j < NQ; ++j) {
-      const int d = EPU * (2 * j + half);
-      Unit x = {};
-      if (live) {
-        if (a.vec_q && d + EPU <= a.key_dim) {
-          x = *(const Unit*)(qp + d);
-        } else {
-#pragma unroll
-          for (int e = 0; e < EPU; ++e)
-            if (d + e < a.key_dim) x[e] = qp[d + e];
-        }
-      }
-      qv[j] = x;
-    }
-  }
-
-  f32x16 o[MB];  // O^T[channel 32 mb + 8 (r / 4) + 4 half + r % 4][column]
-  float m, l;    // the column's reference score and this lane's share of the sum of P
-
-  // Rows [start, stop) in tiles of BK.
-  const int start = 0, stop = end;
-  const int nt = (stop - start + BK - 1) / BK;
+  const int slot = unit / a.kv_heads, kvh = unit % a.kv_heads;
+  if (slot >= a.slots) return;
+  int all;
+  const int per = tiles_per_slot<BK>(a, all);
 
   // Tile loads: wave w fills rows [w BK / 4, (w + 1) BK / 4) of a tile, all
   // in its 32-row group `grp`.
@@ -235,7 +286,7 @@ __global__ void __launch_bounds__(256, 1) tree_kernel(TreeArgs a) {
   uint32_t kofs[S::kIW], vofs[S::kIW];
 #pragma unroll
   for (int i = 0; i < S::kIW; ++i) {
-    const int sl = (wave * S::kIW + i) * 64 + lane;
+    const int sl = (wave * S::kIW + i) * 64 + thread_lane;
     const int r = sl / U;
     const int uk = (sl % U) ^ k_swz<S>(r), uv = (sl % U) ^ v_swz<T, S>(r);
     // units past the head width: an offset past every row, which reads zero
@@ -248,63 +299,117 @@ __global__ void __launch_bounds__(256, 1) tree_kernel(TreeArgs a) {
   }
   const uint32_t lbase = (uint32_t)(uintptr_t)(lds_void_t*)smem;
 
-  auto group_base = [&](int row, const T*& kb, const T*& vb) __attribute__((always_inline)) {
-    if (a.pages != nullptr) {
-      int pg = load_const(a.pages + (int64_t)b * a.max_pages + (row >> a.page_shift));
-      pg = min(max(pg, 0), a.num_pages - 1);
-      const int64_t in = row & ((1 << a.page_shift) - 1);
-      kb = (const T*)a.k + pg * a.ks_b + in * a.ks_pos + (int64_t)kvh * a.ks_h;
-      vb = (const T*)a.v + pg * a.vs_b + in * a.vs_pos + (int64_t)kvh * a.vs_h;
-    } else {
-      kb = (const T*)a.k + (int64_t)b * a.ks_b + (int64_t)row * a.ks_pos + (int64_t)kvh * a.ks_h;
-      vb = (const T*)a.v + (int64_t)b * a.vs_b + (int64_t)row * a.vs_pos + (int64_t)kvh * a.vs_h;
-    }
-  };
-  auto load_tile = [&](int t, int buf) __attribute__((always_inline)) {
-    const int row0 = start + t * BK + grp;
-    const int rows = __builtin_amdgcn_readfirstlane(min(max(stop - row0, 0), 32));
-    const T *kb = (const T*)a.k, *vb = (const T*)a.v;
-    if (rows > 0) group_base(row0, kb, vb);
-    if constexpr (DMA) {
-      const i32x4 rk = rsrc_words((uint64_t)(uintptr_t)kb,
-                                  (uint32_t)(rows * a.ks_pos * (int64_t)sizeof(T)));
-      const i32x4 rv = rsrc_words((uint64_t)(uintptr_t)vb,
-                                  (uint32_t)(rows * a.vs_pos * (int64_t)sizeof(T)));
-      const uint32_t dst = lbase + buf * 2 * kTileB + wave * S::kIW * 1024;
+  int todo = slot * per;
+  const int todo_end = min(all, todo + per);
+  while (todo < todo_end) {
+    // opaque, so that nothing formed from it is kept over the tile loop for
+    // the next sequence (those values took the registers of the loop)
+    int lane = thread_lane;
+    pin(lane);
+    const int hl = lane & 31, half = lane >> 5;
+    const int col = ct * S::kCols + 32 * wq + hl;
+    const int node = col / G;
+    const bool in_range = node < a.nodes;
+    const Share sh = find_share<BK>(a, per, todo, -1);
+    const int b = sh.b, P = sh.P;
+    const int t0 = todo - sh.first, nt = min(todo_end, sh.first + sh.tiles) - todo;
+    todo += nt;
+    // rows [start, stop) of sequence b, in tiles of BK
+    const int start = t0 * BK, stop = min(sh.end, start + nt * BK);
+    const int count = sh.end - P;
+    const bool live = node < count;
+    // a wave without a live column only loads and meets the barriers
+    const bool idle = ct * S::kCols + 32 * wq >= count * G;
+    if (ct * S::kCols >= count * G && (nt < sh.tiles || !a.direct)) continue;
+    const int64_t qrow = ((int64_t)b * a.nodes + (in_range ? node : 0)) * a.q_heads +
+                         kvh * G + (col - node * G);
+    const uint32_t* mask = a.masks + b * a.mask_b + (int64_t)(in_range ? node : 0) * a.words;
+
+    // B operand of S^T: this lane's units of its column's query row (unit
+    // 2 j + half of every pair j), zero past the head width.
+    Unit qv[NQ];
+    {
+      const T* qp = (const T*)a.q + qrow * a.key_dim;
+      // channels past the width: the last ones again, their bits cleared
+      const int on = live ? -1 : 0;
+      if (a.vec_q) {
 #pragma unroll
-      for (int i = 0; i < S::kIW; ++i) lds_dma16(rk, dst + i * 1024, kofs[i]);
+        for (int j = 0; j < NQ; ++j) {
+          const int d = EPU * (2 * j + half);
+          const u32x4 x = *(const u32x4*)(qp + min(d, a.key_dim - EPU));
+          qv[j] = __builtin_bit_cast(Unit, x & (uint32_t)(on & ((d - a.key_dim) >> 31)));
+        }
+      } else {
+        typedef typename std::conditional<F32, int32_t, int16_t>::type Bits;
 #pragma unroll
-      for (int i = 0; i < S::kIW; ++i) lds_dma16(rv, dst + kTileB + i * 1024, vofs[i]);
-    } else {
-      // any head width, stride or alignment: element by element
-      T* dst = (T*)(smem + buf * 2 * kTileB);
-      for (int i = lane; i < kRows * DP; i += 64) {
-        const int r = wave * kRows + i / DP, d = i % DP;
-        const bool in = r - grp < rows;
-        const T kx = in && d < a.key_dim ? kb[(int64_t)(r - grp) * a.ks_pos + d] : from_f32<T>(0.f);
-        const T vx = in && d < a.value_dim ? vb[(int64_t)(r - grp) * a.vs_pos + d] : from_f32<T>(0.f);
-        const int u = d / EPU, e = d % EPU;
-        dst[r * DP + (u ^ k_swz<S>(r)) * EPU + e] = kx;
-        dst[kTileB / (int)sizeof(T) + r * DP + (u ^ v_swz<T, S>(r)) * EPU + e] = vx;
+        for (int j = 0; j < NQ; ++j) {
+#pragma unroll
+          for (int e = 0; e < EPU; ++e) {
+            const int d = EPU * (2 * j + half) + e;
+            const Bits x = __builtin_bit_cast(Bits, qp[min(d, a.key_dim - 1)]);
+            qv[j][e] = __builtin_bit_cast(T, (Bits)(x & on & ((d - a.key_dim) >> 31)));
+          }
+        }
       }
     }
-  };
 
-  // One pass over the rows.  SAFE: a row that one column sees and another
-  // does not may hold an infinity or a NaN, and 0 times it is no 0: the
-  // product takes the finite values alone, and each column adds the others
-  // of the rows that it sees.
-  auto walk = [&](auto safe_) __attribute__((always_inline)) {
-    constexpr bool SAFE = decltype(safe_)::value;
+    f32x16 o[MB];  // O^T[channel 32 mb + 8 (r / 4) + 4 half + r % 4][column]
+    float m, l;    // the column's reference score and this lane's share of the sum of P
+
+    auto group_base = [&](int row, const T*& kb, const T*& vb) __attribute__((always_inline)) {
+      if (a.pages != nullptr) {
+        int pg = load_const(a.pages + (int64_t)b * a.max_pages + (row >> a.page_shift));
+        pg = min(max(pg, 0), a.num_pages - 1);
+        const int64_t in = row & ((1 << a.page_shift) - 1);
+        kb = (const T*)a.k + pg * a.ks_b + in * a.ks_pos + (int64_t)kvh * a.ks_h;
+        vb = (const T*)a.v + pg * a.vs_b + in * a.vs_pos + (int64_t)kvh * a.vs_h;
+      } else {
+        kb = (const T*)a.k + (int64_t)b * a.ks_b + (int64_t)row * a.ks_pos + (int64_t)kvh * a.ks_h;
+        vb = (const T*)a.v + (int64_t)b * a.vs_b + (int64_t)row * a.vs_pos + (int64_t)kvh * a.vs_h;
+      }
+    };
+    auto load_tile = [&](int t, int buf) __attribute__((always_inline)) {
+      const int row0 = start + t * BK + grp;
+      const int rows = __builtin_amdgcn_readfirstlane(min(max(stop - row0, 0), 32));
+      const T *kb = (const T*)a.k, *vb = (const T*)a.v;
+      if (rows > 0) group_base(row0, kb, vb);
+      if constexpr (DMA) {
+        const i32x4 rk = rsrc_words((uint64_t)(uintptr_t)kb,
+                                    (uint32_t)(rows * a.ks_pos * (int64_t)sizeof(T)));
+        const i32x4 rv = rsrc_words((uint64_t)(uintptr_t)vb,
+                                    (uint32_t)(rows * a.vs_pos * (int64_t)sizeof(T)));
+        const uint32_t dst = lbase + buf * 2 * kTileB + wave * S::kIW * 1024;
+#pragma unroll
+        for (int i = 0; i < S::kIW; ++i) lds_dma16(rk, dst + i * 1024, kofs[i]);
+#pragma unroll
+        for (int i = 0; i < S::kIW; ++i) lds_dma16(rv, dst + kTileB + i * 1024, vofs[i]);
+      } else {
+        // any head width, stride or alignment: element by element
+        T* dst = (T*)(smem + buf * 2 * kTileB);
+        for (int i = lane; i < kRows * DP; i += 64) {
+          const int r = wave * kRows + i / DP, d = i % DP;
+          const bool in = r - grp < rows;
+          const T kx =
+              in && d < a.key_dim ? kb[(int64_t)(r - grp) * a.ks_pos + d] : from_f32<T>(0.f);
+          const T vx =
+              in && d < a.value_dim ? vb[(int64_t)(r - grp) * a.vs_pos + d] : from_f32<T>(0.f);
+          const int u = d / EPU, e = d % EPU;
+          dst[r * DP + (u ^ k_swz<S>(r)) * EPU + e] = kx;
+          dst[kTileB / (int)sizeof(T) + r * DP + (u ^ v_swz<T, S>(r)) * EPU + e] = vx;
+        }
+      }
+    };
+
     m = -INFINITY;
     l = 0.f;
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[mb][r] = 0.f;
-    if (nt > 0) load_tile(0, 0);
+    load_tile(0, 0);
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
+#pragma clang loop unroll(disable)
     for (int t = 0; t < nt; ++t) {
       const int buf = t & 1;
       if (t + 1 < nt) load_tile(t + 1, buf ^ 1);
@@ -312,6 +417,7 @@ __global__ void __launch_bounds__(256, 1) tree_kernel(TreeArgs a) {
       const char* vt = kt + kTileB;
 #pragma unroll
       for (int kr = 0; kr < KR; ++kr) {
+        if (idle) break;
         const int g0 = 32 * (wk * KR + kr);       // this wave's keys of the tile
         const int key0 = start + t * BK + g0;
         f32x16 s;
@@ -328,13 +434,14 @@ __global__ void __launch_bounds__(256, 1) tree_kernel(TreeArgs a) {
             s = mfma32x32x16(ka, qv[j], s);
           }
         }
-        uint32_t bits = 0xffffffffu;
-        if (SAFE || key0 + 32 > P) {  // not all of these keys are prefix rows
-          bits = seen_bits(mask, a.words, P, stop, key0, live);
+        if (key0 + 32 > P) {  // not all of these keys are prefix rows
+          const uint32_t bits = seen_bits(mask, a.words, P, stop, key0, live);
           const uint32_t mine = bits >> (4 * half);
 #pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (!(mine & (1u << (8 * (r >> 2) + (r & 3))))) s[r] = -INFINITY;
+          for (int r = 0; r < 16; ++r) {
+            const int keep = (int)(mine << (31 - (8 * (r >> 2) + (r & 3)))) >> 31;  // all bits or none
+            s[r] = __int_as_float((__float_as_int(s[r]) & keep) | (0xff800000 & ~keep));
+          }
         }
         float mx = s[0];
 #pragma unroll
@@ -348,10 +455,7 @@ __global__ void __launch_bounds__(256, 1) tree_kernel(TreeArgs a) {
             const float c = fast_exp2(m - mx);  // 0 while m is -inf
             l *= c;
 #pragma unroll
-            for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-              for (int r = 0; r < 16; ++r)
-                if (!SAFE || finite(o[mb][r])) o[mb][r] *= c;
+            for (int mb = 0; mb < MB; ++mb) o[mb] *= c;
             m = mx;
           }
         }
@@ -366,18 +470,13 @@ __global__ void __launch_bounds__(256, 1) tree_kernel(TreeArgs a) {
         // O^T += V^T P^T.  Any order of the keys will do as long as both
         // operands have the same: slot e of lane half h is key 16 ks +
         // 8 (e / 4) + 4 h + e % 4, which is where P already lies.
-        bool bad = false;
         if constexpr (F32) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int vr = g0 + 8 * (r >> 2) + 4 * half + (r & 3);
 #pragma unroll
             for (int mb = 0; mb < MB; ++mb) {
-              float x = *(const float*)(vt + vr * kRowB + 128 * mb + 4 * hl);
-              if (SAFE && !finite(x)) {
-                bad = true;
-                x = 0.f;
-              }
+              const float x = *(const float*)(vt + vr * kRowB + 128 * mb + 4 * hl);
               o[mb] = mfma32x32x2(x, s[r], o[mb]);
             }
           }
@@ -399,34 +498,8 @@ __global__ void __launch_bounds__(256, 1) tree_kernel(TreeArgs a) {
               const T* p1 = (const T*)(vt + (vr + 8) * kRowB + (u ^ v_swz<T, S>(vr + 8)) * 16 +
                                        8 * (lane & 1));
               const V4 x0 = lds_read_tr4(p0), x1 = lds_read_tr4(p1);
-              V8 x = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
-              if constexpr (SAFE) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                  if (!finite(x[e])) {
-                    bad = true;
-                    x[e] = from_f32<T>(0.f);
-                  }
-              }
+              const V8 x = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
               o[mb] = mfma32x32x16(x, p, o[mb]);
-            }
-          }
-        }
-        if constexpr (SAFE) {
-          if (__ballot(bad) != 0) {
-#pragma clang loop unroll(disable)
-            for (int key = 0; key < 32; ++key) {
-              if (!(bits >> key & 1u)) continue;
-              const int vr = g0 + key;
-#pragma unroll
-              for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                  const int d = 32 * mb + 8 * (r >> 2) + 4 * half + (r & 3);
-                  const T x = *(const T*)(vt + vr * kRowB + ((d / EPU) ^ v_swz<T, S>(vr)) * 16 +
-                                          (d % EPU) * (int)sizeof(T));
-                  if (!finite(x)) o[mb][r] += to_f32(x);
-                }
             }
           }
         }
@@ -434,86 +507,336 @@ __global__ void __launch_bounds__(256, 1) tree_kernel(TreeArgs a) {
       __builtin_amdgcn_s_waitcnt(0);  // the next tile is in LDS
       __syncthreads();
     }
-  };
 
-  walk(std::false_type());
-  bool bad = false;
+    l += __shfl_xor(l, 32);
+    if constexpr (WK > 1) {
+      // the waves of a column tile's keys, joined in LDS by the first of them
+      constexpr int kPart = (MB * 16 + 2) * 64;  // floats per wave
+      float* part = (float*)smem;
+      if (wk > 0) {
+        float* p = part + ((wk - 1) * S::WQ + wq) * kPart + lane;
 #pragma unroll
-  for (int mb = 0; mb < MB; ++mb)
+        for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) bad |= !(fabsf(o[mb][r]) < INFINITY);
-  if (__syncthreads_or(bad)) walk(std::true_type());
-
-  l += __shfl_xor(l, 32);
-  if constexpr (WK > 1) {
-    // the waves of a column tile's keys, joined in LDS by the first of them
-    constexpr int kPart = (MB * 16 + 2) * 64;  // floats per wave
-    float* part = (float*)smem;
-    if (wk > 0) {
-      float* p = part + ((wk - 1) * S::WQ + wq) * kPart + lane;
+          for (int r = 0; r < 16; ++r) p[(mb * 16 + r) * 64] = o[mb][r];
+        p[MB * 16 * 64] = m;
+        p[(MB * 16 + 1) * 64] = l;
+      }
+      __syncthreads();
+      if (wk == 0) {
 #pragma unroll
-      for (int mb = 0; mb < MB; ++mb)
+        for (int w = 0; w < WK - 1; ++w) {
+          const float* p = part + (w * S::WQ + wq) * kPart + lane;
+          const float m1 = p[MB * 16 * 64], l1 = p[(MB * 16 + 1) * 64];
+          const float M = fmaxf(m, m1);
+          const float c0 = weight(m, M), c1 = weight(m1, M);
+          l = l * c0 + l1 * c1;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) p[(mb * 16 + r) * 64] = o[mb][r];
-      p[MB * 16 * 64] = m;
-      p[(MB * 16 + 1) * 64] = l;
-    }
-    __syncthreads();
-    if (wk > 0) return;
+          for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-    for (int w = 0; w < WK - 1; ++w) {
-      const float* p = part + (w * S::WQ + wq) * kPart + lane;
-      const float m1 = p[MB * 16 * 64], l1 = p[(MB * 16 + 1) * 64];
-      const float M = fmaxf(m, m1);
-      // a part that saw no row has l = 0 and O = 0; one that saw a NaN keeps it
-      const float c0 = m == -INFINITY ? 1.f : fast_exp2(m - M);
-      const float c1 = m1 == -INFINITY ? 1.f : fast_exp2(m1 - M);
-      l = l * c0 + l1 * c1;
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float x0 = o[mb][r], x1 = p[(mb * 16 + r) * 64];
-          o[mb][r] = (finite(x0) ? x0 * c0 : x0) + (finite(x1) ? x1 * c1 : x1);
+            for (int r = 0; r < 16; ++r)
+              o[mb][r] = o[mb][r] * c0 + p[(mb * 16 + r) * 64] * c1;
+          m = M;
         }
+      }
+      __syncthreads();  // the next sequence's tiles may overwrite the parts
+      if (wk > 0) continue;
+    }
+    if (nt < sh.tiles || !a.direct) {
+      if (idle) continue;
+      const int64_t seg =
+          ((int64_t)(slot + b) * a.kv_heads + kvh) * a.col_tiles * S::WQ + ct * S::WQ + wq;
+      f32x4* po = (f32x4*)a.part_o + seg * (MB * 4 * 64) + lane;
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          po[(mb * 4 + q) * 64] =
+              (f32x4){o[mb][4 * q], o[mb][4 * q + 1], o[mb][4 * q + 2], o[mb][4 * q + 3]};
+      if (half == 0) a.part_st[seg * 32 + hl] = make_float2(m, l);
+      continue;
+    }
+    // a whole sequence: the output, and whether some of it is not finite
+    float zero = 0.f;  // 0 times anything else is a NaN
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) zero = fmaf(o[mb][r], 0.f, zero);
+    const bool bad = __ballot(live && zero != 0.f) != 0;
+    const int64_t seg =
+        ((int64_t)(slot + b) * a.kv_heads + kvh) * a.col_tiles * S::WQ + ct * S::WQ + wq;
+    if (half == 0) a.part_st[seg * 32 + hl] = make_float2(bad ? 1.f : 0.f, 0.f);
+    if (!in_range) continue;
+    const float inv = live && l != 0.f ? 1.f / l : 0.f;
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) o[mb] = live ? o[mb] * inv : (f32x16){};
+    const int64_t out0 = qrow * DP + 4 * half;
+    if (a.gate != nullptr) {
+      typedef typename Vec4<T>::type V4;
+      const T* gp = (const T*)a.gate + out0;
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const V4 g = *(const V4*)(gp + 32 * mb + 8 * q);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[mb][4 * q + i] *= fast_sigmoid(to_f32(g[i]));
+        }
+    }
+    auto store = [&](auto zero_of_type) __attribute__((always_inline)) {
+      typedef decltype(zero_of_type) TO;
+      typedef TO TO4 __attribute__((ext_vector_type(4)));
+      TO* op = (TO*)a.out + out0;
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *(TO4*)(op + 32 * mb + 8 * q) =
+              (TO4){from_f32<TO>(o[mb][4 * q]), from_f32<TO>(o[mb][4 * q + 1]),
+                    from_f32<TO>(o[mb][4 * q + 2]), from_f32<TO>(o[mb][4 * q + 3])};
+    };
+    switch (a.out_dtype) {
+      case ALPX_F32: store(0.f); break;
+      case ALPX_F16: store((f16_t)0.f); break;
+      default: store((bf16_t)0.f); break;
+    }
+  }
+}
+
+// The result of 32 columns and 32 channels row by row, for sequences with an
+// infinity or a NaN in them.  The products take every row of a tile for
+// every column, and 0 times an infinity is a NaN: here a column takes the
+// rows that it sees, and an infinity among their values comes out as itself
+// however small its weight.  Thread (column, g) takes rows g, g + 8, ...
+template <typename T>
+__device__ __noinline__ void rows_apart(const TreeArgs& a, int b, int kvh, int col, int d0, int P,
+                                        int end, float (&o)[32], float& m, float& l) {
+  const int G = a.group, node = col / G, g = threadIdx.x >> 5;
+  m = -INFINITY;
+  l = 0.f;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) o[i] = 0.f;
+  if (node >= min(end - P, a.nodes)) return;
+  const T* q = (const T*)a.q +
+               (((int64_t)b * a.nodes + node) * a.q_heads + kvh * G + (col - node * G)) * a.key_dim;
+  const uint32_t* mask = a.masks + b * a.mask_b + (int64_t)node * a.words;
+  for (int j = g; j < end; j += 8) {
+    if (j >= P && !(mask[(j - P) >> 5] >> ((j - P) & 31) & 1u)) continue;
+    int64_t ko = (int64_t)b * a.ks_b + j * a.ks_pos, vo = (int64_t)b * a.vs_b + j * a.vs_pos;
+    if (a.pages != nullptr) {
+      int pg = a.pages[(int64_t)b * a.max_pages + (j >> a.page_shift)];
+      pg = min(max(pg, 0), a.num_pages - 1);
+      const int64_t in = j & ((1 << a.page_shift) - 1);
+      ko = pg * a.ks_b + in * a.ks_pos;
+      vo = pg * a.vs_b + in * a.vs_pos;
+    }
+    const T* k = (const T*)a.k + ko + (int64_t)kvh * a.ks_h;
+    const T* v = (const T*)a.v + vo + (int64_t)kvh * a.vs_h;
+    float s = 0.f;
+    for (int d = 0; d < a.key_dim; ++d) s = fmaf(to_f32(q[d]), to_f32(k[d]), s);
+    s *= a.scale_log2;
+    const float M = fmaxf(m, s);
+    const float c = weight(m, M), p = fast_exp2(s - M);
+    l = l * c + p;
+    m = M;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const float x = d0 + i < a.value_dim ? to_f32(v[d0 + i]) : 0.f;
+      const float kept = finite(o[i]) ? o[i] * c : o[i];
+      o[i] = kept + (finite(x) ? p * x : x);
+    }
+  }
+}
+
+// Joins the segments of the sequences that more than one slot has tiles of,
+// and writes zeros for those without a row.  One block per (sequence, kv
+// head, 32 columns, 32 channels); its four waves take the segments in turn
+// and meet in LDS.  A block whose result is not finite forms it again, row
+// by row.
+template <typename T, int DP, int BK>
+__global__ void __launch_bounds__(256) tree_join(TreeArgs a) {
+  constexpr int MB = DP / 32, kFlight = 4;
+  __shared__ float part[34 * 256];  // [4][18][64] of the segments, or [34][256] row by row
+  const int lane = threadIdx.x & 63, hl = lane & 31, half = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int mb = blockIdx.x % MB;
+  const int groups = a.col_tiles;  // of 32 columns
+  const int cg = blockIdx.x / MB % groups;
+  const int kvh = blockIdx.x / MB / groups % a.kv_heads;
+  const int b = blockIdx.x / MB / groups / a.kv_heads;
+  int all;
+  const int per = tiles_per_slot<BK>(a, all);
+  const Share sh = find_share<BK>(a, per, 0, b);
+  const int s0 = sh.first / per, s1 = (sh.first + max(sh.tiles, 1) - 1) / per;
+  const bool whole = a.direct && sh.tiles > 0 && s0 == s1;  // written by its slot
+  if (whole && a.part_st[((((int64_t)(s0 + b) * a.kv_heads + kvh) * groups + cg) * 32)].x == 0.f)
+    return;
+  const int G = a.group, col = 32 * cg + hl, node = col / G;
+  const int count = sh.end - sh.P;
+  float m = -INFINITY, l = 0.f, o[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) o[i] = 0.f;
+  if (!whole && sh.tiles > 0 && 32 * cg < count * G) {
+    for (int s = s0 + w; s <= s1; s += 4 * kFlight) {
+      float2 st[kFlight];
+      f32x4 x[kFlight][4];
+#pragma unroll
+      for (int u = 0; u < kFlight; ++u) {
+        const int su = min(s + 4 * u, s1);  // past the last: its loads again, unused
+        const int64_t seg = ((int64_t)(su + b) * a.kv_heads + kvh) * groups + cg;
+        st[u] = a.part_st[seg * 32 + hl];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          x[u][q] = ((const f32x4*)a.part_o)[(seg * MB + mb) * 256 + q * 64 + lane];
+      }
+      float M = m;
+#pragma unroll
+      for (int u = 0; u < kFlight; ++u)
+        if (s + 4 * u <= s1) M = fmaxf(M, st[u].x);
+      const float c = weight(m, M);
+      l *= c;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[i] *= c;
+#pragma unroll
+      for (int u = 0; u < kFlight; ++u) {
+        if (s + 4 * u > s1) continue;
+        const float cu = weight(st[u].x, M);
+        l += st[u].y * cu;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] += x[u][i >> 2][i & 3] * cu;
+      }
       m = M;
     }
   }
-  if (!in_range) return;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  {
+    float* p = part + w * 18 * 64 + lane;
 #pragma unroll
-  for (int mb = 0; mb < MB; ++mb)
+    for (int i = 0; i < 16; ++i) p[i * 64] = o[i];
+    p[16 * 64] = m;
+    p[17 * 64] = l;
+  }
+  __syncthreads();
+  float M = -INFINITY;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      float r[4];
+  for (int v = 0; v < 4; ++v) M = fmaxf(M, part[(v * 18 + 16) * 64 + lane]);
+  l = 0.f;
+  float r[4] = {0.f, 0.f, 0.f, 0.f};  // wave w writes channels 8 w + 4 half + 0 .. 3
 #pragma unroll
-      for (int i = 0; i < 4; ++i) r[i] = live ? o[mb][4 * q + i] * inv : 0.f;
-      write4<T>(a, qrow, 32 * mb + 8 * q + 4 * half, r);
+  for (int v = 0; v < 4; ++v) {
+    const float c = weight(part[(v * 18 + 16) * 64 + lane], M);
+    l += part[(v * 18 + 17) * 64 + lane] * c;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] += part[(v * 18 + 4 * w + i) * 64 + lane] * c;
+  }
+  bool bad = whole;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) bad |= node < count && !(finite(r[i]) && finite(l));
+  if (__syncthreads_or(bad)) {
+    float x[32];
+    rows_apart<T>(a, b, kvh, 32 * cg + (threadIdx.x & 31), 32 * mb, sh.P, sh.end, x, m, l);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) part[i * 256 + threadIdx.x] = x[i];
+    part[32 * 256 + threadIdx.x] = m;
+    part[33 * 256 + threadIdx.x] = l;
+    __syncthreads();
+    M = -INFINITY;
+    for (int g = 0; g < 8; ++g) M = fmaxf(M, part[32 * 256 + 32 * g + hl]);
+    l = 0.f;
+    for (int i = 0; i < 4; ++i) r[i] = 0.f;
+    for (int g = 0; g < 8; ++g) {
+      const float c = weight(part[32 * 256 + 32 * g + hl], M);
+      l += part[33 * 256 + 32 * g + hl] * c;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float y = part[(8 * w + 4 * half + i) * 256 + 32 * g + hl];
+        r[i] += finite(y) ? y * c : y;
+      }
     }
+  }
+  if (node >= a.nodes) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int64_t qrow =
+      ((int64_t)b * a.nodes + node) * a.q_heads + kvh * G + (col - node * G);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = node < count ? r[i] * inv : 0.f;
+  write4<T>(a, qrow, 32 * mb + 8 * w + 4 * half, r);
 }
 
 struct Kernel {
   const void* fn;
-  int cols;  // columns per block
+  const void* join;
+  int cols;     // columns per block
+  int rows;     // rows per tile
+  int width;    // DP
+  int per_cu;   // blocks on a CU at a time
 };
 
 template <typename T, int DP, int WK, int BK, bool DMA>
 Kernel make() {
-  return {(const void*)tree_kernel<T, DP, WK, BK, DMA>, Shape<T, DP, WK, BK>::kCols};
+  typedef Shape<T, DP, WK, BK> S;
+  return {(const void*)tree_kernel<T, S, DMA>, (const void*)tree_join<T, DP, BK>,
+          S::kCols, BK, DP, S::kPerCu};
 }
 
+// Waves side by side in columns or in keys: few columns leave whole waves
+// without work unless they share the keys.
 template <typename T>
-Kernel pick(int width, bool dma) {
-  constexpr int B64 = sizeof(T) == 4 ? 32 : 64;
-  if (width <= 64) return dma ? make<T, 64, 1, B64, true>() : make<T, 64, 1, B64, false>();
-  if (width <= 128) return dma ? make<T, 128, 1, B64, true>() : make<T, 128, 1, B64, false>();
-  return dma ? make<T, 256, 1, 32, true>() : make<T, 256, 1, 32, false>();
+Kernel pick(int width, int cols, bool dma) {
+  constexpr bool F32 = sizeof(T) == 4;
+  if (width <= 64) {
+    if (!dma) return make<T, 64, 2, 64, false>();
+    return cols <= 64 ? make<T, 64, 2, 64, true>() : make<T, 64, 1, F32 ? 32 : 64, true>();
+  }
+  if (width <= 128) {
+    if (!dma) return make<T, 128, 2, 64, false>();
+    return cols <= 64 ? make<T, 128, 2, 64, true>() : make<T, 128, 1, F32 ? 32 : 64, true>();
+  }
+  if constexpr (F32) {
+    return dma ? make<T, 256, 1, 32, true>() : make<T, 256, 1, 32, false>();
+  } else {
+    if (!dma) return make<T, 256, 1, 32, false>();
+    return cols <= 64 ? make<T, 256, 2, 64, true>() : make<T, 256, 1, 32, true>();
+  }
+}
+
+constexpr int kCus = 256;
+
+struct TreePlan {
+  Kernel kernel;
+  int col_tiles, slots;
+  bool join;
+  size_t segments, part_o, bytes;  // floats of O, bytes in all
+};
+
+TreePlan tree_plan(int batch, int nodes, int q_heads, int kv_heads, int key_dim, int value_dim,
+                   int length, int dtype, bool dma) {
+  TreePlan p = {};
+  const int width = std::max(key_dim, value_dim);
+  const int cols = nodes * (q_heads / kv_heads);
+  p.kernel = dtype == ALPX_F32   ? pick<float>(width, cols, dma)
+             : dtype == ALPX_F16 ? pick<f16_t>(width, cols, dma)
+                                 : pick<bf16_t>(width, cols, dma);
+  p.col_tiles = (cols + p.kernel.cols - 1) / p.kernel.cols;
+  // one round of blocks, every slot at least a tile
+  const int64_t tiles = (int64_t)batch * ((length + p.kernel.rows - 1) / p.kernel.rows);
+  const int64_t share = kCus * p.kernel.per_cu / ((int64_t)kv_heads * p.col_tiles);
+  p.slots = (int)std::min(std::max<int64_t>(share, 1), tiles);
+  p.join = true;
+  p.segments = (size_t)(p.slots + batch) * kv_heads * p.col_tiles * (p.kernel.cols / 32);
+  p.part_o = p.segments * 32 * p.kernel.width;
+  p.bytes = p.part_o * 4 + p.segments * 32 * sizeof(float2);
+  return p;
+}
+
+bool tree_sizes_ok(int batch, int nodes, int q_heads, int kv_heads, int key_dim, int value_dim,
+                   int length) {
+  return batch > 0 && nodes > 0 && q_heads > 0 && kv_heads > 0 && key_dim > 0 && value_dim > 0 &&
+         length > 0 && q_heads % kv_heads == 0 && key_dim <= 256 && value_dim <= 256 &&
+         (int64_t)nodes * (q_heads / kv_heads) <= (1 << 24);
 }
 
 int tree_launch(const char* what, TreeArgs a, int dtype, void* workspace, size_t workspace_bytes,
                 void* stream) {
-  (void)workspace;
-  (void)workspace_bytes;
   if (!a.q || !a.k || !a.v || !a.out || !a.masks || !a.prefix)
     return fail(ALPX_EINVAL, "%s: null buffer", what);
   if (!dtype_ok(dtype) || !dtype_ok(a.out_dtype)) return fail(ALPX_EINVAL, "%s: unknown dtype", what);
@@ -538,21 +861,35 @@ int tree_launch(const char* what, TreeArgs a, int dtype, void* workspace, size_t
                          (uintptr_t)(a.vs_h * es) | (uintptr_t)(a.key_dim * es) |
                          (uintptr_t)(a.value_dim * es);
   const bool dma = (rows & 15) == 0;
-  a.vec_q = (((uintptr_t)a.q | (uintptr_t)(a.key_dim * es)) & 15) == 0 &&
-            (((uintptr_t)a.out | (uintptr_t)(a.value_dim * os)) & (4 * os - 1)) == 0;
-  const int width = std::max(a.key_dim, a.value_dim);
-  const Kernel kernel = dtype == ALPX_F32   ? pick<float>(width, dma)
-                        : dtype == ALPX_F16 ? pick<f16_t>(width, dma)
-                                            : pick<bf16_t>(width, dma);
-  a.col_tiles = (a.nodes * a.group + kernel.cols - 1) / kernel.cols;
-  const int64_t units = (int64_t)a.batch * a.kv_heads;
-  const int64_t blocks = (units + kXcds - 1) / kXcds * kXcds * a.col_tiles;
-  if (blocks > 0x7fffffff) return fail(ALPX_EUNSUPPORTED, "%s: too many sequences", what);
+  a.vec_q = (((uintptr_t)a.q | (uintptr_t)(a.key_dim * es)) & 15) == 0;
+  a.vec_o = a.value_dim % 4 == 0 && ((uintptr_t)a.out & (4 * os - 1)) == 0 &&
+            ((uintptr_t)a.gate & (4 * es - 1)) == 0;
+  const TreePlan p = tree_plan(a.batch, a.nodes, a.q_heads, a.kv_heads, a.key_dim, a.value_dim,
+                               a.length, dtype, dma);
+  if (workspace_bytes < p.bytes || (p.bytes > 0 && !workspace))
+    return fail(ALPX_EINVAL, "%s: workspace holds %zu bytes, needs %zu", what, workspace_bytes,
+                p.bytes);
+  a.col_tiles = p.col_tiles;
+  a.slots = p.slots;
+  a.direct = a.vec_o && a.value_dim == p.kernel.width;
+  a.part_o = (float*)workspace;
+  a.part_st = (float2*)((float*)workspace + p.part_o);
+  const int64_t units = (int64_t)p.slots * a.kv_heads;
+  const int64_t blocks = (units + kXcds - 1) / kXcds * kXcds * p.col_tiles;
+  const int groups = p.col_tiles * (p.kernel.cols / 32);
+  const int64_t joins = (int64_t)a.batch * a.kv_heads * groups * (p.kernel.width / 32);
+  if (blocks > 0x7fffffff || joins > 0x7fffffff)
+    return fail(ALPX_EUNSUPPORTED, "%s: too many sequences", what);
   hipStream_t s = (hipStream_t)stream;
-  TimedRegion timed(ALPX_T_DECODE, s);
   void* args[] = {&a};
-  if (hipLaunchKernel(kernel.fn, dim3((unsigned)blocks), dim3(256), args, 0, s) != hipSuccess) {
-    return check_launch(what);
+  {
+    TimedRegion timed(ALPX_T_DECODE, s);
+    (void)hipLaunchKernel(p.kernel.fn, dim3((unsigned)blocks), dim3(256), args, 0, s);
+  }
+  if (p.join) {
+    a.col_tiles = groups;
+    TimedRegion timed(ALPX_T_DECODE_COMBINE, s);
+    (void)hipLaunchKernel(p.kernel.join, dim3((unsigned)joins), dim3(256), args, 0, s);
   }
   return check_launch(what);
 }
@@ -562,7 +899,16 @@ int tree_launch(const char* what, TreeArgs a, int dtype, void* workspace, size_t
 
 using namespace alpx;
 
-extern "C" size_t alpx_tree_workspace_bytes(int, int, int, int, int, int, int, int) { return 0; }
+extern "C" size_t alpx_tree_workspace_bytes(int batch, int nodes, int q_heads, int kv_heads,
+                                            int key_dim, int value_dim, int length, int dtype) {
+  if (!tree_sizes_ok(batch, nodes, q_heads, kv_heads, key_dim, value_dim, length) || !dtype_ok(dtype))
+    return 0;
+  size_t most = 0;
+  for (const bool dma : {false, true})
+    most = std::max(most, tree_plan(batch, nodes, q_heads, kv_heads, key_dim, value_dim, length,
+                                    dtype, dma).bytes);
+  return most;
+}
 
 extern "C" int alpx_tree_attention(const void* q, const void* key_cache, const void* value_cache,
                                    const uint64_t* masks, int64_t mask_batch_stride,
