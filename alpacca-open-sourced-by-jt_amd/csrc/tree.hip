@@ -69,6 +69,15 @@ __device__ __forceinline__ void lane_rows(const TreeArgs& a, int b, int& P, int&
   end = min(P + n, a.length);
 }
 
+// The same of one sequence for the whole wave, through the scalar cache.
+__device__ __forceinline__ void uniform_rows(const TreeArgs& a, int b, int& P, int& end) {
+  P = min(max(load_const(a.prefix + b), 0), a.length);
+  int n = a.counts != nullptr ? load_const(a.counts + b) : a.nodes;
+  n = min(max(n, 0), a.nodes);
+  P = __builtin_amdgcn_readfirstlane(P);
+  end = __builtin_amdgcn_readfirstlane(min(P + n, a.length));
+}
+
 // Shares of the rows.  The sequences' tiles of BK rows, one sequence after
 // the other, are dealt out in runs of `per` to the slots, so that every slot
 // gets the same number whatever the lengths; a run may end one sequence and
@@ -85,60 +94,59 @@ struct Share {
   int P, end; // its rows
 };
 
-// One wave's sum over its lanes, and inclusive sums.
-__device__ __forceinline__ int wave_sums(int x, int lane, int& total) {
+// Tiles of sequence b0 + lane, and before it (from b0 on).
+template <int BK>
+__device__ __forceinline__ void lane_tiles(const TreeArgs& a, int b0, int& P, int& end, int& nt,
+                                           int& before, int& total) {
+  const int lane = threadIdx.x & 63, b = b0 + lane;
+  P = end = 0;
+  if (b < a.batch) lane_rows(a, b, P, end);
+  nt = (end + BK - 1) / BK;
+  int x = nt;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
     const int y = __shfl_up(x, off);
     if (lane >= off) x += y;
   }
-  total = __shfl(x, 63);
-  return x;
+  total = __builtin_amdgcn_readlane(x, 63);
+  before = x - nt;
 }
 
-// The share of the tile list that holds tile `want` (of sequence want_b if
-// that is >= 0).  Every lane of a wave calls this, and gets the same.
+// The share of tile `want`, or where want_b >= 0 of sequence want_b; want
+// counts in units of the tiles per slot.  Every lane of a wave calls this,
+// and gets the same.
 template <int BK>
-__device__ __forceinline__ Share find_share(const TreeArgs& a, int per, int want, int want_b) {
-  const int lane = threadIdx.x & 63;
-  Share r = {per, 0, -1, 0, 0, 0};
-  int before = 0;
+__device__ __forceinline__ Share find_share(const TreeArgs& a, int want_slot, int want_b, int& all) {
+  int P, end, nt, before, total;
+  lane_tiles<BK>(a, 0, P, end, nt, before, total);
+  all = total;
+  for (int b0 = 64; b0 < a.batch; b0 += 64) {  // the first 64 sequences stay in registers
+    int p, e, n, f, t;
+    lane_tiles<BK>(a, b0, p, e, n, f, t);
+    all += t;
+  }
+  Share r = {};
+  r.b = -1;
+  r.per = max(1, (all + a.slots - 1) / a.slots);
+  const int want = want_slot * r.per;
+  int base = 0;
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    int P = 0, end = 0;
-    const int b = b0 + lane;
-    if (b < a.batch) lane_rows(a, b, P, end);
-    const int nt = (end + BK - 1) / BK;
-    int total;
-    const int incl = before + wave_sums(nt, lane, total);
-    const bool mine = want_b >= 0 ? b == want_b : (want >= incl - nt && want < incl);
+    if (b0 > 0) lane_tiles<BK>(a, b0, P, end, nt, before, total);
+    const int b = b0 + (int)(threadIdx.x & 63), first = base + before;
+    const bool mine = want_b >= 0 ? b == want_b : (want >= first && want < first + nt);
     const unsigned long long hit = __ballot(mine);
     if (hit != 0) {
       const int src = __ffsll((long long)hit) - 1;
       r.b = b0 + src;
       r.tiles = __builtin_amdgcn_readlane(nt, src);
-      r.first = __builtin_amdgcn_readlane(incl, src) - r.tiles;
+      r.first = __builtin_amdgcn_readlane(first, src);
       r.P = __builtin_amdgcn_readlane(P, src);
       r.end = __builtin_amdgcn_readlane(end, src);
       return r;
     }
-    before += total;
+    base += total;
   }
   return r;
-}
-
-// Tiles per slot.
-template <int BK>
-__device__ __forceinline__ int tiles_per_slot(const TreeArgs& a, int& all) {
-  const int lane = threadIdx.x & 63;
-  int sum = 0;
-  for (int b = lane; b < a.batch; b += 64) {
-    int P, end;
-    lane_rows(a, b, P, end);
-    sum += (end + BK - 1) / BK;
-  }
-  (void)wave_sums(sum, lane, all);
-  all = __builtin_amdgcn_readfirstlane(all);
-  return max(1, (all + a.slots - 1) / a.slots);
 }
 
 __device__ __forceinline__ f32x16 mfma32x32x16(f16x8 a, f16x8 b, f32x16 c) {
@@ -153,10 +161,10 @@ __device__ __forceinline__ f32x16 mfma32x32x2(float a, float b, f32x16 c) {
 
 // Shape of a kernel: T, DP (the head width rounded up to 64, 128 or 256), WK
 // waves that share a column tile's keys (4 / WK waves side by side in
-// columns), BK rows per K and V tile.
-template <typename T, int DP_, int WK_, int BK_>
+// columns), BK rows per K and V tile, a ring of RING tiles in LDS.
+template <typename T, int DP_, int WK_, int BK_, int RING_>
 struct Shape {
-  static constexpr int DP = DP_, WK = WK_, BK = BK_;
+  static constexpr int DP = DP_, WK = WK_, BK = BK_, RING = RING_;
   static constexpr int WQ = 4 / WK;
   static constexpr int kCols = 32 * WQ;
   static constexpr int KR = BK / (32 * WK);      // 32-key groups per wave and tile
@@ -165,10 +173,11 @@ struct Shape {
   static constexpr int kRowB = DP * (int)sizeof(T);
   static constexpr int kTileB = BK * kRowB;
   static constexpr int kIW = kTileB / 4096;      // direct loads per wave and tile
+  static constexpr int kTileLoads = 2 * kIW;     // direct loads per wave for a tile's K and V
   static constexpr int MB = DP / 32;             // 32-channel blocks of O^T
   // O and the sums of the waves that share keys are joined in LDS.
   static constexpr int kMergeB = (WK - 1) * WQ * (MB * 16 + 2) * 256;
-  static constexpr int kLds = 4 * kTileB > kMergeB ? 4 * kTileB : kMergeB;
+  static constexpr int kLds = 2 * RING * kTileB > kMergeB ? 2 * RING * kTileB : kMergeB;
   // Blocks per CU (160 KiB of LDS, a little of it the compiler's).
   static constexpr int kPerCu = kLds > 80 * 1024 ? 1 : kLds > 40 * 1024 ? 2 : 4;
   static_assert(BK % (32 * WK) == 0 && kIW >= 1, "tiles split evenly over the waves");
@@ -205,6 +214,17 @@ __device__ __forceinline__ uint32_t seen_bits(const uint32_t* mask, int words, i
   }
   const int left = end - key0;
   return left < 32 ? bits & ((1u << left) - 1u) : bits;
+}
+
+// Waits until at most N of this wave's loads are on their way.  The direct
+// loads are unknown to the compiler; loads of its own among them only make
+// the wait longer.
+template <int N>
+__device__ __forceinline__ void wait_tiles() {
+  static_assert(N >= 0 && N < 64, "vmcnt is 6 bits");
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(N) : "memory");
+#endif
 }
 
 template <typename T>
@@ -262,7 +282,7 @@ __global__ void __launch_bounds__(256, S::kPerCu) tree_kernel(TreeArgs a) {
   constexpr int kTileB = S::kTileB;
   typedef T Unit __attribute__((ext_vector_type(EPU)));
   constexpr int NQ = DP / (2 * EPU);  // units of a query row per lane (half of them)
-  __shared__ __attribute__((aligned(1024))) char smem[S::kLds];  // K 0, V 0, K 1, V 1
+  __shared__ __attribute__((aligned(1024))) char smem[S::kLds];  // K 0, V 0, K 1, V 1, ..
 
   const int tid = threadIdx.x, thread_lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -277,7 +297,10 @@ __global__ void __launch_bounds__(256, S::kPerCu) tree_kernel(TreeArgs a) {
   const int slot = unit / a.kv_heads, kvh = unit % a.kv_heads;
   if (slot >= a.slots) return;
   int all;
-  const int per = tiles_per_slot<BK>(a, all);
+  Share sh = find_share<BK>(a, slot, -1, all);
+  if (sh.b < 0) return;  // fewer tiles than slots
+  int todo = slot * sh.per;
+  const int todo_end = min(all, todo + sh.per);
 
   // Tile loads: wave w fills rows [w BK / 4, (w + 1) BK / 4) of a tile, all
   // in its 32-row group `grp`.
@@ -299,9 +322,7 @@ __global__ void __launch_bounds__(256, S::kPerCu) tree_kernel(TreeArgs a) {
   }
   const uint32_t lbase = (uint32_t)(uintptr_t)(lds_void_t*)smem;
 
-  int todo = slot * per;
-  const int todo_end = min(all, todo + per);
-  while (todo < todo_end) {
+  for (;;) {
     // opaque, so that nothing formed from it is kept over the tile loop for
     // the next sequence (those values took the registers of the loop)
     int lane = thread_lane;
@@ -310,48 +331,19 @@ __global__ void __launch_bounds__(256, S::kPerCu) tree_kernel(TreeArgs a) {
     const int col = ct * S::kCols + 32 * wq + hl;
     const int node = col / G;
     const bool in_range = node < a.nodes;
-    const Share sh = find_share<BK>(a, per, todo, -1);
     const int b = sh.b, P = sh.P;
     const int t0 = todo - sh.first, nt = min(todo_end, sh.first + sh.tiles) - todo;
-    todo += nt;
+    auto segment = [&]() __attribute__((always_inline)) {
     // rows [start, stop) of sequence b, in tiles of BK
     const int start = t0 * BK, stop = min(sh.end, start + nt * BK);
     const int count = sh.end - P;
     const bool live = node < count;
     // a wave without a live column only loads and meets the barriers
     const bool idle = ct * S::kCols + 32 * wq >= count * G;
-    if (ct * S::kCols >= count * G && (nt < sh.tiles || !a.direct)) continue;
+    if (ct * S::kCols >= count * G && (nt < sh.tiles || !a.direct)) return;
     const int64_t qrow = ((int64_t)b * a.nodes + (in_range ? node : 0)) * a.q_heads +
                          kvh * G + (col - node * G);
     const uint32_t* mask = a.masks + b * a.mask_b + (int64_t)(in_range ? node : 0) * a.words;
-
-    // B operand of S^T: this lane's units of its column's query row (unit
-    // 2 j + half of every pair j), zero past the head width.
-    Unit qv[NQ];
-    {
-      const T* qp = (const T*)a.q + qrow * a.key_dim;
-      // channels past the width: the last ones again, their bits cleared
-      const int on = live ? -1 : 0;
-      if (a.vec_q) {
-#pragma unroll
-        for (int j = 0; j < NQ; ++j) {
-          const int d = EPU * (2 * j + half);
-          const u32x4 x = *(const u32x4*)(qp + min(d, a.key_dim - EPU));
-          qv[j] = __builtin_bit_cast(Unit, x & (uint32_t)(on & ((d - a.key_dim) >> 31)));
-        }
-      } else {
-        typedef typename std::conditional<F32, int32_t, int16_t>::type Bits;
-#pragma unroll
-        for (int j = 0; j < NQ; ++j) {
-#pragma unroll
-          for (int e = 0; e < EPU; ++e) {
-            const int d = EPU * (2 * j + half) + e;
-            const Bits x = __builtin_bit_cast(Bits, qp[min(d, a.key_dim - 1)]);
-            qv[j][e] = __builtin_bit_cast(T, (Bits)(x & on & ((d - a.key_dim) >> 31)));
-          }
-        }
-      }
-    }
 
     f32x16 o[MB];  // O^T[channel 32 mb + 8 (r / 4) + 4 half + r % 4][column]
     float m, l;    // the column's reference score and this lane's share of the sum of P
@@ -406,13 +398,46 @@ __global__ void __launch_bounds__(256, S::kPerCu) tree_kernel(TreeArgs a) {
     for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[mb][r] = 0.f;
-    load_tile(0, 0);
-    __builtin_amdgcn_s_waitcnt(0);
+    // the ring's first tiles, the queries while they are on their way
+#pragma unroll
+    for (int i = 0; i < S::RING - 1; ++i) load_tile(i, i);
+    // B operand of S^T: this lane's units of its column's query row (unit
+    // 2 j + half of every pair j), zero past the head width.
+    Unit qv[NQ];
+    {
+      const T* qp = (const T*)a.q + qrow * a.key_dim;
+      // channels past the width: the last ones again, their bits cleared
+      const int on = live ? -1 : 0;
+      if (a.vec_q) {
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) {
+          const int d = EPU * (2 * j + half);
+          const u32x4 x = *(const u32x4*)(qp + min(d, a.key_dim - EPU));
+          qv[j] = __builtin_bit_cast(Unit, x & (uint32_t)(on & ((d - a.key_dim) >> 31)));
+        }
+      } else {
+        typedef typename std::conditional<F32, int32_t, int16_t>::type Bits;
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) {
+#pragma unroll
+          for (int e = 0; e < EPU; ++e) {
+            const int d = EPU * (2 * j + half) + e;
+            const Bits x = __builtin_bit_cast(Bits, qp[min(d, a.key_dim - 1)]);
+            qv[j][e] = __builtin_bit_cast(T, (Bits)(x & on & ((d - a.key_dim) >> 31)));
+          }
+        }
+      }
+    }
+
+    wait_tiles<(S::RING - 2) * S::kTileLoads * DMA>();  // the first tile is in LDS
     __syncthreads();
+    int buf = 0;
 #pragma clang loop unroll(disable)
     for (int t = 0; t < nt; ++t) {
-      const int buf = t & 1;
-      if (t + 1 < nt) load_tile(t + 1, buf ^ 1);
+      // into the place of the tile before this one; past the last tile the
+      // loads fetch nothing and write zeros, so that every turn waits for
+      // the same number
+      load_tile(t + S::RING - 1, buf == 0 ? S::RING - 1 : buf - 1);
       const char* kt = smem + buf * 2 * kTileB;
       const char* vt = kt + kTileB;
 #pragma unroll
@@ -504,9 +529,12 @@ __global__ void __launch_bounds__(256, S::kPerCu) tree_kernel(TreeArgs a) {
           }
         }
       }
-      __builtin_amdgcn_s_waitcnt(0);  // the next tile is in LDS
+      wait_tiles<(S::RING - 2) * S::kTileLoads * DMA>();  // the next tile is in LDS
       __syncthreads();
+      buf = buf + 1 == S::RING ? 0 : buf + 1;
     }
+    __builtin_amdgcn_s_waitcnt(0);  // no load may land behind the loop
+    if constexpr (WK > 1) __syncthreads();  // nor any other wave's
 
     l += __shfl_xor(l, 32);
     if constexpr (WK > 1) {
@@ -540,10 +568,10 @@ __global__ void __launch_bounds__(256, S::kPerCu) tree_kernel(TreeArgs a) {
         }
       }
       __syncthreads();  // the next sequence's tiles may overwrite the parts
-      if (wk > 0) continue;
+      if (wk > 0) return;
     }
     if (nt < sh.tiles || !a.direct) {
-      if (idle) continue;
+      if (idle) return;
       const int64_t seg =
           ((int64_t)(slot + b) * a.kv_heads + kvh) * a.col_tiles * S::WQ + ct * S::WQ + wq;
       f32x4* po = (f32x4*)a.part_o + seg * (MB * 4 * 64) + lane;
@@ -554,7 +582,7 @@ __global__ void __launch_bounds__(256, S::kPerCu) tree_kernel(TreeArgs a) {
           po[(mb * 4 + q) * 64] =
               (f32x4){o[mb][4 * q], o[mb][4 * q + 1], o[mb][4 * q + 2], o[mb][4 * q + 3]};
       if (half == 0) a.part_st[seg * 32 + hl] = make_float2(m, l);
-      continue;
+      return;
     }
     // a whole sequence: the output, and whether some of it is not finite
     float zero = 0.f;  // 0 times anything else is a NaN
@@ -566,7 +594,7 @@ __global__ void __launch_bounds__(256, S::kPerCu) tree_kernel(TreeArgs a) {
     const int64_t seg =
         ((int64_t)(slot + b) * a.kv_heads + kvh) * a.col_tiles * S::WQ + ct * S::WQ + wq;
     if (half == 0) a.part_st[seg * 32 + hl] = make_float2(bad ? 1.f : 0.f, 0.f);
-    if (!in_range) continue;
+    if (!in_range) return;
     const float inv = live && l != 0.f ? 1.f / l : 0.f;
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) o[mb] = live ? o[mb] * inv : (f32x16){};
@@ -600,6 +628,18 @@ __global__ void __launch_bounds__(256, S::kPerCu) tree_kernel(TreeArgs a) {
       case ALPX_F16: store((f16_t)0.f); break;
       default: store((bf16_t)0.f); break;
     }
+    };
+    segment();
+    todo += nt;
+    if (todo >= todo_end) return;
+    // the next sequence that has rows
+    do {
+      sh.first += sh.tiles;
+      ++sh.b;
+      uniform_rows(a, sh.b, sh.P, sh.end);
+      sh.tiles = (sh.end + BK - 1) / BK;
+    } while (sh.tiles == 0);
+    __syncthreads();  // every wave is done with the tiles in LDS
   }
 }
 
@@ -609,8 +649,8 @@ __global__ void __launch_bounds__(256, S::kPerCu) tree_kernel(TreeArgs a) {
 // rows that it sees, and an infinity among their values comes out as itself
 // however small its weight.  Thread (column, g) takes rows g, g + 8, ...
 template <typename T>
-__device__ __noinline__ void rows_apart(const TreeArgs& a, int b, int kvh, int col, int d0, int P,
-                                        int end, float (&o)[32], float& m, float& l) {
+__device__ __forceinline__ void rows_apart(const TreeArgs& a, int b, int kvh, int col, int d0,
+                                           int P, int end, float (&o)[32], float& m, float& l) {
   const int G = a.group, node = col / G, g = threadIdx.x >> 5;
   m = -INFINITY;
   l = 0.f;
@@ -665,9 +705,8 @@ __global__ void __launch_bounds__(256) tree_join(TreeArgs a) {
   const int kvh = blockIdx.x / MB / groups % a.kv_heads;
   const int b = blockIdx.x / MB / groups / a.kv_heads;
   int all;
-  const int per = tiles_per_slot<BK>(a, all);
-  const Share sh = find_share<BK>(a, per, 0, b);
-  const int s0 = sh.first / per, s1 = (sh.first + max(sh.tiles, 1) - 1) / per;
+  const Share sh = find_share<BK>(a, 0, b, all);
+  const int s0 = sh.first / sh.per, s1 = (sh.first + max(sh.tiles, 1) - 1) / sh.per;
   const bool whole = a.direct && sh.tiles > 0 && s0 == s1;  // written by its slot
   if (whole && a.part_st[((((int64_t)(s0 + b) * a.kv_heads + kvh) * groups + cg) * 32)].x == 0.f)
     return;
@@ -732,6 +771,7 @@ __global__ void __launch_bounds__(256) tree_join(TreeArgs a) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) bad |= node < count && !(finite(r[i]) && finite(l));
   if (__syncthreads_or(bad)) {
+    __syncthreads();  // the segments' sums in LDS are read
     float x[32];
     rows_apart<T>(a, b, kvh, 32 * cg + (threadIdx.x & 31), 32 * mb, sh.P, sh.end, x, m, l);
 #pragma unroll
@@ -771,32 +811,34 @@ struct Kernel {
   int per_cu;   // blocks on a CU at a time
 };
 
-template <typename T, int DP, int WK, int BK, bool DMA>
+template <typename T, int DP, int WK, int BK, int RING, bool DMA>
 Kernel make() {
-  typedef Shape<T, DP, WK, BK> S;
+  typedef Shape<T, DP, WK, BK, RING> S;
   return {(const void*)tree_kernel<T, S, DMA>, (const void*)tree_join<T, DP, BK>,
           S::kCols, BK, DP, S::kPerCu};
 }
 
-// Waves side by side in columns or in keys: few columns leave whole waves
-// without work unless they share the keys.
+// Few columns are bound by the rows' way from memory: waves share the keys
+// where that leaves fewer of them without a column, and the ring holds as
+// many tiles as LDS does, most of them on their way.  Many columns are bound
+// by the products: all waves side by side, and room for a second block,
+// whose products run while this one forms its probabilities.
 template <typename T>
 Kernel pick(int width, int cols, bool dma) {
   constexpr bool F32 = sizeof(T) == 4;
+  constexpr int B = F32 ? 32 : 64;
   if (width <= 64) {
-    if (!dma) return make<T, 64, 2, 64, false>();
-    return cols <= 64 ? make<T, 64, 2, 64, true>() : make<T, 64, 1, F32 ? 32 : 64, true>();
+    if (!dma) return make<T, 64, 2, 64, 2, false>();
+    if constexpr (F32)
+      if (cols <= 32) return make<T, 64, 4, 128, 2, true>();
+    return cols <= 64 ? make<T, 64, 2, 64, 4, true>() : make<T, 64, 1, B, 2, true>();
   }
   if (width <= 128) {
-    if (!dma) return make<T, 128, 2, 64, false>();
-    return cols <= 64 ? make<T, 128, 2, 64, true>() : make<T, 128, 1, F32 ? 32 : 64, true>();
+    if (!dma) return make<T, 128, 2, 64, 2, false>();
+    return cols <= 64 ? make<T, 128, 2, 64, F32 ? 2 : 4, true>() : make<T, 128, 1, B, 2, true>();
   }
-  if constexpr (F32) {
-    return dma ? make<T, 256, 1, 32, true>() : make<T, 256, 1, 32, false>();
-  } else {
-    if (!dma) return make<T, 256, 1, 32, false>();
-    return cols <= 64 ? make<T, 256, 2, 64, true>() : make<T, 256, 1, 32, true>();
-  }
+  if (!dma) return make<T, 256, 1, 32, 2, false>();
+  return make<T, 256, 1, 32, F32 ? 2 : 4, true>();
 }
 
 constexpr int kCus = 256;
