@@ -935,11 +935,14 @@ def _enqueue(fn, device, *args):
     """One C-ABI call (arguments without the stream) on torch's current stream
     of ``device``, which need not be the current device."""
     torch = _torch()
-    if device.index == torch.cuda.current_device():
-        _lib.check(fn(*args, _lib.current_stream(device.index)))
-        return
-    with torch.cuda.device(device):
-        _lib.check(fn(*args, _lib.current_stream(device.index)))
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, _lib.current_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _lib.current_stream(index))
+    if rc:
+        _lib.check(rc)
 
 
 def _address(tensor):
@@ -993,7 +996,7 @@ def tree_masks(parents, *, lengths=None, counts=None):
     words = (nodes + 63) // 64
     device = parents.device
     masks = torch.empty((batch, nodes, words), dtype=torch.int64, device=device)
-    depths = torch.empty((batch, nodes), dtype=torch.int32, device=device)
+    depths = parents.new_empty((batch, nodes))
     lanes = None
     if lengths is not None:
         lanes = torch.empty((batch, nodes, 4), dtype=torch.int64, device=device)
@@ -1025,14 +1028,11 @@ def tree_commit(key_cache, value_cache, paths, *, prefix_lens, accepted, block_t
 def paged_resize(block_table, lengths, free_pages, free_count, targets, *, page_size, tokens):
     """Takes every sequence from ``lengths[b]`` to ``targets[b]`` rows (in
     place); returns ``(starts, slots, positions, sequences, granted)``."""
-    torch = _torch()
     batch, max_pages = block_table.shape
     device = block_table.device
     # one buffer: three rows of `tokens`, then starts and grants
-    buf = torch.empty(3 * tokens + 2 * batch + 1, dtype=torch.int32, device=device)
-    slots, positions, sequences = (buf[i * tokens:(i + 1) * tokens] for i in range(3))
-    starts = buf[3 * tokens:3 * tokens + batch + 1]
-    granted = buf[3 * tokens + batch + 1:]
+    slots, positions, sequences, starts, granted = lengths.new_empty(
+        3 * tokens + 2 * batch + 1).split_with_sizes((tokens, tokens, tokens, batch + 1, batch))
     _enqueue(_lib.lib().alpx_paged_resize, device, block_table.data_ptr(), lengths.data_ptr(),
              free_pages.data_ptr(), free_count.data_ptr(), targets.data_ptr(), batch, max_pages,
              page_size, free_pages.shape[0], tokens, starts.data_ptr(), slots.data_ptr(),

@@ -19,6 +19,10 @@ __device__ __forceinline__ int load_const(const int32_t* p) {
 
 // ------------------------------------------------------------------ resize
 
+// Up to this many rows one launch does it all: the block's own loop over the
+// rows costs less than a second launch.
+constexpr int kOneLaunchRows = 4096;
+
 struct ResizeArgs {
   int32_t* table;    // [B, max_pages]
   int32_t* lengths;  // [B]
@@ -34,27 +38,31 @@ struct ResizeArgs {
   bool expand;       // this launch writes the rows' slots too
 };
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 1024;  // largest block
 
-// Inclusive sums over the block of one value per thread; `total`: of all.
-// `part` holds 16 sums and is free again when the call returns.
-__device__ __forceinline__ int64_t block_scan(int64_t x, int64_t* part, int64_t& total) {
+// Inclusive sums over a block of NT threads, of one value per thread, and
+// the sum of all.  A wave's sums meet the others' in `part` (two of them in
+// turn, so that one barrier a call is enough).
+template <int NT>
+__device__ __forceinline__ int64_t block_scan(int64_t x, int64_t (*part)[kThreads / 64], int& turn,
+                                              int64_t& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
     const int64_t y = __shfl_up(x, off);
     if (lane >= off) x += y;
   }
-  if (lane == 63) part[wave] = x;
+  int64_t* p = part[turn];
+  turn ^= 1;
+  if (lane == 63) p[wave] = x;
   __syncthreads();
   int64_t before = 0, all = 0;
 #pragma unroll
-  for (int w = 0; w < kThreads / 64; ++w) {
-    const int64_t s = part[w];
+  for (int w = 0; w < NT / 64; ++w) {
+    const int64_t s = p[w];
     if (w < wave) before += s;
     all += s;
   }
-  __syncthreads();
   total = all;
   return x + before;
 }
@@ -115,40 +123,56 @@ __device__ __forceinline__ void write_row(const ResizeArgs& a, const int32_t* st
 // to it is at most what the stack holds (and its new rows end within
 // `tokens`): a refused one makes later ones that need pages be refused too.
 // Pages move in flat order over the block, whatever each sequence's share.
-// The sums are 64-bit: they run over refused requests, which need not fit.
-__global__ void __launch_bounds__(kThreads) resize_kernel(ResizeArgs a) {
-  __shared__ int64_t part[kThreads / 64];
-  __shared__ int32_t first[kThreads + 1], table_at[kThreads];
+//
+// A tile is NT sequences; more of them go tile by tile.  Sums of pages fit 32
+// bits per tile (max_pages <= 2^20) and share a 64-bit sum; sums of rows run
+// over refused requests, which need not fit, in 64 bits.  Bound by latency:
+// a handful of dependent round trips to memory and block-wide sums.
+template <int NT>
+__global__ void __launch_bounds__(NT) resize_kernel(ResizeArgs a) {
+  __shared__ int64_t part[2][kThreads / 64];
+  __shared__ int32_t first[NT], table_at[NT];
+  __shared__ int32_t starts[NT + 1];
   const int tid = threadIdx.x;
-  const int tiles = (a.batch + kThreads - 1) / kThreads;
+  const int tiles = (a.batch + NT - 1) / NT;
   const int64_t count = max(*a.count, 0);
-  int64_t total, R = 0;
+  int turn = 0;
+  int64_t total;
 
-  // released pages of all sequences
-  for (int t = 0; t < tiles; ++t) {
-    const Change c = change_of(a, t * kThreads + tid);
-    block_scan(max(c.old_pages - c.new_pages, 0), part, total);
-    R += total;
+  // released pages (low half) and needed ones (high half) of the tile
+  const Change c0 = change_of(a, tid);
+  auto pages_of = [](const Change& c) {
+    const int64_t need = max(c.new_pages - c.old_pages, 0);
+    return need << 32 | (uint32_t)max(c.old_pages - c.new_pages, 0);
+  };
+  const int64_t incl0 = block_scan<NT>(pages_of(c0), part, turn, total);
+  const int64_t total0 = total;
+  int64_t R = (uint32_t)total0;
+  for (int t = 1; t < tiles; ++t) {
+    block_scan<NT>(pages_of(change_of(a, t * NT + tid)), part, turn, total);
+    R += (uint32_t)total;
   }
   // the released pages onto the stack
   if (R > 0) {
     int64_t base = 0;
     for (int t = 0; t < tiles; ++t) {
-      const int b = t * kThreads + tid;
-      const Change c = change_of(a, b);
-      const int out = max(c.old_pages - c.new_pages, 0);
-      const int64_t incl = block_scan(out, part, total);
-      first[tid] = (int)(incl - out);
+      const Change c = t == 0 ? c0 : change_of(a, t * NT + tid);
+      const int out = (uint32_t)pages_of(c);
+      int64_t incl = incl0;
+      total = total0;
+      if (t > 0) incl = block_scan<NT>(pages_of(c), part, turn, total);
+      first[tid] = (int)(uint32_t)incl - out;
       table_at[tid] = c.new_pages;
       __syncthreads();
-      for (int i = tid; i < (int)total; i += kThreads) {
-        const int s = find_last(first, kThreads, i);
-        const int64_t at = (int64_t)(t * kThreads + s) * a.max_pages + table_at[s] + (i - first[s]);
+      const int here = (int)(uint32_t)total;
+      for (int i = tid; i < here; i += NT) {
+        const int s = find_last(first, NT, i);
+        const int64_t at = (int64_t)(t * NT + s) * a.max_pages + table_at[s] + (i - first[s]);
         const int64_t place = count + R - 1 - (base + i);
         if (place >= 0 && place < a.num_pages) a.free[place] = a.table[at];
         a.table[at] = -1;
       }
-      base += total;
+      base += here;
       __syncthreads();
     }
   }
@@ -156,33 +180,38 @@ __global__ void __launch_bounds__(kThreads) resize_kernel(ResizeArgs a) {
   const int64_t have = count + R;
   int64_t pages = 0, rows = 0, taken = 0, packed = 0;
   for (int t = 0; t < tiles; ++t) {
-    const int b = t * kThreads + tid;
-    const Change c = change_of(a, b);
+    const int b = t * NT + tid;
+    const Change c = t == 0 ? c0 : change_of(a, b);
     const int need = max(c.new_pages - c.old_pages, 0);
     const int64_t more = max((int64_t)c.target - c.length, (int64_t)0);
-    const int64_t pages_to = pages + block_scan(need, part, total);
-    pages += total;
-    const int64_t rows_to = rows + block_scan(more, part, total);
+    int64_t incl = incl0;
+    total = total0;
+    if (t > 0) incl = block_scan<NT>(pages_of(c), part, turn, total);
+    const int64_t pages_to = pages + (incl >> 32);
+    pages += total >> 32;
+    const int64_t rows_to = rows + block_scan<NT>(more, part, turn, total);
     rows += total;
     const bool ok = c.valid && (need == 0 || pages_to <= have) && (more == 0 || rows_to <= a.tokens);
     const int take = ok ? need : 0;
     const int add = ok ? (int)more : 0;
-    const int64_t take_to = block_scan(take, part, total);
-    const int64_t taken_here = total;
-    const int64_t add_to = packed + block_scan(add, part, total);
-    first[tid] = (int)(take_to - take);
+    const int64_t both = block_scan<NT>((int64_t)take << 32 | add, part, turn, total);
+    const int taken_here = (int)(total >> 32), added_here = (int)(uint32_t)total;
+    const int start = (int)packed + (int)(uint32_t)both - add;
+    first[tid] = (int)(both >> 32) - take;
     table_at[tid] = c.old_pages;
+    starts[tid] = start;
     if (b < a.batch) {
-      a.starts[b] = (int)(add_to - add);
+      a.starts[b] = start;
       a.granted[b] = ok ? 1 : 0;
-      if (ok) a.lengths[b] = c.target;
+      if (ok && c.target != c.length) a.lengths[b] = c.target;
     }
-    packed += total;
+    packed += added_here;
+    if (tid == 0) starts[min(a.batch, NT)] = (int)packed;
     __syncthreads();
-    for (int i = tid; i < (int)taken_here; i += kThreads) {
-      const int s = find_last(first, kThreads, i);
+    for (int i = tid; i < taken_here; i += NT) {
+      const int s = find_last(first, NT, i);
       const int64_t place = have - 1 - (taken + i);
-      a.table[(int64_t)(t * kThreads + s) * a.max_pages + table_at[s] + (i - first[s])] =
+      a.table[(int64_t)(t * NT + s) * a.max_pages + table_at[s] + (i - first[s])] =
           place >= 0 && place < a.num_pages ? a.free[place] : -1;
     }
     taken += taken_here;
@@ -193,8 +222,10 @@ __global__ void __launch_bounds__(kThreads) resize_kernel(ResizeArgs a) {
     *a.count = (int)(have - taken);
   }
   if (!a.expand) return;
-  __syncthreads();  // starts, lengths and table of every thread
-  for (int t = tid; t < a.tokens; t += kThreads) write_row(a, a.starts, t, (int)packed);
+  // (the barrier above: lengths and table of every thread are written)
+  if (tiles > 1) __syncthreads();  // and the last of the starts
+  const int32_t* start = tiles > 1 ? a.starts : starts;
+  for (int t = tid; t < a.tokens; t += NT) write_row(a, start, t, (int)packed);
 }
 
 // The new rows' slots, one thread each, in a launch of its own.
@@ -213,10 +244,6 @@ __global__ void __launch_bounds__(256) slots_kernel(ResizeArgs a) {
   else
     write_row(a, a.starts, t, a.starts[a.batch]);
 }
-
-// Up to this many rows one launch does it all: the block's own loop over the
-// rows costs less than a second launch.
-constexpr int kOneLaunchRows = 4096;
 
 // ------------------------------------------------------------------- masks
 
@@ -408,13 +435,18 @@ extern "C" int alpx_paged_resize(int32_t* block_table, int32_t* lengths, int32_t
   if (!power_of_two(page_size)) return fail(ALPX_EINVAL, "page_size must be a power of two");
   if ((int64_t)num_pages * page_size > 0x7fffffff || (int64_t)max_pages * page_size > 0x7fffffff)
     return fail(ALPX_EUNSUPPORTED, "%s: 2^31 rows or more", what);
+  if (max_pages > 1 << 20) return fail(ALPX_EUNSUPPORTED, "%s: more than 2^20 pages a sequence", what);
   ResizeArgs a = {block_table, lengths,   free_pages, free_count, targets,
                   starts,      slots,     positions,  sequences,  granted,
                   batch,       max_pages, __builtin_ctz((unsigned)page_size), num_pages, tokens,
                   tokens <= kOneLaunchRows};
   hipStream_t s = (hipStream_t)stream;
   TimedRegion timed(ALPX_T_AUX, s);
-  hipLaunchKernelGGL(resize_kernel, dim3(1), dim3(kThreads), 0, s, a);
+  // a block as large as the work that it finds
+  if (batch <= 256 && tokens <= 1024)
+    hipLaunchKernelGGL(resize_kernel<256>, dim3(1), dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL(resize_kernel<kThreads>, dim3(1), dim3(kThreads), 0, s, a);
   if (!a.expand)
     hipLaunchKernelGGL(slots_kernel, dim3((unsigned)((tokens + 255) / 256)), dim3(256), 0, s, a);
   return check_launch(what);

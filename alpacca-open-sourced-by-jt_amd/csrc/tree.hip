@@ -159,44 +159,74 @@ __device__ __forceinline__ f32x16 mfma32x32x2(float a, float b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
 }
 
-// Shape of a kernel: T, DP (the head width rounded up to 64, 128 or 256), WK
-// waves that share a column tile's keys (4 / WK waves side by side in
-// columns), BK rows per K and V tile, a ring of RING tiles in LDS.
-template <typename T, int DP_, int WK_, int BK_, int RING_>
+// Shape of a kernel: T, DP (the head width rounded up to 64, 128 or 256), WC
+// columns per wave (32, or 16 on the 16 x 16 MFMA), WQ waves side by side in
+// columns, WK waves that share a column's keys, BK rows per K and V tile, a
+// ring of RING tiles in LDS.
+template <typename T_, int DP_, int WC_, int WQ_, int WK_, int BK_, int RING_>
 struct Shape {
-  static constexpr int DP = DP_, WK = WK_, BK = BK_, RING = RING_;
-  static constexpr int WQ = 4 / WK;
-  static constexpr int kCols = 32 * WQ;
-  static constexpr int KR = BK / (32 * WK);      // 32-key groups per wave and tile
+  typedef T_ T;
+  static constexpr int DP = DP_, WC = WC_, WQ = WQ_, WK = WK_, BK = BK_, RING = RING_;
+  static constexpr int NW = WQ * WK;             // waves
+  static constexpr int kCols = WC * WQ;
+  static constexpr int LPC = 64 / WC;            // lanes per column
+  static constexpr int KG = BK / WK < 32 ? BK / WK : 32;  // keys of a wave at a time
+  static constexpr int KR = BK / (KG * WK);      // such groups per tile
+  static constexpr int NS = KG / LPC;            // scores per lane
   static constexpr int EPU = 16 / (int)sizeof(T);  // elements per 16-byte unit
   static constexpr int U = DP / EPU;             // units per row
+  static constexpr int NQ = U / LPC;             // units of the query row per lane
   static constexpr int kRowB = DP * (int)sizeof(T);
   static constexpr int kTileB = BK * kRowB;
-  static constexpr int kIW = kTileB / 4096;      // direct loads per wave and tile
-  static constexpr int kTileLoads = 2 * kIW;     // direct loads per wave for a tile's K and V
-  static constexpr int MB = DP / 32;             // 32-channel blocks of O^T
+  static constexpr int kIW = kTileB / (1024 * NW);  // direct loads per wave and tile
+  static constexpr int kTileLoads = 2 * kIW;     // the same for K and V
+  static constexpr int NF = DP / (4 * LPC);      // 4-channel pieces of O^T per lane
   // O and the sums of the waves that share keys are joined in LDS.
-  static constexpr int kMergeB = (WK - 1) * WQ * (MB * 16 + 2) * 256;
+  static constexpr int kPart = (4 * NF + 2) * 64;  // floats per wave
+  static constexpr int kMergeB = (WK - 1) * WQ * kPart * 4;
   static constexpr int kLds = 2 * RING * kTileB > kMergeB ? 2 * RING * kTileB : kMergeB;
-  // Blocks per CU (160 KiB of LDS, a little of it the compiler's).
-  static constexpr int kPerCu = kLds > 80 * 1024 ? 1 : kLds > 40 * 1024 ? 2 : 4;
-  static_assert(BK % (32 * WK) == 0 && kIW >= 1, "tiles split evenly over the waves");
+  // Blocks per CU: 160 KiB of LDS, and registers for 16 or 8 waves.
+  static constexpr int kLdsBlocks = 160 * 1024 / kLds, kWaveBlocks = (DP == 64 ? 16 : 8) / NW;
+  static constexpr int kPerCu = kLdsBlocks < kWaveBlocks ? kLdsBlocks : kWaveBlocks;
+  static_assert(WC == 32 || WC == 16, "MFMA shapes");
+  static_assert(BK % (KG * WK) == 0 && kIW >= 1 && kCols % 32 == 0, "tiles split evenly");
+  static_assert(KG == 32 || (WC == 16 && KG == 16 && sizeof(T) == 4), "16-bit products take 32 keys");
   // The rows a wave loads lie in one 32-row group of the tile, so a page of
   // 32 rows or more is looked up once per wave and tile.
-  static_assert(BK / 4 <= 32 && 32 % (BK / 4) == 0, "a wave's rows share a page");
+  static_assert(BK / NW <= 32 && 32 % (BK / NW) == 0, "a wave's rows share a page");
 };
 
-// Swizzles (16-byte unit u of row r is stored at u ^ swz).  K is read 32
-// rows at a time, one unit each; 16-bit V by transposing reads of 8 rows,
-// four units each; float V in whole 128-byte pieces of a row, any order.
+// Swizzles (16-byte unit u of row r is stored at u ^ swz), which spread what
+// the lanes of a read take over the banks.  K: one unit each of 16 or 32
+// rows.  16-bit V: transposing reads of two or four units each of 16 or 8
+// rows.  Float V: 64 or 128 bytes each of rows four apart.
 template <typename S>
 __device__ __forceinline__ int k_swz(int r) {
   return S::kRowB >= 256 ? (r & 15) : (r & 7);
 }
-template <typename T, typename S>
+template <typename S>
 __device__ __forceinline__ int v_swz(int r) {
-  if (sizeof(T) == 4) return 0;
+  if (sizeof(typename S::T) == 4) return 4 * ((r >> 2) & 3);
   return S::kRowB >= 256 ? (((r & 7) << 1) | ((r >> 3) & 1)) : (r & 7);
+}
+
+// One unit step of S^T: keys of `ka` against the column's `q`.
+template <int WC, typename Unit, typename Acc>
+__device__ __forceinline__ Acc score_step(Unit ka, Unit q, Acc s) {
+  if constexpr (sizeof(ka[0]) == 4) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (WC == 32)
+        s = mfma32x32x2(ka[e], q[e], s);
+      else
+        s = mfma16x16x4(ka[e], q[e], s);
+    }
+    return s;
+  } else if constexpr (WC == 32) {
+    return mfma32x32x16(ka, q, s);
+  } else {
+    return mfma16x16x32(ka, q, s);
+  }
 }
 
 // Which of the 32 keys from `key0` a column sees, one bit each: mask words
@@ -274,19 +304,28 @@ __device__ __forceinline__ void write4(const TreeArgs& a, int64_t row, int d0, f
 
 // One block: slot `s`, kv head and column tile; it walks its run of tiles,
 // sequence by sequence.
-template <typename T, typename S, bool DMA>
-__global__ void __launch_bounds__(256, S::kPerCu) tree_kernel(TreeArgs a) {
-  constexpr int DP = S::DP, WK = S::WK, BK = S::BK;
+//
+// Lane (cl, sub) of a wave owns column cl and, of every 4 LPC keys or
+// channels, the four from 4 sub on: the order in which an MFMA leaves its
+// result.  Both products take their inner index in that order too, so the
+// probabilities are an operand where they lie.
+template <typename S, bool DMA>
+__global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(TreeArgs a) {
+  typedef typename S::T T;
   constexpr bool F32 = sizeof(T) == 4;
-  constexpr int MB = S::MB, KR = S::KR, EPU = S::EPU, U = S::U, kRowB = S::kRowB;
-  constexpr int kTileB = S::kTileB;
+  constexpr int BK = S::BK, WC = S::WC, LPC = S::LPC, KG = S::KG, EPU = S::EPU, U = S::U;
+  constexpr int NF = S::NF, NS = S::NS, NQ = S::NQ, kRowB = S::kRowB, kTileB = S::kTileB;
+  constexpr int DB = WC;             // channels of one MFMA of O^T
+  constexpr int NB = S::DP / DB;     // such blocks
+  constexpr int KB = WC == 32 ? 1 : KG / 16;  // MFMA blocks of a key group
   typedef T Unit __attribute__((ext_vector_type(EPU)));
-  constexpr int NQ = DP / (2 * EPU);  // units of a query row per lane (half of them)
+  typedef typename std::conditional<WC == 32, f32x16, f32x4>::type Acc;
+  constexpr int NA = WC == 32 ? 16 : 4;
   __shared__ __attribute__((aligned(1024))) char smem[S::kLds];  // K 0, V 0, K 1, V 1, ..
 
   const int tid = threadIdx.x, thread_lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wq = wave % S::WQ, wk = wave / S::WQ;
+  const int wk = wave % S::WK, wq = wave / S::WK;  // a column's waves on different SIMDs
   const int G = a.group;
 
   // The column tiles of one (slot, kv head) run next to each other on one
@@ -302,16 +341,16 @@ __global__ void __launch_bounds__(256, S::kPerCu) tree_kernel(TreeArgs a) {
   int todo = slot * sh.per;
   const int todo_end = min(all, todo + sh.per);
 
-  // Tile loads: wave w fills rows [w BK / 4, (w + 1) BK / 4) of a tile, all
+  // Tile loads: wave w fills rows [w BK / NW, (w + 1) BK / NW) of a tile, all
   // in its 32-row group `grp`.
-  constexpr int kRows = BK / 4;
+  constexpr int kRows = BK / S::NW;
   const int grp = wave * kRows / 32 * 32;
   uint32_t kofs[S::kIW], vofs[S::kIW];
 #pragma unroll
   for (int i = 0; i < S::kIW; ++i) {
     const int sl = (wave * S::kIW + i) * 64 + thread_lane;
     const int r = sl / U;
-    const int uk = (sl % U) ^ k_swz<S>(r), uv = (sl % U) ^ v_swz<T, S>(r);
+    const int uk = (sl % U) ^ k_swz<S>(r), uv = (sl % U) ^ v_swz<S>(r);
     // units past the head width: an offset past every row, which reads zero
     kofs[i] = uk * EPU < a.key_dim
                   ? (uint32_t)(((int64_t)(r - grp) * a.ks_pos + EPU * uk) * (int64_t)sizeof(T))
@@ -327,307 +366,301 @@ __global__ void __launch_bounds__(256, S::kPerCu) tree_kernel(TreeArgs a) {
     // the next sequence (those values took the registers of the loop)
     int lane = thread_lane;
     pin(lane);
-    const int hl = lane & 31, half = lane >> 5;
-    const int col = ct * S::kCols + 32 * wq + hl;
+    const int cl = lane % WC, sub = lane / WC;
+    const int col = ct * S::kCols + WC * wq + cl;
     const int node = col / G;
     const bool in_range = node < a.nodes;
     const int b = sh.b, P = sh.P;
     const int t0 = todo - sh.first, nt = min(todo_end, sh.first + sh.tiles) - todo;
     auto segment = [&]() __attribute__((always_inline)) {
-    // rows [start, stop) of sequence b, in tiles of BK
-    const int start = t0 * BK, stop = min(sh.end, start + nt * BK);
-    const int count = sh.end - P;
-    const bool live = node < count;
-    // a wave without a live column only loads and meets the barriers
-    const bool idle = ct * S::kCols + 32 * wq >= count * G;
-    if (ct * S::kCols >= count * G && (nt < sh.tiles || !a.direct)) return;
-    const int64_t qrow = ((int64_t)b * a.nodes + (in_range ? node : 0)) * a.q_heads +
-                         kvh * G + (col - node * G);
-    const uint32_t* mask = a.masks + b * a.mask_b + (int64_t)(in_range ? node : 0) * a.words;
+      // rows [start, stop) of sequence b, in tiles of BK
+      const int start = t0 * BK, stop = min(sh.end, start + nt * BK);
+      const int count = sh.end - P;
+      const bool live = node < count;
+      // a wave without a live column only loads and meets the barriers
+      const bool idle = ct * S::kCols + WC * wq >= count * G;
+      if (ct * S::kCols >= count * G && (nt < sh.tiles || !a.direct)) return;
+      const int64_t qrow = ((int64_t)b * a.nodes + (in_range ? node : 0)) * a.q_heads + kvh * G +
+                           (col - node * G);
+      const uint32_t* mask = a.masks + b * a.mask_b + (int64_t)(in_range ? node : 0) * a.words;
 
-    f32x16 o[MB];  // O^T[channel 32 mb + 8 (r / 4) + 4 half + r % 4][column]
-    float m, l;    // the column's reference score and this lane's share of the sum of P
-
-    auto group_base = [&](int row, const T*& kb, const T*& vb) __attribute__((always_inline)) {
-      if (a.pages != nullptr) {
-        int pg = load_const(a.pages + (int64_t)b * a.max_pages + (row >> a.page_shift));
-        pg = min(max(pg, 0), a.num_pages - 1);
-        const int64_t in = row & ((1 << a.page_shift) - 1);
-        kb = (const T*)a.k + pg * a.ks_b + in * a.ks_pos + (int64_t)kvh * a.ks_h;
-        vb = (const T*)a.v + pg * a.vs_b + in * a.vs_pos + (int64_t)kvh * a.vs_h;
-      } else {
-        kb = (const T*)a.k + (int64_t)b * a.ks_b + (int64_t)row * a.ks_pos + (int64_t)kvh * a.ks_h;
-        vb = (const T*)a.v + (int64_t)b * a.vs_b + (int64_t)row * a.vs_pos + (int64_t)kvh * a.vs_h;
-      }
-    };
-    auto load_tile = [&](int t, int buf) __attribute__((always_inline)) {
-      const int row0 = start + t * BK + grp;
-      const int rows = __builtin_amdgcn_readfirstlane(min(max(stop - row0, 0), 32));
-      const T *kb = (const T*)a.k, *vb = (const T*)a.v;
-      if (rows > 0) group_base(row0, kb, vb);
-      if constexpr (DMA) {
-        const i32x4 rk = rsrc_words((uint64_t)(uintptr_t)kb,
-                                    (uint32_t)(rows * a.ks_pos * (int64_t)sizeof(T)));
-        const i32x4 rv = rsrc_words((uint64_t)(uintptr_t)vb,
-                                    (uint32_t)(rows * a.vs_pos * (int64_t)sizeof(T)));
-        const uint32_t dst = lbase + buf * 2 * kTileB + wave * S::kIW * 1024;
-#pragma unroll
-        for (int i = 0; i < S::kIW; ++i) lds_dma16(rk, dst + i * 1024, kofs[i]);
-#pragma unroll
-        for (int i = 0; i < S::kIW; ++i) lds_dma16(rv, dst + kTileB + i * 1024, vofs[i]);
-      } else {
-        // any head width, stride or alignment: element by element
-        T* dst = (T*)(smem + buf * 2 * kTileB);
-        for (int i = lane; i < kRows * DP; i += 64) {
-          const int r = wave * kRows + i / DP, d = i % DP;
-          const bool in = r - grp < rows;
-          const T kx =
-              in && d < a.key_dim ? kb[(int64_t)(r - grp) * a.ks_pos + d] : from_f32<T>(0.f);
-          const T vx =
-              in && d < a.value_dim ? vb[(int64_t)(r - grp) * a.vs_pos + d] : from_f32<T>(0.f);
-          const int u = d / EPU, e = d % EPU;
-          dst[r * DP + (u ^ k_swz<S>(r)) * EPU + e] = kx;
-          dst[kTileB / (int)sizeof(T) + r * DP + (u ^ v_swz<T, S>(r)) * EPU + e] = vx;
+      auto group_base = [&](int row, const T*& kb, const T*& vb) __attribute__((always_inline)) {
+        if (a.pages != nullptr) {
+          int pg = load_const(a.pages + (int64_t)b * a.max_pages + (row >> a.page_shift));
+          pg = min(max(pg, 0), a.num_pages - 1);
+          const int64_t in = row & ((1 << a.page_shift) - 1);
+          kb = (const T*)a.k + pg * a.ks_b + in * a.ks_pos + (int64_t)kvh * a.ks_h;
+          vb = (const T*)a.v + pg * a.vs_b + in * a.vs_pos + (int64_t)kvh * a.vs_h;
+        } else {
+          kb = (const T*)a.k + (int64_t)b * a.ks_b + (int64_t)row * a.ks_pos + (int64_t)kvh * a.ks_h;
+          vb = (const T*)a.v + (int64_t)b * a.vs_b + (int64_t)row * a.vs_pos + (int64_t)kvh * a.vs_h;
         }
-      }
-    };
-
-    m = -INFINITY;
-    l = 0.f;
+      };
+      auto load_tile = [&](int t, int buf) __attribute__((always_inline)) {
+        const int row0 = start + t * BK + grp;
+        const int rows = __builtin_amdgcn_readfirstlane(min(max(stop - row0, 0), 32));
+        const T *kb = (const T*)a.k, *vb = (const T*)a.v;
+        if (rows > 0) group_base(row0, kb, vb);
+        if constexpr (DMA) {
+          const i32x4 rk = rsrc_words((uint64_t)(uintptr_t)kb,
+                                      (uint32_t)(rows * a.ks_pos * (int64_t)sizeof(T)));
+          const i32x4 rv = rsrc_words((uint64_t)(uintptr_t)vb,
+                                      (uint32_t)(rows * a.vs_pos * (int64_t)sizeof(T)));
+          const uint32_t dst = lbase + buf * 2 * kTileB + wave * S::kIW * 1024;
 #pragma unroll
-    for (int mb = 0; mb < MB; ++mb)
+          for (int i = 0; i < S::kIW; ++i) lds_dma16(rk, dst + i * 1024, kofs[i]);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) o[mb][r] = 0.f;
-    // the ring's first tiles, the queries while they are on their way
-#pragma unroll
-    for (int i = 0; i < S::RING - 1; ++i) load_tile(i, i);
-    // B operand of S^T: this lane's units of its column's query row (unit
-    // 2 j + half of every pair j), zero past the head width.
-    Unit qv[NQ];
-    {
-      const T* qp = (const T*)a.q + qrow * a.key_dim;
-      // channels past the width: the last ones again, their bits cleared
-      const int on = live ? -1 : 0;
-      if (a.vec_q) {
-#pragma unroll
-        for (int j = 0; j < NQ; ++j) {
-          const int d = EPU * (2 * j + half);
-          const u32x4 x = *(const u32x4*)(qp + min(d, a.key_dim - EPU));
-          qv[j] = __builtin_bit_cast(Unit, x & (uint32_t)(on & ((d - a.key_dim) >> 31)));
-        }
-      } else {
-        typedef typename std::conditional<F32, int32_t, int16_t>::type Bits;
-#pragma unroll
-        for (int j = 0; j < NQ; ++j) {
-#pragma unroll
-          for (int e = 0; e < EPU; ++e) {
-            const int d = EPU * (2 * j + half) + e;
-            const Bits x = __builtin_bit_cast(Bits, qp[min(d, a.key_dim - 1)]);
-            qv[j][e] = __builtin_bit_cast(T, (Bits)(x & on & ((d - a.key_dim) >> 31)));
+          for (int i = 0; i < S::kIW; ++i) lds_dma16(rv, dst + kTileB + i * 1024, vofs[i]);
+        } else {
+          // any head width, stride or alignment: element by element
+          T* dst = (T*)(smem + buf * 2 * kTileB);
+          for (int i = lane; i < kRows * S::DP; i += 64) {
+            const int r = wave * kRows + i / S::DP, d = i % S::DP;
+            const bool in = r - grp < rows;
+            const T kx =
+                in && d < a.key_dim ? kb[(int64_t)(r - grp) * a.ks_pos + d] : from_f32<T>(0.f);
+            const T vx =
+                in && d < a.value_dim ? vb[(int64_t)(r - grp) * a.vs_pos + d] : from_f32<T>(0.f);
+            const int u = d / EPU, e = d % EPU;
+            dst[r * S::DP + (u ^ k_swz<S>(r)) * EPU + e] = kx;
+            dst[kTileB / (int)sizeof(T) + r * S::DP + (u ^ v_swz<S>(r)) * EPU + e] = vx;
           }
         }
-      }
-    }
+      };
 
-    wait_tiles<(S::RING - 2) * S::kTileLoads * DMA>();  // the first tile is in LDS
-    __syncthreads();
-    int buf = 0;
-#pragma clang loop unroll(disable)
-    for (int t = 0; t < nt; ++t) {
-      // into the place of the tile before this one; past the last tile the
-      // loads fetch nothing and write zeros, so that every turn waits for
-      // the same number
-      load_tile(t + S::RING - 1, buf == 0 ? S::RING - 1 : buf - 1);
-      const char* kt = smem + buf * 2 * kTileB;
-      const char* vt = kt + kTileB;
+      // the ring's first tiles, the queries while they are on their way
 #pragma unroll
-      for (int kr = 0; kr < KR; ++kr) {
-        if (idle) break;
-        const int g0 = 32 * (wk * KR + kr);       // this wave's keys of the tile
-        const int key0 = start + t * BK + g0;
-        f32x16 s;
+      for (int i = 0; i < S::RING - 1; ++i) load_tile(i, i);
+      // B operand of S^T: this lane's units of its column's query row (unit
+      // LPC j + sub), zero past the head width.
+      Unit qv[NQ];
+      {
+        const T* qp = (const T*)a.q + qrow * a.key_dim;
+        // channels past the width: the last ones again, their bits cleared
+        const int on = live ? -1 : 0;
+        if (a.vec_q) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = 0.f;
-        const int row = g0 + hl;
-#pragma unroll
-        for (int j = 0; j < NQ; ++j) {
-          const Unit ka = *(const Unit*)(kt + row * kRowB + ((2 * j + half) ^ k_swz<S>(row)) * 16);
-          if constexpr (F32) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s = mfma32x32x2(ka[e], qv[j][e], s);
-          } else {
-            s = mfma32x32x16(ka, qv[j], s);
-          }
-        }
-        if (key0 + 32 > P) {  // not all of these keys are prefix rows
-          const uint32_t bits = seen_bits(mask, a.words, P, stop, key0, live);
-          const uint32_t mine = bits >> (4 * half);
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int keep = (int)(mine << (31 - (8 * (r >> 2) + (r & 3)))) >> 31;  // all bits or none
-            s[r] = __int_as_float((__float_as_int(s[r]) & keep) | (0xff800000 & ~keep));
-          }
-        }
-        float mx = s[0];
-#pragma unroll
-        for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
-        mx *= a.scale_log2;
-        // the reference moves only when a score exceeds it by more than
-        // kRescale, so P <= 2^kRescale and the sums keep their range
-        if (__ballot(mx > m + kRescale) != 0) {
-          mx = fmaxf(mx, __shfl_xor(mx, 32));
-          if (mx > m + kRescale) {
-            const float c = fast_exp2(m - mx);  // 0 while m is -inf
-            l *= c;
-#pragma unroll
-            for (int mb = 0; mb < MB; ++mb) o[mb] *= c;
-            m = mx;
-          }
-        }
-        const float off = m == -INFINITY ? 0.f : m;
-        float ps = 0.f;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          s[r] = fast_exp2(fmaf(s[r], a.scale_log2, -off));
-          ps += s[r];
-        }
-        l += ps;
-        // O^T += V^T P^T.  Any order of the keys will do as long as both
-        // operands have the same: slot e of lane half h is key 16 ks +
-        // 8 (e / 4) + 4 h + e % 4, which is where P already lies.
-        if constexpr (F32) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int vr = g0 + 8 * (r >> 2) + 4 * half + (r & 3);
-#pragma unroll
-            for (int mb = 0; mb < MB; ++mb) {
-              const float x = *(const float*)(vt + vr * kRowB + 128 * mb + 4 * hl);
-              o[mb] = mfma32x32x2(x, s[r], o[mb]);
-            }
+          for (int j = 0; j < NQ; ++j) {
+            const int d = EPU * (LPC * j + sub);
+            const u32x4 x = *(const u32x4*)(qp + min(d, a.key_dim - EPU));
+            qv[j] = __builtin_bit_cast(Unit, x & (uint32_t)(on & ((d - a.key_dim) >> 31)));
           }
         } else {
-          typedef typename Vec8<T>::type V8;
-          typedef typename Vec4<T>::type V4;
+          typedef typename std::conditional<F32, int32_t, int16_t>::type Bits;
 #pragma unroll
-          for (int ks = 0; ks < 2; ++ks) {
-            V8 p;
+          for (int j = 0; j < NQ; ++j) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) p[e] = from_f32<T>(s[8 * ks + e]);
-            // transposing reads: lane 4 k + q of 16 supplies row k, channels
-            // 4 q .. 4 q + 3, and receives channel lane % 16 of the four rows
-            const int vr = g0 + 16 * ks + 4 * half + ((lane & 15) >> 2);
-#pragma unroll
-            for (int mb = 0; mb < MB; ++mb) {
-              const int u = 4 * mb + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-              const T* p0 = (const T*)(vt + vr * kRowB + (u ^ v_swz<T, S>(vr)) * 16 + 8 * (lane & 1));
-              const T* p1 = (const T*)(vt + (vr + 8) * kRowB + (u ^ v_swz<T, S>(vr + 8)) * 16 +
-                                       8 * (lane & 1));
-              const V4 x0 = lds_read_tr4(p0), x1 = lds_read_tr4(p1);
-              const V8 x = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
-              o[mb] = mfma32x32x16(x, p, o[mb]);
+            for (int e = 0; e < EPU; ++e) {
+              const int d = EPU * (LPC * j + sub) + e;
+              const Bits x = __builtin_bit_cast(Bits, qp[min(d, a.key_dim - 1)]);
+              qv[j][e] = __builtin_bit_cast(T, (Bits)(x & on & ((d - a.key_dim) >> 31)));
             }
           }
         }
       }
-      wait_tiles<(S::RING - 2) * S::kTileLoads * DMA>();  // the next tile is in LDS
-      __syncthreads();
-      buf = buf + 1 == S::RING ? 0 : buf + 1;
-    }
-    __builtin_amdgcn_s_waitcnt(0);  // no load may land behind the loop
-    if constexpr (WK > 1) __syncthreads();  // nor any other wave's
 
-    l += __shfl_xor(l, 32);
-    if constexpr (WK > 1) {
-      // the waves of a column tile's keys, joined in LDS by the first of them
-      constexpr int kPart = (MB * 16 + 2) * 64;  // floats per wave
-      float* part = (float*)smem;
-      if (wk > 0) {
-        float* p = part + ((wk - 1) * S::WQ + wq) * kPart + lane;
+      Acc o[NB];              // O^T[channel DB n + 4 LPC (r / 4) + 4 sub + r % 4][column]
+      float m = -INFINITY;    // the column's reference score
+      float l = 0.f;          // this lane's share of the sum of P
 #pragma unroll
-        for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) p[(mb * 16 + r) * 64] = o[mb][r];
-        p[MB * 16 * 64] = m;
-        p[(MB * 16 + 1) * 64] = l;
-      }
+      for (int n = 0; n < NB; ++n) o[n] = (Acc)(0.f);
+      wait_tiles<(S::RING - 2) * S::kTileLoads * DMA>();  // the first tile is in LDS
       __syncthreads();
-      if (wk == 0) {
+      int buf = 0;
+#pragma clang loop unroll(disable)
+      for (int t = 0; t < nt; ++t) {
+        // into the place of the tile before this one; past the last tile the
+        // loads fetch nothing and write zeros, so that every turn waits for
+        // the same number
+        load_tile(t + S::RING - 1, buf == 0 ? S::RING - 1 : buf - 1);
+        const char* kt = smem + buf * 2 * kTileB;
+        const char* vt = kt + kTileB;
 #pragma unroll
-        for (int w = 0; w < WK - 1; ++w) {
-          const float* p = part + (w * S::WQ + wq) * kPart + lane;
-          const float m1 = p[MB * 16 * 64], l1 = p[(MB * 16 + 1) * 64];
+        for (int kr = 0; kr < S::KR; ++kr) {
+          if (idle) break;
+          const int g0 = KG * (wk * S::KR + kr);  // this wave's keys of the tile
+          const int key0 = start + t * BK + g0;
+          Acc sa[KB];
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb) sa[kb] = (Acc)(0.f);
+#pragma unroll
+          for (int j = 0; j < NQ; ++j)
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+              const int row = g0 + WC * kb + cl;
+              const Unit ka =
+                  *(const Unit*)(kt + row * kRowB + ((LPC * j + sub) ^ k_swz<S>(row)) * 16);
+              sa[kb] = score_step<WC>(ka, qv[j], sa[kb]);
+            }
+          float s[NS];  // score r is of key g0 + 4 LPC (r / 4) + 4 sub + r % 4
+#pragma unroll
+          for (int r = 0; r < NS; ++r) s[r] = sa[r / NA][r % NA];
+          if (key0 + KG > P) {  // not all of these keys are prefix rows
+            const uint32_t mine = seen_bits(mask, a.words, P, stop, key0, live) >> (4 * sub);
+#pragma unroll
+            for (int r = 0; r < NS; ++r) {
+              // all bits or none
+              const int keep = (int)(mine << (31 - (4 * LPC * (r >> 2) + (r & 3)))) >> 31;
+              s[r] = __int_as_float((__float_as_int(s[r]) & keep) | (0xff800000 & ~keep));
+            }
+          }
+          float mx = s[0];
+#pragma unroll
+          for (int r = 1; r < NS; ++r) mx = fmaxf(mx, s[r]);
+          mx *= a.scale_log2;
+          // the reference moves only when a score exceeds it by more than
+          // kRescale, so P <= 2^kRescale and the sums keep their range
+          if (__ballot(mx > m + kRescale) != 0) {
+            if constexpr (LPC == 4) mx = fmaxf(mx, __shfl_xor(mx, 16));
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            if (mx > m + kRescale) {
+              const float c = fast_exp2(m - mx);  // 0 while m is -inf
+              l *= c;
+#pragma unroll
+              for (int n = 0; n < NB; ++n) o[n] *= c;
+              m = mx;
+            }
+          }
+          const float off = m == -INFINITY ? 0.f : m;
+          float ps = 0.f;
+#pragma unroll
+          for (int r = 0; r < NS; ++r) {
+            s[r] = fast_exp2(fmaf(s[r], a.scale_log2, -off));
+            ps += s[r];
+          }
+          l += ps;
+          if constexpr (F32) {
+#pragma unroll
+            for (int r = 0; r < NS; ++r) {
+              const int vr = g0 + 4 * LPC * (r >> 2) + 4 * sub + (r & 3);
+#pragma unroll
+              for (int n = 0; n < NB; ++n) {
+                const int u = (DB * n + cl) / 4;
+                const float x = *(const float*)(vt + vr * kRowB + (u ^ v_swz<S>(vr)) * 16 + 4 * (cl & 3));
+                if constexpr (WC == 32)
+                  o[n] = mfma32x32x2(x, s[r], o[n]);
+                else
+                  o[n] = mfma16x16x4(x, s[r], o[n]);
+              }
+            }
+          } else {
+            typedef typename Vec8<T>::type V8;
+            typedef typename Vec4<T>::type V4;
+#pragma unroll
+            for (int ks = 0; ks < NS / 8; ++ks) {
+              V8 p;  // rounded to the cache's type for its product
+#pragma unroll
+              for (int e = 0; e < 8; ++e) p[e] = from_f32<T>(s[8 * ks + e]);
+              // transposing reads: lane 4 k + q of 16 supplies row k, channels
+              // 4 q .. 4 q + 3, and receives channel lane % 16 of the four rows
+              const int vr = g0 + 8 * LPC * ks + 4 * sub + ((lane & 15) >> 2);
+#pragma unroll
+              for (int n = 0; n < NB; ++n) {
+                const int u = DB / 8 * n + (WC == 32 ? 2 * ((lane >> 4) & 1) : 0) + ((lane & 3) >> 1);
+                const T* p0 = (const T*)(vt + vr * kRowB + (u ^ v_swz<S>(vr)) * 16 + 8 * (lane & 1));
+                const int vr1 = vr + 4 * LPC;
+                const T* p1 =
+                    (const T*)(vt + vr1 * kRowB + (u ^ v_swz<S>(vr1)) * 16 + 8 * (lane & 1));
+                const V4 x0 = lds_read_tr4(p0), x1 = lds_read_tr4(p1);
+                const V8 x = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
+                if constexpr (WC == 32)
+                  o[n] = mfma32x32x16(x, p, o[n]);
+                else
+                  o[n] = mfma16x16x32(x, p, o[n]);
+              }
+            }
+          }
+        }
+        wait_tiles<(S::RING - 2) * S::kTileLoads * DMA>();  // the next tile is in LDS
+        __syncthreads();
+        buf = buf + 1 == S::RING ? 0 : buf + 1;
+      }
+      __builtin_amdgcn_s_waitcnt(0);  // no load may land behind the loop
+      if constexpr (S::WK > 1) __syncthreads();  // nor any other wave's
+
+      if constexpr (LPC == 4) l += __shfl_xor(l, 16);
+      l += __shfl_xor(l, 32);
+      if constexpr (S::WK > 1) {
+        // the waves of a column tile's keys, joined in LDS by the first of them
+        float* part = (float*)smem;
+        if (wk > 0) {
+          float* p = part + ((wk - 1) * S::WQ + wq) * S::kPart + lane;
+#pragma unroll
+          for (int i = 0; i < 4 * NF; ++i) p[i * 64] = o[i / NA][i % NA];
+          p[4 * NF * 64] = m;
+          p[(4 * NF + 1) * 64] = l;
+        }
+        __syncthreads();
+        if (wk > 0) return;
+#pragma unroll
+        for (int w = 0; w < S::WK - 1; ++w) {
+          const float* p = part + (w * S::WQ + wq) * S::kPart + lane;
+          const float m1 = p[4 * NF * 64], l1 = p[(4 * NF + 1) * 64];
           const float M = fmaxf(m, m1);
           const float c0 = weight(m, M), c1 = weight(m1, M);
           l = l * c0 + l1 * c1;
 #pragma unroll
-          for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-              o[mb][r] = o[mb][r] * c0 + p[(mb * 16 + r) * 64] * c1;
+          for (int i = 0; i < 4 * NF; ++i)
+            o[i / NA][i % NA] = o[i / NA][i % NA] * c0 + p[i * 64] * c1;
           m = M;
         }
       }
-      __syncthreads();  // the next sequence's tiles may overwrite the parts
-      if (wk > 0) return;
-    }
-    if (nt < sh.tiles || !a.direct) {
-      if (idle) return;
-      const int64_t seg =
-          ((int64_t)(slot + b) * a.kv_heads + kvh) * a.col_tiles * S::WQ + ct * S::WQ + wq;
-      f32x4* po = (f32x4*)a.part_o + seg * (MB * 4 * 64) + lane;
+      // piece f of this lane: channels 4 LPC f + 4 sub + 0 .. 3
+      auto piece = [&](int f) __attribute__((always_inline)) {
+        const int i = 4 * f;
+        return (f32x4){o[i / NA][i % NA], o[i / NA][i % NA + 1], o[i / NA][i % NA + 2],
+                       o[i / NA][i % NA + 3]};
+      };
+      const int64_t seg = (((int64_t)(slot + b) * a.kv_heads + kvh) * a.col_tiles + ct) *
+                              (S::kCols / 32) + WC * wq / 32;
+      const int c32 = (WC * wq) % 32 + cl;  // column in its group of 32
+      if (nt < sh.tiles || !a.direct) {
+        if (idle) return;
+        // [piece of 8 channels][4 of them][column]
+        f32x4* po = (f32x4*)a.part_o + seg * (S::DP * 8) + c32;
 #pragma unroll
-      for (int mb = 0; mb < MB; ++mb)
+        for (int f = 0; f < NF; ++f) po[(LPC * f + sub) * 32] = piece(f);
+        if (sub == 0) a.part_st[seg * 32 + c32] = make_float2(m, l);
+        return;
+      }
+      // a whole sequence: the output, and whether some of it is not finite
+      float zero = 0.f;  // 0 times anything else is a NaN
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          po[(mb * 4 + q) * 64] =
-              (f32x4){o[mb][4 * q], o[mb][4 * q + 1], o[mb][4 * q + 2], o[mb][4 * q + 3]};
-      if (half == 0) a.part_st[seg * 32 + hl] = make_float2(m, l);
-      return;
-    }
-    // a whole sequence: the output, and whether some of it is not finite
-    float zero = 0.f;  // 0 times anything else is a NaN
+      for (int i = 0; i < 4 * NF; ++i) zero = fmaf(o[i / NA][i % NA], 0.f, zero);
+      const bool bad = __ballot(live && zero != 0.f) != 0;
+      if (sub == 0) a.part_st[seg * 32 + c32] = make_float2(bad ? 1.f : 0.f, 0.f);
+      if (!in_range) return;
+      const float inv = live && l != 0.f ? 1.f / l : 0.f;
 #pragma unroll
-    for (int mb = 0; mb < MB; ++mb)
+      for (int n = 0; n < NB; ++n) o[n] = live ? o[n] * inv : (Acc)(0.f);
+      const int64_t out0 = qrow * S::DP + 4 * sub;
+      if (a.gate != nullptr) {
+        typedef typename Vec4<T>::type V4;
+        const T* gp = (const T*)a.gate + out0;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) zero = fmaf(o[mb][r], 0.f, zero);
-    const bool bad = __ballot(live && zero != 0.f) != 0;
-    const int64_t seg =
-        ((int64_t)(slot + b) * a.kv_heads + kvh) * a.col_tiles * S::WQ + ct * S::WQ + wq;
-    if (half == 0) a.part_st[seg * 32 + hl] = make_float2(bad ? 1.f : 0.f, 0.f);
-    if (!in_range) return;
-    const float inv = live && l != 0.f ? 1.f / l : 0.f;
+        for (int f = 0; f < NF; ++f) {
+          const V4 g = *(const V4*)(gp + 4 * LPC * f);
 #pragma unroll
-    for (int mb = 0; mb < MB; ++mb) o[mb] = live ? o[mb] * inv : (f32x16){};
-    const int64_t out0 = qrow * DP + 4 * half;
-    if (a.gate != nullptr) {
-      typedef typename Vec4<T>::type V4;
-      const T* gp = (const T*)a.gate + out0;
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const V4 g = *(const V4*)(gp + 32 * mb + 8 * q);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[mb][4 * q + i] *= fast_sigmoid(to_f32(g[i]));
+          for (int i = 0; i < 4; ++i)
+            o[4 * f / NA][4 * f % NA + i] *= F32 ? stable_sigmoid(to_f32(g[i])) : fast_sigmoid(to_f32(g[i]));
         }
-    }
-    auto store = [&](auto zero_of_type) __attribute__((always_inline)) {
-      typedef decltype(zero_of_type) TO;
-      typedef TO TO4 __attribute__((ext_vector_type(4)));
-      TO* op = (TO*)a.out + out0;
+      }
+      auto store = [&](auto zero_of_type) __attribute__((always_inline)) {
+        typedef decltype(zero_of_type) TO;
+        typedef TO TO4 __attribute__((ext_vector_type(4)));
+        TO* op = (TO*)a.out + out0;
 #pragma unroll
-      for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          *(TO4*)(op + 32 * mb + 8 * q) =
-              (TO4){from_f32<TO>(o[mb][4 * q]), from_f32<TO>(o[mb][4 * q + 1]),
-                    from_f32<TO>(o[mb][4 * q + 2]), from_f32<TO>(o[mb][4 * q + 3])};
-    };
-    switch (a.out_dtype) {
-      case ALPX_F32: store(0.f); break;
-      case ALPX_F16: store((f16_t)0.f); break;
-      default: store((bf16_t)0.f); break;
-    }
+        for (int f = 0; f < NF; ++f) {
+          const f32x4 x = piece(f);
+          *(TO4*)(op + 4 * LPC * f) = (TO4){from_f32<TO>(x[0]), from_f32<TO>(x[1]),
+                                            from_f32<TO>(x[2]), from_f32<TO>(x[3])};
+        }
+      };
+      switch (a.out_dtype) {
+        case ALPX_F32: store(0.f); break;
+        case ALPX_F16: store((f16_t)0.f); break;
+        default: store((bf16_t)0.f); break;
+      }
     };
     segment();
     todo += nt;
@@ -708,8 +741,10 @@ __global__ void __launch_bounds__(256) tree_join(TreeArgs a) {
   const Share sh = find_share<BK>(a, 0, b, all);
   const int s0 = sh.first / sh.per, s1 = (sh.first + max(sh.tiles, 1) - 1) / sh.per;
   const bool whole = a.direct && sh.tiles > 0 && s0 == s1;  // written by its slot
-  if (whole && a.part_st[((((int64_t)(s0 + b) * a.kv_heads + kvh) * groups + cg) * 32)].x == 0.f)
-    return;
+  if (whole) {  // the two waves of 16 columns have a mark each
+    const float2* mark = a.part_st + (((int64_t)(s0 + b) * a.kv_heads + kvh) * groups + cg) * 32;
+    if (mark[0].x == 0.f && mark[16].x == 0.f) return;
+  }
   const int G = a.group, col = 32 * cg + hl, node = col / G;
   const int count = sh.end - sh.P;
   float m = -INFINITY, l = 0.f, o[16];
@@ -805,40 +840,58 @@ __global__ void __launch_bounds__(256) tree_join(TreeArgs a) {
 struct Kernel {
   const void* fn;
   const void* join;
+  int threads;
   int cols;     // columns per block
   int rows;     // rows per tile
   int width;    // DP
   int per_cu;   // blocks on a CU at a time
 };
 
-template <typename T, int DP, int WK, int BK, int RING, bool DMA>
+template <typename S, bool DMA>
 Kernel make() {
-  typedef Shape<T, DP, WK, BK, RING> S;
-  return {(const void*)tree_kernel<T, S, DMA>, (const void*)tree_join<T, DP, BK>,
-          S::kCols, BK, DP, S::kPerCu};
+  return {(const void*)tree_kernel<S, DMA>, (const void*)tree_join<typename S::T, S::DP, S::BK>,
+          64 * S::NW, S::kCols, S::BK, S::DP, S::kPerCu};
 }
 
-// Few columns are bound by the rows' way from memory: waves share the keys
-// where that leaves fewer of them without a column, and the ring holds as
-// many tiles as LDS does, most of them on their way.  Many columns are bound
-// by the products: all waves side by side, and room for a second block,
-// whose products run while this one forms its probabilities.
+// Few columns are bound by the rows' way from memory: 16 columns a wave, so
+// that there are waves enough to hide each other's waits, and a ring of as
+// many tiles as LDS holds, most of them on their way.  Many columns are
+// bound by the products: 32 a wave, which halves the operand reads, and room
+// for a second block, whose products run while this one forms its
+// probabilities.
 template <typename T>
 Kernel pick(int width, int cols, bool dma) {
-  constexpr bool F32 = sizeof(T) == 4;
-  constexpr int B = F32 ? 32 : 64;
-  if (width <= 64) {
-    if (!dma) return make<T, 64, 2, 64, 2, false>();
-    if constexpr (F32)
-      if (cols <= 32) return make<T, 64, 4, 128, 2, true>();
-    return cols <= 64 ? make<T, 64, 2, 64, 4, true>() : make<T, 64, 1, B, 2, true>();
+  if constexpr (sizeof(T) == 4) {
+    if (width <= 64) {
+      if (!dma) return make<Shape<T, 64, 16, 4, 2, 64, 2>, false>();
+      return cols <= 32   ? make<Shape<T, 64, 16, 2, 4, 128, 2>, true>()
+             : cols <= 64 ? make<Shape<T, 64, 16, 4, 2, 64, 4>, true>()
+                          : make<Shape<T, 64, 32, 4, 1, 32, 2>, true>();
+    }
+    if (width <= 128) {
+      if (!dma) return make<Shape<T, 128, 16, 4, 2, 64, 2>, false>();
+      return cols <= 32   ? make<Shape<T, 128, 16, 2, 4, 64, 2>, true>()
+             : cols <= 64 ? make<Shape<T, 128, 16, 4, 2, 64, 2>, true>()
+                          : make<Shape<T, 128, 32, 4, 1, 32, 2>, true>();
+    }
+    if (!dma) return make<Shape<T, 256, 16, 4, 2, 32, 2>, false>();
+    return cols <= 64 ? make<Shape<T, 256, 16, 4, 2, 32, 2>, true>()
+                      : make<Shape<T, 256, 32, 4, 1, 32, 2>, true>();
+  } else {
+    if (width <= 64) {
+      if (!dma) return make<Shape<T, 64, 16, 4, 2, 64, 2>, false>();
+      return cols <= 64 ? make<Shape<T, 64, 16, 4, 2, 64, 4>, true>()
+                        : make<Shape<T, 64, 32, 4, 1, 64, 2>, true>();
+    }
+    if (width <= 128) {
+      if (!dma) return make<Shape<T, 128, 16, 4, 2, 64, 2>, false>();
+      return cols <= 64 ? make<Shape<T, 128, 16, 4, 2, 64, 4>, true>()
+                        : make<Shape<T, 128, 32, 4, 1, 64, 2>, true>();
+    }
+    if (!dma) return make<Shape<T, 256, 16, 8, 1, 32, 2>, false>();
+    return cols <= 128 ? make<Shape<T, 256, 16, 8, 1, 32, 4>, true>()
+                       : make<Shape<T, 256, 32, 4, 1, 32, 4>, true>();
   }
-  if (width <= 128) {
-    if (!dma) return make<T, 128, 2, 64, 2, false>();
-    return cols <= 64 ? make<T, 128, 2, 64, F32 ? 2 : 4, true>() : make<T, 128, 1, B, 2, true>();
-  }
-  if (!dma) return make<T, 256, 1, 32, 2, false>();
-  return make<T, 256, 1, 32, F32 ? 2 : 4, true>();
 }
 
 constexpr int kCus = 256;
@@ -926,7 +979,7 @@ int tree_launch(const char* what, TreeArgs a, int dtype, void* workspace, size_t
   void* args[] = {&a};
   {
     TimedRegion timed(ALPX_T_DECODE, s);
-    (void)hipLaunchKernel(p.kernel.fn, dim3((unsigned)blocks), dim3(256), args, 0, s);
+    (void)hipLaunchKernel(p.kernel.fn, dim3((unsigned)blocks), dim3(p.kernel.threads), args, 0, s);
   }
   if (p.join) {
     a.col_tiles = groups;

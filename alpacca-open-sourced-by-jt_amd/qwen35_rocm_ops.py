@@ -1199,6 +1199,9 @@ class Qwen35RocmOps:
         """An int32 device tensor of ``shape``; a host sequence (one axis) is
         checked against ``[low, high]`` and uploaded."""
         torch = self.torch
+        if (isinstance(value, torch.Tensor) and value.dtype == torch.int32 and value.shape == shape
+                and value.get_device() == self.device_index and value.is_contiguous()):
+            return value
         if not torch.is_tensor(value) or value.device.type != "cuda":
             host = [int(v) for v in value]
             if (len(host),) != tuple(shape) or any(
@@ -1374,7 +1377,7 @@ class Qwen35RocmOps:
         block_table = self._device_ints(block_table, "block table", (batch, max_pages))
         for name, value in (("lengths", lengths), ("free_pages", free_pages),
                             ("free_count", free_count)):
-            if not torch.is_tensor(value) or value.device.type != "cuda" or value.dim() != 1:
+            if not torch.is_tensor(value) or not value.is_cuda or value.dim() != 1:
                 raise TypeError(f"{name} must be a one-dimensional device tensor")
         lengths = self._device_ints(lengths, "lengths", (batch,))
         free_pages = self._device_ints(free_pages, "free_pages", _shape(free_pages))
