@@ -26,6 +26,23 @@
 namespace alpx {
 namespace {
 
+// lds_dma16 for bytes that no other block reads (the nontemporal hint).
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // m0 is reserved; the clobber is intended
+__device__ __forceinline__ void lds_dma16_once(i32x4 r, uint32_t lds, uint32_t voff) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds"
+               :
+               : "s"(lds), "v"(voff), "s"(r)
+               : "memory", "m0");
+#else
+  (void)r;
+  (void)lds;
+  (void)voff;
+#endif
+}
+#pragma clang diagnostic pop
+
 struct TreeArgs {
   const void* q;      // [B, N, Hq, D]
   const void* k;
@@ -181,6 +198,10 @@ struct Shape {
   static constexpr int kIW = kTileB / (1024 * NW);  // direct loads per wave and tile
   static constexpr int kTileLoads = 2 * kIW;     // the same for K and V
   static constexpr int NF = DP / (4 * LPC);      // 4-channel pieces of O^T per lane
+  // The narrow kernels have one column tile: nobody reads a tile twice.
+  // (The hint on V, on K and V / on V / on neither, 16 x 16 drafts on 8192
+  // rows: @@ us.)
+  static constexpr bool kOnce = WC == 16;
   // O and the sums of the waves that share keys are joined in LDS.
   static constexpr int kPart = (4 * NF + 2) * 64;  // floats per wave
   static constexpr int kMergeB = (WK - 1) * WQ * kPart * 4;
@@ -410,7 +431,12 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
 #pragma unroll
           for (int i = 0; i < S::kIW; ++i) lds_dma16(rk, dst + i * 1024, kofs[i]);
 #pragma unroll
-          for (int i = 0; i < S::kIW; ++i) lds_dma16(rv, dst + kTileB + i * 1024, vofs[i]);
+          for (int i = 0; i < S::kIW; ++i) {
+            if (S::kOnce)
+              lds_dma16_once(rv, dst + kTileB + i * 1024, vofs[i]);
+            else
+              lds_dma16(rv, dst + kTileB + i * 1024, vofs[i]);
+          }
         } else {
           // any head width, stride or alignment: element by element
           T* dst = (T*)(smem + buf * 2 * kTileB);
@@ -475,38 +501,44 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
         load_tile(t + S::RING - 1, buf == 0 ? S::RING - 1 : buf - 1);
         const char* kt = smem + buf * 2 * kTileB;
         const char* vt = kt + kTileB;
-#pragma unroll
-        for (int kr = 0; kr < S::KR; ++kr) {
-          if (idle) break;
-          const int g0 = KG * (wk * S::KR + kr);  // this wave's keys of the tile
+        if (!idle) {
+          const int g0 = KG * S::KR * wk;  // this wave's keys of the tile
           const int key0 = start + t * BK + g0;
-          Acc sa[KB];
+          // All of them through each step together, so that one group's
+          // products run beside the other's softmax.
+          Acc sa[S::KR * KB];
 #pragma unroll
-          for (int kb = 0; kb < KB; ++kb) sa[kb] = (Acc)(0.f);
+          for (int kb = 0; kb < S::KR * KB; ++kb) sa[kb] = (Acc)(0.f);
 #pragma unroll
           for (int j = 0; j < NQ; ++j)
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb) {
+            for (int kb = 0; kb < S::KR * KB; ++kb) {
               const int row = g0 + WC * kb + cl;
               const Unit ka =
                   *(const Unit*)(kt + row * kRowB + ((LPC * j + sub) ^ k_swz<S>(row)) * 16);
               sa[kb] = score_step<WC>(ka, qv[j], sa[kb]);
             }
-          float s[NS];  // score r is of key g0 + 4 LPC (r / 4) + 4 sub + r % 4
+          constexpr int NT = S::KR * NS;
+          float s[NT];  // score r is of key g0 + 4 LPC (r / 4) + 4 sub + r % 4
 #pragma unroll
-          for (int r = 0; r < NS; ++r) s[r] = sa[r / NA][r % NA];
-          if (key0 + KG > P) {  // not all of these keys are prefix rows
-            const uint32_t mine = seen_bits(mask, a.words, P, stop, key0, live) >> (4 * sub);
+          for (int r = 0; r < NT; ++r) s[r] = sa[r / NA][r % NA];
+          if (key0 + KG * S::KR > P) {  // not all of these keys are prefix rows
 #pragma unroll
-            for (int r = 0; r < NS; ++r) {
-              // all bits or none
-              const int keep = (int)(mine << (31 - (4 * LPC * (r >> 2) + (r & 3)))) >> 31;
-              s[r] = __int_as_float((__float_as_int(s[r]) & keep) | (0xff800000 & ~keep));
+            for (int kr = 0; kr < S::KR; ++kr) {
+              const uint32_t mine =
+                  seen_bits(mask, a.words, P, stop, key0 + KG * kr, live) >> (4 * sub);
+#pragma unroll
+              for (int r = 0; r < NS; ++r) {
+                // all bits or none
+                const int keep = (int)(mine << (31 - (4 * LPC * (r >> 2) + (r & 3)))) >> 31;
+                float& x = s[kr * NS + r];
+                x = __int_as_float((__float_as_int(x) & keep) | (0xff800000 & ~keep));
+              }
             }
           }
           float mx = s[0];
 #pragma unroll
-          for (int r = 1; r < NS; ++r) mx = fmaxf(mx, s[r]);
+          for (int r = 1; r < NT; ++r) mx = fmaxf(mx, s[r]);
           mx *= a.scale_log2;
           // the reference moves only when a score exceeds it by more than
           // kRescale, so P <= 2^kRescale and the sums keep their range
@@ -524,52 +556,59 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
           const float off = m == -INFINITY ? 0.f : m;
           float ps = 0.f;
 #pragma unroll
-          for (int r = 0; r < NS; ++r) {
-            s[r] = fast_exp2(fmaf(s[r], a.scale_log2, -off));
-            ps += s[r];
-          }
-          l += ps;
-          if constexpr (F32) {
+          for (int kr = 0; kr < S::KR; ++kr) {
+            float* p_ = s + kr * NS;
 #pragma unroll
             for (int r = 0; r < NS; ++r) {
-              const int vr = g0 + 4 * LPC * (r >> 2) + 4 * sub + (r & 3);
-#pragma unroll
-              for (int n = 0; n < NB; ++n) {
-                const int u = (DB * n + cl) / 4;
-                const float x = *(const float*)(vt + vr * kRowB + (u ^ v_swz<S>(vr)) * 16 + 4 * (cl & 3));
-                if constexpr (WC == 32)
-                  o[n] = mfma32x32x2(x, s[r], o[n]);
-                else
-                  o[n] = mfma16x16x4(x, s[r], o[n]);
-              }
+              p_[r] = fast_exp2(fmaf(p_[r], a.scale_log2, -off));
+              ps += p_[r];
             }
-          } else {
-            typedef typename Vec8<T>::type V8;
-            typedef typename Vec4<T>::type V4;
+            if constexpr (F32) {
 #pragma unroll
-            for (int ks = 0; ks < NS / 8; ++ks) {
-              V8 p;  // rounded to the cache's type for its product
+              for (int r = 0; r < NS; ++r) {
+                const int vr = g0 + KG * kr + 4 * LPC * (r >> 2) + 4 * sub + (r & 3);
 #pragma unroll
-              for (int e = 0; e < 8; ++e) p[e] = from_f32<T>(s[8 * ks + e]);
-              // transposing reads: lane 4 k + q of 16 supplies row k, channels
-              // 4 q .. 4 q + 3, and receives channel lane % 16 of the four rows
-              const int vr = g0 + 8 * LPC * ks + 4 * sub + ((lane & 15) >> 2);
+                for (int n = 0; n < NB; ++n) {
+                  const int u = (DB * n + cl) / 4;
+                  const float x =
+                      *(const float*)(vt + vr * kRowB + (u ^ v_swz<S>(vr)) * 16 + 4 * (cl & 3));
+                  if constexpr (WC == 32)
+                    o[n] = mfma32x32x2(x, p_[r], o[n]);
+                  else
+                    o[n] = mfma16x16x4(x, p_[r], o[n]);
+                }
+              }
+            } else {
+              typedef typename Vec8<T>::type V8;
+              typedef typename Vec4<T>::type V4;
 #pragma unroll
-              for (int n = 0; n < NB; ++n) {
-                const int u = DB / 8 * n + (WC == 32 ? 2 * ((lane >> 4) & 1) : 0) + ((lane & 3) >> 1);
-                const T* p0 = (const T*)(vt + vr * kRowB + (u ^ v_swz<S>(vr)) * 16 + 8 * (lane & 1));
-                const int vr1 = vr + 4 * LPC;
-                const T* p1 =
-                    (const T*)(vt + vr1 * kRowB + (u ^ v_swz<S>(vr1)) * 16 + 8 * (lane & 1));
-                const V4 x0 = lds_read_tr4(p0), x1 = lds_read_tr4(p1);
-                const V8 x = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
-                if constexpr (WC == 32)
-                  o[n] = mfma32x32x16(x, p, o[n]);
-                else
-                  o[n] = mfma16x16x32(x, p, o[n]);
+              for (int ks = 0; ks < NS / 8; ++ks) {
+                V8 p;  // rounded to the cache's type for its product
+#pragma unroll
+                for (int e = 0; e < 8; ++e) p[e] = from_f32<T>(p_[8 * ks + e]);
+                // transposing reads: lane 4 k + q of 16 supplies row k, channels
+                // 4 q .. 4 q + 3, and receives channel lane % 16 of the four rows
+                const int vr = g0 + KG * kr + 8 * LPC * ks + 4 * sub + ((lane & 15) >> 2);
+#pragma unroll
+                for (int n = 0; n < NB; ++n) {
+                  const int u =
+                      DB / 8 * n + (WC == 32 ? 2 * ((lane >> 4) & 1) : 0) + ((lane & 3) >> 1);
+                  const T* p0 =
+                      (const T*)(vt + vr * kRowB + (u ^ v_swz<S>(vr)) * 16 + 8 * (lane & 1));
+                  const int vr1 = vr + 4 * LPC;
+                  const T* p1 =
+                      (const T*)(vt + vr1 * kRowB + (u ^ v_swz<S>(vr1)) * 16 + 8 * (lane & 1));
+                  const V4 x0 = lds_read_tr4(p0), x1 = lds_read_tr4(p1);
+                  const V8 x = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
+                  if constexpr (WC == 32)
+                    o[n] = mfma32x32x16(x, p, o[n]);
+                  else
+                    o[n] = mfma16x16x32(x, p, o[n]);
+                }
               }
             }
           }
+          l += ps;
         }
         wait_tiles<(S::RING - 2) * S::kTileLoads * DMA>();  // the next tile is in LDS
         __syncthreads();
