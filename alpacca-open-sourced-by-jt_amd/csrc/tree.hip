@@ -198,6 +198,9 @@ struct Shape {
   static constexpr int kIW = kTileB / (1024 * NW);  // direct loads per wave and tile
   static constexpr int kTileLoads = 2 * kIW;     // the same for K and V
   static constexpr int NF = DP / (4 * LPC);      // 4-channel pieces of O^T per lane
+  // The wide 16-bit kernels run the products of two tiles beside the softmax
+  // of a third (see the loop).
+  static constexpr bool kPipe = WC == 32 && sizeof(T) == 2 && RING == 2;
   // The narrow kernels have one column tile: nobody reads a tile twice.
   // (The hint on V, on K and V / on V / on neither, 16 x 16 drafts on 8192
   // rows: @@ us.)
@@ -206,8 +209,9 @@ struct Shape {
   static constexpr int kPart = (4 * NF + 2) * 64;  // floats per wave
   static constexpr int kMergeB = (WK - 1) * WQ * kPart * 4;
   static constexpr int kLds = 2 * RING * kTileB > kMergeB ? 2 * RING * kTileB : kMergeB;
-  // Blocks per CU: 160 KiB of LDS, and registers for 16 or 8 waves.
-  static constexpr int kLdsBlocks = 160 * 1024 / kLds, kWaveBlocks = (DP == 64 ? 16 : 8) / NW;
+  // Blocks per CU: 160 KiB of LDS, and registers for 16, 8 or 4 waves.
+  static constexpr int kLdsBlocks = 160 * 1024 / kLds;
+  static constexpr int kWaveBlocks = (DP == 64 && !kPipe ? 16 : DP == 256 && WC == 32 ? 4 : 8) / NW;
   static constexpr int kPerCu = kLdsBlocks < kWaveBlocks ? kLdsBlocks : kWaveBlocks;
   static_assert(WC == 32 || WC == 16, "MFMA shapes");
   static_assert(BK % (KG * WK) == 0 && kIW >= 1 && kCols % 32 == 0, "tiles split evenly");
@@ -228,6 +232,7 @@ __device__ __forceinline__ int k_swz(int r) {
 template <typename S>
 __device__ __forceinline__ int v_swz(int r) {
   if (sizeof(typename S::T) == 4) return 4 * ((r >> 2) & 3);
+  if (S::WC == 32) return S::kRowB >= 256 ? 4 * (r & 3) : 4 * ((r >> 1) & 1);
   return S::kRowB >= 256 ? (((r & 7) << 1) | ((r >> 3) & 1)) : (r & 7);
 }
 
@@ -417,29 +422,36 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
           vb = (const T*)a.v + (int64_t)b * a.vs_b + (int64_t)row * a.vs_pos + (int64_t)kvh * a.vs_h;
         }
       };
-      auto load_tile = [&](int t, int buf) __attribute__((always_inline)) {
+      // K, V or both of tile t to LDS bytes kdst and vdst; rows past the end
+      // (all of them past the last tile) are zeros
+      auto load = [&](int t, bool k, bool v, uint32_t kdst, uint32_t vdst)
+                      __attribute__((always_inline)) {
         const int row0 = start + t * BK + grp;
         const int rows = __builtin_amdgcn_readfirstlane(min(max(stop - row0, 0), 32));
         const T *kb = (const T*)a.k, *vb = (const T*)a.v;
         if (rows > 0) group_base(row0, kb, vb);
         if constexpr (DMA) {
-          const i32x4 rk = rsrc_words((uint64_t)(uintptr_t)kb,
-                                      (uint32_t)(rows * a.ks_pos * (int64_t)sizeof(T)));
-          const i32x4 rv = rsrc_words((uint64_t)(uintptr_t)vb,
-                                      (uint32_t)(rows * a.vs_pos * (int64_t)sizeof(T)));
-          const uint32_t dst = lbase + buf * 2 * kTileB + wave * S::kIW * 1024;
+          if (k) {
+            const i32x4 rk = rsrc_words((uint64_t)(uintptr_t)kb,
+                                        (uint32_t)(rows * a.ks_pos * (int64_t)sizeof(T)));
+            const uint32_t dst = lbase + kdst + wave * S::kIW * 1024;
 #pragma unroll
-          for (int i = 0; i < S::kIW; ++i) lds_dma16(rk, dst + i * 1024, kofs[i]);
+            for (int i = 0; i < S::kIW; ++i) lds_dma16(rk, dst + i * 1024, kofs[i]);
+          }
+          if (v) {
+            const i32x4 rv = rsrc_words((uint64_t)(uintptr_t)vb,
+                                        (uint32_t)(rows * a.vs_pos * (int64_t)sizeof(T)));
+            const uint32_t dst = lbase + vdst + wave * S::kIW * 1024;
 #pragma unroll
-          for (int i = 0; i < S::kIW; ++i) {
-            if (S::kOnce)
-              lds_dma16_once(rv, dst + kTileB + i * 1024, vofs[i]);
-            else
-              lds_dma16(rv, dst + kTileB + i * 1024, vofs[i]);
+            for (int i = 0; i < S::kIW; ++i) {
+              if (S::kOnce)
+                lds_dma16_once(rv, dst + i * 1024, vofs[i]);
+              else
+                lds_dma16(rv, dst + i * 1024, vofs[i]);
+            }
           }
         } else {
           // any head width, stride or alignment: element by element
-          T* dst = (T*)(smem + buf * 2 * kTileB);
           for (int i = lane; i < kRows * S::DP; i += 64) {
             const int r = wave * kRows + i / S::DP, d = i % S::DP;
             const bool in = r - grp < rows;
@@ -448,15 +460,23 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
             const T vx =
                 in && d < a.value_dim ? vb[(int64_t)(r - grp) * a.vs_pos + d] : from_f32<T>(0.f);
             const int u = d / EPU, e = d % EPU;
-            dst[r * S::DP + (u ^ k_swz<S>(r)) * EPU + e] = kx;
-            dst[kTileB / (int)sizeof(T) + r * S::DP + (u ^ v_swz<S>(r)) * EPU + e] = vx;
+            ((T*)(smem + kdst))[r * S::DP + (u ^ k_swz<S>(r)) * EPU + e] = kx;
+            ((T*)(smem + vdst))[r * S::DP + (u ^ v_swz<S>(r)) * EPU + e] = vx;
           }
         }
       };
+      auto load_tile = [&](int t, int buf) __attribute__((always_inline)) {
+        load(t, true, true, buf * 2 * kTileB, (buf * 2 + 1) * kTileB);
+      };
 
       // the ring's first tiles, the queries while they are on their way
+      if constexpr (S::kPipe) {
+        load(0, true, false, 0, 0);
+        load(1, true, false, kTileB, 0);
+      } else {
 #pragma unroll
-      for (int i = 0; i < S::RING - 1; ++i) load_tile(i, i);
+        for (int i = 0; i < S::RING - 1; ++i) load_tile(i, i);
+      }
       // B operand of S^T: this lane's units of its column's query row (unit
       // LPC j + sub), zero past the head width.
       Unit qv[NQ];
@@ -490,129 +510,282 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
       float l = 0.f;          // this lane's share of the sum of P
 #pragma unroll
       for (int n = 0; n < NB; ++n) o[n] = (Acc)(0.f);
-      wait_tiles<(S::RING - 2) * S::kTileLoads * DMA>();  // the first tile is in LDS
-      __syncthreads();
-      int buf = 0;
-#pragma clang loop unroll(disable)
-      for (int t = 0; t < nt; ++t) {
-        // into the place of the tile before this one; past the last tile the
-        // loads fetch nothing and write zeros, so that every turn waits for
-        // the same number
-        load_tile(t + S::RING - 1, buf == 0 ? S::RING - 1 : buf - 1);
-        const char* kt = smem + buf * 2 * kTileB;
-        const char* vt = kt + kTileB;
-        if (!idle) {
-          const int g0 = KG * S::KR * wk;  // this wave's keys of the tile
-          const int key0 = start + t * BK + g0;
-          // All of them through each step together, so that one group's
-          // products run beside the other's softmax.
-          Acc sa[S::KR * KB];
+      if constexpr (S::kPipe) {
+        // Turn t: PV of tile t - 1, the softmax of tile t and QK of tile
+        // t + 1, so that the products run beside the exponentials of the same
+        // wave, while K of tile t + 2 and V of tile t are on their way.  K
+        // tiles at 0 and kTileB, V tiles at 2 and 3 kTileB.
+        typedef typename Vec8<T>::type V8;
+        typedef typename Vec4<T>::type V4;
+        constexpr int KR = S::KR, NV = 2 * KR * NB, NK = KR * NQ, NE = 16 * KR;
+        Acc sc[KR];
+        V8 pv[2 * KR];
+        float pend = 1.f;  // what O still has to be multiplied by
+        bool pend_any = false;
+        // byte offsets of this lane's operands: K row cl of a group, unit
+        // 2 j + sub (16 units on: 256 bytes); V row 4 sub + (lane % 16) / 4
+        // of 8, channels 32 n + 16 ((lane / 16) % 2) + 4 (lane % 4)
+        constexpr int KA = NQ < 8 ? NQ : 8, VA = NB < 4 ? NB : 4;
+        int kadr[KA], vadr[VA];
+        const int vrow = 4 * sub + ((lane & 15) >> 2);
 #pragma unroll
-          for (int kb = 0; kb < S::KR * KB; ++kb) sa[kb] = (Acc)(0.f);
+        for (int j = 0; j < KA; ++j) kadr[j] = cl * kRowB + ((2 * j + sub) ^ k_swz<S>(cl)) * 16;
 #pragma unroll
-          for (int j = 0; j < NQ; ++j)
+        for (int n = 0; n < VA; ++n)
+          vadr[n] = 2 * kTileB + vrow * kRowB +
+                    ((4 * n + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ v_swz<S>(vrow)) * 16 +
+                    8 * (lane & 1);
+        auto k_operand = [&](int buf, int kr, int j) __attribute__((always_inline)) {
+          return *(const Unit*)(smem + kadr[j % KA] + buf + 32 * kr * kRowB + j / KA * 256);
+        };
+        auto v_operand = [&](int buf, int ks, int n) __attribute__((always_inline)) {
+          const char* p = smem + vadr[n % VA] + buf + 16 * ks * kRowB + n / VA * 256;
+          const V4 x0 = lds_read_tr4((const T*)p), x1 = lds_read_tr4((const T*)(p + 8 * kRowB));
+          return __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
+        };
+        // V 1 and P are zeros for the product of turn 0
 #pragma unroll
-            for (int kb = 0; kb < S::KR * KB; ++kb) {
-              const int row = g0 + WC * kb + cl;
-              const Unit ka =
-                  *(const Unit*)(kt + row * kRowB + ((LPC * j + sub) ^ k_swz<S>(row)) * 16);
-              sa[kb] = score_step<WC>(ka, qv[j], sa[kb]);
+        for (int i = 0; i < S::kIW; ++i)
+          *(u32x4*)(smem + 3 * kTileB + ((wave * S::kIW + i) * 64 + lane) * 16) = (u32x4){};
+#pragma unroll
+        for (int i = 0; i < 2 * KR; ++i) pv[i] = (V8){};
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+#pragma unroll
+        for (int kr = 0; kr < KR; ++kr) {
+          sc[kr] = (Acc)(0.f);
+#pragma unroll
+          for (int j = 0; j < NQ; ++j) sc[kr] = mfma32x32x16(k_operand(0, kr, j), qv[j], sc[kr]);
+        }
+        __syncthreads();  // K 0 is read before turn 0 refills it
+        auto turn = [&](auto parity, int t) __attribute__((always_inline)) {
+          constexpr int Q = decltype(parity)::value;  // t & 1
+          if (t + 2 < nt) load(t + 2, true, false, Q * kTileB, 0);
+          if (t < nt) load(t, false, true, 0, (2 + Q) * kTileB);
+          if (!idle) {
+            // O holds tiles up to t - 2 and is about to take P of tile t - 1,
+            // formed against the reference that moved there
+            if (__builtin_expect(pend_any, 0)) {
+#pragma unroll
+              for (int n = 0; n < NB; ++n) o[n] *= pend;
+              pend = 1.f;
+              pend_any = false;
             }
-          constexpr int NT = S::KR * NS;
-          float s[NT];  // score r is of key g0 + 4 LPC (r / 4) + 4 sub + r % 4
+            const int key0 = start + t * BK;
+            // not all of these keys are prefix rows, or turn nt, whose scores
+            // are of no tile
+            if (key0 + BK > min(P, stop)) {
 #pragma unroll
-          for (int r = 0; r < NT; ++r) s[r] = sa[r / NA][r % NA];
-          if (key0 + KG * S::KR > P) {  // not all of these keys are prefix rows
+              for (int kr = 0; kr < KR; ++kr) {
+                const uint32_t mine =
+                    seen_bits(mask, a.words, P, stop, key0 + 32 * kr, live) >> (4 * sub);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                  const int keep = (int)(mine << (31 - (8 * (r >> 2) + (r & 3)))) >> 31;
+                  sc[kr][r] = __int_as_float((__float_as_int(sc[kr][r]) & keep) |
+                                             (0xff800000 & ~keep));
+                }
+              }
+            }
+            float mx = sc[0][0];
+#pragma unroll
+            for (int r = 1; r < NE; ++r) mx = fmaxf(mx, sc[r / 16][r % 16]);
+            mx *= a.scale_log2;
+            if (__builtin_expect(__ballot(mx > m + kRescale) != 0, 0)) {
+              mx = fmaxf(mx, __shfl_xor(mx, 32));
+              if (mx > m + kRescale) {
+                pend = fast_exp2(m - mx);
+                l *= pend;
+                m = mx;
+              }
+              pend_any = true;
+            }
+            const float off = m == -INFINITY ? 0.f : m;
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(1);
+            float ps = 0.f;
+            V8 pn[2 * KR];
+            // Step i: product i of NV + NK and its share of the exponentials,
+            // all of them before their registers take tile t + 1's scores.
+            // Operands are read AHEAD steps before their product; the order
+            // is kept as written (left to itself the scheduler reads each
+            // operand right before its product and waits for it).
+            constexpr int N = NV + NK, LAST = NV + (KR - 1) * NQ, AHEAD = 4;
+            u32x4 opd[N];
+            auto read = [&](auto i_) __attribute__((always_inline)) {
+              constexpr int i = decltype(i_)::value;
+              if constexpr (i < NV)
+                opd[i] = __builtin_bit_cast(u32x4, v_operand((Q ^ 1) * kTileB, i / NB, i % NB));
+              else
+                opd[i] = __builtin_bit_cast(
+                    u32x4, k_operand((Q ^ 1) * kTileB, (i - NV) / NQ, (i - NV) % NQ));
+            };
+            static_for<0, AHEAD>(read);
+            static_for<0, N>([&](auto i_) __attribute__((always_inline)) {
+              constexpr int i = decltype(i_)::value;
+              if constexpr (i + AHEAD < N) read(Par<i + AHEAD>());
+              const V8 x = __builtin_bit_cast(V8, opd[i]);
+              if constexpr (i < NV) {
+                o[i % NB] = mfma32x32x16(x, pv[i / NB], o[i % NB]);
+              } else {
+                constexpr int kr = (i - NV) / NQ, j = (i - NV) % NQ;
+                if constexpr (j == 0)
+                  sc[kr] = mfma32x32x16(x, qv[j], (Acc)(0.f));
+                else
+                  sc[kr] = mfma32x32x16(x, qv[j], sc[kr]);
+              }
+              constexpr int e0 = i < LAST ? i * NE / LAST : NE;
+              constexpr int e1 = i + 1 < LAST ? (i + 1) * NE / LAST : NE;
+              static_for<e0, e1>([&](auto e_) __attribute__((always_inline)) {
+                constexpr int e = decltype(e_)::value;
+                const float p = fast_exp2(fmaf(sc[e / 16][e % 16], a.scale_log2, -off));
+                ps += p;
+                pn[e / 8][e % 8] = from_f32<T>(p);
+              });
+              __builtin_amdgcn_sched_barrier(0);
+            });
+            __builtin_amdgcn_s_setprio(0);
+            __builtin_amdgcn_sched_barrier(0);
+            l += ps;
+#pragma unroll
+            for (int i = 0; i < 2 * KR; ++i) {
+              pv[i] = pn[i];
+              pin(pv[i]);
+            }
+          }
+          __builtin_amdgcn_s_waitcnt(0);
+          __syncthreads();
+        };
+#pragma clang loop unroll(disable)
+        for (int t = 0; t <= nt; t += 2) {
+          turn(Par<0>(), t);
+          if (t + 1 <= nt) turn(Par<1>(), t + 1);
+        }
+      } else {
+        wait_tiles<(S::RING - 2) * S::kTileLoads * DMA>();  // the first tile is in LDS
+        __syncthreads();
+        int buf = 0;
+#pragma clang loop unroll(disable)
+        for (int t = 0; t < nt; ++t) {
+          // into the place of the tile before this one; past the last tile the
+          // loads fetch nothing and write zeros, so that every turn waits for
+          // the same number
+          load_tile(t + S::RING - 1, buf == 0 ? S::RING - 1 : buf - 1);
+          const char* kt = smem + buf * 2 * kTileB;
+          const char* vt = kt + kTileB;
+          if (!idle) {
+            const int g0 = KG * S::KR * wk;  // this wave's keys of the tile
+            const int key0 = start + t * BK + g0;
+            // All of them through each step together, so that one group's
+            // products run beside the other's softmax.
+            Acc sa[S::KR * KB];
+#pragma unroll
+            for (int kb = 0; kb < S::KR * KB; ++kb) sa[kb] = (Acc)(0.f);
+#pragma unroll
+            for (int j = 0; j < NQ; ++j)
+#pragma unroll
+              for (int kb = 0; kb < S::KR * KB; ++kb) {
+                const int row = g0 + WC * kb + cl;
+                const Unit ka =
+                    *(const Unit*)(kt + row * kRowB + ((LPC * j + sub) ^ k_swz<S>(row)) * 16);
+                sa[kb] = score_step<WC>(ka, qv[j], sa[kb]);
+              }
+            constexpr int NT = S::KR * NS;
+            float s[NT];  // score r is of key g0 + 4 LPC (r / 4) + 4 sub + r % 4
+#pragma unroll
+            for (int r = 0; r < NT; ++r) s[r] = sa[r / NA][r % NA];
+            if (key0 + KG * S::KR > P) {  // not all of these keys are prefix rows
+#pragma unroll
+              for (int kr = 0; kr < S::KR; ++kr) {
+                const uint32_t mine =
+                    seen_bits(mask, a.words, P, stop, key0 + KG * kr, live) >> (4 * sub);
+#pragma unroll
+                for (int r = 0; r < NS; ++r) {
+                  // all bits or none
+                  const int keep = (int)(mine << (31 - (4 * LPC * (r >> 2) + (r & 3)))) >> 31;
+                  float& x = s[kr * NS + r];
+                  x = __int_as_float((__float_as_int(x) & keep) | (0xff800000 & ~keep));
+                }
+              }
+            }
+            float mx = s[0];
+#pragma unroll
+            for (int r = 1; r < NT; ++r) mx = fmaxf(mx, s[r]);
+            mx *= a.scale_log2;
+            // the reference moves only when a score exceeds it by more than
+            // kRescale, so P <= 2^kRescale and the sums keep their range
+            if (__ballot(mx > m + kRescale) != 0) {
+              if constexpr (LPC == 4) mx = fmaxf(mx, __shfl_xor(mx, 16));
+              mx = fmaxf(mx, __shfl_xor(mx, 32));
+              if (mx > m + kRescale) {
+                const float c = fast_exp2(m - mx);  // 0 while m is -inf
+                l *= c;
+#pragma unroll
+                for (int n = 0; n < NB; ++n) o[n] *= c;
+                m = mx;
+              }
+            }
+            const float off = m == -INFINITY ? 0.f : m;
+            float ps = 0.f;
 #pragma unroll
             for (int kr = 0; kr < S::KR; ++kr) {
-              const uint32_t mine =
-                  seen_bits(mask, a.words, P, stop, key0 + KG * kr, live) >> (4 * sub);
+              float* p_ = s + kr * NS;
 #pragma unroll
               for (int r = 0; r < NS; ++r) {
-                // all bits or none
-                const int keep = (int)(mine << (31 - (4 * LPC * (r >> 2) + (r & 3)))) >> 31;
-                float& x = s[kr * NS + r];
-                x = __int_as_float((__float_as_int(x) & keep) | (0xff800000 & ~keep));
+                p_[r] = fast_exp2(fmaf(p_[r], a.scale_log2, -off));
+                ps += p_[r];
               }
-            }
-          }
-          float mx = s[0];
+              if constexpr (F32) {
 #pragma unroll
-          for (int r = 1; r < NT; ++r) mx = fmaxf(mx, s[r]);
-          mx *= a.scale_log2;
-          // the reference moves only when a score exceeds it by more than
-          // kRescale, so P <= 2^kRescale and the sums keep their range
-          if (__ballot(mx > m + kRescale) != 0) {
-            if constexpr (LPC == 4) mx = fmaxf(mx, __shfl_xor(mx, 16));
-            mx = fmaxf(mx, __shfl_xor(mx, 32));
-            if (mx > m + kRescale) {
-              const float c = fast_exp2(m - mx);  // 0 while m is -inf
-              l *= c;
+                for (int r = 0; r < NS; ++r) {
+                  const int vr = g0 + KG * kr + 4 * LPC * (r >> 2) + 4 * sub + (r & 3);
 #pragma unroll
-              for (int n = 0; n < NB; ++n) o[n] *= c;
-              m = mx;
-            }
-          }
-          const float off = m == -INFINITY ? 0.f : m;
-          float ps = 0.f;
-#pragma unroll
-          for (int kr = 0; kr < S::KR; ++kr) {
-            float* p_ = s + kr * NS;
-#pragma unroll
-            for (int r = 0; r < NS; ++r) {
-              p_[r] = fast_exp2(fmaf(p_[r], a.scale_log2, -off));
-              ps += p_[r];
-            }
-            if constexpr (F32) {
-#pragma unroll
-              for (int r = 0; r < NS; ++r) {
-                const int vr = g0 + KG * kr + 4 * LPC * (r >> 2) + 4 * sub + (r & 3);
-#pragma unroll
-                for (int n = 0; n < NB; ++n) {
-                  const int u = (DB * n + cl) / 4;
-                  const float x =
-                      *(const float*)(vt + vr * kRowB + (u ^ v_swz<S>(vr)) * 16 + 4 * (cl & 3));
-                  if constexpr (WC == 32)
-                    o[n] = mfma32x32x2(x, p_[r], o[n]);
-                  else
-                    o[n] = mfma16x16x4(x, p_[r], o[n]);
+                  for (int n = 0; n < NB; ++n) {
+                    const int u = (DB * n + cl) / 4;
+                    const float x =
+                        *(const float*)(vt + vr * kRowB + (u ^ v_swz<S>(vr)) * 16 + 4 * (cl & 3));
+                    if constexpr (WC == 32)
+                      o[n] = mfma32x32x2(x, p_[r], o[n]);
+                    else
+                      o[n] = mfma16x16x4(x, p_[r], o[n]);
+                  }
                 }
-              }
-            } else {
-              typedef typename Vec8<T>::type V8;
-              typedef typename Vec4<T>::type V4;
+              } else {
+                typedef typename Vec8<T>::type V8;
+                typedef typename Vec4<T>::type V4;
 #pragma unroll
-              for (int ks = 0; ks < NS / 8; ++ks) {
-                V8 p;  // rounded to the cache's type for its product
+                for (int ks = 0; ks < NS / 8; ++ks) {
+                  V8 p;  // rounded to the cache's type for its product
 #pragma unroll
-                for (int e = 0; e < 8; ++e) p[e] = from_f32<T>(p_[8 * ks + e]);
-                // transposing reads: lane 4 k + q of 16 supplies row k, channels
-                // 4 q .. 4 q + 3, and receives channel lane % 16 of the four rows
-                const int vr = g0 + KG * kr + 8 * LPC * ks + 4 * sub + ((lane & 15) >> 2);
+                  for (int e = 0; e < 8; ++e) p[e] = from_f32<T>(p_[8 * ks + e]);
+                  // transposing reads: lane 4 k + q of 16 supplies row k, channels
+                  // 4 q .. 4 q + 3, and receives channel lane % 16 of the four rows
+                  const int vr = g0 + KG * kr + 8 * LPC * ks + 4 * sub + ((lane & 15) >> 2);
 #pragma unroll
-                for (int n = 0; n < NB; ++n) {
-                  const int u =
-                      DB / 8 * n + (WC == 32 ? 2 * ((lane >> 4) & 1) : 0) + ((lane & 3) >> 1);
-                  const T* p0 =
-                      (const T*)(vt + vr * kRowB + (u ^ v_swz<S>(vr)) * 16 + 8 * (lane & 1));
-                  const int vr1 = vr + 4 * LPC;
-                  const T* p1 =
-                      (const T*)(vt + vr1 * kRowB + (u ^ v_swz<S>(vr1)) * 16 + 8 * (lane & 1));
-                  const V4 x0 = lds_read_tr4(p0), x1 = lds_read_tr4(p1);
-                  const V8 x = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
-                  if constexpr (WC == 32)
-                    o[n] = mfma32x32x16(x, p, o[n]);
-                  else
-                    o[n] = mfma16x16x32(x, p, o[n]);
+                  for (int n = 0; n < NB; ++n) {
+                    const int u =
+                        DB / 8 * n + (WC == 32 ? 2 * ((lane >> 4) & 1) : 0) + ((lane & 3) >> 1);
+                    const T* p0 =
+                        (const T*)(vt + vr * kRowB + (u ^ v_swz<S>(vr)) * 16 + 8 * (lane & 1));
+                    const int vr1 = vr + 4 * LPC;
+                    const T* p1 =
+                        (const T*)(vt + vr1 * kRowB + (u ^ v_swz<S>(vr1)) * 16 + 8 * (lane & 1));
+                    const V4 x0 = lds_read_tr4(p0), x1 = lds_read_tr4(p1);
+                    const V8 x = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
+                    if constexpr (WC == 32)
+                      o[n] = mfma32x32x16(x, p, o[n]);
+                    else
+                      o[n] = mfma16x16x32(x, p, o[n]);
+                  }
                 }
               }
             }
+            l += ps;
           }
-          l += ps;
+          wait_tiles<(S::RING - 2) * S::kTileLoads * DMA>();  // the next tile is in LDS
+          __syncthreads();
+          buf = buf + 1 == S::RING ? 0 : buf + 1;
         }
-        wait_tiles<(S::RING - 2) * S::kTileLoads * DMA>();  // the next tile is in LDS
-        __syncthreads();
-        buf = buf + 1 == S::RING ? 0 : buf + 1;
       }
       __builtin_amdgcn_s_waitcnt(0);  // no load may land behind the loop
       if constexpr (S::WK > 1) __syncthreads();  // nor any other wave's
@@ -929,7 +1102,7 @@ Kernel pick(int width, int cols, bool dma) {
     }
     if (!dma) return make<Shape<T, 256, 16, 8, 1, 32, 2>, false>();
     return cols <= 128 ? make<Shape<T, 256, 16, 8, 1, 32, 4>, true>()
-                       : make<Shape<T, 256, 32, 4, 1, 32, 4>, true>();
+                       : make<Shape<T, 256, 32, 4, 1, 64, 2>, true>();
   }
 }
 
