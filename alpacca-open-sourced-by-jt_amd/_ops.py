@@ -966,7 +966,7 @@ def tree_attention(q, key_cache, value_cache, masks, *, length, prefix_lens, cou
     batch, nodes, q_heads, key_dim = q.shape
     kv_heads, value_dim = value_cache.shape[2:]
     if out is None:
-        out = torch.empty((batch, nodes, q_heads, value_dim),
+        out = torch.empty(batch, nodes, q_heads, value_dim,
                           dtype=q.dtype if out_dtype is None else out_dtype, device=q.device)
     code = _lib.dtype_code(torch, q.dtype)
     nbytes = _tree_bytes(batch, nodes, q_heads, kv_heads, key_dim, value_dim, length, code)
@@ -995,11 +995,11 @@ def tree_masks(parents, *, lengths=None, counts=None):
     batch, nodes = parents.shape
     words = (nodes + 63) // 64
     device = parents.device
-    masks = torch.empty((batch, nodes, words), dtype=torch.int64, device=device)
-    depths = parents.new_empty((batch, nodes))
+    masks = torch.empty(batch, nodes, words, dtype=torch.int64, device=device)
+    depths = torch.empty_like(parents)
     lanes = None
     if lengths is not None:
-        lanes = torch.empty((batch, nodes, 4), dtype=torch.int64, device=device)
+        lanes = torch.empty(batch, nodes, 4, dtype=torch.int64, device=device)
     _enqueue(_lib.lib().alpx_tree_masks, device, parents.data_ptr(), _address(counts),
              _address(lengths), masks.data_ptr(), depths.data_ptr(), _address(lanes), batch, nodes,
              words)
@@ -1049,8 +1049,8 @@ def attention_prologue_rows(query_gate, key, value, q_norm, k_norm, key_pages, v
     tokens, q_heads, joint = query_gate.shape
     pages, page_size, kv_heads, dim = key_pages.shape
     value_dim = value_pages.shape[3]
-    query, gate = torch.empty((2, tokens, q_heads, dim), dtype=query_gate.dtype,
-                              device=query_gate.device)
+    query = torch.empty(tokens, q_heads, dim, dtype=query_gate.dtype, device=query_gate.device)
+    gate = torch.empty_like(query)
     _enqueue(_lib.lib().alpx_attention_prologue_rows, query_gate.device, query_gate.data_ptr(),
              key.data_ptr(), value.data_ptr(), q_norm.data_ptr(), k_norm.data_ptr(),
              query.data_ptr(), gate.data_ptr(), key_pages.data_ptr(), value_pages.data_ptr(),

@@ -33,7 +33,7 @@ from __future__ import annotations
 import importlib
 import math
 from dataclasses import dataclass
-from typing import Any, Sequence
+from typing import Any, NamedTuple, Sequence
 
 from . import _lib, _ops
 
@@ -167,8 +167,7 @@ class RocmPagedAttentionWorkspace:
         }
 
 
-@dataclass(frozen=True)
-class RocmTreeMasks:
+class RocmTreeMasks(NamedTuple):
     """Draft trees (extension): visibility words ``masks [batch, nodes,
     ceil(nodes / 64)]`` (int64, bit j % 64 of word j / 64 is draft j),
     ``depths [batch, nodes]`` (int32, -1 past a sequence's drafts) and, where
@@ -179,8 +178,7 @@ class RocmTreeMasks:
     position_lanes: Any
 
 
-@dataclass(frozen=True)
-class RocmPagedRows:
+class RocmPagedRows(NamedTuple):
     """New rows of a page pool (extension), packed in the order of sequences:
     ``starts [batch + 1]``; per row, -1 past the last, its pool row
     ``slots``, its position in its sequence ``positions`` and that sequence
@@ -237,6 +235,11 @@ class Qwen35RocmOps:
                 allow_integer: bool = False) -> Any:
         """Contract check of qwen35_rocm_ops.py:134-165, widened to fp16/bf16."""
         torch = self.torch
+        # all of it at once (a tensor on the host has device -1)
+        if (isinstance(value, torch.Tensor) and value.get_device() == self.device_index
+                and value.dtype in (self._int_dtypes if allow_integer else self._float_dtypes)
+                and (dimensions is None or value.dim() == dimensions) and value.is_contiguous()):
+            return value
         if not isinstance(value, torch.Tensor):
             raise TypeError(f"{name} must be a PyTorch tensor")
         if not value.is_cuda:
@@ -269,9 +272,11 @@ class Qwen35RocmOps:
 
     @staticmethod
     def _same_dtype(what: str, *tensors: Any) -> None:
-        dtypes = {t.dtype for t in tensors}
-        if len(dtypes) != 1:
-            raise TypeError(f"{what} tensors must share one dtype, got {sorted(map(str, dtypes))}")
+        dtype = tensors[0].dtype
+        for t in tensors:
+            if t.dtype != dtype:
+                dtypes = sorted({str(t.dtype) for t in tensors})
+                raise TypeError(f"{what} tensors must share one dtype, got {dtypes}")
 
     # ------------------------------------------------------------ workspaces
 
