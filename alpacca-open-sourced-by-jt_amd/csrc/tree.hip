@@ -422,57 +422,67 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
           vb = (const T*)a.v + (int64_t)b * a.vs_b + (int64_t)row * a.vs_pos + (int64_t)kvh * a.vs_h;
         }
       };
-      // K, V or both of tile t to LDS bytes kdst and vdst; rows past the end
-      // (all of them past the last tile) are zeros
-      auto load = [&](int t, bool k, bool v, uint32_t kdst, uint32_t vdst)
-                      __attribute__((always_inline)) {
+      // Where tile t's K and V lie; rows past the end (all of them past the
+      // last tile) read as zeros.
+      struct Source {
+        const T *k, *v;
+        int rows;
+        i32x4 rk, rv;
+      };
+      auto source = [&](int t) __attribute__((always_inline)) {
+        Source s;
         const int row0 = start + t * BK + grp;
-        const int rows = __builtin_amdgcn_readfirstlane(min(max(stop - row0, 0), 32));
-        const T *kb = (const T*)a.k, *vb = (const T*)a.v;
-        if (rows > 0) group_base(row0, kb, vb);
+        s.rows = __builtin_amdgcn_readfirstlane(min(max(stop - row0, 0), 32));
+        s.k = (const T*)a.k;
+        s.v = (const T*)a.v;
+        if (s.rows > 0) group_base(row0, s.k, s.v);
+        s.rk = rsrc_words((uint64_t)(uintptr_t)s.k,
+                          (uint32_t)(s.rows * a.ks_pos * (int64_t)sizeof(T)));
+        s.rv = rsrc_words((uint64_t)(uintptr_t)s.v,
+                          (uint32_t)(s.rows * a.vs_pos * (int64_t)sizeof(T)));
+        return s;
+      };
+      // load i of this wave's share of a K (V) tile, to LDS byte dst
+      auto load_k = [&](const Source& s, int i, uint32_t dst) __attribute__((always_inline)) {
+        lds_dma16(s.rk, lbase + dst + (wave * S::kIW + i) * 1024, kofs[i]);
+      };
+      auto load_v = [&](const Source& s, int i, uint32_t dst) __attribute__((always_inline)) {
+        if (S::kOnce)
+          lds_dma16_once(s.rv, lbase + dst + (wave * S::kIW + i) * 1024, vofs[i]);
+        else
+          lds_dma16(s.rv, lbase + dst + (wave * S::kIW + i) * 1024, vofs[i]);
+      };
+      auto load_tile = [&](int t, int buf) __attribute__((always_inline)) {
+        const Source s = source(t);
+        const uint32_t dst = buf * 2 * kTileB;
         if constexpr (DMA) {
-          if (k) {
-            const i32x4 rk = rsrc_words((uint64_t)(uintptr_t)kb,
-                                        (uint32_t)(rows * a.ks_pos * (int64_t)sizeof(T)));
-            const uint32_t dst = lbase + kdst + wave * S::kIW * 1024;
 #pragma unroll
-            for (int i = 0; i < S::kIW; ++i) lds_dma16(rk, dst + i * 1024, kofs[i]);
-          }
-          if (v) {
-            const i32x4 rv = rsrc_words((uint64_t)(uintptr_t)vb,
-                                        (uint32_t)(rows * a.vs_pos * (int64_t)sizeof(T)));
-            const uint32_t dst = lbase + vdst + wave * S::kIW * 1024;
+          for (int i = 0; i < S::kIW; ++i) load_k(s, i, dst);
 #pragma unroll
-            for (int i = 0; i < S::kIW; ++i) {
-              if (S::kOnce)
-                lds_dma16_once(rv, dst + i * 1024, vofs[i]);
-              else
-                lds_dma16(rv, dst + i * 1024, vofs[i]);
-            }
-          }
+          for (int i = 0; i < S::kIW; ++i) load_v(s, i, dst + kTileB);
         } else {
           // any head width, stride or alignment: element by element
           for (int i = lane; i < kRows * S::DP; i += 64) {
             const int r = wave * kRows + i / S::DP, d = i % S::DP;
-            const bool in = r - grp < rows;
-            const T kx =
-                in && d < a.key_dim ? kb[(int64_t)(r - grp) * a.ks_pos + d] : from_f32<T>(0.f);
-            const T vx =
-                in && d < a.value_dim ? vb[(int64_t)(r - grp) * a.vs_pos + d] : from_f32<T>(0.f);
+            const int64_t row = r - grp;
+            const bool in = row < s.rows;
+            const T kx = in && d < a.key_dim ? s.k[row * a.ks_pos + d] : from_f32<T>(0.f);
+            const T vx = in && d < a.value_dim ? s.v[row * a.vs_pos + d] : from_f32<T>(0.f);
             const int u = d / EPU, e = d % EPU;
-            ((T*)(smem + kdst))[r * S::DP + (u ^ k_swz<S>(r)) * EPU + e] = kx;
-            ((T*)(smem + vdst))[r * S::DP + (u ^ v_swz<S>(r)) * EPU + e] = vx;
+            T* k = (T*)(smem + dst);
+            k[r * S::DP + (u ^ k_swz<S>(r)) * EPU + e] = kx;
+            k[kTileB / (int)sizeof(T) + r * S::DP + (u ^ v_swz<S>(r)) * EPU + e] = vx;
           }
         }
-      };
-      auto load_tile = [&](int t, int buf) __attribute__((always_inline)) {
-        load(t, true, true, buf * 2 * kTileB, (buf * 2 + 1) * kTileB);
       };
 
       // the ring's first tiles, the queries while they are on their way
       if constexpr (S::kPipe) {
-        load(0, true, false, 0, 0);
-        load(1, true, false, kTileB, 0);
+        const Source s0 = source(0), s1 = source(1);
+#pragma unroll
+        for (int i = 0; i < S::kIW; ++i) load_k(s0, i, 0);
+#pragma unroll
+        for (int i = 0; i < S::kIW; ++i) load_k(s1, i, kTileB);
       } else {
 #pragma unroll
         for (int i = 0; i < S::RING - 1; ++i) load_tile(i, i);
@@ -560,9 +570,20 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
         __syncthreads();  // K 0 is read before turn 0 refills it
         auto turn = [&](auto parity, int t) __attribute__((always_inline)) {
           constexpr int Q = decltype(parity)::value;  // t & 1
-          if (t + 2 < nt) load(t + 2, true, false, Q * kTileB, 0);
-          if (t < nt) load(t, false, true, 0, (2 + Q) * kTileB);
-          if (!idle) {
+          // the turn's loads (past the last tile they fetch nothing and write
+          // zeros where nothing is read): spread over the steps, since a wave
+          // that issues them in one go waits for the address unit meanwhile
+          const Source sk = source(t + 2), sv = source(t);
+          auto load = [&](int i) __attribute__((always_inline)) {
+            if (i < S::kIW)
+              load_v(sv, i, (2 + Q) * kTileB);
+            else
+              load_k(sk, i - S::kIW, Q * kTileB);
+          };
+          if (idle) {
+#pragma unroll
+            for (int i = 0; i < S::kTileLoads; ++i) load(i);
+          } else {
             // O holds tiles up to t - 2 and is about to take P of tile t - 1,
             // formed against the reference that moved there
             if (__builtin_expect(pend_any, 0)) {
@@ -634,6 +655,9 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
                 else
                   sc[kr] = mfma32x32x16(x, qv[j], sc[kr]);
               }
+              // loads first, in the steps' first three quarters
+              constexpr int d0 = i * S::kTileLoads * 4 / (3 * N), d1 = (i + 1) * S::kTileLoads * 4 / (3 * N);
+              if constexpr (d1 > d0 && d0 < S::kTileLoads) load(d0);
               constexpr int e0 = i < LAST ? i * NE / LAST : NE;
               constexpr int e1 = i + 1 < LAST ? (i + 1) * NE / LAST : NE;
               static_for<e0, e1>([&](auto e_) __attribute__((always_inline)) {
