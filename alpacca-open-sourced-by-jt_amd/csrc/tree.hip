@@ -63,8 +63,9 @@ struct TreeArgs {
   int length, batch, nodes, q_heads, kv_heads, group, key_dim, value_dim;
   int col_tiles;      // column tiles per (sequence, kv head)
   int slots;          // shares of the rows per (kv head, column tile)
-  float* part_o;      // partial states, see `segment_of`
-  float2* part_st;
+  float* part_o;      // segments of O, [segment, kv head, column group][DP / 4][32] x 4
+  float2* part_st;    // reference score and sum of P of their columns
+  int4* found;        // [batch]: first and last slot of a sequence, P, end
   float scale_log2;
   int out_dtype;
   int vec_q, vec_o;   // q rows may be read, out rows written in vectors
@@ -95,73 +96,134 @@ __device__ __forceinline__ void uniform_rows(const TreeArgs& a, int b, int& P, i
   end = __builtin_amdgcn_readfirstlane(min(P + n, a.length));
 }
 
-// Shares of the rows.  The sequences' tiles of BK rows, one sequence after
-// the other, are dealt out in runs of `per` to the slots, so that every slot
-// gets the same number whatever the lengths; a run may end one sequence and
-// begin another.  Slot s leaves the partial state of its tiles of sequence b
-// in segment s + b: both rise along the list, so no two segments share a
-// number, and there are at most slots + batch.  A run that holds a whole
-// sequence writes its output and leaves no partial state, only a mark
-// whether that output is finite.
+// Shares of the rows: every slot gets a run of tiles of BK rows, cut on the
+// device since only it knows the lengths.
+//
+// Where the sequences divide well, a run belongs to one of them: the shortest
+// run length is searched with which all sequences' runs fit the slots, and
+// each sequence is cut into equal runs.  Otherwise the sequences' tiles, one
+// sequence after the other, are dealt out in runs of equal length, and a run
+// may end one sequence and begin another, which costs it about kTurnOver
+// tiles of waiting (for the next queries and first tiles).
+//
+// Slot s leaves the partial state of its tiles of sequence b in segment
+// s + b: both rise along the runs, so no two segments share a number, and
+// there are at most slots + batch.  A run that holds a whole sequence writes
+// its output and leaves no partial state, only a mark whether that output is
+// finite.
 struct Share {
-  int per;    // tiles per slot
-  int first;  // tiles before the sequence
-  int b;      // the sequence, -1: none
-  int tiles;  // its tiles
-  int P, end; // its rows
+  int b;       // the sequence, -1: none
+  int P, end;  // its rows: [0, P) the prefix, [P, end) the drafts
+  int tiles;   // its tiles
+  int t0, nt;  // the slot's: nt tiles of it from t0 on
+  int left;    // and as many of the next sequences
+  int s1;      // the last slot that has tiles of it
+  int per;     // tiles per slot
 };
+constexpr int kTurnOver = 4;
 
-// Tiles of sequence b0 + lane, and before it (from b0 on).
-template <int BK>
-__device__ __forceinline__ void lane_tiles(const TreeArgs& a, int b0, int& P, int& end, int& nt,
-                                           int& before, int& total) {
-  const int lane = threadIdx.x & 63, b = b0 + lane;
-  P = end = 0;
-  if (b < a.batch) lane_rows(a, b, P, end);
-  nt = (end + BK - 1) / BK;
-  int x = nt;
+__device__ __forceinline__ int wave_total(int x) {
 #pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int y = __shfl_up(x, off);
-    if (lane >= off) x += y;
-  }
-  total = __builtin_amdgcn_readlane(x, 63);
-  before = x - nt;
+  for (int off = 32; off >= 1; off >>= 1) x += __shfl_xor(x, off);
+  return __builtin_amdgcn_readfirstlane(x);
 }
 
-// The share of tile `want`, or where want_b >= 0 of sequence want_b; want
-// counts in units of the tiles per slot.  Every lane of a wave calls this,
-// and gets the same.
-template <int BK>
-__device__ __forceinline__ Share find_share(const TreeArgs& a, int want_slot, int want_b, int& all) {
-  int P, end, nt, before, total;
-  lane_tiles<BK>(a, 0, P, end, nt, before, total);
-  all = total;
-  for (int b0 = 64; b0 < a.batch; b0 += 64) {  // the first 64 sequences stay in registers
-    int p, e, n, f, t;
-    lane_tiles<BK>(a, b0, p, e, n, f, t);
-    all += t;
+// Exclusive sums over the lanes.
+__device__ __forceinline__ int wave_before(int x) {
+  const int lane = threadIdx.x & 63;
+  int y = x;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int z = __shfl_up(y, off);
+    if (lane >= off) y += z;
   }
+  return y - x;
+}
+
+__device__ __forceinline__ int div_up(int x, int y) {
+  return (int)(((unsigned)x + (unsigned)y - 1u) / (unsigned)y);
+}
+
+// The first share of slot `slot`.  Every lane of a wave calls this, and gets
+// the same.  `first_of_all`: sequences without a row are noted for the join (the
+// others are by the slot that begins them).
+template <int BK>
+__device__ __forceinline__ Share find_share(const TreeArgs& a, int slot, bool first_of_all) {
+  const int lane = threadIdx.x & 63;
+  auto rows_of = [&](int b0, int& P, int& end) __attribute__((always_inline)) {
+    P = end = 0;
+    if (b0 + lane < a.batch) lane_rows(a, b0 + lane, P, end);
+    return (end + BK - 1) / BK;
+  };
+  int P, end;
+  int nt = rows_of(0, P, end);  // the first 64 sequences stay in registers
+  int all = wave_total(nt);
+  auto note_empty = [&](int b, int tiles) __attribute__((always_inline)) {
+    if (first_of_all && tiles == 0 && b < a.batch) a.found[b] = make_int4(0, -1, 0, 0);
+  };
+  note_empty(lane, nt);
+  for (int b0 = 64; b0 < a.batch; b0 += 64) {
+    int p, e;
+    const int n = rows_of(b0, p, e);
+    all += wave_total(n);
+    note_empty(b0 + lane, n);
+  }
+  const int per = max(1, div_up(all, a.slots));
   Share r = {};
   r.b = -1;
-  r.per = max(1, (all + a.slots - 1) / a.slots);
-  const int want = want_slot * r.per;
+  int lo = per, hi = per;
+  if (a.batch <= 64) {
+    bool fits = wave_total(div_up(nt, per)) <= a.slots;
+    if (!fits && a.slots > a.batch) {
+      hi = min(div_up(all, a.slots - a.batch), per + kTurnOver + 1);
+      while (hi - lo > 1) {  // lo does not fit, hi does or is too long
+        const int mid = (lo + hi) >> 1;
+        if (wave_total(div_up(nt, mid)) <= a.slots) hi = mid; else lo = mid;
+      }
+      fits = hi <= per + kTurnOver;
+    }
+    if (fits) {
+      const int runs = div_up(nt, hi), before = wave_before(runs);
+      const bool mine = slot >= before && slot < before + runs;
+      const unsigned long long hit = __ballot(mine);
+      if (hit == 0) return r;
+      const int src = __ffsll((long long)hit) - 1;
+      const int n = __builtin_amdgcn_readlane(runs, src);
+      r.b = src;
+      r.P = __builtin_amdgcn_readlane(P, src);
+      r.end = __builtin_amdgcn_readlane(end, src);
+      r.tiles = __builtin_amdgcn_readlane(nt, src);
+      const int s0 = __builtin_amdgcn_readlane(before, src);
+      r.s1 = s0 + n - 1;
+      const int q = r.tiles / n, more = r.tiles - q * n, i = slot - s0;
+      r.t0 = i * q + min(i, more);
+      r.nt = q + (i < more ? 1 : 0);
+      return r;
+    }
+  }
+  const int want = slot * per;
   int base = 0;
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
-    if (b0 > 0) lane_tiles<BK>(a, b0, P, end, nt, before, total);
-    const int b = b0 + (int)(threadIdx.x & 63), first = base + before;
-    const bool mine = want_b >= 0 ? b == want_b : (want >= first && want < first + nt);
+    if (b0 > 0) nt = rows_of(b0, P, end);
+    const int first = base + wave_before(nt);
+    const bool mine = want >= first && want < first + nt;
     const unsigned long long hit = __ballot(mine);
     if (hit != 0) {
       const int src = __ffsll((long long)hit) - 1;
+      const int f = __builtin_amdgcn_readlane(first, src);
       r.b = b0 + src;
-      r.tiles = __builtin_amdgcn_readlane(nt, src);
-      r.first = __builtin_amdgcn_readlane(first, src);
       r.P = __builtin_amdgcn_readlane(P, src);
       r.end = __builtin_amdgcn_readlane(end, src);
+      r.tiles = __builtin_amdgcn_readlane(nt, src);
+      r.s1 = (f + r.tiles - 1) / per;
+      r.per = per;
+      r.t0 = want - f;
+      const int run = min(per, all - want);
+      r.nt = min(run, r.tiles - r.t0);
+      r.left = run - r.nt;
       return r;
     }
-    base += total;
+    base += __builtin_amdgcn_readlane(first + nt, 63) - base;
   }
   return r;
 }
@@ -361,11 +423,8 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
   const int unit = (at / a.col_tiles) * kXcds + xcd;
   const int slot = unit / a.kv_heads, kvh = unit % a.kv_heads;
   if (slot >= a.slots) return;
-  int all;
-  Share sh = find_share<BK>(a, slot, -1, all);
+  Share sh = find_share<BK>(a, slot, unit == 0 && ct == 0 && wave == 0);
   if (sh.b < 0) return;  // fewer tiles than slots
-  int todo = slot * sh.per;
-  const int todo_end = min(all, todo + sh.per);
 
   // Tile loads: wave w fills rows [w BK / NW, (w + 1) BK / NW) of a tile, all
   // in its 32-row group `grp`.
@@ -397,7 +456,9 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
     const int node = col / G;
     const bool in_range = node < a.nodes;
     const int b = sh.b, P = sh.P;
-    const int t0 = todo - sh.first, nt = min(todo_end, sh.first + sh.tiles) - todo;
+    const int t0 = sh.t0, nt = sh.nt;
+    if (t0 == 0 && kvh == 0 && ct == 0 && tid == 0)
+      a.found[b] = make_int4(slot, sh.s1, P, sh.end);
     auto segment = [&]() __attribute__((always_inline)) {
       // rows [start, stop) of sequence b, in tiles of BK
       const int start = t0 * BK, stop = min(sh.end, start + nt * BK);
@@ -899,15 +960,17 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
       }
     };
     segment();
-    todo += nt;
-    if (todo >= todo_end) return;
+    if (sh.left == 0) return;
     // the next sequence that has rows
     do {
-      sh.first += sh.tiles;
       ++sh.b;
       uniform_rows(a, sh.b, sh.P, sh.end);
       sh.tiles = (sh.end + BK - 1) / BK;
     } while (sh.tiles == 0);
+    sh.t0 = 0;
+    sh.nt = min(sh.left, sh.tiles);
+    sh.left -= sh.nt;
+    sh.s1 = slot + (sh.tiles - sh.nt + sh.per - 1) / sh.per;
     __syncthreads();  // every wave is done with the tiles in LDS
   }
 }
@@ -962,7 +1025,7 @@ __device__ __forceinline__ void rows_apart(const TreeArgs& a, int b, int kvh, in
 // head, 32 columns, 32 channels); its four waves take the segments in turn
 // and meet in LDS.  A block whose result is not finite forms it again, row
 // by row.
-template <typename T, int DP, int BK>
+template <typename T, int DP>
 __global__ void __launch_bounds__(256) tree_join(TreeArgs a) {
   constexpr int MB = DP / 32, kFlight = 4;
   __shared__ float part[34 * 256];  // [4][18][64] of the segments, or [34][256] row by row
@@ -973,20 +1036,20 @@ __global__ void __launch_bounds__(256) tree_join(TreeArgs a) {
   const int cg = blockIdx.x / MB % groups;
   const int kvh = blockIdx.x / MB / groups % a.kv_heads;
   const int b = blockIdx.x / MB / groups / a.kv_heads;
-  int all;
-  const Share sh = find_share<BK>(a, 0, b, all);
-  const int s0 = sh.first / sh.per, s1 = (sh.first + max(sh.tiles, 1) - 1) / sh.per;
-  const bool whole = a.direct && sh.tiles > 0 && s0 == s1;  // written by its slot
+  const int32_t* found = (const int32_t*)(a.found + b);
+  const int s0 = load_const(found), s1 = load_const(found + 1);
+  const int P = load_const(found + 2), end = load_const(found + 3);
+  const bool whole = a.direct && s0 == s1;  // written by its slot
   if (whole) {  // the two waves of 16 columns have a mark each
     const float2* mark = a.part_st + (((int64_t)(s0 + b) * a.kv_heads + kvh) * groups + cg) * 32;
     if (mark[0].x == 0.f && mark[16].x == 0.f) return;
   }
   const int G = a.group, col = 32 * cg + hl, node = col / G;
-  const int count = sh.end - sh.P;
+  const int count = end - P;
   float m = -INFINITY, l = 0.f, o[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) o[i] = 0.f;
-  if (!whole && sh.tiles > 0 && 32 * cg < count * G) {
+  if (!whole && 32 * cg < count * G) {
     for (int s = s0 + w; s <= s1; s += 4 * kFlight) {
       float2 st[kFlight];
       f32x4 x[kFlight][4];
@@ -1044,7 +1107,7 @@ __global__ void __launch_bounds__(256) tree_join(TreeArgs a) {
   if (__syncthreads_or(bad)) {
     __syncthreads();  // the segments' sums in LDS are read
     float x[32];
-    rows_apart<T>(a, b, kvh, 32 * cg + (threadIdx.x & 31), 32 * mb, sh.P, sh.end, x, m, l);
+    rows_apart<T>(a, b, kvh, 32 * cg + (threadIdx.x & 31), 32 * mb, P, end, x, m, l);
 #pragma unroll
     for (int i = 0; i < 32; ++i) part[i * 256 + threadIdx.x] = x[i];
     part[32 * 256 + threadIdx.x] = m;
@@ -1073,6 +1136,8 @@ __global__ void __launch_bounds__(256) tree_join(TreeArgs a) {
   write4<T>(a, qrow, 32 * mb + 8 * w + 4 * half, r);
 }
 
+constexpr int kCus = 256;
+
 struct Kernel {
   const void* fn;
   const void* join;
@@ -1085,7 +1150,7 @@ struct Kernel {
 
 template <typename S, bool DMA>
 Kernel make() {
-  return {(const void*)tree_kernel<S, DMA>, (const void*)tree_join<typename S::T, S::DP, S::BK>,
+  return {(const void*)tree_kernel<S, DMA>, (const void*)tree_join<typename S::T, S::DP>,
           64 * S::NW, S::kCols, S::BK, S::DP, S::kPerCu};
 }
 
@@ -1095,17 +1160,23 @@ Kernel make() {
 // bound by the products: 32 a wave, which halves the operand reads, and room
 // for a second block, whose products run while this one forms its
 // probabilities.
+//
+// float32: where tiles of 128 rows are fewer than CUs, tiles of 32 rows give
+// more of them one (8 drafts on 508 rows, 32/8 heads of 64 / 128: 12.2 ->
+// 9.3 / 13.6 -> 11.2 us; 4 x 8 on 8192 rows 31 -> 33 / 59 -> 64).
 template <typename T>
-Kernel pick(int width, int cols, bool dma) {
+Kernel pick(int width, int cols, bool dma, bool few) {
   if constexpr (sizeof(T) == 4) {
     if (width <= 64) {
       if (!dma) return make<Shape<T, 64, 16, 4, 2, 64, 2>, false>();
+      if (cols <= 32 && few) return make<Shape<T, 64, 16, 2, 2, 32, 4>, true>();
       return cols <= 32   ? make<Shape<T, 64, 16, 2, 4, 128, 2>, true>()
              : cols <= 64 ? make<Shape<T, 64, 16, 4, 2, 64, 4>, true>()
                           : make<Shape<T, 64, 32, 4, 1, 32, 2>, true>();
     }
     if (width <= 128) {
       if (!dma) return make<Shape<T, 128, 16, 4, 2, 64, 2>, false>();
+      if (cols <= 32 && few) return make<Shape<T, 128, 16, 2, 2, 32, 2>, true>();
       return cols <= 32   ? make<Shape<T, 128, 16, 2, 4, 64, 2>, true>()
              : cols <= 64 ? make<Shape<T, 128, 16, 4, 2, 64, 2>, true>()
                           : make<Shape<T, 128, 32, 4, 1, 32, 2>, true>();
@@ -1130,12 +1201,9 @@ Kernel pick(int width, int cols, bool dma) {
   }
 }
 
-constexpr int kCus = 256;
-
 struct TreePlan {
   Kernel kernel;
   int col_tiles, slots;
-  bool join;
   size_t segments, part_o, bytes;  // floats of O, bytes in all
 };
 
@@ -1144,18 +1212,18 @@ TreePlan tree_plan(int batch, int nodes, int q_heads, int kv_heads, int key_dim,
   TreePlan p = {};
   const int width = std::max(key_dim, value_dim);
   const int cols = nodes * (q_heads / kv_heads);
-  p.kernel = dtype == ALPX_F32   ? pick<float>(width, cols, dma)
-             : dtype == ALPX_F16 ? pick<f16_t>(width, cols, dma)
-                                 : pick<bf16_t>(width, cols, dma);
+  const bool few = (int64_t)batch * kv_heads * ((length + 127) / 128) < kCus;
+  p.kernel = dtype == ALPX_F32   ? pick<float>(width, cols, dma, few)
+             : dtype == ALPX_F16 ? pick<f16_t>(width, cols, dma, few)
+                                 : pick<bf16_t>(width, cols, dma, few);
   p.col_tiles = (cols + p.kernel.cols - 1) / p.kernel.cols;
   // one round of blocks, every slot at least a tile
   const int64_t tiles = (int64_t)batch * ((length + p.kernel.rows - 1) / p.kernel.rows);
   const int64_t share = kCus * p.kernel.per_cu / ((int64_t)kv_heads * p.col_tiles);
   p.slots = (int)std::min(std::max<int64_t>(share, 1), tiles);
-  p.join = true;
   p.segments = (size_t)(p.slots + batch) * kv_heads * p.col_tiles * (p.kernel.cols / 32);
   p.part_o = p.segments * 32 * p.kernel.width;
-  p.bytes = p.part_o * 4 + p.segments * 32 * sizeof(float2);
+  p.bytes = p.part_o * 4 + p.segments * 32 * sizeof(float2) + (size_t)batch * sizeof(int4);
   return p;
 }
 
@@ -1204,7 +1272,8 @@ int tree_launch(const char* what, TreeArgs a, int dtype, void* workspace, size_t
   a.slots = p.slots;
   a.direct = a.vec_o && a.value_dim == p.kernel.width;
   a.part_o = (float*)workspace;
-  a.part_st = (float2*)((float*)workspace + p.part_o);
+  a.part_st = (float2*)(a.part_o + p.part_o);
+  a.found = (int4*)(a.part_st + p.segments * 32);
   const int64_t units = (int64_t)p.slots * a.kv_heads;
   const int64_t blocks = (units + kXcds - 1) / kXcds * kXcds * p.col_tiles;
   const int groups = p.col_tiles * (p.kernel.cols / 32);
@@ -1217,11 +1286,9 @@ int tree_launch(const char* what, TreeArgs a, int dtype, void* workspace, size_t
     TimedRegion timed(ALPX_T_DECODE, s);
     (void)hipLaunchKernel(p.kernel.fn, dim3((unsigned)blocks), dim3(p.kernel.threads), args, 0, s);
   }
-  if (p.join) {
-    a.col_tiles = groups;
-    TimedRegion timed(ALPX_T_DECODE_COMBINE, s);
-    (void)hipLaunchKernel(p.kernel.join, dim3((unsigned)joins), dim3(256), args, 0, s);
-  }
+  a.col_tiles = groups;
+  TimedRegion timed(ALPX_T_DECODE_COMBINE, s);
+  (void)hipLaunchKernel(p.kernel.join, dim3((unsigned)joins), dim3(256), args, 0, s);
   return check_launch(what);
 }
 
