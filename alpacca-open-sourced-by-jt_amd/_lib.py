@@ -51,7 +51,7 @@ SIGNATURES = {
                                         _c_int, _c_ptr]),
     "alpx_paged_resize": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int,
                                    _c_int, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
-                                   _c_ptr, _c_ptr]),
+                                   _c_ptr, _c_ptr, _c_ptr]),
     "alpx_attention_prologue_rows": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
                                               _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_ptr, _c_ptr,
                                               _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,

@@ -1030,13 +1030,15 @@ def paged_resize(block_table, lengths, free_pages, free_count, targets, *, page_
     place); returns ``(starts, slots, positions, sequences, granted)``."""
     batch, max_pages = block_table.shape
     device = block_table.device
-    # one buffer: three rows of `tokens`, then starts and grants
-    slots, positions, sequences, starts, granted = lengths.new_empty(
-        3 * tokens + 2 * batch + 1).split_with_sizes((tokens, tokens, tokens, batch + 1, batch))
+    # one buffer: three rows of `tokens`, starts, grants and the call's scratch
+    buffer = lengths.new_empty(3 * tokens + 3 * batch + 2)
+    slots, positions, sequences, starts, granted, _ = buffer.split_with_sizes(
+        (tokens, tokens, tokens, batch + 1, batch, batch + 1))
     _enqueue(_lib.lib().alpx_paged_resize, device, block_table.data_ptr(), lengths.data_ptr(),
              free_pages.data_ptr(), free_count.data_ptr(), targets.data_ptr(), batch, max_pages,
              page_size, free_pages.shape[0], tokens, starts.data_ptr(), slots.data_ptr(),
-             positions.data_ptr(), sequences.data_ptr(), granted.data_ptr())
+             positions.data_ptr(), sequences.data_ptr(), granted.data_ptr(),
+             granted.data_ptr() + 4 * batch)
     return starts, slots, positions, sequences, granted
 
 

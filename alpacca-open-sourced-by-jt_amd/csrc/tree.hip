@@ -1265,7 +1265,9 @@ int tree_launch(const char* what, TreeArgs a, int dtype, void* workspace, size_t
             ((uintptr_t)a.gate & (4 * es - 1)) == 0;
   const TreePlan p = tree_plan(a.batch, a.nodes, a.q_heads, a.kv_heads, a.key_dim, a.value_dim,
                                a.length, dtype, dma);
-  if (workspace_bytes < p.bytes || (p.bytes > 0 && !workspace))
+  if (((uintptr_t)workspace & 15) != 0)
+    return fail(ALPX_EINVAL, "%s: workspace must be 16-byte aligned", what);
+  if (workspace_bytes < p.bytes || !workspace)
     return fail(ALPX_EINVAL, "%s: workspace holds %zu bytes, needs %zu", what, workspace_bytes,
                 p.bytes);
   a.col_tiles = p.col_tiles;

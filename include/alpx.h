@@ -696,8 +696,9 @@ int alpx_recurrent_prefill_prep(const float* current, const float* conv_weight,
  * stride and alignment; rows of 16-byte multiples run fastest.  Arithmetic
  * is fp32 (fp16 / bf16: the probabilities are rounded to the cache's type
  * for their product, the sums are not).
- * workspace: alpx_tree_workspace_bytes bytes (0: none is needed); scratch,
- * which calls that may overlap must not share.
+ * workspace: alpx_tree_workspace_bytes bytes (0 for sizes that the calls
+ * refuse), 16-byte aligned; scratch, which calls that may overlap must not
+ * share.  Two launches.
  */
 size_t alpx_tree_workspace_bytes(int batch, int nodes, int q_heads, int kv_heads, int key_dim,
                                  int value_dim, int length, int dtype);
@@ -766,11 +767,13 @@ int alpx_tree_commit_paged(void* key_pages, void* value_pages, const int32_t* bl
  * positions[t] in its sequence sequences[t]; all three are [tokens], -1 past
  * the last new row.  Cutting sequences back by the rows of the last call
  * restores the stack.  page_size a power of two; pool and sequences of less
- * than 2^31 rows, max_pages of at most 2^20.  One launch, two for more than 4096 tokens. */
+ * than 2^31 rows, max_pages of at most 2^20.  scratch: batch + 1 int32 of the
+ * call's own.  One launch, two for more than 4096 tokens. */
 int alpx_paged_resize(int32_t* block_table, int32_t* lengths, int32_t* free_pages,
                       int32_t* free_count, const int32_t* targets, int batch, int max_pages,
                       int page_size, int num_pages, int tokens, int32_t* starts, int32_t* slots,
-                      int32_t* positions, int32_t* sequences, int32_t* granted, void* stream);
+                      int32_t* positions, int32_t* sequences, int32_t* granted,
+                      int32_t* scratch, void* stream);
 
 /* alpx_attention_prologue for packed tokens of any sequences and positions
  * (an extension): token t of query_gate [T, Hq, 2D], key [T, Hkv, D] and
