@@ -59,7 +59,7 @@ __device__ __forceinline__ int64_t block_scan(int64_t x, int64_t (*part)[kThread
   if (lane == 63) p[wave] = x;
   __syncthreads();
   int64_t before = 0, all = 0;
-#pragma unroll
+#pragma unroll 4
   for (int w = 0; w < NT / 64; ++w) {
     const int64_t s = p[w];
     if (w < wave) before += s;
@@ -355,7 +355,7 @@ __device__ __forceinline__ char* commit_row(const CommitArgs& a, char* base, int
 // before that, so no row is written before it has been read.  Bound by
 // latency: path, table, row, one round trip each (one thread per unit that
 // took its rows in turn, eight at a time: 9.4 us for 128 sequences of up to
-// 16 accepted drafts, 32 KiB each; this one @@).
+// 16 accepted drafts, 32 KiB each; this one 4.2).
 constexpr int kUnits = 64, kSteps = 4;          // units of a block, steps of a thread
 constexpr int kChunk = 256 / kUnits * kSteps;   // steps of a block at a time
 static_assert(kChunk <= 64, "a wave holds a chunk's steps in its lanes");

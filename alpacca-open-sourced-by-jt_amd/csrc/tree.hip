@@ -264,12 +264,13 @@ struct Shape {
   // of a third (see the loop).
   static constexpr bool kPipe = WC == 32 && sizeof(T) == 2 && RING == 2;
   // The narrow kernels have one column tile: nobody reads a tile twice.
-  // (The hint on V, on K and V / on V / on neither, 16 x 16 drafts on 8192
-  // rows: @@ us.)
+  // (The hint on K and V / on V / on neither, 16 x 16 drafts on 8192 rows:
+  // 97 / 86 / 103 us.)
   static constexpr bool kOnce = WC == 16;
   // O and the sums of the waves that share keys are joined in LDS.
   static constexpr int kPart = (4 * NF + 2) * 64;  // floats per wave
   static constexpr int kMergeB = (WK - 1) * WQ * kPart * 4;
+  static constexpr int kRowsApartB = 34 * 256 * 4;  // see sort_out
   static constexpr int kLds = 2 * RING * kTileB > kMergeB ? 2 * RING * kTileB : kMergeB;
   // Blocks per CU: 160 KiB of LDS, and registers for 16, 8 or 4 waves.
   static constexpr int kLdsBlocks = 160 * 1024 / kLds;
@@ -390,15 +391,99 @@ __device__ __forceinline__ void write4(const TreeArgs& a, int64_t row, int d0, f
   }
 }
 
+// The result of 32 columns and 32 channels row by row, for sequences with an
+// infinity or a NaN in them.  The products take every row of a tile for
+// every column, and 0 times an infinity is a NaN: here a column takes the
+// rows that it sees, and an infinity among their values comes out as itself
+// however small its weight.  Thread (column, g), g < 8, takes rows g, g + 8, ...
+template <typename T>
+__device__ __forceinline__ void rows_apart(const TreeArgs& a, int b, int kvh, int col, int d0,
+                                           int P, int end, float (&o)[32], float& m, float& l) {
+  const int G = a.group, node = col / G, g = threadIdx.x >> 5;
+  m = -INFINITY;
+  l = 0.f;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) o[i] = 0.f;
+  if (node >= min(end - P, a.nodes)) return;
+  const T* q = (const T*)a.q +
+               (((int64_t)b * a.nodes + node) * a.q_heads + kvh * G + (col - node * G)) * a.key_dim;
+  const uint32_t* mask = a.masks + b * a.mask_b + (int64_t)node * a.words;
+  for (int j = g; j < end; j += 8) {
+    if (j >= P && !(mask[(j - P) >> 5] >> ((j - P) & 31) & 1u)) continue;
+    int64_t ko = (int64_t)b * a.ks_b + j * a.ks_pos, vo = (int64_t)b * a.vs_b + j * a.vs_pos;
+    if (a.pages != nullptr) {
+      int pg = a.pages[(int64_t)b * a.max_pages + (j >> a.page_shift)];
+      pg = min(max(pg, 0), a.num_pages - 1);
+      const int64_t in = j & ((1 << a.page_shift) - 1);
+      ko = pg * a.ks_b + in * a.ks_pos;
+      vo = pg * a.vs_b + in * a.vs_pos;
+    }
+    const T* k = (const T*)a.k + ko + (int64_t)kvh * a.ks_h;
+    const T* v = (const T*)a.v + vo + (int64_t)kvh * a.vs_h;
+    float s = 0.f;
+    for (int d = 0; d < a.key_dim; ++d) s = fmaf(to_f32(q[d]), to_f32(k[d]), s);
+    s *= a.scale_log2;
+    const float M = fmaxf(m, s);
+    const float c = weight(m, M), p = fast_exp2(s - M);
+    l = l * c + p;
+    m = M;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const float x = d0 + i < a.value_dim ? to_f32(v[d0 + i]) : 0.f;
+      const float kept = finite(o[i]) ? o[i] * c : o[i];
+      o[i] = kept + (finite(x) ? p * x : x);
+    }
+  }
+}
+
+// The output of columns 32 cg + 0 .. 31 and channels 32 mb + 0 .. 31 that way.
+// Every thread of the block calls it; those past 256 only meet the barriers.
+// `part`: 34 x 256 floats of LDS.
+template <typename T>
+__device__ __forceinline__ void sort_out(const TreeArgs& a, int b, int kvh, int cg, int mb, int P,
+                                         int end, float* part) {
+  const int tid = threadIdx.x, lane = tid & 63, hl = lane & 31, half = lane >> 5, w = tid >> 6;
+  const int G = a.group, col = 32 * cg + hl, node = col / G;
+  if (tid < 256) {
+    float x[32], m, l;
+    rows_apart<T>(a, b, kvh, col, 32 * mb, P, end, x, m, l);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) part[i * 256 + tid] = x[i];
+    part[32 * 256 + tid] = m;
+    part[33 * 256 + tid] = l;
+  }
+  __syncthreads();
+  if (tid < 256 && node < a.nodes) {
+    float M = -INFINITY, l = 0.f, r[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int g = 0; g < 8; ++g) M = fmaxf(M, part[32 * 256 + 32 * g + hl]);
+    for (int g = 0; g < 8; ++g) {
+      const float c = weight(part[32 * 256 + 32 * g + hl], M);
+      l += part[33 * 256 + 32 * g + hl] * c;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float y = part[(8 * w + 4 * half + i) * 256 + 32 * g + hl];
+        r[i] += finite(y) ? y * c : y;
+      }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = node < end - P ? r[i] * inv : 0.f;
+    const int64_t row = ((int64_t)b * a.nodes + node) * a.q_heads + kvh * G + (col - node * G);
+    write4<T>(a, row, 32 * mb + 8 * w + 4 * half, r);
+  }
+  __syncthreads();  // `part` is read
+}
+
 // One block: slot `s`, kv head and column tile; it walks its run of tiles,
-// sequence by sequence.
+// sequence by sequence.  ALONE: slot `s` is sequence `s`.
 //
 // Lane (cl, sub) of a wave owns column cl and, of every 4 LPC keys or
 // channels, the four from 4 sub on: the order in which an MFMA leaves its
 // result.  Both products take their inner index in that order too, so the
 // probabilities are an operand where they lie.
-template <typename S, bool DMA>
+template <typename S, bool DMA, bool ALONE>
 __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(TreeArgs a) {
+  static_assert(!ALONE || (S::kLds >= S::kRowsApartB && S::NW >= 4), "sort_out's space and threads");
   typedef typename S::T T;
   constexpr bool F32 = sizeof(T) == 4;
   constexpr int BK = S::BK, WC = S::WC, LPC = S::LPC, KG = S::KG, EPU = S::EPU, U = S::U;
@@ -423,8 +508,16 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
   const int unit = (at / a.col_tiles) * kXcds + xcd;
   const int slot = unit / a.kv_heads, kvh = unit % a.kv_heads;
   if (slot >= a.slots) return;
-  Share sh = find_share<BK>(a, slot, unit == 0 && ct == 0 && wave == 0);
-  if (sh.b < 0) return;  // fewer tiles than slots
+  Share sh;
+  if constexpr (ALONE) {  // a slot per sequence
+    sh = {};
+    sh.b = slot;
+    uniform_rows(a, slot, sh.P, sh.end);
+    sh.tiles = sh.nt = (sh.end + BK - 1) / BK;
+  } else {
+    sh = find_share<BK>(a, slot, unit == 0 && ct == 0 && wave == 0);
+    if (sh.b < 0) return;  // fewer tiles than slots
+  }
 
   // Tile loads: wave w fills rows [w BK / NW, (w + 1) BK / NW) of a tile, all
   // in its 32-row group `grp`.
@@ -457,8 +550,9 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
     const bool in_range = node < a.nodes;
     const int b = sh.b, P = sh.P;
     const int t0 = sh.t0, nt = sh.nt;
-    if (t0 == 0 && kvh == 0 && ct == 0 && tid == 0)
+    if (!ALONE && t0 == 0 && kvh == 0 && ct == 0 && tid == 0)
       a.found[b] = make_int4(slot, sh.s1, P, sh.end);
+    bool again = false;  // alone: some of the output is not finite
     auto segment = [&]() __attribute__((always_inline)) {
       // rows [start, stop) of sequence b, in tiles of BK
       const int start = t0 * BK, stop = min(sh.end, start + nt * BK);
@@ -925,7 +1019,8 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
 #pragma unroll
       for (int i = 0; i < 4 * NF; ++i) zero = fmaf(o[i / NA][i % NA], 0.f, zero);
       const bool bad = __ballot(live && zero != 0.f) != 0;
-      if (sub == 0) a.part_st[seg * 32 + c32] = make_float2(bad ? 1.f : 0.f, 0.f);
+      if (!ALONE && sub == 0) a.part_st[seg * 32 + c32] = make_float2(bad ? 1.f : 0.f, 0.f);
+      again |= bad;
       if (!in_range) return;
       const float inv = live && l != 0.f ? 1.f / l : 0.f;
 #pragma unroll
@@ -960,6 +1055,14 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
       }
     };
     segment();
+    if constexpr (ALONE) {
+      if (__syncthreads_or(again)) {
+        for (int i = 0; i < S::kCols / 32 * (S::DP / 32); ++i)
+          sort_out<T>(a, b, kvh, ct * (S::kCols / 32) + i / (S::DP / 32), i % (S::DP / 32), P,
+                      sh.end, (float*)smem);
+      }
+      return;
+    }
     if (sh.left == 0) return;
     // the next sequence that has rows
     do {
@@ -972,51 +1075,6 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
     sh.left -= sh.nt;
     sh.s1 = slot + (sh.tiles - sh.nt + sh.per - 1) / sh.per;
     __syncthreads();  // every wave is done with the tiles in LDS
-  }
-}
-
-// The result of 32 columns and 32 channels row by row, for sequences with an
-// infinity or a NaN in them.  The products take every row of a tile for
-// every column, and 0 times an infinity is a NaN: here a column takes the
-// rows that it sees, and an infinity among their values comes out as itself
-// however small its weight.  Thread (column, g) takes rows g, g + 8, ...
-template <typename T>
-__device__ __forceinline__ void rows_apart(const TreeArgs& a, int b, int kvh, int col, int d0,
-                                           int P, int end, float (&o)[32], float& m, float& l) {
-  const int G = a.group, node = col / G, g = threadIdx.x >> 5;
-  m = -INFINITY;
-  l = 0.f;
-#pragma unroll
-  for (int i = 0; i < 32; ++i) o[i] = 0.f;
-  if (node >= min(end - P, a.nodes)) return;
-  const T* q = (const T*)a.q +
-               (((int64_t)b * a.nodes + node) * a.q_heads + kvh * G + (col - node * G)) * a.key_dim;
-  const uint32_t* mask = a.masks + b * a.mask_b + (int64_t)node * a.words;
-  for (int j = g; j < end; j += 8) {
-    if (j >= P && !(mask[(j - P) >> 5] >> ((j - P) & 31) & 1u)) continue;
-    int64_t ko = (int64_t)b * a.ks_b + j * a.ks_pos, vo = (int64_t)b * a.vs_b + j * a.vs_pos;
-    if (a.pages != nullptr) {
-      int pg = a.pages[(int64_t)b * a.max_pages + (j >> a.page_shift)];
-      pg = min(max(pg, 0), a.num_pages - 1);
-      const int64_t in = j & ((1 << a.page_shift) - 1);
-      ko = pg * a.ks_b + in * a.ks_pos;
-      vo = pg * a.vs_b + in * a.vs_pos;
-    }
-    const T* k = (const T*)a.k + ko + (int64_t)kvh * a.ks_h;
-    const T* v = (const T*)a.v + vo + (int64_t)kvh * a.vs_h;
-    float s = 0.f;
-    for (int d = 0; d < a.key_dim; ++d) s = fmaf(to_f32(q[d]), to_f32(k[d]), s);
-    s *= a.scale_log2;
-    const float M = fmaxf(m, s);
-    const float c = weight(m, M), p = fast_exp2(s - M);
-    l = l * c + p;
-    m = M;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const float x = d0 + i < a.value_dim ? to_f32(v[d0 + i]) : 0.f;
-      const float kept = finite(o[i]) ? o[i] * c : o[i];
-      o[i] = kept + (finite(x) ? p * x : x);
-    }
   }
 }
 
@@ -1104,28 +1162,9 @@ __global__ void __launch_bounds__(256) tree_join(TreeArgs a) {
   bool bad = whole;
 #pragma unroll
   for (int i = 0; i < 4; ++i) bad |= node < count && !(finite(r[i]) && finite(l));
-  if (__syncthreads_or(bad)) {
-    __syncthreads();  // the segments' sums in LDS are read
-    float x[32];
-    rows_apart<T>(a, b, kvh, 32 * cg + (threadIdx.x & 31), 32 * mb, P, end, x, m, l);
-#pragma unroll
-    for (int i = 0; i < 32; ++i) part[i * 256 + threadIdx.x] = x[i];
-    part[32 * 256 + threadIdx.x] = m;
-    part[33 * 256 + threadIdx.x] = l;
-    __syncthreads();
-    M = -INFINITY;
-    for (int g = 0; g < 8; ++g) M = fmaxf(M, part[32 * 256 + 32 * g + hl]);
-    l = 0.f;
-    for (int i = 0; i < 4; ++i) r[i] = 0.f;
-    for (int g = 0; g < 8; ++g) {
-      const float c = weight(part[32 * 256 + 32 * g + hl], M);
-      l += part[33 * 256 + 32 * g + hl] * c;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float y = part[(8 * w + 4 * half + i) * 256 + 32 * g + hl];
-        r[i] += finite(y) ? y * c : y;
-      }
-    }
+  if (__syncthreads_or(bad)) {  // (a barrier: the segments' sums in LDS are read)
+    sort_out<T>(a, b, kvh, cg, mb, P, end, part);
+    return;
   }
   if (node >= a.nodes) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -1140,6 +1179,7 @@ constexpr int kCus = 256;
 
 struct Kernel {
   const void* fn;
+  const void* alone;  // the same with a slot per sequence, or null
   const void* join;
   int threads;
   int cols;     // columns per block
@@ -1150,7 +1190,9 @@ struct Kernel {
 
 template <typename S, bool DMA>
 Kernel make() {
-  return {(const void*)tree_kernel<S, DMA>, (const void*)tree_join<typename S::T, S::DP>,
+  const void* alone = nullptr;
+  if constexpr (S::WC == 16 && DMA) alone = (const void*)tree_kernel<S, DMA, true>;
+  return {(const void*)tree_kernel<S, DMA, false>, alone, (const void*)tree_join<typename S::T, S::DP>,
           64 * S::NW, S::kCols, S::BK, S::DP, S::kPerCu};
 }
 
@@ -1201,14 +1243,26 @@ Kernel pick(int width, int cols, bool dma, bool few) {
   }
 }
 
+// Narrow calls run as one launch, a slot per sequence and nothing to join,
+// while a sequence's K is short: the shares of the rows and the second launch
+// cost 4 to 5 us, which a few tiles that follow each other do not (8 drafts,
+// 32/8 heads, two launches -> one: bf16, 128 wide, 136 rows 11.4 -> 8.7 us
+// and 520 rows 12.3 -> 13.6; float32, 64 wide, 136 rows 10.5 -> 8.9 and 264
+// rows 10.8 -> 12.4).  Where every CU has a sequence anyway, splitting one
+// gains nothing for four times as many rows (32 sequences: bf16, 128 wide, 520
+// rows 22.8 -> 18.3 us); beyond that a single long sequence among short ones
+// would hold the call up.
+constexpr int64_t kAloneBytes = 48 * 1024;
+
 struct TreePlan {
   Kernel kernel;
   int col_tiles, slots;
+  bool alone;
   size_t segments, part_o, bytes;  // floats of O, bytes in all
 };
 
 TreePlan tree_plan(int batch, int nodes, int q_heads, int kv_heads, int key_dim, int value_dim,
-                   int length, int dtype, bool dma) {
+                   int length, int dtype, bool dma, bool vec_o) {
   TreePlan p = {};
   const int width = std::max(key_dim, value_dim);
   const int cols = nodes * (q_heads / kv_heads);
@@ -1217,10 +1271,19 @@ TreePlan tree_plan(int batch, int nodes, int q_heads, int kv_heads, int key_dim,
              : dtype == ALPX_F16 ? pick<f16_t>(width, cols, dma, few)
                                  : pick<bf16_t>(width, cols, dma, few);
   p.col_tiles = (cols + p.kernel.cols - 1) / p.kernel.cols;
+  const bool direct = vec_o && value_dim == p.kernel.width;
   // one round of blocks, every slot at least a tile
   const int64_t tiles = (int64_t)batch * ((length + p.kernel.rows - 1) / p.kernel.rows);
   const int64_t share = kCus * p.kernel.per_cu / ((int64_t)kv_heads * p.col_tiles);
   p.slots = (int)std::min(std::max<int64_t>(share, 1), tiles);
+  const bool all_busy = (int64_t)batch * kv_heads * p.col_tiles >= kCus;
+  p.alone = direct && p.kernel.alone &&
+            (int64_t)length * p.kernel.width * (int64_t)dtype_size(dtype) <=
+                (all_busy ? 4 : 1) * kAloneBytes;
+  if (p.alone) {
+    p.slots = batch;
+    return p;
+  }
   p.segments = (size_t)(p.slots + batch) * kv_heads * p.col_tiles * (p.kernel.cols / 32);
   p.part_o = p.segments * 32 * p.kernel.width;
   p.bytes = p.part_o * 4 + p.segments * 32 * sizeof(float2) + (size_t)batch * sizeof(int4);
@@ -1252,6 +1315,11 @@ int tree_launch(const char* what, TreeArgs a, int dtype, void* workspace, size_t
   const int64_t es = (int64_t)dtype_size(dtype), os = (int64_t)dtype_size(a.out_dtype);
   if ((int64_t)a.nodes * a.group > (1 << 24))
     return fail(ALPX_EUNSUPPORTED, "%s: too many drafts", what);
+  if (a.ks_pos < 0 || a.ks_b < 0 || a.ks_h < 0 || a.vs_pos < 0 || a.vs_b < 0 || a.vs_h < 0)
+    return fail(ALPX_EINVAL, "%s: strides must not be negative", what);
+  // (sums of tiles and of rows past the end stay in 31 bits)
+  if (a.length > (1 << 30) || (int64_t)a.batch * ((int64_t)a.length / 32 + 1) >= ((int64_t)1 << 31))
+    return fail(ALPX_EUNSUPPORTED, "%s: too many rows", what);
   if (32 * std::max(a.ks_pos, a.vs_pos) * es >= ((int64_t)1 << 31))
     return fail(ALPX_EUNSUPPORTED, "%s: rows too far apart", what);
   const uintptr_t rows = (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)(a.ks_pos * es) |
@@ -1263,11 +1331,19 @@ int tree_launch(const char* what, TreeArgs a, int dtype, void* workspace, size_t
   a.vec_q = (((uintptr_t)a.q | (uintptr_t)(a.key_dim * es)) & 15) == 0;
   a.vec_o = a.value_dim % 4 == 0 && ((uintptr_t)a.out & (4 * os - 1)) == 0 &&
             ((uintptr_t)a.gate & (4 * es - 1)) == 0;
+  // rows of values that are not finite read q and gate after others wrote out
+  const int64_t cells = (int64_t)a.batch * a.nodes * a.q_heads;
+  const uintptr_t out = (uintptr_t)a.out, out_end = out + (uintptr_t)(cells * a.value_dim * os);
+  auto meets_out = [&](const void* x, int64_t width) {
+    return x && (uintptr_t)x < out_end && out < (uintptr_t)x + (uintptr_t)(cells * width * es);
+  };
+  if (meets_out(a.q, a.key_dim) || meets_out(a.gate, a.value_dim))
+    return fail(ALPX_EINVAL, "%s: out must not overlap q or gate", what);
   const TreePlan p = tree_plan(a.batch, a.nodes, a.q_heads, a.kv_heads, a.key_dim, a.value_dim,
-                               a.length, dtype, dma);
+                               a.length, dtype, dma, a.vec_o);
   if (((uintptr_t)workspace & 15) != 0)
     return fail(ALPX_EINVAL, "%s: workspace must be 16-byte aligned", what);
-  if (workspace_bytes < p.bytes || !workspace)
+  if (workspace_bytes < p.bytes || (p.bytes > 0 && !workspace))
     return fail(ALPX_EINVAL, "%s: workspace holds %zu bytes, needs %zu", what, workspace_bytes,
                 p.bytes);
   a.col_tiles = p.col_tiles;
@@ -1286,8 +1362,9 @@ int tree_launch(const char* what, TreeArgs a, int dtype, void* workspace, size_t
   void* args[] = {&a};
   {
     TimedRegion timed(ALPX_T_DECODE, s);
-    (void)hipLaunchKernel(p.kernel.fn, dim3((unsigned)blocks), dim3(p.kernel.threads), args, 0, s);
+    (void)hipLaunchKernel(p.alone ? p.kernel.alone : p.kernel.fn, dim3((unsigned)blocks), dim3(p.kernel.threads), args, 0, s);
   }
+  if (p.alone) return check_launch(what);
   a.col_tiles = groups;
   TimedRegion timed(ALPX_T_DECODE_COMBINE, s);
   (void)hipLaunchKernel(p.kernel.join, dim3((unsigned)joins), dim3(256), args, 0, s);
@@ -1303,10 +1380,10 @@ extern "C" size_t alpx_tree_workspace_bytes(int batch, int nodes, int q_heads, i
                                             int key_dim, int value_dim, int length, int dtype) {
   if (!tree_sizes_ok(batch, nodes, q_heads, kv_heads, key_dim, value_dim, length) || !dtype_ok(dtype))
     return 0;
-  size_t most = 0;
-  for (const bool dma : {false, true})
+  size_t most = 0;  // whatever the call's alignment
+  for (int i = 0; i < 4; ++i)
     most = std::max(most, tree_plan(batch, nodes, q_heads, kv_heads, key_dim, value_dim, length,
-                                    dtype, dma).bytes);
+                                    dtype, i & 1, i & 2).bytes);
   return most;
 }
 
@@ -1314,8 +1391,9 @@ extern "C" int alpx_tree_attention(const void* q, const void* key_cache, const v
                                    const uint64_t* masks, int64_t mask_batch_stride,
                                    int mask_words, const int32_t* prefix_lens,
                                    const int32_t* counts, int length, const void* gate, void* out,
-                                   void* workspace, size_t workspace_bytes, int batch, int nodes, int q_heads, int kv_heads, int key_dim,
-                                   int value_dim, int64_t k_pos_stride, int64_t k_batch_stride,
+                                   void* workspace, size_t workspace_bytes, int batch, int nodes,
+                                   int q_heads, int kv_heads, int key_dim, int value_dim,
+                                   int64_t k_pos_stride, int64_t k_batch_stride,
                                    int64_t k_head_stride, int64_t v_pos_stride,
                                    int64_t v_batch_stride, int64_t v_head_stride, float scale,
                                    int dtype, int out_dtype, void* stream) {

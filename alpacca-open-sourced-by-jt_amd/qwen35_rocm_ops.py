@@ -1208,6 +1208,8 @@ class Qwen35RocmOps:
                 and value.get_device() == self.device_index and value.is_contiguous()):
             return value
         if not torch.is_tensor(value) or value.device.type != "cuda":
+            if len(shape) != 1:
+                raise TypeError(f"{name} must remain on the ROCm device")
             host = [int(v) for v in value]
             if (len(host),) != tuple(shape) or any(
                     (low is not None and v < low) or (high is not None and v > high)
@@ -1297,7 +1299,8 @@ class Qwen35RocmOps:
         ``masks [B or 1, N, words]`` (``tree_masks``).  Drafts at or past
         ``counts[b]``, and drafts that see no row, give zeros.  ``length``
         bounds every sequence's rows, drafts included; device lengths past it
-        are clamped.  Returns ``[B, N, Hq, Dv]``."""
+        are clamped.  ``out`` must not overlap an input.  Returns
+        ``[B, N, Hq, Dv]``."""
         key_cache = self._tensor(key_cache, "attention key cache", dimensions=4)
         value_cache = self._tensor(value_cache, "attention value cache", dimensions=4)
         capacity, batch, kv_heads, _ = _shape(key_cache)

@@ -698,7 +698,8 @@ int alpx_recurrent_prefill_prep(const float* current, const float* conv_weight,
  * for their product, the sums are not).
  * workspace: alpx_tree_workspace_bytes bytes (0 for sizes that the calls
  * refuse), 16-byte aligned; scratch, which calls that may overlap must not
- * share.  Two launches.
+ * share.  out must not overlap any input.  One launch for few drafts on few
+ * rows, otherwise two.
  */
 size_t alpx_tree_workspace_bytes(int batch, int nodes, int q_heads, int kv_heads, int key_dim,
                                  int value_dim, int length, int dtype);

@@ -225,6 +225,24 @@ def test_infinities_and_nan_stay_with_the_drafts_that_see_them(gpu, ops, dtype, 
     case.check(case.call(ops))
 
 
+@pytest.mark.parametrize("spare", [0, 100, 2000])
+@pytest.mark.parametrize("batch", [3, 70])
+@pytest.mark.parametrize("dtype,d,nodes", [("f32", 64, 8), ("f32", 128, 3), ("f32", 256, 9),
+                                           ("f16", 64, 16), ("bf16", 128, 16), ("bf16", 256, 30)])
+def test_short_sequences_in_short_and_long_caches(gpu, ops, dtype, d, nodes, batch, spare):
+    # a block per sequence, or shares of the rows and a join; empty sequences,
+    # some with values that are not finite
+    rng = np.random.default_rng(d + batch)
+    prefix, counts = rng.integers(0, 40, batch), rng.integers(0, nodes + 1, batch)
+    prefix[1], counts[1] = 0, 0
+    prefix[2], counts[2] = 40, nodes
+    case = Case(gpu, 21, dtype=dtype, d=d, hq=8, hkv=4, nodes=nodes, prefix=prefix.tolist(),
+                counts=counts.tolist(), spare=spare, gate=True)
+    case.v[41, 2, 1, 3], case.v[40 + nodes - 1, 2, 3, d - 1] = np.inf, np.nan
+    case.k[42, 2, 2, 0] = np.nan
+    case.check(case.call(ops))
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_an_infinity_in_the_prefix_reaches_every_draft(gpu, ops, dtype):
     case = Case(gpu, 12, dtype=dtype, d=64, hq=4, hkv=2, nodes=9, prefix=[1500])
