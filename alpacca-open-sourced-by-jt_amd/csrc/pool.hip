@@ -6,6 +6,7 @@
 
 #include "alpx_common.h"
 #include "timing.h"
+#include "wave_scan.h"
 
 namespace alpx {
 namespace {
@@ -49,11 +50,7 @@ template <int NT>
 __device__ __forceinline__ int64_t block_scan(int64_t x, int64_t (*part)[kThreads / 64], int& turn,
                                               int64_t& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int64_t y = __shfl_up(x, off);
-    if (lane >= off) x += y;
-  }
+  x = wave_inclusive(x);
   int64_t* p = part[turn];
   turn ^= 1;
   if (lane == 63) p[wave] = x;

@@ -22,6 +22,7 @@
 #include "alpx_common.h"
 #include "prefill_run.h"
 #include "timing.h"
+#include "wave_scan.h"
 
 namespace alpx {
 namespace {
@@ -121,24 +122,6 @@ struct Share {
   int per;     // tiles per slot
 };
 constexpr int kTurnOver = 4;
-
-__device__ __forceinline__ int wave_total(int x) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) x += __shfl_xor(x, off);
-  return __builtin_amdgcn_readfirstlane(x);
-}
-
-// Exclusive sums over the lanes.
-__device__ __forceinline__ int wave_before(int x) {
-  const int lane = threadIdx.x & 63;
-  int y = x;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int z = __shfl_up(y, off);
-    if (lane >= off) y += z;
-  }
-  return y - x;
-}
 
 __device__ __forceinline__ int div_up(int x, int y) {
   return (int)(((unsigned)x + (unsigned)y - 1u) / (unsigned)y);
