@@ -661,8 +661,9 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
       if constexpr (S::kPipe) {
         // Turn t: PV of tile t - 1, the softmax of tile t and QK of tile
         // t + 1, so that the products run beside the exponentials of the same
-        // wave, while K of tile t + 2 and V of tile t are on their way.  K
-        // tiles at 0 and kTileB, V tiles at 2 and 3 kTileB.
+        // wave, while K of tile t + 2 and V of tile t are on their way.  The
+        // first turn has no PV, the last one (turn nt) nothing else.  K tiles
+        // at 0 and kTileB, V tiles at 2 and 3 kTileB.
         typedef typename Vec8<T>::type V8;
         typedef typename Vec4<T>::type V4;
         constexpr int KR = S::KR, NV = 2 * KR * NB, NK = KR * NQ, NE = 16 * KR;
@@ -691,12 +692,6 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
           const V4 x0 = lds_read_tr4((const T*)p), x1 = lds_read_tr4((const T*)(p + 8 * kRowB));
           return __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
         };
-        // V 1 and P are zeros for the product of turn 0
-#pragma unroll
-        for (int i = 0; i < S::kIW; ++i)
-          *(u32x4*)(smem + 3 * kTileB + ((wave * S::kIW + i) * 64 + lane) * 16) = (u32x4){};
-#pragma unroll
-        for (int i = 0; i < 2 * KR; ++i) pv[i] = (V8){};
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
 #pragma unroll
@@ -706,12 +701,20 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
           for (int j = 0; j < NQ; ++j) sc[kr] = mfma32x32x16(k_operand(0, kr, j), qv[j], sc[kr]);
         }
         __syncthreads();  // K 0 is read before turn 0 refills it
-        auto turn = [&](auto parity, int t) __attribute__((always_inline)) {
-          constexpr int Q = decltype(parity)::value;  // t & 1
+        auto turn = [&](auto parity, auto place, int t) __attribute__((always_inline)) {
+          constexpr int Q = decltype(parity)::value;  // t & 1, but for the last
+          constexpr bool FIRST = decltype(place)::value == 0, LAST = decltype(place)::value == 2;
+          // the other place of each pair: tile t - 1 of V, tile t + 1 of K
+          const int behind = LAST ? ((nt & 1) ^ 1) * kTileB : (Q ^ 1) * kTileB;
           // the turn's loads (past the last tile they fetch nothing and write
           // zeros where nothing is read): spread over the steps, since a wave
           // that issues them in one go waits for the address unit meanwhile
-          const Source sk = source(t + 2), sv = source(t);
+          constexpr int NL = LAST ? 0 : S::kTileLoads;
+          Source sk, sv;
+          if constexpr (!LAST) {
+            sk = source(t + 2);
+            sv = source(t);
+          }
           auto load = [&](int i) __attribute__((always_inline)) {
             if (i < S::kIW)
               load_v(sv, i, (2 + Q) * kTileB);
@@ -720,7 +723,7 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
           };
           if (idle) {
 #pragma unroll
-            for (int i = 0; i < S::kTileLoads; ++i) load(i);
+            for (int i = 0; i < NL; ++i) load(i);
           } else {
             // O holds tiles up to t - 2 and is about to take P of tile t - 1,
             // formed against the reference that moved there
@@ -731,9 +734,7 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
               pend_any = false;
             }
             const int key0 = start + t * BK;
-            // not all of these keys are prefix rows, or turn nt, whose scores
-            // are of no tile
-            if (key0 + BK > min(P, stop)) {
+            if (!LAST && key0 + BK > P) {  // not all of these keys are prefix rows
 #pragma unroll
               for (int kr = 0; kr < KR; ++kr) {
                 const uint32_t mine =
@@ -746,83 +747,95 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
                 }
               }
             }
-            float mx = sc[0][0];
+            if constexpr (!LAST) {
+              float mx = sc[0][0];
 #pragma unroll
-            for (int r = 1; r < NE; ++r) mx = fmaxf(mx, sc[r / 16][r % 16]);
-            mx *= a.scale_log2;
-            if (__builtin_expect(__ballot(mx > m + kRescale) != 0, 0)) {
-              mx = fmaxf(mx, __shfl_xor(mx, 32));
-              if (mx > m + kRescale) {
-                pend = fast_exp2(m - mx);
-                l *= pend;
-                m = mx;
+              for (int r = 1; r < NE; ++r) mx = fmaxf(mx, sc[r / 16][r % 16]);
+              mx *= a.scale_log2;
+              if (__builtin_expect(__ballot(mx > m + kRescale) != 0, 0)) {
+                mx = fmaxf(mx, __shfl_xor(mx, 32));
+                if (mx > m + kRescale) {
+                  pend = fast_exp2(m - mx);
+                  l *= pend;
+                  m = mx;
+                }
+                pend_any = true;
               }
-              pend_any = true;
             }
             const float off = m == -INFINITY ? 0.f : m;
             __builtin_amdgcn_sched_barrier(0);
             __builtin_amdgcn_s_setprio(1);
             float ps = 0.f;
             V8 pn[2 * KR];
-            // Step i: product i of NV + NK and its share of the exponentials,
+            auto probability = [&](auto e_) __attribute__((always_inline)) {
+              constexpr int e = decltype(e_)::value;
+              const float p = fast_exp2(fmaf(sc[e / 16][e % 16], a.scale_log2, -off));
+              ps += p;
+              pn[e / 8][e % 8] = from_f32<T>(p);
+            };
+            if constexpr (FIRST) static_for<0, NE>(probability);
+            // Step i: product i of NP + NS and its share of the exponentials,
             // all of them before their registers take tile t + 1's scores.
             // Operands are read AHEAD steps before their product; the order
             // is kept as written (left to itself the scheduler reads each
             // operand right before its product and waits for it).
-            constexpr int N = NV + NK, LAST = NV + (KR - 1) * NQ, AHEAD = 4;
+            constexpr int NP = FIRST ? 0 : NV, N = NP + (LAST ? 0 : NK), AHEAD = 4;
+            constexpr int BY = NP + (KR - 1) * NQ;  // the exponentials' last step
             u32x4 opd[N];
             auto read = [&](auto i_) __attribute__((always_inline)) {
               constexpr int i = decltype(i_)::value;
-              if constexpr (i < NV)
-                opd[i] = __builtin_bit_cast(u32x4, v_operand((Q ^ 1) * kTileB, i / NB, i % NB));
+              if constexpr (i < NP)
+                opd[i] = __builtin_bit_cast(u32x4, v_operand(behind, i / NB, i % NB));
               else
                 opd[i] = __builtin_bit_cast(
-                    u32x4, k_operand((Q ^ 1) * kTileB, (i - NV) / NQ, (i - NV) % NQ));
+                    u32x4, k_operand(behind, (i - NP) / NQ, (i - NP) % NQ));
             };
             static_for<0, AHEAD>(read);
             static_for<0, N>([&](auto i_) __attribute__((always_inline)) {
               constexpr int i = decltype(i_)::value;
               if constexpr (i + AHEAD < N) read(Par<i + AHEAD>());
               const V8 x = __builtin_bit_cast(V8, opd[i]);
-              if constexpr (i < NV) {
+              if constexpr (i < NP) {
                 o[i % NB] = mfma32x32x16(x, pv[i / NB], o[i % NB]);
               } else {
-                constexpr int kr = (i - NV) / NQ, j = (i - NV) % NQ;
+                constexpr int kr = (i - NP) / NQ, j = (i - NP) % NQ;
                 if constexpr (j == 0)
                   sc[kr] = mfma32x32x16(x, qv[j], (Acc)(0.f));
                 else
                   sc[kr] = mfma32x32x16(x, qv[j], sc[kr]);
               }
               // loads first, in the steps' first three quarters
-              constexpr int d0 = i * S::kTileLoads * 4 / (3 * N), d1 = (i + 1) * S::kTileLoads * 4 / (3 * N);
-              if constexpr (d1 > d0 && d0 < S::kTileLoads) load(d0);
-              constexpr int e0 = i < LAST ? i * NE / LAST : NE;
-              constexpr int e1 = i + 1 < LAST ? (i + 1) * NE / LAST : NE;
-              static_for<e0, e1>([&](auto e_) __attribute__((always_inline)) {
-                constexpr int e = decltype(e_)::value;
-                const float p = fast_exp2(fmaf(sc[e / 16][e % 16], a.scale_log2, -off));
-                ps += p;
-                pn[e / 8][e % 8] = from_f32<T>(p);
-              });
+              constexpr int d0 = i * NL * 4 / (3 * N), d1 = (i + 1) * NL * 4 / (3 * N);
+              static_for<(d0 < NL ? d0 : NL), (d1 < NL ? d1 : NL)>(
+                  [&](auto d_) __attribute__((always_inline)) { load(decltype(d_)::value); });
+              if constexpr (!FIRST && !LAST)
+                static_for<(i < BY ? i * NE / BY : NE), (i + 1 < BY ? (i + 1) * NE / BY : NE)>(
+                    probability);
               __builtin_amdgcn_sched_barrier(0);
             });
             __builtin_amdgcn_s_setprio(0);
             __builtin_amdgcn_sched_barrier(0);
-            l += ps;
+            if constexpr (!LAST) {
+              l += ps;
 #pragma unroll
-            for (int i = 0; i < 2 * KR; ++i) {
-              pv[i] = pn[i];
-              pin(pv[i]);
+              for (int i = 0; i < 2 * KR; ++i) {
+                pv[i] = pn[i];
+                pin(pv[i]);
+              }
             }
           }
-          __builtin_amdgcn_s_waitcnt(0);
-          __syncthreads();
+          if constexpr (!LAST) {
+            __builtin_amdgcn_s_waitcnt(0);
+            __syncthreads();
+          }
         };
+        turn(Par<0>(), Par<0>(), 0);
 #pragma clang loop unroll(disable)
-        for (int t = 0; t <= nt; t += 2) {
-          turn(Par<0>(), t);
-          if (t + 1 <= nt) turn(Par<1>(), t + 1);
+        for (int t = 1; t < nt; t += 2) {
+          turn(Par<1>(), Par<1>(), t);
+          if (t + 1 < nt) turn(Par<0>(), Par<1>(), t + 1);
         }
+        turn(Par<0>(), Par<2>(), nt);
       } else {
         wait_tiles<(S::RING - 2) * S::kTileLoads * DMA>();  // the first tile is in LDS
         __syncthreads();
