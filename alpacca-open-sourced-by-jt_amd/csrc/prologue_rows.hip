@@ -68,7 +68,10 @@ __device__ __forceinline__ void store8(T* p, const Row8<T>& r) {
 // One token per block row, D / 8 lanes per head row, eight channels per
 // lane; grid y shares out a token's rows (query heads, key heads, value
 // heads, in this order).  Dv = D, R a multiple of 8: the partner of a
-// rotated channel lies R / 8 lanes away.
+// rotated channel lies R / 8 lanes away.  Bound by memory: 4133 tokens of
+// 16/2 heads of 256 in bf16, 152 MB, 25.8 us = 5.9 TB/s (a copy of 1 GiB ran
+// at 5.2; part of these outputs stays in cache).  8 tokens of 32/8 heads of
+// 64, float32: 4.5 us, the latency of the angles and of one row.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) prologue_rows_kernel(RowsProArgs a) {
   constexpr int kLanes = D / 8, kRows = kThreads / kLanes;

@@ -11,10 +11,17 @@
 // The drafts of one sequence read the same rows, so a block takes columns =
 // (draft, query head of one kv head) pairs, up to 128 of them, against one
 // stream of K and V tiles: the cache is read once for all of them.  S^T =
-// K Q^T and O^T = V^T P^T on 32 x 32 MFMA tiles: a lane owns one column
-// (lane % 32), keys lie in its registers, so its mask is one word per 32
-// keys, the softmax needs one exchange with the lane 32 away, and P feeds
-// the second product from the registers the first one wrote.
+// K Q^T and O^T = V^T P^T on MFMA tiles of 16 or 32 columns: a lane owns one
+// column, keys lie in its registers, so its mask is one word per 32 keys,
+// the softmax needs one or two exchanges with the other lanes of the column,
+// and P feeds the second product from the registers the first one wrote.
+//
+// Few columns are bound by the rows' way from memory (16 sequences of 16
+// drafts on 8192 rows, 32/8 heads of 128, fp16: 78 us = 6.9 TB/s in the
+// loop, 90 with both ends of the launch, 7 more for the join), many by the
+// products and what they read from LDS (4 of 64 on 32768 rows, 16/2 heads of
+// 256, bf16: 165 us = 830 TFLOP/s, join 10), short ones by latency (8 on 508
+// rows, float32: 7.0 + 4.4 us).
 #include <math.h>
 
 #include <algorithm>

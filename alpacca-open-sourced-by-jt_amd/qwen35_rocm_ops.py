@@ -1258,6 +1258,8 @@ class Qwen35RocmOps:
         value_width = int(value_cache.shape[3])
         if length > capacity:
             raise ValueError("attention cache length exceeds capacity")
+        if length >= 2 ** 31:
+            raise ValueError("attention cache length exceeds 2^31 rows")
         if query_batch != batch or width != key_width:
             raise ValueError("attention query does not match K cache batch/head width")
         if nodes <= 0:
@@ -1395,10 +1397,13 @@ class Qwen35RocmOps:
         size = _positive_integer("page_size", page_size)
         if size & (size - 1):
             raise ValueError("page_size must be a power of two")
+        if size * max(max_pages, free_pages.numel()) >= 2 ** 31:
+            raise ValueError("a page pool or block table holds less than 2^31 rows")
+        if _nonnegative_integer("tokens", tokens) >= 2 ** 31:
+            raise ValueError("tokens must be less than 2^31")
         targets = self._device_ints(targets, "targets", (batch,), low=0, high=max_pages * size)
         return RocmPagedRows(*_ops.paged_resize(block_table, lengths, free_pages, free_count,
-                                                targets, page_size=size,
-                                                tokens=_nonnegative_integer("tokens", tokens)))
+                                                targets, page_size=size, tokens=tokens))
 
     def paged_attention_prologue_rows_(self, query_gate: Any, key: Any, value: Any,
                                        query_norm: Any, key_norm: Any, key_pages: Any,

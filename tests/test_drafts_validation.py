@@ -258,6 +258,28 @@ def test_facade_tree_attention_refusals(ops, paged):
             _attend(ops, paged, **changes)
 
 
+def test_facade_refuses_numbers_past_32_bits(ops, monkeypatch):
+    # a C int would take the low 32 bits of them
+    wide = torch.zeros(1, dtype=torch.int32).expand(2, 2 ** 28)
+    monkeypatch.setattr(ops, "_paged", lambda keys, values, table: (keys, values))
+    with pytest.raises(ValueError, match="2\\^31"):
+        _attend(ops, True, length=2 ** 32 + 5, block_table=wide)
+    # (only the checks of host tensors stand between the call and its sizes)
+    monkeypatch.setattr(ops, "_device_ints", lambda value, *a, **k: value)
+
+    class OnDevice(torch.Tensor):
+        is_cuda = True
+
+    def ints(*shape):
+        return _i32(*shape).as_subclass(OnDevice)
+    for kw in (dict(page_size=2 ** 32, tokens=2), dict(page_size=2 ** 30, tokens=2),
+               dict(page_size=32, tokens=2 ** 32 + 2)):
+        with pytest.raises(ValueError, match="2\\^31"):
+            ops.paged_resize_(ints(2, 2), ints(2), ints(4), ints(1), ints(2), **kw)
+    with pytest.raises(AssertionError, match="passed"):
+        ops.paged_resize_(ints(2, 2), ints(2), ints(4), ints(1), ints(2), page_size=32, tokens=2)
+
+
 def test_facade_masks_commit_and_resize_refusals(ops):
     with pytest.raises(ValueError, match=r"\[batch, nodes\]"):
         ops.tree_masks([[-1, 0]])
