@@ -1209,6 +1209,16 @@ Kernel make() {
 // float32: where tiles of 128 rows are fewer than CUs, tiles of 32 rows give
 // more of them one (8 drafts on 508 rows, 32/8 heads of 64 / 128: 12.2 ->
 // 9.3 / 13.6 -> 11.2 us; 4 x 8 on 8192 rows 31 -> 33 / 59 -> 64).
+//
+// 16 bits, 64 wide: tiles of 128 rows, which halves the barriers (8 x 16
+// drafts on 65536 rows 223 -> 199 us, 16 x 8 on 1000 rows 16.1 -> 14.9), and
+// two of them rather than four, which leaves LDS for a second block (four: 187
+// and 15.4, but 128 x 8 on 264 rows 22 -> 34).  256 wide: 64 columns take 64
+// rows by two waves a column rather than 32 by one (4 x 8 drafts on 32768 rows
+// 63 -> 57 us); 128 columns have waves enough.  float32, 256 wide: four waves
+// have the registers of eight, 32 columns 180 -> 122 us (4 x 4 drafts on 8192
+// rows), 64 columns 238 -> 189 (4 x 16); 64 wide, 64 columns: room for a second
+// block 62.3 -> 59.2 (4 x 16 on 8192).
 template <typename T>
 Kernel pick(int width, int cols, bool dma, bool few) {
   if constexpr (sizeof(T) == 4) {
@@ -1216,7 +1226,7 @@ Kernel pick(int width, int cols, bool dma, bool few) {
       if (!dma) return make<Shape<T, 64, 16, 4, 2, 64, 2>, false>();
       if (cols <= 32 && few) return make<Shape<T, 64, 16, 2, 2, 32, 4>, true>();
       return cols <= 32   ? make<Shape<T, 64, 16, 2, 4, 128, 2>, true>()
-             : cols <= 64 ? make<Shape<T, 64, 16, 4, 2, 64, 4>, true>()
+             : cols <= 64 ? make<Shape<T, 64, 16, 4, 2, 64, 2>, true>()
                           : make<Shape<T, 64, 32, 4, 1, 32, 2>, true>();
     }
     if (width <= 128) {
@@ -1227,12 +1237,13 @@ Kernel pick(int width, int cols, bool dma, bool few) {
                           : make<Shape<T, 128, 32, 4, 1, 32, 2>, true>();
     }
     if (!dma) return make<Shape<T, 256, 16, 4, 2, 32, 2>, false>();
-    return cols <= 64 ? make<Shape<T, 256, 16, 4, 2, 32, 2>, true>()
-                      : make<Shape<T, 256, 32, 4, 1, 32, 2>, true>();
+    return cols <= 32   ? make<Shape<T, 256, 16, 2, 2, 32, 2>, true>()
+           : cols <= 64 ? make<Shape<T, 256, 16, 4, 1, 32, 2>, true>()
+                        : make<Shape<T, 256, 32, 4, 1, 32, 2>, true>();
   } else {
     if (width <= 64) {
       if (!dma) return make<Shape<T, 64, 16, 4, 2, 64, 2>, false>();
-      return cols <= 64 ? make<Shape<T, 64, 16, 4, 2, 64, 4>, true>()
+      return cols <= 64 ? make<Shape<T, 64, 16, 4, 2, 128, 2>, true>()
                         : make<Shape<T, 64, 32, 4, 1, 64, 2>, true>();
     }
     if (width <= 128) {
@@ -1241,8 +1252,9 @@ Kernel pick(int width, int cols, bool dma, bool few) {
                         : make<Shape<T, 128, 32, 4, 1, 64, 2>, true>();
     }
     if (!dma) return make<Shape<T, 256, 16, 8, 1, 32, 2>, false>();
-    return cols <= 128 ? make<Shape<T, 256, 16, 8, 1, 32, 4>, true>()
-                       : make<Shape<T, 256, 32, 4, 1, 64, 2>, true>();
+    return cols <= 64    ? make<Shape<T, 256, 16, 4, 2, 64, 2>, true>()
+           : cols <= 128 ? make<Shape<T, 256, 16, 8, 1, 32, 4>, true>()
+                         : make<Shape<T, 256, 32, 4, 1, 64, 2>, true>();
   }
 }
 
