@@ -25,6 +25,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "alpx_common.h"
 #include "prefill_run.h"
@@ -253,6 +254,12 @@ struct Shape {
   // The wide 16-bit kernels run the products of two tiles beside the softmax
   // of a third (see the loop).
   static constexpr bool kPipe = WC == 32 && sizeof(T) == 2 && RING == 2;
+  // fp16 probabilities are formed 2^kLift times as large as their reference
+  // says (the sums too, so it cancels): with kRescale they stay below 2^15, and
+  // weights down to 2^-21 of the largest, not 2^-14, keep all their bits.  Many
+  // rows of small weight beside a large one are what a first row that every
+  // draft attends to leaves.
+  static constexpr float kLift = std::is_same<T, f16_t>::value ? 7.f : 0.f;
   // The narrow kernels have one column tile: nobody reads a tile twice.
   // (The hint on K and V / on V / on neither, 16 x 16 drafts on 8192 rows:
   // 97 / 86 / 103 us.)
@@ -769,7 +776,7 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
                 pend_any = true;
               }
             }
-            const float off = m == -INFINITY ? 0.f : m;
+            const float off = m == -INFINITY ? 0.f : m - S::kLift;
             __builtin_amdgcn_sched_barrier(0);
             __builtin_amdgcn_s_setprio(1);
             float ps = 0.f;
@@ -907,7 +914,7 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
                 m = mx;
               }
             }
-            const float off = m == -INFINITY ? 0.f : m;
+            const float off = m == -INFINITY ? 0.f : m - S::kLift;
             float ps = 0.f;
 #pragma unroll
             for (int kr = 0; kr < S::KR; ++kr) {

@@ -261,6 +261,37 @@ def test_scores_of_large_spread(gpu, ops):
     assert (np.abs(got - want) <= 1e-4 + 2.0 ** -24 * 8 * 300 * 8 * weight).all()
 
 
+@pytest.mark.parametrize("gap", [7.0, 11.0, 15.0])
+@pytest.mark.parametrize("dtype,d,nodes", [("f16", 64, 4), ("f16", 128, 4), ("f16", 256, 4),
+                                           ("f16", 64, 70), ("f16", 128, 70), ("f16", 256, 70),
+                                           ("f16", 256, 130), ("bf16", 128, 4), ("bf16", 128, 70)])
+def test_many_small_weights_beside_a_large_one(gpu, ops, dtype, d, nodes, gap):
+    # the first row's score lies `gap` above all others, whose values alone
+    # are seen in the output: their weights are e^-gap of the largest, below
+    # fp16's smallest normal number for the larger gaps
+    # (more sequences and heads than the device has blocks at a time, so that
+    # most runs are whole sequences)
+    case = Case(gpu, 22, dtype=dtype, d=d, hq=8, hkv=8, nodes=nodes, prefix=[600, 500] * 20)
+    case.k *= 0.0
+    case.q = I.round_to(0.125 * case.q, dtype)
+    case.q[..., 0], case.k[0, :, :, 0] = 8.0, gap * d ** 0.5 / 8.0
+    case.k = I.round_to(case.k, dtype)
+    case.v = np.abs(case.v)
+    case.v[0] = 0.0
+    got = case.call(ops)[:2].double().cpu().numpy()
+    case.batch = 2  # the first two sequences against the oracle
+    want, weight = case.want()
+    u = _half_step(dtype)
+    # an output is a sum of positive terms: each term's and the result's
+    # rounding, float32 sums of 700 terms, and for fp16 half a step of its
+    # subnormals per row (values below 5) where the largest probability is at
+    # least 2^7, and for the output; no absolute slack, the outputs of gap 15
+    # are 1e-4
+    rows = np.array(case.rows[:2]).reshape(-1, 1, 1, 1)
+    low = rows * 2.0 ** -32 * 5 + 2.0 ** -25 if dtype == "f16" else 0.0
+    assert (np.abs(got - want) <= 2 * u * weight + 700 * 2.0 ** -24 * weight + low).all()
+
+
 @pytest.mark.parametrize("out_dtype", ["f32", "f16", "bf16"])
 def test_output_types_and_out_buffer(gpu, ops, out_dtype):
     import torch
