@@ -161,6 +161,8 @@ TREES = [
     dict(dtype="bf16", d=128, hq=8, hkv=2, nodes=16, prefix=[3000, 17, 1500]),
     dict(dtype="f16", d=256, hq=8, hkv=1, nodes=20, prefix=[2500]),
     dict(dtype="f32", d=128, hq=8, hkv=8, nodes=4, prefix=[2000, 900]),
+    # the most drafts that one tree of masks holds
+    dict(dtype="f16", d=64, hq=2, hkv=1, nodes=1024, prefix=[5, 100], counts=[1000, 1024]),
 ]
 
 
@@ -683,3 +685,41 @@ def test_a_step_of_drafts(gpu, ops, dtype, d, hq, hkv):
             for flat, rows_b in ((flat_k, state[b][0]), (flat_v, state[b][1])):
                 want = T.commit(rows_b, prefix[b], paths[b], taken[b])[:n]
                 assert np.array_equal(flat[at].float().cpu().numpy(), want)
+
+
+def test_rows_past_32_bit_offsets(gpu, ops):
+    """Caches of more than 2^31 elements: attention over all of their rows,
+    contiguous and paged, rows written and moved at their end."""
+    import torch
+    rows, heads, d, P = 300032, 64, 128, 300000
+    k, v = (torch.zeros(rows, 1, heads, d, dtype=torch.bfloat16, device=gpu) for _ in range(2))
+    assert k.numel() > 2 ** 31
+    v[P - 1], v[P], v[P + 1], v[P + 2] = 32768.0, 4096.0, 512.0, float("nan")
+    q = torch.randn(1, 2, heads, d, device=gpu).to(torch.bfloat16)
+    masks = torch.tensor([[[1], [3]]], dtype=torch.int64, device=gpu)
+    kw = dict(length=rows, prefix_lens=_ints(gpu, [P]))
+    out = ops.tree_attention(q, k, v, masks, **kw)
+    # every weight is 1: sums of whole numbers, one rounding
+    want = torch.tensor([36864 / 300001, 37376 / 300002], dtype=torch.float64)
+    off = (out[0].double().cpu() - want[:, None, None]).abs()
+    assert (off <= 2.0 ** -8 * want[:, None, None]).all()
+    kp, vp = (x.reshape(rows // 64, 64, heads, d) for x in (k, v))
+    table = torch.arange(rows // 64, dtype=torch.int32, device=gpu)[None]
+    assert torch.equal(ops.paged_tree_attention(q, kp, vp, table, masks, **kw), out)
+
+    ops.paged_tree_commit_(kp, vp, table, _ints(gpu, [[1]]), prefix_lens=_ints(gpu, [P]),
+                           accepted=_ints(gpu, [1]))
+    assert (v[P] == 512.0).all() and (v[P - 1] == 32768.0).all()
+    ops.tree_commit_(k, v, _ints(gpu, [[1]]), prefix_lens=_ints(gpu, [P - 2]),
+                     accepted=_ints(gpu, [1]))
+    assert (v[P - 2] == 32768.0).all() and not v[P - 3].any()
+
+    args = [torch.randn(2, n * d, device=gpu).to(torch.bfloat16) for n in (2 * heads, heads, heads)]
+    args += [torch.ones(d, device=gpu)] * 2
+    small = [torch.zeros(1, 2, heads, d, dtype=torch.bfloat16, device=gpu) for _ in range(2)]
+    lanes = torch.tensor([[P, P, P, 0], [7, 7, 7, 0]], dtype=torch.int64, device=gpu)
+    kw = dict(sections=(11, 11, 10, 0), frequency_base=1e7, epsilon=1e-6)
+    ops.paged_attention_prologue_rows_(*args, kp, vp, _ints(gpu, [rows - 1, 7]), lanes, **kw)
+    ops.paged_attention_prologue_rows_(*args, *small, _ints(gpu, [0, 1]), lanes, **kw)
+    for pool, rows_ in zip((k, v), small):
+        assert torch.equal(pool[rows - 1, 0], rows_[0, 0]) and torch.equal(pool[7, 0], rows_[0, 1])
