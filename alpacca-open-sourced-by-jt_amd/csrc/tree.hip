@@ -420,15 +420,16 @@ __device__ __forceinline__ void rows_apart(const TreeArgs& a, int b, int kvh, in
     float s = 0.f;
     for (int d = 0; d < a.key_dim; ++d) s = fmaf(to_f32(q[d]), to_f32(k[d]), s);
     s *= a.scale_log2;
+    const bool none = s == -INFINITY;  // no weight, also while m is -inf
     const float M = fmaxf(m, s);
-    const float c = weight(m, M), p = fast_exp2(s - M);
+    const float c = weight(m, M), p = none ? 0.f : fast_exp2(s - M);
     l = l * c + p;
     m = M;
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
       const float x = d0 + i < a.value_dim ? to_f32(v[d0 + i]) : 0.f;
       const float kept = finite(o[i]) ? o[i] * c : o[i];
-      o[i] = kept + (finite(x) ? p * x : x);
+      o[i] = kept + (finite(x) || none ? p * x : x);
     }
   }
 }

@@ -246,6 +246,26 @@ def test_short_sequences_in_short_and_long_caches(gpu, ops, dtype, d, nodes, bat
     case.check(case.call(ops))
 
 
+@pytest.mark.parametrize("spare", [0, 2000])
+@pytest.mark.parametrize("nodes", [5, 40])
+@pytest.mark.parametrize("dtype,d", [("f32", 64), ("f16", 128), ("bf16", 256), ("bf16", 48)])
+def test_rows_that_score_minus_infinity_weigh_nothing(gpu, ops, dtype, d, nodes, spare):
+    # an infinity in K makes a NaN of the queries of its sign and is nothing to
+    # the others, which share their columns' blocks: in the first row that a
+    # draft sees (of the prefix, of the drafts) and in a later one.  A weight
+    # of exactly 0 times an infinity in V is a NaN
+    case = Case(gpu, 23, dtype=dtype, d=d, hq=8, hkv=2, nodes=nodes, prefix=[20, 0, 40],
+                spare=spare)
+    case.k[0, 0, :, 1], case.k[9, 2, 0, 1] = np.inf, np.inf
+    case.k[0, 1, 0, 1], case.k[0, 1, 1, 1] = np.inf, -np.inf
+    case.q[1, 0, :4, 1], case.q[1, 0, 4:, 1] = 1.0, -1.0  # this draft sees that row alone
+    case.v[0, 0, 1, 3] = np.inf
+    want, _ = case.want()
+    for b in range(3):  # both kinds are there
+        assert 0 < np.isnan(want[b, :, :4]).all(-1).sum() < 4 * nodes
+    case.check(case.call(ops))
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_an_infinity_in_the_prefix_reaches_every_draft(gpu, ops, dtype):
     case = Case(gpu, 12, dtype=dtype, d=64, hq=4, hkv=2, nodes=9, prefix=[1500])
