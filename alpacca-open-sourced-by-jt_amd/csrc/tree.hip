@@ -420,9 +420,9 @@ __device__ __forceinline__ void rows_apart(const TreeArgs& a, int b, int kvh, in
     float s = 0.f;
     for (int d = 0; d < a.key_dim; ++d) s = fmaf(to_f32(q[d]), to_f32(k[d]), s);
     s *= a.scale_log2;
-    const bool none = s == -INFINITY;  // no weight, also while m is -inf
-    const float M = fmaxf(m, s);
-    const float c = weight(m, M), p = none ? 0.f : fast_exp2(s - M);
+    const bool none = s == -INFINITY;  // no weight; m tells that a row was seen
+    const float M = fmaxf(fmaxf(m, s), -__FLT_MAX__);
+    const float c = weight(m, M), p = fast_exp2(s - M);
     l = l * c + p;
     m = M;
 #pragma unroll
@@ -463,7 +463,8 @@ __device__ __forceinline__ void sort_out(const TreeArgs& a, int b, int kvh, int 
         r[i] += finite(y) ? y * c : y;
       }
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    // no row seen: zeros; rows that all score -inf: 0 / 0
+    const float inv = l == 0.f ? (M == -INFINITY ? 0.f : NAN) : 1.f / l;
 #pragma unroll
     for (int i = 0; i < 4; ++i) r[i] = node < end - P ? r[i] * inv : 0.f;
     const int64_t row = ((int64_t)b * a.nodes + node) * a.q_heads + kvh * G + (col - node * G);
@@ -1029,7 +1030,8 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
       float zero = 0.f;  // 0 times anything else is a NaN
 #pragma unroll
       for (int i = 0; i < 4 * NF; ++i) zero = fmaf(o[i / NA][i % NA], 0.f, zero);
-      const bool bad = __ballot(live && zero != 0.f) != 0;
+      // (a sum of 0: no row seen, or all of them at -inf)
+      const bool bad = __ballot(live && (zero != 0.f || l == 0.f)) != 0;
       if (!ALONE && sub == 0) a.part_st[seg * 32 + c32] = make_float2(bad ? 1.f : 0.f, 0.f);
       again |= bad;
       if (!in_range) return;
@@ -1170,15 +1172,15 @@ __global__ void __launch_bounds__(256) tree_join(TreeArgs a) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) r[i] += part[(v * 18 + 4 * w + i) * 64 + lane] * c;
   }
-  bool bad = whole;
+  bool bad = whole || (node < count && (!finite(l) || l == 0.f));
 #pragma unroll
-  for (int i = 0; i < 4; ++i) bad |= node < count && !(finite(r[i]) && finite(l));
+  for (int i = 0; i < 4; ++i) bad |= node < count && !finite(r[i]);
   if (__syncthreads_or(bad)) {  // (a barrier: the segments' sums in LDS are read)
     sort_out<T>(a, b, kvh, cg, mb, P, end, part);
     return;
   }
   if (node >= a.nodes) return;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = 1.f / l;  // of a column with a row; the others are zeros
   const int64_t qrow =
       ((int64_t)b * a.nodes + node) * a.q_heads + kvh * G + (col - node * G);
 #pragma unroll

@@ -691,8 +691,9 @@ int alpx_recurrent_prefill_prep(const float* current, const float* conv_weight,
  * share one tree).  prefix_lens and counts (null: `nodes` drafts each) are
  * device int32 [batch]; the sequence's rows are clamped to [0, length], and
  * nothing behind them is read.  A draft at or past counts[b], and one that
- * sees no row, yields zeros.  Infinities and NaN in rows that a draft does
- * not see stay out of its result.  Head widths up to 256 of any dtype,
+ * sees no row, yields zeros; one that sees rows which all score -inf, NaN
+ * (0 / 0).  Infinities and NaN in rows that a draft does not see stay out of
+ * its result.  Head widths up to 256 of any dtype,
  * stride and alignment; rows of 16-byte multiples run fastest.  Arithmetic
  * is fp32 (fp16 / bf16: the probabilities are rounded to the cache's type
  * for their product, the sums are not).

@@ -266,6 +266,21 @@ def test_rows_that_score_minus_infinity_weigh_nothing(gpu, ops, dtype, d, nodes,
     case.check(case.call(ops))
 
 
+@pytest.mark.parametrize("spare", [0, 2000])
+@pytest.mark.parametrize("nodes", [5, 40])
+@pytest.mark.parametrize("dtype,d", [("f32", 64), ("f16", 128), ("bf16", 256), ("bf16", 48)])
+def test_scores_that_are_all_minus_infinity_have_no_softmax(gpu, ops, dtype, d, nodes, spare):
+    # 0 / 0 is a NaN, which a draft that sees no row (zeros) does not get
+    case = Case(gpu, 24, dtype=dtype, d=d, hq=8, hkv=2, nodes=nodes, prefix=[0, 3, 0], spare=spare)
+    case.k[0, 0, 0, 1], case.q[0, 0, :4, 1] = np.inf, -1.0  # a draft that sees its own row alone
+    case.k[:, 1, 0, 1], case.q[1, :, :4, 1] = np.inf, -2.0  # every row of a sequence
+    case.sees[2, 1] = False
+    got = case.call(ops)
+    case.check(got)
+    assert got[0, 0, :4].isnan().all() and got[1, :, :4].isnan().all()
+    assert not got[2, 1].any() and got[1, :, 4:].isfinite().all()
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_an_infinity_in_the_prefix_reaches_every_draft(gpu, ops, dtype):
     case = Case(gpu, 12, dtype=dtype, d=64, hq=4, hkv=2, nodes=9, prefix=[1500])
