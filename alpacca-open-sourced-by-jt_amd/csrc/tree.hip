@@ -370,13 +370,17 @@ __device__ __forceinline__ void store4(void* out, int64_t at, const float (&r)[4
 }
 
 // Output channels d0 .. d0 + 3 of row `row` = (b, draft, head): the gate,
-// then the one rounding.
+// then the one rounding.  `sees`: the draft sees a row; one that sees none
+// gets zeros whatever its gate holds.
 template <typename T>
-__device__ __forceinline__ void write4(const TreeArgs& a, int64_t row, int d0, float (&r)[4]) {
+__device__ __forceinline__ void write4(const TreeArgs& a, int64_t row, int d0, float (&r)[4],
+                                       bool sees) {
   const int n = a.value_dim - d0;
   if (n <= 0) return;
   const int64_t at = row * a.value_dim + d0;
-  if (a.gate != nullptr) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = sees ? r[i] : 0.f;
+  if (a.gate != nullptr && sees) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (i < n) r[i] *= stable_sigmoid(to_f32(((const T*)a.gate)[at + i]));
@@ -463,12 +467,11 @@ __device__ __forceinline__ void sort_out(const TreeArgs& a, int b, int kvh, int 
         r[i] += finite(y) ? y * c : y;
       }
     }
-    // no row seen: zeros; rows that all score -inf: 0 / 0
-    const float inv = l == 0.f ? (M == -INFINITY ? 0.f : NAN) : 1.f / l;
+    const float inv = l == 0.f ? NAN : 1.f / l;  // (rows that all score -inf: 0 / 0)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = node < end - P ? r[i] * inv : 0.f;
+    for (int i = 0; i < 4; ++i) r[i] *= inv;
     const int64_t row = ((int64_t)b * a.nodes + node) * a.q_heads + kvh * G + (col - node * G);
-    write4<T>(a, row, 32 * mb + 8 * w + 4 * half, r);
+    write4<T>(a, row, 32 * mb + 8 * w + 4 * half, r, M != -INFINITY);
   }
   __syncthreads();  // `part` is read
 }
@@ -1036,10 +1039,10 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
       again |= bad;
       if (!in_range) return;
       const float inv = live && l != 0.f ? 1.f / l : 0.f;
+      const int64_t out0 = qrow * S::DP + 4 * sub;
 #pragma unroll
       for (int n = 0; n < NB; ++n) o[n] = live ? o[n] * inv : (Acc)(0.f);
-      const int64_t out0 = qrow * S::DP + 4 * sub;
-      if (a.gate != nullptr) {
+      if (a.gate != nullptr && live) {  // the others are zeros whatever their gate holds
         typedef typename Vec4<T>::type V4;
         const T* gp = (const T*)a.gate + out0;
 #pragma unroll
@@ -1184,8 +1187,8 @@ __global__ void __launch_bounds__(256) tree_join(TreeArgs a) {
   const int64_t qrow =
       ((int64_t)b * a.nodes + node) * a.q_heads + kvh * G + (col - node * G);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) r[i] = node < count ? r[i] * inv : 0.f;
-  write4<T>(a, qrow, 32 * mb + 8 * w + 4 * half, r);
+  for (int i = 0; i < 4; ++i) r[i] *= inv;
+  write4<T>(a, qrow, 32 * mb + 8 * w + 4 * half, r, node < count);
 }
 
 constexpr int kCus = 256;

@@ -281,6 +281,27 @@ def test_scores_that_are_all_minus_infinity_have_no_softmax(gpu, ops, dtype, d, 
     assert not got[2, 1].any() and got[1, :, 4:].isfinite().all()
 
 
+@pytest.mark.parametrize("spare", [0, 2000])
+@pytest.mark.parametrize("dtype,d,nodes", [("f32", 64, 6), ("f16", 128, 6), ("bf16", 256, 6),
+                                           ("bf16", 64, 40), ("bf16", 48, 6)])
+def test_gates_of_drafts_without_rows_are_not_read_into_their_zeros(gpu, ops, dtype, d, nodes,
+                                                                   spare):
+    # what a caller leaves in the gate of drafts past the counts, and of a
+    # draft that sees no row
+    case = Case(gpu, 25, dtype=dtype, d=d, hq=8, hkv=2, nodes=nodes, prefix=[33, 0, 40, 0],
+                counts=[nodes - 2, 0, 0, nodes - 1], gate=True, spare=spare)
+    case.sees[3, 2] = False
+    empty = [(b, i) for b in range(4) for i in range(case.counts[b], nodes)] + [(3, 2)]
+    for b, i in empty:
+        case.gate[b, i] = np.nan
+        case.gate[b, i, 1], case.gate[b, i, 2] = np.inf, -np.inf
+    got = case.call(ops)
+    for b, i in empty:
+        assert (got[b, i] == 0).all()
+        case.gate[b, i] = 0.0
+    case.check(got)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_an_infinity_in_the_prefix_reaches_every_draft(gpu, ops, dtype):
     case = Case(gpu, 12, dtype=dtype, d=64, hq=4, hkv=2, nodes=9, prefix=[1500])
