@@ -580,7 +580,8 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
         }
       };
       // Where tile t's K and V lie; rows past the end (all of them past the
-      // last tile) read as zeros.
+      // last tile) read as zeros, or, where rows lie over each other, as what
+      // the rows before hold there (no column sees them).
       struct Source {
         const T *k, *v;
         int rows;
@@ -593,10 +594,13 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
         s.k = (const T*)a.k;
         s.v = (const T*)a.v;
         if (s.rows > 0) group_base(row0, s.k, s.v);
+        // to the last row's last value: rows may lie over each other
+        const uint32_t rows_k = (uint32_t)((s.rows - 1) * a.ks_pos * (int64_t)sizeof(T));
+        const uint32_t rows_v = (uint32_t)((s.rows - 1) * a.vs_pos * (int64_t)sizeof(T));
         s.rk = rsrc_words((uint64_t)(uintptr_t)s.k,
-                          (uint32_t)(s.rows * a.ks_pos * (int64_t)sizeof(T)));
+                          s.rows > 0 ? rows_k + a.key_dim * (uint32_t)sizeof(T) : 0u);
         s.rv = rsrc_words((uint64_t)(uintptr_t)s.v,
-                          (uint32_t)(s.rows * a.vs_pos * (int64_t)sizeof(T)));
+                          s.rows > 0 ? rows_v + a.value_dim * (uint32_t)sizeof(T) : 0u);
         return s;
       };
       // load i of this wave's share of a K (V) tile, to LDS byte dst

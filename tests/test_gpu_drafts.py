@@ -408,6 +408,32 @@ def test_strides_of_a_cache_that_is_no_workspace(gpu):
         case.check(out)
 
 
+@pytest.mark.parametrize("dtype,d", [("f16", 64), ("bf16", 256), ("f32", 128)])
+def test_rows_that_lie_over_each_other(gpu, dtype, d):
+    """The C entry point with one row for all positions (a stride of 0) and
+    with rows that begin inside the one before, aligned and not."""
+    import torch
+    lib = importlib.import_module(PKG + "._lib")
+    code = dict(f32=lib.F32, f16=lib.F16, bf16=lib.BF16)[dtype]
+    for step in (0, 16, 3):
+        case = Case(gpu, 27, dtype=dtype, d=d, hq=4, hkv=2, nodes=6, prefix=[75, 20])
+        span = (case.length - 1) * step + d
+        flat = _normal(np.random.default_rng(step), dtype, 2, 2, 2, span)  # K / V, sequence, head
+        at = np.arange(case.length)[:, None] * step + np.arange(d)
+        case.k, case.v = (x[:, :, at].transpose(2, 0, 1, 3) for x in flat)
+        kv = [_up(gpu, x, dtype) for x in flat]
+        q, out = _up(gpu, case.q, dtype), torch.empty(2, 6, 4, d, dtype=_td(dtype), device=gpu)
+        masks, prefix = _up(gpu, T.mask_words(case.sees)), _ints(gpu, case.prefix)
+        need = lib.lib().alpx_tree_workspace_bytes(2, 6, 4, 2, d, d, case.length, code)
+        ws = torch.empty(max(need, 1), dtype=torch.uint8, device=gpu)
+        strides = (step, 2 * span, span)
+        lib.check(lib.lib().alpx_tree_attention(
+            q.data_ptr(), kv[0].data_ptr(), kv[1].data_ptr(), masks.data_ptr(), 6, 1,
+            prefix.data_ptr(), None, case.length, None, out.data_ptr(), ws.data_ptr(), need, 2, 6,
+            4, 2, d, d, *strides, *strides, d ** -0.5, code, code, lib.stream_handle(torch, gpu)))
+        case.check(out)
+
+
 def test_tree_attention_on_another_stream_and_in_a_graph(gpu, ops):
     """Two captured calls of different sizes, replayed several times with
     eager calls and synchronisations between them."""
