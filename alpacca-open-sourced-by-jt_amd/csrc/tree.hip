@@ -355,6 +355,16 @@ __device__ __forceinline__ float weight(float m, float M) {
   return m == -INFINITY ? 1.f : fast_exp2(m - M);
 }
 
+// What a gate lets through: the same form wherever a value is stored, the one
+// of the prefill's.
+template <typename T>
+__device__ __forceinline__ float gate_weight(T g) {
+  if constexpr (std::is_same<T, float>::value)
+    return stable_sigmoid(g);
+  else
+    return fast_sigmoid(to_f32(g));
+}
+
 template <typename TO>
 __device__ __forceinline__ void store4(void* out, int64_t at, const float (&r)[4], int n,
                                        bool vec) {
@@ -383,7 +393,7 @@ __device__ __forceinline__ void write4(const TreeArgs& a, int64_t row, int d0, f
   if (a.gate != nullptr && sees) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (i < n) r[i] *= stable_sigmoid(to_f32(((const T*)a.gate)[at + i]));
+      if (i < n) r[i] *= gate_weight(((const T*)a.gate)[at + i]);
   }
   switch (a.out_dtype) {
     case ALPX_F32: store4<float>(a.out, at, r, n, a.vec_o); break;
@@ -1053,8 +1063,7 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
         for (int f = 0; f < NF; ++f) {
           const V4 g = *(const V4*)(gp + 4 * LPC * f);
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            o[4 * f / NA][4 * f % NA + i] *= F32 ? stable_sigmoid(to_f32(g[i])) : fast_sigmoid(to_f32(g[i]));
+          for (int i = 0; i < 4; ++i) o[4 * f / NA][4 * f % NA + i] *= gate_weight((T)g[i]);
         }
       }
       auto store = [&](auto zero_of_type) __attribute__((always_inline)) {

@@ -434,6 +434,26 @@ def test_rows_that_lie_over_each_other(gpu, dtype, d):
         case.check(out)
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_gates_give_the_same_bits_by_every_store(gpu, dtype):
+    """One key row each, so that a float32 output is v * sigmoid(gate) with no
+    sum in it: whole rows written in vectors, by the joining launch, and
+    value by value to an output that is not aligned."""
+    import torch
+    ops = importlib.import_module(PKG + ".qwen35_rocm_ops").Qwen35RocmOps()
+    case = Case(gpu, 26, dtype=dtype, d=64, hq=8, hkv=2, nodes=1, prefix=[0] * 40, gate=True)
+    flat = torch.empty(40 * 8 * 64 + 1, dtype=torch.float32, device=gpu)
+    outs = [case.call(ops, out_dtype=torch.float32),
+            case.call(ops, out_dtype=torch.float32, out=flat[1:].reshape(40, 1, 8, 64))]
+    case.k, case.v = (np.concatenate([x, np.zeros((3000,) + x.shape[1:], x.dtype)])
+                      for x in (case.k, case.v))
+    case.length += 3000
+    outs.append(case.call(ops, out_dtype=torch.float32))
+    for got in outs:
+        case.check(got, "f32")
+        assert torch.equal(got, outs[0])
+
+
 def test_tree_attention_on_another_stream_and_in_a_graph(gpu, ops):
     """Two captured calls of different sizes, replayed several times with
     eager calls and synchronisations between them."""
