@@ -26,6 +26,7 @@
 
 #include <algorithm>
 #include <type_traits>
+#include <utility>
 
 #include "alpx_common.h"
 #include "prefill_run.h"
@@ -77,7 +78,7 @@ struct TreeArgs {
   int4* found;        // [batch]: first and last slot of a sequence, P, end
   float scale_log2;
   int out_dtype;
-  int vec_q, vec_o;   // q rows may be read, out rows written in vectors
+  int vec_k, vec_q, vec_o;  // rows of K and of q may be read, of out written in vectors
   int direct;         // vec_o, value_dim = DP: a slot writes its whole sequences
 };
 
@@ -229,6 +230,14 @@ __device__ __forceinline__ f32x16 mfma32x32x2(float a, float b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
 }
 
+// fp16 probabilities are formed 2^kLift times as large as their reference
+// says (the sums too, so it cancels): with kRescale they stay below 2^15, and
+// weights down to 2^-21 of the largest, not 2^-14, keep all their bits.  Many
+// rows of small weight beside a large one are what a first row that every
+// draft attends to leaves.
+template <typename T>
+constexpr float kLift = std::is_same<T, f16_t>::value ? 7.f : 0.f;
+
 // Shape of a kernel: T, DP (the head width rounded up to 64, 128 or 256), WC
 // columns per wave (32, or 16 on the 16 x 16 MFMA), WQ waves side by side in
 // columns, WK waves that share a column's keys, BK rows per K and V tile, a
@@ -254,12 +263,6 @@ struct Shape {
   // The wide 16-bit kernels run the products of two tiles beside the softmax
   // of a third (see the loop).
   static constexpr bool kPipe = WC == 32 && sizeof(T) == 2 && RING == 2;
-  // fp16 probabilities are formed 2^kLift times as large as their reference
-  // says (the sums too, so it cancels): with kRescale they stay below 2^15, and
-  // weights down to 2^-21 of the largest, not 2^-14, keep all their bits.  Many
-  // rows of small weight beside a large one are what a first row that every
-  // draft attends to leaves.
-  static constexpr float kLift = std::is_same<T, f16_t>::value ? 7.f : 0.f;
   // The narrow kernels have one column tile: nobody reads a tile twice.
   // (The hint on K and V / on V / on neither, 16 x 16 drafts on 8192 rows:
   // 97 / 86 / 103 us.)
@@ -267,7 +270,6 @@ struct Shape {
   // O and the sums of the waves that share keys are joined in LDS.
   static constexpr int kPart = (4 * NF + 2) * 64;  // floats per wave
   static constexpr int kMergeB = (WK - 1) * WQ * kPart * 4;
-  static constexpr int kRowsApartB = 34 * 256 * 4;  // see sort_out
   static constexpr int kLds = 2 * RING * kTileB > kMergeB ? 2 * RING * kTileB : kMergeB;
   // Blocks per CU: 160 KiB of LDS, and registers for 16, 8 or 4 waves.
   static constexpr int kLdsBlocks = 160 * 1024 / kLds;
@@ -402,86 +404,177 @@ __device__ __forceinline__ void write4(const TreeArgs& a, int64_t row, int d0, f
   }
 }
 
-// The result of 32 columns and 32 channels row by row, for sequences with an
-// infinity or a NaN in them.  The products take every row of a tile for
-// every column, and 0 times an infinity is a NaN: here a column takes the
-// rows that it sees, and an infinity among their values comes out as itself
-// however small its weight.  Thread (column, g), g < 8, takes rows g, g + 8, ...
+// The 16 bytes of a row of `width` from channel d on, zeros past its end.
 template <typename T>
-__device__ __forceinline__ void rows_apart(const TreeArgs& a, int b, int kvh, int col, int d0,
-                                           int P, int end, float (&o)[32], float& m, float& l) {
-  const int G = a.group, node = col / G, g = threadIdx.x >> 5;
-  m = -INFINITY;
-  l = 0.f;
-#pragma unroll
-  for (int i = 0; i < 32; ++i) o[i] = 0.f;
-  if (node >= min(end - P, a.nodes)) return;
-  const T* q = (const T*)a.q +
-               (((int64_t)b * a.nodes + node) * a.q_heads + kvh * G + (col - node * G)) * a.key_dim;
-  const uint32_t* mask = a.masks + b * a.mask_b + (int64_t)node * a.words;
-  for (int j = g; j < end; j += 8) {
-    if (j >= P && !(mask[(j - P) >> 5] >> ((j - P) & 31) & 1u)) continue;
-    int64_t ko = (int64_t)b * a.ks_b + j * a.ks_pos, vo = (int64_t)b * a.vs_b + j * a.vs_pos;
-    if (a.pages != nullptr) {
-      int pg = a.pages[(int64_t)b * a.max_pages + (j >> a.page_shift)];
-      pg = min(max(pg, 0), a.num_pages - 1);
-      const int64_t in = j & ((1 << a.page_shift) - 1);
-      ko = pg * a.ks_b + in * a.ks_pos;
-      vo = pg * a.vs_b + in * a.vs_pos;
-    }
-    const T* k = (const T*)a.k + ko + (int64_t)kvh * a.ks_h;
-    const T* v = (const T*)a.v + vo + (int64_t)kvh * a.vs_h;
-    float s = 0.f;
-    for (int d = 0; d < a.key_dim; ++d) s = fmaf(to_f32(q[d]), to_f32(k[d]), s);
-    s *= a.scale_log2;
-    const bool none = s == -INFINITY;  // no weight; m tells that a row was seen
-    const float M = fmaxf(fmaxf(m, s), -__FLT_MAX__);
-    const float c = weight(m, M), p = fast_exp2(s - M);
-    l = l * c + p;
-    m = M;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const float x = d0 + i < a.value_dim ? to_f32(v[d0 + i]) : 0.f;
-      const float kept = finite(o[i]) ? o[i] * c : o[i];
-      o[i] = kept + (finite(x) || none ? p * x : x);
-    }
+__device__ __forceinline__ auto row_unit(const T* row, int d, int width, bool vec) {
+  constexpr int EPU = 16 / (int)sizeof(T);
+  typedef T Unit __attribute__((ext_vector_type(EPU)));
+  Unit x = {};
+  if (vec) {
+    if (d < width) x = *(const Unit*)(row + d);
+  } else {
+    for (int e = 0; e < EPU; ++e)
+      if (d + e < width) x[e] = row[d + e];
   }
+  return x;
 }
 
-// The output of columns 32 cg + 0 .. 31 and channels 32 mb + 0 .. 31 that way.
-// Every thread of the block calls it; those past 256 only meet the barriers.
-// `part`: 34 x 256 floats of LDS.
+// The output of columns 32 cg + 0 .. 31 and channels 32 mb + 0 .. 31 of a
+// sequence whose V holds an infinity or a NaN.  The products take every row
+// of a tile for every column, and 0 times either is a NaN, whether the column
+// does not see the row or its weight is below the smallest number.  Here V
+// enters the product with its infinities and NaN replaced by zeros, and those
+// are counted apart, for each column among the rows that it sees: products of
+// 0 / 1 matrices again, in the tiles that hold any.  An infinity that a column
+// sees comes out as itself however small its weight (a NaN where the weight is
+// exactly 0: a score of -inf).  One infinity in a prefix, one kv head of one
+// sequence: 4 x 64 drafts on 32768 rows, 256 wide, 200 us -> 3.0 ms (every
+// head's: 5.8), 16 x 16 on 8192, 128 wide, 97 us -> 0.55 ms; row by row, with
+// one column a thread, it took 135 (494) and 18 ms.
+//
+// Waves 0 to 3 take 16 columns each, two of them every other 32 rows, operands
+// straight from memory (few registers: the kernels that call this keep what
+// their own loops need).  Every thread of the block calls it; those past 256
+// only meet the barriers.  `part`: kApart floats of LDS.
+constexpr int kApart = 4 * 11 * 64;
 template <typename T>
-__device__ __forceinline__ void sort_out(const TreeArgs& a, int b, int kvh, int cg, int mb, int P,
-                                         int end, float* part) {
-  const int tid = threadIdx.x, lane = tid & 63, hl = lane & 31, half = lane >> 5, w = tid >> 6;
-  const int G = a.group, col = 32 * cg + hl, node = col / G;
-  if (tid < 256) {
-    float x[32], m, l;
-    rows_apart<T>(a, b, kvh, col, 32 * mb, P, end, x, m, l);
+__device__ __forceinline__ void set_apart(const TreeArgs& a, int b, int kvh, int cg, int mb, int P,
+                                          int end, float* part) {
+  constexpr int EPU = 16 / (int)sizeof(T);
+  const int lane = threadIdx.x & 63, cl = lane & 15, sub = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int G = a.group, col = 32 * cg + 16 * (w & 1) + cl, node = col / G;
+  const bool in_range = node < a.nodes, live = node < end - P;
+  const int64_t row = ((int64_t)b * a.nodes + (in_range ? node : 0)) * a.q_heads + kvh * G +
+                      (col - node * G);
+  if (w < 4) {
+    const T* q = (const T*)a.q + row * a.key_dim;
+    const uint32_t* mask = a.masks + b * a.mask_b + (int64_t)(in_range ? node : 0) * a.words;
+    f32x4 o[2] = {};  // channels 16 n + 4 sub + 0 .. 3 of the 32
+    uint32_t found = 0;  // infinities seen: bit 4 n + i for inf, 8 + 4 n + i for -inf
+    float m = -INFINITY, l = 0.f;
+#pragma clang loop unroll(disable)
+    for (int j0 = 32 * (w >> 1); j0 < end; j0 += 64) {
+      int64_t ko = (int64_t)b * a.ks_b + j0 * a.ks_pos, vo = (int64_t)b * a.vs_b + j0 * a.vs_pos;
+      if (a.pages != nullptr) {  // (a page holds whole groups of 32 rows)
+        int pg = load_const(a.pages + (int64_t)b * a.max_pages + (j0 >> a.page_shift));
+        pg = min(max(pg, 0), a.num_pages - 1);
+        const int64_t in = j0 & ((1 << a.page_shift) - 1);
+        ko = pg * a.ks_b + in * a.ks_pos;
+        vo = pg * a.vs_b + in * a.vs_pos;
+      }
+      const int rows = end - j0;
+      const T* k = (const T*)a.k + ko + (int64_t)kvh * a.ks_h;
+      const T* v = (const T*)a.v + vo + (int64_t)kvh * a.vs_h;
+      // (32 rows lie within 2^31 bytes)
+      const T* k0 = k + min(cl, rows - 1) * (uint32_t)a.ks_pos;
+      const T* k1 = k + min(16 + cl, rows - 1) * (uint32_t)a.ks_pos;
+      f32x4 sc[2] = {};
+      for (int d0 = 0; d0 < a.key_dim; d0 += 4 * EPU) {
+        const int d = d0 + EPU * sub;
+        const auto qd = row_unit(q, d, a.key_dim, a.vec_q);
+        sc[0] = score_step<16>(row_unit(k0, d, a.key_dim, a.vec_k), qd, sc[0]);
+        sc[1] = score_step<16>(row_unit(k1, d, a.key_dim, a.vec_k), qd, sc[1]);
+      }
+      // score r is of key 16 (r / 4) + 4 sub + r % 4
+      const uint32_t seen = seen_bits(mask, a.words, P, end, j0, live) >> (4 * sub);
+      float s[8], mx = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) part[i * 256 + tid] = x[i];
-    part[32 * 256 + tid] = m;
-    part[33 * 256 + tid] = l;
-  }
-  __syncthreads();
-  if (tid < 256 && node < a.nodes) {
-    float M = -INFINITY, l = 0.f, r[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int g = 0; g < 8; ++g) M = fmaxf(M, part[32 * 256 + 32 * g + hl]);
-    for (int g = 0; g < 8; ++g) {
-      const float c = weight(part[32 * 256 + 32 * g + hl], M);
-      l += part[33 * 256 + 32 * g + hl] * c;
+      for (int r = 0; r < 8; ++r) {
+        const bool keep = seen >> (16 * (r >> 2) + (r & 3)) & 1;
+        s[r] = keep ? sc[r >> 2][r & 3] * a.scale_log2 : -INFINITY;
+        // (the reference is finite from the first row that is seen)
+        if (keep) mx = fmaxf(mx, fmaxf(s[r], -__FLT_MAX__));
+      }
+      mx = fmaxf(mx, __shfl_xor(mx, 16));
+      mx = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32)));
+      const float c = weight(m, mx), off = mx == -INFINITY ? 0.f : mx - kLift<T>;
+      m = mx;
+      l *= c;
+      uint32_t none = 0;  // rows that are seen without weight
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float y = part[(8 * w + 4 * half + i) * 256 + 32 * g + hl];
-        r[i] += finite(y) ? y * c : y;
+      for (int r = 0; r < 8; ++r) {
+        if (s[r] == -INFINITY) none |= seen & 1u << (16 * (r >> 2) + (r & 3));
+        s[r] = fast_exp2(s[r] - off);
+        l += s[r];
+      }
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        // x[r]: this lane's channel 16 n + cl of the key of score r
+        const int channel = 32 * mb + 16 * n + cl;
+        float x[8];
+        bool odd = false;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const int key = 16 * (r >> 2) + 4 * sub + (r & 3);
+          x[r] = to_f32(v[min(key, rows - 1) * (uint32_t)a.vs_pos + min(channel, a.value_dim - 1)]);
+          if (key >= rows) x[r] = 0.f;
+          odd |= !finite(x[r]);
+        }
+        // the product of f(r).first at key and channel, f(r).second at key and column
+        typedef std::pair<float, float> Two;
+        auto product = [&](auto f, f32x4 acc) __attribute__((always_inline)) {
+          if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int r = 0; r < 8; ++r) acc = mfma16x16x4(f(r).first, f(r).second, acc);
+          } else {
+            typename Vec8<T>::type xs, ps;
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+              xs[r] = from_f32<T>(f(r).first);
+              ps[r] = from_f32<T>(f(r).second);
+            }
+            acc = mfma16x16x32(xs, ps, acc);
+          }
+          return acc;
+        };
+        o[n] = product([&](int r) { return Two(finite(x[r]) ? x[r] : 0.f, s[r]); }, o[n] * c);
+        if (__ballot(odd) == 0) continue;
+        // a row that is seen counts an infinity of its sign, and a NaN as
+        // both; one without weight counts either as both
+#pragma unroll
+        for (int sign = 0; sign < 2; ++sign) {
+          const float other = sign == 0 ? -INFINITY : INFINITY;
+          f32x4 count = product([&](int r) {
+            return Two(finite(x[r]) || x[r] == other ? 0.f : 1.f,
+                       (float)(seen >> (16 * (r >> 2) + (r & 3)) & 1));
+          }, (f32x4)(0.f));
+          count = product([&](int r) {
+            return Two(x[r] == other ? 1.f : 0.f, (float)(none >> (16 * (r >> 2) + (r & 3)) & 1));
+          }, count);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) found |= (uint32_t)(count[i] > 0.f) << (8 * sign + 4 * n + i);
+        }
       }
     }
-    const float inv = l == 0.f ? NAN : 1.f / l;  // (rows that all score -inf: 0 / 0)
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    float* to = part + w * 11 * 64 + lane;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] *= inv;
-    const int64_t row = ((int64_t)b * a.nodes + node) * a.q_heads + kvh * G + (col - node * G);
-    write4<T>(a, row, 32 * mb + 8 * w + 4 * half, r, M != -INFINITY);
+    for (int i = 0; i < 8; ++i) to[i * 64] = o[i >> 2][i & 3];
+    to[8 * 64] = m;
+    to[9 * 64] = l;
+    to[10 * 64] = __uint_as_float(found);
+  }
+  __syncthreads();
+  if (w < 4 && in_range) {  // wave w writes channels 16 n + 4 sub + 0 .. 3 of its columns
+    const int n = w >> 1;
+    const float* p0 = part + (w & 1) * 11 * 64 + lane;
+    const float* p1 = p0 + 2 * 11 * 64;
+    const float m0 = p0[8 * 64], m1 = p1[8 * 64], M = fmaxf(m0, m1);
+    const float c0 = weight(m0, M), c1 = weight(m1, M);
+    const float l = p0[9 * 64] * c0 + p1[9 * 64] * c1;
+    const uint32_t found = __float_as_uint(p0[10 * 64]) | __float_as_uint(p1[10 * 64]);
+    const float inv = l == 0.f ? NAN : 1.f / l;  // (rows that all score -inf: 0 / 0)
+    float r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = 4 * n + i;
+      r[i] = (p0[at * 64] * c0 + p1[at * 64] * c1) * inv;
+      if (found >> at & 1) r[i] += INFINITY;
+      if (found >> (8 + at) & 1) r[i] -= INFINITY;
+    }
+    write4<T>(a, row, 32 * mb + 16 * n + 4 * sub, r, M != -INFINITY);
   }
   __syncthreads();  // `part` is read
 }
@@ -495,7 +588,7 @@ __device__ __forceinline__ void sort_out(const TreeArgs& a, int b, int kvh, int 
 // probabilities are an operand where they lie.
 template <typename S, bool DMA, bool ALONE>
 __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(TreeArgs a) {
-  static_assert(!ALONE || (S::kLds >= S::kRowsApartB && S::NW >= 4), "sort_out's space and threads");
+  static_assert(!ALONE || (S::kLds >= kApart * 4 && S::NW >= 4), "set_apart's space and threads");
   typedef typename S::T T;
   constexpr bool F32 = sizeof(T) == 4;
   constexpr int BK = S::BK, WC = S::WC, LPC = S::LPC, KG = S::KG, EPU = S::EPU, U = S::U;
@@ -795,7 +888,7 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
                 pend_any = true;
               }
             }
-            const float off = m == -INFINITY ? 0.f : m - S::kLift;
+            const float off = m == -INFINITY ? 0.f : m - kLift<T>;
             __builtin_amdgcn_sched_barrier(0);
             __builtin_amdgcn_s_setprio(1);
             float ps = 0.f;
@@ -933,7 +1026,7 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
                 m = mx;
               }
             }
-            const float off = m == -INFINITY ? 0.f : m - S::kLift;
+            const float off = m == -INFINITY ? 0.f : m - kLift<T>;
             float ps = 0.f;
 #pragma unroll
             for (int kr = 0; kr < S::KR; ++kr) {
@@ -1047,8 +1140,9 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
       float zero = 0.f;  // 0 times anything else is a NaN
 #pragma unroll
       for (int i = 0; i < 4 * NF; ++i) zero = fmaf(o[i / NA][i % NA], 0.f, zero);
-      // (a sum of 0: no row seen, or all of them at -inf)
-      const bool bad = __ballot(live && (zero != 0.f || l == 0.f)) != 0;
+      // (a sum of 0: no row seen, or all of them at -inf; a sum that is a NaN
+      // makes one of every channel, as it should)
+      const bool bad = __ballot(live && l == l && (zero != 0.f || l == 0.f)) != 0;
       if (!ALONE && sub == 0) a.part_st[seg * 32 + c32] = make_float2(bad ? 1.f : 0.f, 0.f);
       again |= bad;
       if (!in_range) return;
@@ -1087,7 +1181,7 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
     if constexpr (ALONE) {
       if (__syncthreads_or(again)) {
         for (int i = 0; i < S::kCols / 32 * (S::DP / 32); ++i)
-          sort_out<T>(a, b, kvh, ct * (S::kCols / 32) + i / (S::DP / 32), i % (S::DP / 32), P,
+          set_apart<T>(a, b, kvh, ct * (S::kCols / 32) + i / (S::DP / 32), i % (S::DP / 32), P,
                       sh.end, (float*)smem);
       }
       return;
@@ -1110,12 +1204,13 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
 // Joins the segments of the sequences that more than one slot has tiles of,
 // and writes zeros for those without a row.  One block per (sequence, kv
 // head, 32 columns, 32 channels); its four waves take the segments in turn
-// and meet in LDS.  A block whose result is not finite forms it again, row
-// by row.
+// and meet in LDS.  A block whose result is not finite forms it again
+// (set_apart).
 template <typename T, int DP>
 __global__ void __launch_bounds__(256) tree_join(TreeArgs a) {
   constexpr int MB = DP / 32, kFlight = 4;
-  __shared__ float part[34 * 256];  // [4][18][64] of the segments, or [34][256] row by row
+  __shared__ float part[4 * 18 * 64];  // of the segments, or set_apart's
+  static_assert(kApart <= 4 * 18 * 64, "set_apart's space");
   const int lane = threadIdx.x & 63, hl = lane & 31, half = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int mb = blockIdx.x % MB;
@@ -1188,11 +1283,12 @@ __global__ void __launch_bounds__(256) tree_join(TreeArgs a) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) r[i] += part[(v * 18 + 4 * w + i) * 64 + lane] * c;
   }
-  bool bad = whole || (node < count && (!finite(l) || l == 0.f));
+  bool bad = l == 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) bad |= node < count && !finite(r[i]);
+  for (int i = 0; i < 4; ++i) bad |= l == l && !finite(r[i]);
+  bad = whole || (bad && node < count);
   if (__syncthreads_or(bad)) {  // (a barrier: the segments' sums in LDS are read)
-    sort_out<T>(a, b, kvh, cg, mb, P, end, part);
+    set_apart<T>(a, b, kvh, cg, mb, P, end, part);
     return;
   }
   if (node >= a.nodes) return;
@@ -1376,6 +1472,7 @@ int tree_launch(const char* what, TreeArgs a, int dtype, void* workspace, size_t
                          (uintptr_t)(a.vs_h * es) | (uintptr_t)(a.key_dim * es) |
                          (uintptr_t)(a.value_dim * es);
   const bool dma = (rows & 15) == 0;
+  a.vec_k = dma;
   a.vec_q = (((uintptr_t)a.q | (uintptr_t)(a.key_dim * es)) & 15) == 0;
   a.vec_o = a.value_dim % 4 == 0 && ((uintptr_t)a.out & (4 * os - 1)) == 0 &&
             ((uintptr_t)a.gate & (4 * es - 1)) == 0;

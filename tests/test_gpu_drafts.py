@@ -302,6 +302,67 @@ def test_gates_of_drafts_without_rows_are_not_read_into_their_zeros(gpu, ops, dt
     case.check(got)
 
 
+@pytest.mark.parametrize("spare", [0, 2000])
+@pytest.mark.parametrize("dtype,d,nodes", [("f32", 64, 6), ("f16", 128, 6), ("bf16", 256, 40),
+                                           ("f16", 80, 40), ("bf16", 33, 6)])
+def test_infinities_of_both_signs_by_rows_and_channels(gpu, ops, dtype, d, nodes, spare):
+    # scattered over prefix and drafts, a channel with both signs, one of
+    # nothing else, beside scores whose weights are below the smallest number
+    case = Case(gpu, 28, dtype=dtype, d=d, hq=8, hkv=2, nodes=nodes, prefix=[70, 0, 33],
+                counts=[nodes, nodes, nodes - 1], gate=True, spare=spare, scale=8.0, page=32)
+    rows = case.rng.integers(0, 33, (3, 12))
+    for b in range(3):
+        for i, r in enumerate(rows[b] % case.rows[b]):
+            case.v[r, b, i % 2, (5 * i) % d] = [np.inf, -np.inf, np.nan][i % 3]
+    case.v[:, 0, 0, 7] = np.inf
+    case.v[2, 2, 1, 9], case.v[3, 2, 1, 9] = np.inf, -np.inf
+    got = case.call(ops)
+    # the oracle's weights are products' sums in 64 bits; float32 scores of up
+    # to 150 move a weight by 2^-24 * sqrt(d) * 150 (as in scores of large spread)
+    want, weight = case.want()
+    got = got.double().cpu().numpy()
+    fine = np.isfinite(want)
+    assert np.array_equal(np.isfinite(got), fine) and np.array_equal(np.isnan(got), np.isnan(want))
+    assert np.array_equal(got[np.isinf(want)], want[np.isinf(want)])
+    u = _half_step(dtype)
+    tol = (u + 2.0 ** -24 * 16 * 150) * weight + u * np.abs(want)
+    assert (np.abs(got - want)[fine] <= tol[fine] + 1e-4).all()
+
+
+def test_an_infinity_does_not_hold_a_call_up(gpu, ops):
+    # the results that it enters are formed again, in a small multiple of the
+    # call's time (walking the rows one by one took 600 of them)
+    import torch
+    batch, nodes, hq, hkv, d, rows = 2, 48, 16, 2, 256, 16384
+    q = torch.randn(batch, nodes, hq, d, device=gpu).to(torch.bfloat16)
+    k, v = (torch.randn(rows, batch, hkv, d, device=gpu).to(torch.bfloat16) for _ in range(2))
+    masks = ops.tree_masks(torch.arange(nodes, dtype=torch.int32, device=gpu)[None] - 1).masks
+    kw = dict(length=rows, prefix_lens=_ints(gpu, [rows - nodes] * batch))
+
+    def time():
+        ops.tree_attention(q, k, v, masks, **kw)
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        for _ in range(5):
+            ops.tree_attention(q, k, v, masks, **kw)
+        b.record()
+        b.synchronize()
+        return a.elapsed_time(b)
+
+    usual = time()
+    want = ops.tree_attention(q, k, v, masks, **kw).float()
+    v[-1, 0, 1, 3], v[100, 1, 0, 7] = float("inf"), float("-inf")
+    assert time() < 60 * usual
+    got = ops.tree_attention(q, k, v, masks, **kw).float()
+    # the last draft of sequence 0 alone sees the first, every draft of 1 the second
+    want[0, -1, 8:, 3], want[1, :, :8, 7] = float("inf"), float("-inf")
+    fine = want.isfinite()
+    assert torch.equal(got[~fine], want[~fine])
+    # two summations of the same terms, each with P and the result rounded once
+    tol = 2 * 2.0 ** -8 * (want.abs() + v[torch.isfinite(v)].float().abs().mean())
+    assert ((got - want).abs()[fine] <= tol[fine]).all()
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_an_infinity_in_the_prefix_reaches_every_draft(gpu, ops, dtype):
     case = Case(gpu, 12, dtype=dtype, d=64, hq=4, hkv=2, nodes=9, prefix=[1500])
