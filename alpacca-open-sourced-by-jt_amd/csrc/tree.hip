@@ -89,21 +89,24 @@ __device__ __forceinline__ int load_const(const int32_t* p) {
       *(const __attribute__((address_space(4))) int32_t*)(uintptr_t)p);
 }
 
-// Rows of sequence b: its prefix [0, P), its drafts [P, end).
+// Rows of sequence b: its prefix [0, P), its drafts [P, end).  A sequence
+// without drafts has none: nobody reads its prefix.
+__device__ __forceinline__ void rows_from(const TreeArgs& a, int prefix, int count, int& P,
+                                          int& end) {
+  P = min(max(prefix, 0), a.length);
+  end = min(P + min(max(count, 0), a.nodes), a.length);
+  if (end == P) P = end = 0;
+}
 __device__ __forceinline__ void lane_rows(const TreeArgs& a, int b, int& P, int& end) {
-  P = min(max(a.prefix[b], 0), a.length);
-  int n = a.counts != nullptr ? a.counts[b] : a.nodes;
-  n = min(max(n, 0), a.nodes);
-  end = min(P + n, a.length);
+  rows_from(a, a.prefix[b], a.counts != nullptr ? a.counts[b] : a.nodes, P, end);
 }
 
 // The same of one sequence for the whole wave, through the scalar cache.
 __device__ __forceinline__ void uniform_rows(const TreeArgs& a, int b, int& P, int& end) {
-  P = min(max(load_const(a.prefix + b), 0), a.length);
-  int n = a.counts != nullptr ? load_const(a.counts + b) : a.nodes;
-  n = min(max(n, 0), a.nodes);
+  rows_from(a, load_const(a.prefix + b), a.counts != nullptr ? load_const(a.counts + b) : a.nodes,
+            P, end);
   P = __builtin_amdgcn_readfirstlane(P);
-  end = __builtin_amdgcn_readfirstlane(min(P + n, a.length));
+  end = __builtin_amdgcn_readfirstlane(end);
 }
 
 // Shares of the rows: every slot gets a run of tiles of BK rows, cut on the
@@ -659,13 +662,16 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
       a.found[b] = make_int4(slot, sh.s1, P, sh.end);
     bool again = false;  // alone: some of the output is not finite
     auto segment = [&]() __attribute__((always_inline)) {
-      // rows [start, stop) of sequence b, in tiles of BK
-      const int start = t0 * BK, stop = min(sh.end, start + nt * BK);
+      // rows [start, stop) of sequence b, in tiles of BK: none where no column
+      // of the block has a draft
       const int count = sh.end - P;
+      const bool none = ct * S::kCols >= count * G;
+      if (none && (nt < sh.tiles || !a.direct)) return;
+      const int turns = none ? 0 : nt;
+      const int start = t0 * BK, stop = none ? start : min(sh.end, start + nt * BK);
       const bool live = node < count;
       // a wave without a live column only loads and meets the barriers
       const bool idle = ct * S::kCols + WC * wq >= count * G;
-      if (ct * S::kCols >= count * G && (nt < sh.tiles || !a.direct)) return;
       const int64_t qrow = ((int64_t)b * a.nodes + (in_range ? node : 0)) * a.q_heads + kvh * G +
                            (col - node * G);
       const uint32_t* mask = a.masks + b * a.mask_b + (int64_t)(in_range ? node : 0) * a.words;
@@ -788,7 +794,7 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
         // Turn t: PV of tile t - 1, the softmax of tile t and QK of tile
         // t + 1, so that the products run beside the exponentials of the same
         // wave, while K of tile t + 2 and V of tile t are on their way.  The
-        // first turn has no PV, the last one (turn nt) nothing else.  K tiles
+        // first turn has no PV, the last one (turn `turns`) nothing else.  K tiles
         // at 0 and kTileB, V tiles at 2 and 3 kTileB.
         typedef typename Vec8<T>::type V8;
         typedef typename Vec4<T>::type V4;
@@ -831,7 +837,7 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
           constexpr int Q = decltype(parity)::value;  // t & 1, but for the last
           constexpr bool FIRST = decltype(place)::value == 0, LAST = decltype(place)::value == 2;
           // the other place of each pair: tile t - 1 of V, tile t + 1 of K
-          const int behind = LAST ? ((nt & 1) ^ 1) * kTileB : (Q ^ 1) * kTileB;
+          const int behind = LAST ? ((turns & 1) ^ 1) * kTileB : (Q ^ 1) * kTileB;
           // the turn's loads (past the last tile they fetch nothing and write
           // zeros where nothing is read): spread over the steps, since a wave
           // that issues them in one go waits for the address unit meanwhile
@@ -957,17 +963,17 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
         };
         turn(Par<0>(), Par<0>(), 0);
 #pragma clang loop unroll(disable)
-        for (int t = 1; t < nt; t += 2) {
+        for (int t = 1; t < turns; t += 2) {
           turn(Par<1>(), Par<1>(), t);
-          if (t + 1 < nt) turn(Par<0>(), Par<1>(), t + 1);
+          if (t + 1 < turns) turn(Par<0>(), Par<1>(), t + 1);
         }
-        turn(Par<0>(), Par<2>(), nt);
+        turn(Par<0>(), Par<2>(), turns);
       } else {
         wait_tiles<(S::RING - 2) * S::kTileLoads * DMA>();  // the first tile is in LDS
         __syncthreads();
         int buf = 0;
 #pragma clang loop unroll(disable)
-        for (int t = 0; t < nt; ++t) {
+        for (int t = 0; t < turns; ++t) {
           // into the place of the tile before this one; past the last tile the
           // loads fetch nothing and write zeros, so that every turn waits for
           // the same number

@@ -515,6 +515,37 @@ def test_gates_give_the_same_bits_by_every_store(gpu, dtype):
         assert torch.equal(got, outs[0])
 
 
+def test_sequences_without_drafts_are_not_read(gpu, ops):
+    # idle places of a batch, and columns past the counts: no time for their
+    # rows (a third of the cache's reading would show them)
+    import torch
+    batch, nodes, rows = 8, 64, 16384
+    q = torch.randn(batch, nodes, 32, 128, device=gpu).to(torch.bfloat16)
+    k, v = (torch.randn(rows, batch, 8, 128, device=gpu).to(torch.bfloat16) for _ in range(2))
+    masks = ops.tree_masks(torch.arange(nodes, dtype=torch.int32, device=gpu)[None] - 1).masks
+    prefix = _ints(gpu, [rows - nodes] * batch)
+
+    def time(counts):
+        kw = dict(length=rows, prefix_lens=prefix, counts=_ints(gpu, counts))
+        out = ops.tree_attention(q, k, v, masks, **kw)
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        for _ in range(10):
+            ops.tree_attention(q, k, v, masks, **kw)
+        b.record()
+        b.synchronize()
+        return a.elapsed_time(b), out
+
+    full, want = time([nodes] * batch)
+    none, out = time([0] * batch)
+    assert not out.any() and none < full / 3
+    one, out = time([0] * 3 + [nodes] + [0] * 4)
+    assert one < full / 2 and not out[:3].any() and not out[4:].any()
+    # P and the result rounded once on each side; 16384 weighted values' mean size is below 1
+    off = (out[3].float() - want[3].float()).abs()
+    assert (off <= 2 * 2.0 ** -8 * (want[3].float().abs() + 1.0)).all()
+
+
 def test_tree_attention_on_another_stream_and_in_a_graph(gpu, ops):
     """Two captured calls of different sizes, replayed several times with
     eager calls and synchronisations between them."""
