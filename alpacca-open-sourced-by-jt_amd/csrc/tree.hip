@@ -703,13 +703,13 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
         s.k = (const T*)a.k;
         s.v = (const T*)a.v;
         if (s.rows > 0) group_base(row0, s.k, s.v);
-        // to the last row's last value: rows may lie over each other
-        const uint32_t rows_k = (uint32_t)((s.rows - 1) * a.ks_pos * (int64_t)sizeof(T));
-        const uint32_t rows_v = (uint32_t)((s.rows - 1) * a.vs_pos * (int64_t)sizeof(T));
-        s.rk = rsrc_words((uint64_t)(uintptr_t)s.k,
-                          s.rows > 0 ? rows_k + a.key_dim * (uint32_t)sizeof(T) : 0u);
-        s.rv = rsrc_words((uint64_t)(uintptr_t)s.v,
-                          s.rows > 0 ? rows_v + a.value_dim * (uint32_t)sizeof(T) : 0u);
+        // to the last row's last value, since rows may lie over each other
+        // (32 rows lie within 2^31 bytes)
+        auto bytes = [&](int64_t pitch, int width) __attribute__((always_inline)) {
+          return s.rows > 0 ? ((s.rows - 1) * (uint32_t)pitch + width) * (uint32_t)sizeof(T) : 0u;
+        };
+        s.rk = rsrc_words((uint64_t)(uintptr_t)s.k, bytes(a.ks_pos, a.key_dim));
+        s.rv = rsrc_words((uint64_t)(uintptr_t)s.v, bytes(a.vs_pos, a.value_dim));
         return s;
       };
       // load i of this wave's share of a K (V) tile, to LDS byte dst
