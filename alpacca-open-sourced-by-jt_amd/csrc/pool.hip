@@ -463,6 +463,8 @@ extern "C" int alpx_paged_resize(int32_t* block_table, int32_t* lengths, int32_t
   if ((int64_t)num_pages * page_size > 0x7fffffff || (int64_t)max_pages * page_size > 0x7fffffff)
     return fail(ALPX_EUNSUPPORTED, "%s: 2^31 rows or more", what);
   if (max_pages > 1 << 20) return fail(ALPX_EUNSUPPORTED, "%s: more than 2^20 pages a sequence", what);
+  // (the new rows' launch counts its threads in 31 bits)
+  if (tokens > 0x7fffffff - 255) return fail(ALPX_EUNSUPPORTED, "%s: more than 2^31 - 256 tokens", what);
   ResizeArgs a = {block_table, lengths,   free_pages, free_count, targets,
                   starts,      slots,     positions,  sequences,  granted, scratch,
                   batch,       max_pages, __builtin_ctz((unsigned)page_size), num_pages, tokens,

@@ -1399,8 +1399,8 @@ class Qwen35RocmOps:
             raise ValueError("page_size must be a power of two")
         if size * max(max_pages, free_pages.numel()) >= 2 ** 31:
             raise ValueError("a page pool or block table holds less than 2^31 rows")
-        if _nonnegative_integer("tokens", tokens) >= 2 ** 31:
-            raise ValueError("tokens must be less than 2^31")
+        if _nonnegative_integer("tokens", tokens) > 2 ** 31 - 256:
+            raise ValueError("tokens must be at most 2^31 - 256")
         targets = self._device_ints(targets, "targets", (batch,), low=0, high=max_pages * size)
         return RocmPagedRows(*_ops.paged_resize(block_table, lengths, free_pages, free_count,
                                                 targets, page_size=size, tokens=tokens))

@@ -769,8 +769,8 @@ int alpx_tree_commit_paged(void* key_pages, void* value_pages, const int32_t* bl
  * positions[t] in its sequence sequences[t]; all three are [tokens], -1 past
  * the last new row.  Cutting sequences back by the rows of the last call
  * restores the stack.  page_size a power of two; pool and sequences of less
- * than 2^31 rows, max_pages of at most 2^20.  scratch: batch + 1 int32 of the
- * call's own.  One launch, two for more than 4096 tokens. */
+ * than 2^31 rows, max_pages of at most 2^20, tokens of at most 2^31 - 256.
+ * scratch: batch + 1 int32 of the call's own.  One launch, two for more than 4096 tokens. */
 int alpx_paged_resize(int32_t* block_table, int32_t* lengths, int32_t* free_pages,
                       int32_t* free_count, const int32_t* targets, int batch, int max_pages,
                       int page_size, int num_pages, int tokens, int32_t* starts, int32_t* slots,

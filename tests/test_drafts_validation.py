@@ -153,6 +153,15 @@ def test_paged_resize_refusals(L):
     _refused(L, name, args, "EUNSUPPORTED", "2^20", max_pages=(1 << 20) + 1, page_size=1)
 
 
+def test_paged_resize_refuses_tokens_past_its_grid(L):
+    # blocks of 256 rows are counted in 31 bits
+    args = dict(table=FAKE, lengths=FAKE, free=FAKE, count=FAKE, targets=FAKE, batch=2, max_pages=4,
+                page_size=32, num_pages=9, tokens=2 ** 31 - 255, starts=FAKE, slots=FAKE,
+                positions=FAKE, sequences=FAKE, granted=FAKE, scratch=FAKE, stream=None)
+    for tokens in (2 ** 31 - 255, 2 ** 31 - 1):
+        _refused(L, "alpx_paged_resize", args, "EUNSUPPORTED", "tokens", tokens=tokens)
+
+
 def test_prologue_rows_refusals(L):
     name = "alpx_attention_prologue_rows"
     sections = (ctypes.c_int * 4)(11, 11, 10, 0)
@@ -278,6 +287,21 @@ def test_facade_refuses_numbers_past_32_bits(ops, monkeypatch):
             ops.paged_resize_(ints(2, 2), ints(2), ints(4), ints(1), ints(2), **kw)
     with pytest.raises(AssertionError, match="passed"):
         ops.paged_resize_(ints(2, 2), ints(2), ints(4), ints(1), ints(2), page_size=32, tokens=2)
+
+
+def test_facade_refuses_tokens_past_the_grid(ops, monkeypatch):
+    monkeypatch.setattr(ops, "_device_ints", lambda value, *a, **k: value)
+
+    class OnDevice(torch.Tensor):
+        is_cuda = True
+
+    def ints(*shape):
+        return _i32(*shape).as_subclass(OnDevice)
+    for tokens, error, text in ((2 ** 31 - 256, AssertionError, "passed"),
+                                (2 ** 31 - 255, ValueError, "2\\^31")):
+        with pytest.raises(error, match=text):
+            ops.paged_resize_(ints(2, 2), ints(2), ints(4), ints(1), ints(2), page_size=32,
+                              tokens=tokens)
 
 
 def test_facade_masks_commit_and_resize_refusals(ops):
