@@ -1440,10 +1440,24 @@ TreePlan tree_plan(int batch, int nodes, int q_heads, int kv_heads, int key_dim,
   return p;
 }
 
+// Sums of tiles, and of rows past the end, stay in 31 bits.
+bool too_many_rows(int batch, int length) {
+  return length > (1 << 30) || (int64_t)batch * ((int64_t)length / 32 + 1) >= ((int64_t)1 << 31);
+}
+
+// Blocks of the two launches; false: more threads than a grid holds.
+bool tree_grids(const TreePlan& p, int batch, int kv_heads, int64_t& blocks, int64_t& joins) {
+  const int64_t units = (int64_t)p.slots * kv_heads;
+  blocks = (units + kXcds - 1) / kXcds * kXcds * p.col_tiles;
+  joins = (int64_t)batch * kv_heads * p.col_tiles * (p.kernel.cols / 32) * (p.kernel.width / 32);
+  return blocks * p.kernel.threads <= 0xffffffff && joins * 256 <= 0xffffffff;
+}
+
 bool tree_sizes_ok(int batch, int nodes, int q_heads, int kv_heads, int key_dim, int value_dim,
                    int length) {
   return batch > 0 && nodes > 0 && q_heads > 0 && kv_heads > 0 && key_dim > 0 && value_dim > 0 &&
-         length > 0 && q_heads % kv_heads == 0 && key_dim <= 256 && value_dim <= 256 &&
+         length > 0 && !too_many_rows(batch, length) && q_heads % kv_heads == 0 && key_dim <= 256 &&
+         value_dim <= 256 &&
          (int64_t)nodes * (q_heads / kv_heads) <= (1 << 24);
 }
 
@@ -1467,8 +1481,7 @@ int tree_launch(const char* what, TreeArgs a, int dtype, void* workspace, size_t
     return fail(ALPX_EUNSUPPORTED, "%s: too many drafts", what);
   if (a.ks_pos < 0 || a.ks_b < 0 || a.ks_h < 0 || a.vs_pos < 0 || a.vs_b < 0 || a.vs_h < 0)
     return fail(ALPX_EINVAL, "%s: strides must not be negative", what);
-  // (sums of tiles and of rows past the end stay in 31 bits)
-  if (a.length > (1 << 30) || (int64_t)a.batch * ((int64_t)a.length / 32 + 1) >= ((int64_t)1 << 31))
+  if (too_many_rows(a.batch, a.length))
     return fail(ALPX_EUNSUPPORTED, "%s: too many rows", what);
   if (32 * std::max(a.ks_pos, a.vs_pos) * es >= ((int64_t)1 << 31))
     return fail(ALPX_EUNSUPPORTED, "%s: rows too far apart", what);
@@ -1492,6 +1505,9 @@ int tree_launch(const char* what, TreeArgs a, int dtype, void* workspace, size_t
     return fail(ALPX_EINVAL, "%s: out must not overlap q or gate", what);
   const TreePlan p = tree_plan(a.batch, a.nodes, a.q_heads, a.kv_heads, a.key_dim, a.value_dim,
                                a.length, dtype, dma, a.vec_o);
+  int64_t blocks, joins;
+  if (!tree_grids(p, a.batch, a.kv_heads, blocks, joins))
+    return fail(ALPX_EUNSUPPORTED, "%s: too many sequences", what);
   if (((uintptr_t)workspace & 15) != 0)
     return fail(ALPX_EINVAL, "%s: workspace must be 16-byte aligned", what);
   if (workspace_bytes < p.bytes || (p.bytes > 0 && !workspace))
@@ -1503,12 +1519,6 @@ int tree_launch(const char* what, TreeArgs a, int dtype, void* workspace, size_t
   a.part_o = (float*)workspace;
   a.part_st = (float2*)(a.part_o + p.part_o);
   a.found = (int4*)(a.part_st + p.segments * 32);
-  const int64_t units = (int64_t)p.slots * a.kv_heads;
-  const int64_t blocks = (units + kXcds - 1) / kXcds * kXcds * p.col_tiles;
-  const int groups = p.col_tiles * (p.kernel.cols / 32);
-  const int64_t joins = (int64_t)a.batch * a.kv_heads * groups * (p.kernel.width / 32);
-  if (blocks > 0x7fffffff || joins > 0x7fffffff)
-    return fail(ALPX_EUNSUPPORTED, "%s: too many sequences", what);
   hipStream_t s = (hipStream_t)stream;
   void* args[] = {&a};
   {
@@ -1516,7 +1526,7 @@ int tree_launch(const char* what, TreeArgs a, int dtype, void* workspace, size_t
     (void)hipLaunchKernel(p.alone ? p.kernel.alone : p.kernel.fn, dim3((unsigned)blocks), dim3(p.kernel.threads), args, 0, s);
   }
   if (p.alone) return check_launch(what);
-  a.col_tiles = groups;
+  a.col_tiles = p.col_tiles * (p.kernel.cols / 32);  // groups of 32 columns
   TimedRegion timed(ALPX_T_DECODE_COMBINE, s);
   (void)hipLaunchKernel(p.kernel.join, dim3((unsigned)joins), dim3(256), args, 0, s);
   return check_launch(what);
@@ -1532,9 +1542,12 @@ extern "C" size_t alpx_tree_workspace_bytes(int batch, int nodes, int q_heads, i
   if (!tree_sizes_ok(batch, nodes, q_heads, kv_heads, key_dim, value_dim, length) || !dtype_ok(dtype))
     return 0;
   size_t most = 0;  // whatever the call's alignment
-  for (int i = 0; i < 4; ++i)
-    most = std::max(most, tree_plan(batch, nodes, q_heads, kv_heads, key_dim, value_dim, length,
-                                    dtype, i & 1, i & 2).bytes);
+  for (int i = 0; i < 4; ++i) {
+    const TreePlan p = tree_plan(batch, nodes, q_heads, kv_heads, key_dim, value_dim, length, dtype,
+                                 i & 1, i & 2);
+    int64_t blocks, joins;
+    if (tree_grids(p, batch, kv_heads, blocks, joins)) most = std::max(most, p.bytes);
+  }
   return most;
 }
 

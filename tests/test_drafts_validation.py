@@ -102,6 +102,21 @@ def test_tree_workspace_is_zero_for_sizes_that_are_refused(L):
         assert size(*dict(good, **{key: bad}).values()) == 0
 
 
+def test_tree_workspace_is_zero_for_rows_and_sequences_past_the_range(L):
+    good = dict(batch=2, nodes=8, q_heads=8, kv_heads=2, key_dim=64, value_dim=64, length=4000,
+                dtype=1)
+    size = L.lib().alpx_tree_workspace_bytes
+    for bad in (dict(length=(1 << 30) + 1), dict(length=2 ** 31 - 1), dict(length=1 << 30, batch=64),
+                dict(batch=2 ** 31 - 1, length=32), dict(nodes=1 << 24),
+                dict(batch=1 << 20, nodes=1 << 10, q_heads=1 << 10, kv_heads=1 << 10)):
+        args = dict(good, **bad)
+        assert size(*args.values()) == 0
+        # as the call: no workspace that it would take
+        names = ("batch", "nodes", "q_heads", "kv_heads", "key_dim", "value_dim", "length", "dtype")
+        call = dict(dict(TREE, words=1 << 20, out=1 << 60), **{k: args[k] for k in names})
+        _refused(L, "alpx_tree_attention", call, "EUNSUPPORTED", "too many")
+
+
 def test_tree_masks_refusals(L):
     name = "alpx_tree_masks"
     args = dict(parents=FAKE, counts=None, lengths=FAKE, masks=FAKE, depths=FAKE, lanes=FAKE,
