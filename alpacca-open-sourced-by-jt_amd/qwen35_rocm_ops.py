@@ -32,6 +32,7 @@ from __future__ import annotations
 
 import importlib
 import math
+import operator
 from dataclasses import dataclass
 from typing import Any, NamedTuple, Sequence
 
@@ -1210,7 +1211,13 @@ class Qwen35RocmOps:
         if not torch.is_tensor(value) or value.device.type != "cuda":
             if len(shape) != 1:
                 raise TypeError(f"{name} must remain on the ROCm device")
-            host = [int(v) for v in value]
+            host = list(value)
+            if any(isinstance(v, bool) or not hasattr(v, "__index__") for v in host):
+                raise ValueError(f"{name} must hold integers")
+            try:
+                host = [operator.index(v) for v in host]
+            except TypeError:  # (a tensor's number that is not whole)
+                raise ValueError(f"{name} must hold integers") from None
             if (len(host),) != tuple(shape) or any(
                     (low is not None and v < low) or (high is not None and v > high)
                     for v in host):

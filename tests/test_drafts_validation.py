@@ -304,6 +304,20 @@ def test_facade_refuses_numbers_past_32_bits(ops, monkeypatch):
         ops.paged_resize_(ints(2, 2), ints(2), ints(4), ints(1), ints(2), page_size=32, tokens=2)
 
 
+def test_facade_takes_whole_host_numbers_only(ops):
+    import numpy as np
+    for bad in ([3.7, 1], [3.0, 1], [True, 1], np.array([1.5, 2.0]), torch.tensor([1.5, 2.0]),
+                ["1", 2], [None, 1]):
+        for key in ("prefix_lens", "counts"):
+            with pytest.raises(ValueError, match="integers"):
+                _attend(ops, **{key: bad})
+    ops.device = "cpu"  # where the accepted ones go
+    for good in ([3, 1], (0, 8), iter([3, 1]), np.array([1, 2], dtype=np.int64), np.array([1, 2], dtype=np.int8),
+                 torch.tensor([1, 2])):
+        with pytest.raises(AssertionError, match="passed"):
+            _attend(ops, counts=good)
+
+
 def test_facade_refuses_tokens_past_the_grid(ops, monkeypatch):
     monkeypatch.setattr(ops, "_device_ints", lambda value, *a, **k: value)
 
