@@ -667,6 +667,21 @@ def test_resize_sequences_of_calls_match_oracle(gpu, ops, batch, page, most, tok
         pool.step(ops, targets, 0 if turn == 1 else tokens)
 
 
+@pytest.mark.parametrize("batch,tokens", [(1025, 4096), (2500, 4000), (5000, 30000)])
+def test_resize_writes_rows_of_many_sequences(gpu, ops, batch, tokens):
+    # several tiles of sequences whose rows the same launch writes, and more
+    # sequences than the rows' own launch keeps in LDS
+    rng = np.random.default_rng(batch)
+    pool = Pool(gpu, rng, batch, 8, 4, batch * 6, rng.integers(0, 9, batch))
+    for turn in range(3):
+        grow = np.where(rng.random(batch) < 0.7, rng.integers(0, 2 if tokens < 5000 else 9, batch),
+                        -rng.integers(0, 9, batch))
+        if turn == 1:
+            grow[-1] = 1  # the last sequence's rows
+        r = pool.step(ops, np.clip(np.array(pool.lengths) + grow, 0, 32), tokens)
+        assert int(r.starts[-1]) > batch // 4
+
+
 def test_resize_back_restores_the_stack(gpu, ops):
     rng = np.random.default_rng(1)
     pool = Pool(gpu, rng, 40, 20, 32, 600, rng.integers(0, 300, 40))
