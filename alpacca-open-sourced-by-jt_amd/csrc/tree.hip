@@ -532,6 +532,10 @@ __device__ __forceinline__ void set_apart(const TreeArgs& a, int b, int kvh, int
           return acc;
         };
         o[n] = product([&](int r) { return Two(finite(x[r]) ? x[r] : 0.f, s[r]); }, o[n] * c);
+        if constexpr (sizeof(T) == 2)  // P in two parts, as in the narrow kernels
+          o[n] = product([&](int r) {
+            return Two(finite(x[r]) ? x[r] : 0.f, s[r] - to_f32(from_f32<T>(s[r])));
+          }, o[n]);
         if (__ballot(odd) == 0) continue;
         // a row that is seen counts an infinity of its sign, and a NaN as
         // both; one without weight counts either as both
@@ -906,6 +910,10 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
               pn[e / 8][e % 8] = from_f32<T>(p);
             };
             if constexpr (FIRST) static_for<0, NE>(probability);
+            // P is rounded to the cache's type for its product, as the
+            // prefill's: these kernels are bound by the products (the rest of
+            // P as a second one: 4 x 63 on 4133 rows, 128 wide, 28.9 -> 32.0
+            // us, 4 x 64 on 32768, 256 wide, 152 -> 185).
             // Step i: product i of NP + NS and its share of the exponentials,
             // all of them before their registers take tile t + 1's scores.
             // Operands are read AHEAD steps before their product; the order
@@ -1058,32 +1066,42 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
                   }
                 }
               } else {
+                static_assert(WC == 16, "32 columns of 16 bits run the turns above");
                 typedef typename Vec8<T>::type V8;
                 typedef typename Vec4<T>::type V4;
 #pragma unroll
                 for (int ks = 0; ks < NS / 8; ++ks) {
-                  V8 p;  // rounded to the cache's type for its product
+                  // P enters its product in two parts, rounded and the rest:
+                  // rounded alone it was as far off as the output's rounding
+                  // (bf16, rms of the result 2.3e-3, in two parts 1.67e-3, the
+                  // output's share).  A product behind the other, 16 x 16
+                  // drafts on 8192 rows, 128 wide: 65.2 -> 65.6 us (69 with
+                  // both to an accumulator back to back); 8 x 16 on 65536, 64
+                  // wide: 197 -> 198 (192 -> 200 on another card)
+                  V8 p, rest;
 #pragma unroll
-                  for (int e = 0; e < 8; ++e) p[e] = from_f32<T>(p_[8 * ks + e]);
+                  for (int e = 0; e < 8; ++e) {
+                    p[e] = from_f32<T>(p_[8 * ks + e]);
+                    rest[e] = from_f32<T>(fmaf(to_f32(p[e]), -1.f, p_[8 * ks + e]));
+                  }
                   // transposing reads: lane 4 k + q of 16 supplies row k, channels
                   // 4 q .. 4 q + 3, and receives channel lane % 16 of the four rows
                   const int vr = g0 + KG * kr + 8 * LPC * ks + 4 * sub + ((lane & 15) >> 2);
+                  V8 x[NB];
 #pragma unroll
                   for (int n = 0; n < NB; ++n) {
-                    const int u =
-                        DB / 8 * n + (WC == 32 ? 2 * ((lane >> 4) & 1) : 0) + ((lane & 3) >> 1);
+                    const int u = DB / 8 * n + ((lane & 3) >> 1);
                     const T* p0 =
                         (const T*)(vt + vr * kRowB + (u ^ v_swz<S>(vr)) * 16 + 8 * (lane & 1));
                     const int vr1 = vr + 4 * LPC;
                     const T* p1 =
                         (const T*)(vt + vr1 * kRowB + (u ^ v_swz<S>(vr1)) * 16 + 8 * (lane & 1));
                     const V4 x0 = lds_read_tr4(p0), x1 = lds_read_tr4(p1);
-                    const V8 x = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
-                    if constexpr (WC == 32)
-                      o[n] = mfma32x32x16(x, p, o[n]);
-                    else
-                      o[n] = mfma16x16x32(x, p, o[n]);
+                    x[n] = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
+                    o[n] = mfma16x16x32(x[n], p, o[n]);
                   }
+#pragma unroll
+                  for (int n = 0; n < NB; ++n) o[n] = mfma16x16x32(x[n], rest, o[n]);
                 }
               }
             }

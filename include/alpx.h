@@ -695,8 +695,10 @@ int alpx_recurrent_prefill_prep(const float* current, const float* conv_weight,
  * (0 / 0).  Infinities and NaN in rows that a draft does not see stay out of
  * its result.  Head widths up to 256 of any dtype,
  * stride and alignment; rows of 16-byte multiples run fastest.  Arithmetic
- * is fp32 (fp16 / bf16: the probabilities are rounded to the cache's type
- * for their product, the sums are not).
+ * is fp32; for their product the probabilities of fp16 / bf16 caches are
+ * taken in two parts of that type, or, for more than 64 columns (drafts times
+ * query heads of a kv head; 128 for widths above 128), rounded to it; their
+ * sums are not.
  * workspace: alpx_tree_workspace_bytes bytes (0 for sizes that the calls
  * refuse), 16-byte aligned; scratch, which calls that may overlap must not
  * share.  out must not overlap any input.  One launch for few drafts on few

@@ -370,6 +370,24 @@ def test_an_infinity_in_the_prefix_reaches_every_draft(gpu, ops, dtype):
     case.check(case.call(ops))
 
 
+@pytest.mark.parametrize("spare", [0, 2000])
+@pytest.mark.parametrize("dtype,d,nodes,hq", [("f16", 64, 16, 8), ("bf16", 64, 1, 8),
+                                              ("bf16", 128, 16, 8), ("f16", 128, 3, 8),
+                                              ("bf16", 256, 32, 8), ("f16", 256, 5, 6),
+                                              ("bf16", 48, 9, 8), ("f16", 33, 9, 8)])
+def test_few_columns_are_exact_to_the_output_s_rounding(gpu, ops, dtype, d, nodes, hq, spare):
+    # up to 64 columns (128 at width 256) P enters its product in two parts,
+    # which leaves (eps / 2)^2 of it: 2^-16 of the terms for bf16.  A float32
+    # output shows that beside float32 sums and exponentials (2^-24 * sqrt(256)
+    # * 8 for scores of up to 8, and as much again)
+    case = Case(gpu, 29, dtype=dtype, d=d, hq=hq, hkv=2, nodes=nodes, prefix=[20, 300, 0, 700],
+                spare=spare)
+    got = case.call(ops, out_dtype=_td("f32")).double().cpu().numpy()
+    want, weight = case.want()
+    off = np.abs(got - want)
+    assert (off <= (_half_step(dtype) ** 2 + 2.0 ** -16) * weight).all(), (off / weight).max()
+
+
 def test_scores_of_large_spread(gpu, ops):
     # scores of several hundreds: the reference has to move, and stale parts
     # have to weigh nothing
