@@ -6,7 +6,7 @@
 // itself, in a tree):
 //   out[b, i, h] = softmax_j(scale * q[b, i, h] . K[j, h / G]) . V[j, h / G]
 // over the rows it sees, times sigmoid(gate) where given; a draft that sees
-// no row, and drafts at or past n_b, give zeros.
+// no row, and drafts at or past n_b, give zeros, whatever their gate holds.
 //
 // The drafts of one sequence read the same rows, so a block takes columns =
 // (draft, query head of one kv head) pairs, up to 128 of them, against one
@@ -20,8 +20,9 @@
 // drafts on 8192 rows, 32/8 heads of 128, fp16: 78 us = 6.9 TB/s in the
 // loop, 90 with both ends of the launch, 7 more for the join), many by the
 // products and what they read from LDS (4 of 64 on 32768 rows, 16/2 heads of
-// 256, bf16: 165 us = 830 TFLOP/s, join 10), short ones by latency (8 on 508
-// rows, float32: 7.0 + 4.4 us).
+// 256, bf16: 166 us with the join = 830 TFLOP/s from a graph; back to back,
+// at the power limit, 170 to 178 and 10), short ones by latency (8 on 508
+// rows, float32: 7.2 + 4.3 us).
 #include <math.h>
 
 #include <algorithm>
@@ -735,7 +736,10 @@ __global__ void __launch_bounds__(64 * S::NW, S::kPerCu* S::NW / 4) tree_kernel(
 #pragma unroll
           for (int i = 0; i < S::kIW; ++i) load_v(s, i, dst + kTileB);
         } else {
-          // any head width, stride or alignment: element by element
+          // any head width, stride or alignment: element by element, through
+          // registers (4 x 8 drafts on 4096 rows: 33 wide bf16 43.6 us,
+          // float32 60.2, against 18.5 and 27.4 for rows of 40 and 36 by
+          // direct loads; 100 wide bf16 76, 104 wide 25; 250 wide 52, 248 26)
           for (int i = lane; i < kRows * S::DP; i += 64) {
             const int r = wave * kRows + i / S::DP, d = i % S::DP;
             const int64_t row = r - grp;
@@ -1363,8 +1367,10 @@ Kernel make() {
 // rows by two waves a column rather than 32 by one (4 x 8 drafts on 32768 rows
 // 63 -> 57 us); 128 columns have waves enough.  float32, 256 wide: four waves
 // have the registers of eight, 32 columns 180 -> 122 us (4 x 4 drafts on 8192
-// rows), 64 columns 238 -> 189 (4 x 16); 64 wide, 64 columns: room for a second
-// block 62.3 -> 59.2 (4 x 16 on 8192).
+// rows), 64 columns 238 -> 184 (4 x 16); 64 wide, 64 columns: room for a second
+// block 62.3 -> 54-59 (4 x 16 on 8192).  More columns, 32 a wave: 4 x 64 on
+// 8192 rows 148 us (64 wide), 280 (128), 314 (256, 16/2 heads): 71 to 80% of
+// what a large float32 product reaches.
 template <typename T>
 Kernel pick(int width, int cols, bool dma, bool few) {
   if constexpr (sizeof(T) == 4) {
@@ -1409,7 +1415,9 @@ Kernel pick(int width, int cols, bool dma, bool few) {
 // cost 4 to 5 us, which a few tiles that follow each other do not (8 drafts,
 // 32/8 heads, two launches -> one: bf16, 128 wide, 136 rows 11.4 -> 8.7 us
 // and 520 rows 12.3 -> 13.6; float32, 64 wide, 136 rows 10.5 -> 8.9 and 264
-// rows 10.8 -> 12.4).  Where every CU has a sequence anyway, splitting one
+// rows 10.8 -> 12.4; 256 wide, bf16 96 rows 13.9 -> 12.8 and 136 rows 14.1 ->
+// 14.8, float32 32 rows 16.5 -> 13.5 and 48 rows 16.0 -> 18.4 with 16/2 heads,
+// 15.6 -> 14.9 with 32/8).  Where every CU has a sequence anyway, splitting one
 // gains nothing for four times as many rows (32 sequences: bf16, 128 wide, 520
 // rows 22.8 -> 18.3 us); beyond that a single long sequence among short ones
 // would hold the call up.

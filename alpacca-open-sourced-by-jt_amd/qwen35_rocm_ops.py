@@ -1308,7 +1308,9 @@ class Qwen35RocmOps:
         ``masks [B or 1, N, words]`` (``tree_masks``).  Drafts at or past
         ``counts[b]``, and drafts that see no row, give zeros.  ``length``
         bounds every sequence's rows, drafts included; device lengths past it
-        are clamped.  ``out`` must not overlap an input.  Returns
+        are clamped, and drafts whose row lies past it give zeros.  The plan
+        goes by it: a few drafts on short sequences take one launch only where
+        it says that they are short.  ``out`` must not overlap an input.  Returns
         ``[B, N, Hq, Dv]``."""
         key_cache = self._tensor(key_cache, "attention key cache", dimensions=4)
         value_cache = self._tensor(value_cache, "attention value cache", dimensions=4)
@@ -1380,8 +1382,8 @@ class Qwen35RocmOps:
         [num_pages]``, of which ``free_count [1]`` are in use; growing ones
         then take theirs from its top, in the order of sequences.  A request
         is granted while the pages needed up to and with it are there and its
-        new rows end within ``tokens``; a refused one keeps its length and
-        pages.  ``block_table [B, max_pages]`` (-1 past a sequence's pages),
+        new rows end within ``tokens`` (behind those of every request before
+        it, refused ones too); a refused one keeps its length and pages.  ``block_table [B, max_pages]`` (-1 past a sequence's pages),
         ``lengths``, ``free_pages`` and ``free_count`` (all int32) are
         updated in place.  Returns where the new rows lie: ``slots`` go to
         ``paged_attention_prologue_rows_``."""

@@ -690,8 +690,9 @@ int alpx_recurrent_prefill_prep(const float* current, const float* conv_weight,
  * j / 64 is draft row j; mask_batch_stride words between sequences, 0: all
  * share one tree).  prefix_lens and counts (null: `nodes` drafts each) are
  * device int32 [batch]; the sequence's rows are clamped to [0, length], and
- * nothing behind them is read.  A draft at or past counts[b], and one that
- * sees no row, yields zeros; one that sees rows which all score -inf, NaN
+ * nothing behind them is read.  A draft at or past counts[b], one whose own
+ * row lies past length, and one that sees no row yield zeros, whatever their
+ * gate holds; one that sees rows which all score -inf, NaN
  * (0 / 0).  Infinities and NaN in rows that a draft does not see stay out of
  * its result.  Head widths up to 256 of any dtype,
  * stride and alignment; rows of 16-byte multiples run fastest.  Arithmetic
@@ -761,7 +762,8 @@ int alpx_tree_commit_paged(void* key_pages, void* value_pages, const int32_t* bl
  * free_count[0] are in use; then growing sequences take their pages from its
  * top, in the order of sequences.  A request is granted while the pages
  * needed up to and with it are at most what the stack then holds, and its
- * new rows end within `tokens`; one that needs no page is not held up by a
+ * new rows end within `tokens` (behind those of every request before it,
+ * refused ones too); one that needs no page is not held up by a
  * lack of them.  A target (or length) outside [0, max_pages * page_size] is
  * refused.  block_table, lengths, free_pages and free_count are updated in
  * place; granted [batch] holds 1 or 0, and a refused sequence keeps its

@@ -28,8 +28,9 @@ package and its HIP library) never imports it and has no CPU fallback.
 Parity pinning.  The reference ships no tests, golden vectors or fixtures
 for this path, so every oracle function is pinned by closed forms,
 invariants and special cases in ``tests/test_oracle.py`` (each test names
-the mistake it would catch).  No function of this package is left
-"parity unpinned".
+the mistake it would catch); no function that the reference has a
+counterpart of is left "parity unpinned".  ``oracle.drafts`` has none there:
+``tests/test_oracle_drafts.py`` pins it by hand-written cases.
 """
 
 from . import attention, drafts, gdn, inputs, layer, rope  # noqa: F401
