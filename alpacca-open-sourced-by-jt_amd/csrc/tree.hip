@@ -1466,9 +1466,17 @@ TreePlan tree_plan(int batch, int nodes, int q_heads, int kv_heads, int key_dim,
   return p;
 }
 
-// Sums of tiles, and of rows past the end, stay in 31 bits.
+// Sums of tiles, also rounded up to whole runs of every slot, and of rows past
+// the end stay in 31 bits.
 bool too_many_rows(int batch, int length) {
-  return length > (1 << 30) || (int64_t)batch * ((int64_t)length / 32 + 1) >= ((int64_t)1 << 31);
+  constexpr int64_t kSlots = kCus * 8;  // no plan has more
+  return length > (1 << 30) ||
+         (int64_t)batch * ((int64_t)length / 32 + 1) >= ((int64_t)1 << 31) - kSlots;
+}
+
+// Masks of every draft, and 32-bit words of them that an int counts.
+bool bad_words(int words, int64_t batch_stride, int nodes) {
+  return words < 0 || words >= 1 << 30 || (int64_t)words * 64 < nodes || batch_stride < 0;
 }
 
 // Blocks of the two launches; false: more threads than a grid holds.
@@ -1587,7 +1595,7 @@ extern "C" int alpx_tree_attention(const void* q, const void* key_cache, const v
                                    int64_t k_head_stride, int64_t v_pos_stride,
                                    int64_t v_batch_stride, int64_t v_head_stride, float scale,
                                    int dtype, int out_dtype, void* stream) {
-  if (mask_words < 0 || (int64_t)mask_words * 64 < nodes || mask_batch_stride < 0)
+  if (bad_words(mask_words, mask_batch_stride, nodes))
     return fail(ALPX_EINVAL, "alpx_tree_attention: mask_words must cover every draft");
   TreeArgs a = {};
   a.q = q;
@@ -1635,7 +1643,7 @@ extern "C" int alpx_tree_attention_paged(const void* q, const void* key_pages,
     return fail(ALPX_EINVAL, "alpx_tree_attention_paged: sizes must be positive");
   if (length > (int64_t)max_pages * page_size)
     return fail(ALPX_ERANGE, "attention cache length exceeds capacity");
-  if (mask_words < 0 || (int64_t)mask_words * 64 < nodes || mask_batch_stride < 0)
+  if (bad_words(mask_words, mask_batch_stride, nodes))
     return fail(ALPX_EINVAL, "alpx_tree_attention_paged: mask_words must cover every draft");
   TreeArgs a = {};
   a.q = q;

@@ -117,6 +117,19 @@ def test_tree_workspace_is_zero_for_rows_and_sequences_past_the_range(L):
         _refused(L, "alpx_tree_attention", call, "EUNSUPPORTED", "too many")
 
 
+def test_tree_attention_refuses_counts_past_31_bits(L):
+    # a slot's first tile is slot x tiles per slot, rounded up: with up to 2048
+    # slots the tiles have to end that far below 2^31; mask words count twice
+    # (2048 sequences of 2^20 - 1 tiles are 2^31 - 2048)
+    size = L.lib().alpx_tree_workspace_bytes
+    rows = 32 * (2 ** 20 - 2)
+    assert size(2048, 8, 8, 2, 64, 64, rows, 1) == 0 < size(2000, 8, 8, 2, 64, 64, rows, 1)
+    _refused(L, "alpx_tree_attention", dict(TREE, out=1 << 60), "EUNSUPPORTED", "too many rows",
+             batch=2048, length=rows)
+    for name, args in (("alpx_tree_attention", TREE), ("alpx_tree_attention_paged", PAGED)):
+        _refused(L, name, args, "EINVAL", "mask_words", words=1 << 30)
+
+
 def test_tree_masks_refusals(L):
     name = "alpx_tree_masks"
     args = dict(parents=FAKE, counts=None, lengths=FAKE, masks=FAKE, depths=FAKE, lanes=FAKE,
