@@ -56,6 +56,26 @@ SIGNATURES = {
                                               _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_ptr, _c_ptr,
                                               _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
                                               _c_ptr, ctypes.c_double, _c_float, _c_ptr]),
+    "alpx_rotary_append_rows": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64,
+                                         _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int,
+                                         _c_int, _c_int, _c_int, ctypes.c_double,
+                                         ctypes.c_double, _c_ptr]),
+    "alpx_q4_append_rows": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
+                                     _c_ptr, _c_int, _c_int, _c_ptr, _c_ptr, _c_int, _c_int,
+                                     _c_int, _c_int, _c_int, _c_int, _c_int, ctypes.c_double,
+                                     ctypes.c_double, _c_ptr]),
+    "alpx_q4_rows": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_int,
+                              _c_int, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr]),
+    "alpx_q4_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+                                          _c_int]),
+    "alpx_q4_attention": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int,
+                                   _c_int, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr,
+                                   _c_ptr, _c_size, _c_int, _c_int, _c_int, _c_int, _c_int,
+                                   _c_float, _c_int, _c_int, _c_ptr]),
+    "alpx_verify_workspace_bytes": (_c_size, [_c_int, _c_int, _c_i64]),
+    "alpx_verify_drafts": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
+                                    _c_ptr, _c_ptr, _c_ptr, _c_size, _c_int, _c_int, _c_i64,
+                                    _c_int, _c_ptr]),
     "alpx_kv_append_paged": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int,
                                       _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
                                       _c_i64, _c_ptr, _c_ptr]),
@@ -179,6 +199,9 @@ SIGNATURES = {
 # alpx_timed_kernel ids
 (T_KV_APPEND, T_DECODE, T_DECODE_COMBINE, T_PREFILL, T_GDN_CHUNK, T_GDN_STEP, T_AUX, T_LAYER,
  T_RECURRENT_STEP) = range(9)
+
+# alpx_rotary_style
+ROTARY_STYLES = {"norm": 0, "neox": 1}
 
 # alpx_row_norm modes
 NORM_L2, NORM_RMS, NORM_RMS_GATE = 0, 1, 2

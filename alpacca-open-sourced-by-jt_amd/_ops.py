@@ -1060,3 +1060,108 @@ def attention_prologue_rows(query_gate, key, value, q_norm, k_norm, key_pages, v
              _lib.dtype_code(torch, query_gate.dtype), tokens, q_heads, kv_heads, dim, value_dim,
              _sections(sections), float(frequency_base), float(eps))
     return query, gate
+
+
+def _rotary(query, key, *, rotary_dim, style, frequency_base, frequency_scale):
+    """The query's buffers and the arguments of a rotation."""
+    torch = _torch()
+    out = None if query is None else torch.empty_like(query)
+    tokens, kv_heads, dim = key.shape
+    sizes = (_lib.dtype_code(torch, key.dtype), tokens, 0 if query is None else query.shape[1],
+             kv_heads, dim)
+    return out, sizes, (rotary_dim, _lib.ROTARY_STYLES[style], float(frequency_base),
+                        float(frequency_scale))
+
+
+def rotary_append_rows(query, key, value, key_pages, value_pages, slots, positions, **rotary):
+    """Rotates ``query [T, Hq, D]`` (or None) and ``key [T, Hkv, D]`` by
+    ``positions`` and writes the latter with ``value [T, Hkv, Dv]`` to pool
+    rows ``slots``; returns the rotated query."""
+    out, sizes, turn = _rotary(query, key, **rotary)
+    _enqueue(_lib.lib().alpx_rotary_append_rows, key.device, _address(query), key.data_ptr(),
+             value.data_ptr(), _address(out), key_pages.data_ptr(), value_pages.data_ptr(),
+             key_pages.shape[0] * key_pages.shape[1], slots.data_ptr(), _address(positions),
+             *sizes, value.shape[2], *turn)
+    return out
+
+
+# ------------------------------------------------------- 4-bit page pools
+
+
+def q4_append_rows(query, key, value, pool, slots, positions, **rotary):
+    """``rotary_append_rows`` into a pool ``(key codes, key scales, value
+    codes, value scales)``."""
+    out, sizes, turn = _rotary(query, key, **rotary)
+    codes = pool[0]
+    _enqueue(_lib.lib().alpx_q4_append_rows, key.device, _address(query), key.data_ptr(),
+             value.data_ptr(), _address(out), *(x.data_ptr() for x in pool), codes.shape[2],
+             codes.shape[0], slots.data_ptr(), _address(positions), *sizes, *turn)
+    return out
+
+
+def q4_rows(pool, slots, dtype):
+    """Rows ``slots [T]`` of a pool as numbers: ``(key, value)``, each ``[T,
+    Hkv, D]``."""
+    torch = _torch()
+    codes = pool[0]
+    pages, kv_heads, page_size, half = codes.shape
+    rows = slots.shape[0]
+    key = torch.empty(rows, kv_heads, 2 * half, dtype=dtype, device=codes.device)
+    value = torch.empty_like(key)
+    _enqueue(_lib.lib().alpx_q4_rows, codes.device, *(x.data_ptr() for x in pool), page_size,
+             pages, slots.data_ptr(), rows, kv_heads, 2 * half, key.data_ptr(), value.data_ptr(),
+             _lib.dtype_code(torch, dtype))
+    return key, value
+
+
+@functools.lru_cache(maxsize=1024)
+def _q4_bytes(*sizes):
+    """``alpx_q4_workspace_bytes``, a pure function of the sizes."""
+    return _lib.lib().alpx_q4_workspace_bytes(*sizes)
+
+
+def q4_attention(q, pool, block_table, *, length, prefix_lens, counts, scale, gate=None,
+                 out_dtype=None, out=None):
+    """Tokens ``q [B, N, Hq, D]`` over a pool of codes; returns ``[B, N, Hq,
+    D]``.  The workspace is the call's own, as ``tree_attention``'s."""
+    torch = _torch()
+    batch, nodes, q_heads, dim = q.shape
+    pages, kv_heads, page_size, _ = pool[0].shape
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype if out_dtype is None else out_dtype,
+                          device=q.device)
+    code = _lib.dtype_code(torch, q.dtype)
+    nbytes = _q4_bytes(batch, nodes, q_heads, kv_heads, dim, length, code)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    _enqueue(_lib.lib().alpx_q4_attention, q.device, q.data_ptr(),
+             *(x.data_ptr() for x in pool), block_table.data_ptr(), block_table.shape[1],
+             page_size, pages, prefix_lens.data_ptr(), _address(counts), length, _address(gate),
+             out.data_ptr(), _address(ws), nbytes, batch, nodes, q_heads, kv_heads, dim,
+             float(scale), code, _lib.dtype_code(torch, out.dtype))
+    return out
+
+
+# ------------------------------------------------------- drafts verified
+
+
+@functools.lru_cache(maxsize=1024)
+def _verify_bytes(*sizes):
+    """``alpx_verify_workspace_bytes``, a pure function of the sizes."""
+    return _lib.lib().alpx_verify_workspace_bytes(*sizes)
+
+
+def verify_drafts(tokens, target, uniforms, *, parents=None, draft=None, counts=None):
+    """``(paths [B, N], accepted [B], new tokens [B, N])`` of drafts ``tokens
+    [B, N]``."""
+    torch = _torch()
+    batch, nodes, vocab = target.shape
+    # one buffer: paths, new tokens, counts
+    buffer = tokens.new_empty((2 * nodes + 1) * batch)
+    paths, new, accepted = buffer.split_with_sizes((batch * nodes, batch * nodes, batch))
+    nbytes = _verify_bytes(batch, nodes, vocab)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=target.device)
+    _enqueue(_lib.lib().alpx_verify_drafts, target.device, tokens.data_ptr(), target.data_ptr(),
+             _address(draft), _address(parents), _address(counts), uniforms.data_ptr(),
+             paths.data_ptr(), accepted.data_ptr(), new.data_ptr(), ws.data_ptr(), nbytes, batch,
+             nodes, vocab, _lib.dtype_code(torch, target.dtype))
+    return paths.view(batch, nodes), accepted, new.view(batch, nodes)

@@ -1,0 +1,509 @@
+// Packed tokens of any sequences and positions on their way into a page pool:
+// queries and keys turned by their positions, keys and values written to
+// their rows, as they are or as 4-bit codes; and rows of codes read back.
+//
+//   theta_p = position * scale * base^(-2 p / (2 R)), p < R
+//   (a, b) -> (a cos - b sin, a sin + b cos)
+// of channels (2 p, 2 p + 1) ("norm") or (p, p + R) ("neox"); channels from
+// 2 R on stay.  A group of 32 channels of a 4-bit row is stored as
+//   least = f16(min), step = f16((max - least) / 15),
+//   code = clamp(round((x - least) / step), 0, 15), 0 where the step is 0,
+// in float64, rounded through float32: where a code, a step or a least value
+// changes must not depend on the order of operations.
+#include <math.h>
+
+#include <algorithm>
+
+#include "alpx_common.h"
+#include "q4_internal.h"
+#include "rope_internal.h"
+#include "timing.h"
+
+namespace alpx {
+namespace {
+
+constexpr int kThreads = 256;
+
+struct RotaryArgs {
+  const void* q;     // [T, Hq, D]
+  const void* k;     // [T, Hkv, D]
+  const void* v;     // [T, Hkv, Dv]
+  void* q_out;       // [T, Hq, D]
+  void* kc;          // [rows, Hkv, D], or codes
+  void* vc;          // [rows, Hkv, Dv], or codes
+  f16_t* ks;         // scales, for codes
+  f16_t* vs;
+  const int32_t* slots;      // [T], rows of the pool; others write no row
+  const int32_t* positions;  // [T]; unused with R = 0
+  int64_t rows;
+  int Hq, Hkv, D, Dv, R, page_shift;
+  bool neox;
+  bool vec;   // rows may be read and written in vectors of 8 channels
+  bool pvec;  // and the partners of a neox rotation too
+  double inv[kMaxPairs];
+};
+
+// theta reduced to [-pi, pi]: an fma by each of the two parts of 2 pi loses
+// nothing that counts, since theta / 2 pi stays below 2^31.
+__device__ __forceinline__ double reduced(double theta) {
+  constexpr double kTwoPi = 6.283185307179586232, kRest = 2.4492935982947064e-16;
+  const double n = rint(theta * 0.15915494309189535);
+  return fma(-n, kRest, fma(-n, kTwoPi, theta));
+}
+
+template <typename T>
+struct Row8 {
+  T x[8];
+};
+template <typename T>
+__device__ __forceinline__ Row8<T> load8(const T* p, int n, bool vec) {
+  Row8<T> r = {};
+  if (vec) {
+    constexpr int kVecs = sizeof(T) * 8 / 16;
+    u32x4 w[kVecs];
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) w[i] = ((const u32x4*)p)[i];
+    __builtin_memcpy(&r, w, sizeof(r));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) r.x[i] = p[i];
+  }
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const Row8<T>& r, int n, bool vec) {
+  if (vec) {
+    constexpr int kVecs = sizeof(T) * 8 / 16;
+    u32x4 w[kVecs];
+    __builtin_memcpy(w, &r, sizeof(r));
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) ((u32x4*)p)[i] = w[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) p[i] = r.x[i];
+  }
+}
+
+// The 8 channels from c0 of a row turned by its token's angles, in A (float,
+// or double where the result is coded).
+template <typename A, typename T, typename Angle>
+__device__ __forceinline__ void turn8(const RotaryArgs& a, const T* row, int c0, int n,
+                                      const Row8<T>& raw, const Angle* cs, A (&y)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = (A)to_f32(raw.x[i]);
+  if (c0 >= 2 * a.R) return;
+  if (!a.neox) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      if (c0 + i >= 2 * a.R) continue;
+      const Angle r = cs[(c0 + i) >> 1];
+      const A lo = y[i], hi = y[i + 1];
+      y[i] = lo * r.x - hi * r.y;
+      y[i + 1] = lo * r.y + hi * r.x;
+    }
+    return;
+  }
+  Row8<T> far = {};
+  if (a.pvec) {  // all eight lie in one half
+    far = load8(row + (c0 < a.R ? c0 + a.R : c0 - a.R), 8, true);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int c = c0 + i;
+      if (i < n && c < 2 * a.R) far.x[i] = row[c < a.R ? c + a.R : c - a.R];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int c = c0 + i;
+    if (c >= 2 * a.R) continue;
+    const bool first = c < a.R;
+    const Angle r = cs[first ? c : c - a.R];
+    const A p = (A)to_f32(far.x[i]);
+    y[i] = first ? y[i] * r.x - p * r.y : p * r.y + y[i] * r.x;
+  }
+}
+
+// The token's angles, once for all of its heads.
+__device__ __forceinline__ void token_angles(const RotaryArgs& a, int t, float2* cs) {
+  for (int p = threadIdx.x; p < a.R; p += kThreads) {
+    float c, s;
+    rope_cs((double)a.positions[t], a.inv[p], c, s);
+    cs[p] = make_float2(c, s);
+  }
+}
+__device__ __forceinline__ void token_angles(const RotaryArgs& a, int t, double2* cs) {
+  for (int p = threadIdx.x; p < a.R; p += kThreads) {
+    double c, s;
+    sincos(reduced((double)a.positions[t] * a.inv[p]), &s, &c);
+    cs[p] = make_double2(c, s);
+  }
+}
+
+// One token per grid row, eight channels per thread; grid y shares out a
+// token's rows (queries, keys, values, in this order).
+template <typename T>
+__global__ void __launch_bounds__(kThreads) rotary_rows_kernel(RotaryArgs a) {
+  __shared__ float2 cs[kMaxPairs];
+  const int t = blockIdx.x;
+  const int slot = a.slots[t];
+  const bool stored = slot >= 0 && slot < a.rows;
+  const int per = (a.D + 7) >> 3, per_v = (a.Dv + 7) >> 3;
+  const int turned = (a.Hq + a.Hkv) * per, items = turned + a.Hkv * per_v;
+  token_angles(a, t, cs);
+  __syncthreads();
+  for (int j = blockIdx.y * kThreads + threadIdx.x; j < items; j += kThreads * gridDim.y) {
+    if (j >= turned) {
+      if (!stored) return;
+      const int h = (j - turned) / per_v, c0 = 8 * ((j - turned) - h * per_v);
+      const int n = min(8, a.Dv - c0);
+      const Row8<T> r = load8((const T*)a.v + ((int64_t)t * a.Hkv + h) * a.Dv + c0, n, a.vec);
+      store8((T*)a.vc + ((int64_t)slot * a.Hkv + h) * a.Dv + c0, r, n, a.vec);
+      continue;
+    }
+    const int row = j / per, c0 = 8 * (j - row * per), n = min(8, a.D - c0);
+    const bool is_q = row < a.Hq;
+    if (!is_q && !stored) continue;
+    const int h = is_q ? row : row - a.Hq;
+    const T* src = is_q ? (const T*)a.q + ((int64_t)t * a.Hq + h) * a.D
+                        : (const T*)a.k + ((int64_t)t * a.Hkv + h) * a.D;
+    float y[8];
+    turn8(a, src, c0, n, load8(src + c0, n, a.vec), cs, y);
+    Row8<T> out;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out.x[i] = from_f32<T>(y[i]);
+    T* dst = is_q ? (T*)a.q_out + ((int64_t)t * a.Hq + h) * a.D
+                  : (T*)a.kc + ((int64_t)slot * a.Hkv + h) * a.D;
+    store8(dst + c0, out, n, a.vec);
+  }
+}
+
+__device__ __forceinline__ double over_group(double x, bool largest) {
+#pragma unroll
+  for (int off = 1; off <= 2; off <<= 1) {
+    const double o = __shfl_xor(x, off);
+    x = largest ? fmax(x, o) : fmin(x, o);
+  }
+  return x;
+}
+
+// Through float32, in two roundings: left to itself the compiler makes one
+// (and a long one) of them.
+__device__ __forceinline__ f16_t to_half(double x) {
+  float y = (float)x;
+  asm("" : "+v"(y));
+  return (f16_t)y;
+}
+
+// The codes of 8 channels, and the step and least value of the group of four
+// neighbouring threads that share them.
+__device__ __forceinline__ uint32_t codes8(const double (&x)[8], f16_t& step, f16_t& least) {
+  double lo = x[0], hi = x[0];
+  bool finite = true;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    lo = fmin(lo, x[i]);
+    hi = fmax(hi, x[i]);
+    finite = finite && __builtin_isfinite(x[i]);
+  }
+  lo = over_group(lo, false);
+  hi = over_group(hi, true);
+  finite = over_group(finite ? 1.0 : 0.0, false) != 0.0;
+  constexpr double kMost = 65504.0;
+  least = to_half(fmin(fmax(lo, -kMost), kMost));
+  step = to_half(fmin(fmax((hi - (double)least) / 15.0, 0.0), kMost));
+  if (!finite) {  // the whole group reads as NaN
+    least = (f16_t)__builtin_nanf("");
+    step = (f16_t)0.f;
+  }
+  const double m = (double)least, d = (double)step;
+  if (!(d > 0.0)) return 0u;
+  const float inv = 1.f / (float)d;
+  uint32_t word = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    // the float quotient is some 1e-6 off: next to a border the exact one
+    // decides
+    float c = (float)(x[i] - m) * inv;
+    const float down = floorf(c);
+    if (fabsf(c - down - 0.5f) < 1e-4f) c = (float)rint((x[i] - m) / d);
+    c = fminf(fmaxf(rintf(c), 0.f), 15.f);
+    word |= (uint32_t)c << (4 * i);
+  }
+  return word;
+}
+
+// The same with the pool's rows as codes.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) q4_append_kernel(RotaryArgs a) {
+  __shared__ double2 cs[kMaxPairs];
+  const int t = blockIdx.x;
+  const int slot = a.slots[t];
+  const bool stored = slot >= 0 && slot < a.rows;
+  const int per = a.D >> 3, groups = a.D / kQ4Group, size = 1 << a.page_shift;
+  const int turned = (a.Hq + a.Hkv) * per, items = turned + a.Hkv * per;
+  token_angles(a, t, cs);
+  __syncthreads();
+  // rows are whole groups of four threads, so a group's threads stay together
+  for (int j = blockIdx.y * kThreads + threadIdx.x; j < items; j += kThreads * gridDim.y) {
+    const int row = j / per, c0 = 8 * (j - row * per);
+    if (row < a.Hq) {
+      const int64_t at = ((int64_t)t * a.Hq + row) * a.D;
+      const T* src = (const T*)a.q + at;
+      const Row8<T> raw = load8(src + c0, 8, a.vec);
+      double y[8];
+      turn8(a, src, c0, 8, raw, cs, y);
+      Row8<T> out;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) out.x[i] = from_f32<T>((float)y[i]);
+      store8((T*)a.q_out + at + c0, out, 8, a.vec);
+      continue;
+    }
+    if (!stored) return;
+    const bool is_k = row < a.Hq + a.Hkv;
+    const int h = is_k ? row - a.Hq : row - a.Hq - a.Hkv;
+    const T* src = (const T*)(is_k ? a.k : a.v) + ((int64_t)t * a.Hkv + h) * a.D;
+    const Row8<T> raw = load8(src + c0, 8, a.vec);
+    double y[8];
+    if (is_k) {
+      turn8(a, src, c0, 8, raw, cs, y);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = (double)to_f32(raw.x[i]);
+    }
+    f16_t step, least;
+    const uint32_t word = codes8(y, step, least);
+    const int64_t head = (int64_t)(slot >> a.page_shift) * a.Hkv + h;
+    const int r = slot & (size - 1), g = c0 / kQ4Group;
+    ((uint32_t*)(is_k ? a.kc : a.vc))[(head * size + r) * per + (c0 >> 3)] = word;
+    if ((c0 & (kQ4Group - 1)) == 0) {
+      f16_t* s = (is_k ? a.ks : a.vs) + (head * 2 * groups + g) * size + r;
+      s[0] = step;
+      s[(int64_t)groups * size] = least;
+    }
+  }
+}
+
+struct Q4RowsArgs {
+  const uint32_t* codes[2];  // K, V
+  const f16_t* scales[2];
+  void* out[2];              // [T, Hkv, D]
+  const int32_t* slots;      // [T]
+  int64_t rows, items;       // rows of the pool; 8-channel items of one of K, V
+  int Hkv, D, page_shift;
+};
+
+// Eight channels per thread; grid y: K, V.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) q4_rows_kernel(Q4RowsArgs a) {
+  const int per = a.D >> 3, groups = a.D / kQ4Group, size = 1 << a.page_shift;
+  const int which = blockIdx.y;
+  const uint32_t* codes = which ? a.codes[1] : a.codes[0];
+  const f16_t* scales = which ? a.scales[1] : a.scales[0];
+  T* dst = (T*)(which ? a.out[1] : a.out[0]);
+  for (int64_t j = (int64_t)blockIdx.x * kThreads + threadIdx.x; j < a.items;
+       j += (int64_t)gridDim.x * kThreads) {
+    const int64_t row = j / per;
+    const int o = (int)(j - row * per);
+    const int t = (int)(row / a.Hkv), h = (int)(row - (int64_t)t * a.Hkv);
+    const int slot = a.slots[t];
+    Row8<T> out = {};
+    if (slot >= 0 && slot < a.rows) {
+      const int64_t head = (int64_t)(slot >> a.page_shift) * a.Hkv + h;
+      const int r = slot & (size - 1);
+      const uint32_t word = codes[(head * size + r) * per + o];
+      const f16_t* s = scales + (head * 2 * groups + o / 4) * size + r;
+      const float step = (float)s[0], least = (float)s[(int64_t)groups * size];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        out.x[i] = from_f32<T>(fmaf((float)((word >> (4 * i)) & 15u), step, least));
+    }
+    store8(dst + 8 * j, out, 8, true);
+  }
+}
+
+// The host's part that both forms of the append share; 0 or a status.
+int rotary_args(const char* what, RotaryArgs& a, const void* query, const void* key,
+                const void* value, void* query_out, void* key_rows, void* value_rows,
+                const int32_t* slots, const int32_t* positions, int dtype, int tokens, int q_heads,
+                int kv_heads, int head_dim, int value_dim, int rotary_dim, int style, double base,
+                double scale) {
+  if (!key || !value || !key_rows || !value_rows || !slots || (q_heads > 0 && (!query || !query_out)) ||
+      (rotary_dim > 0 && !positions))
+    return fail(ALPX_EINVAL, "%s: null buffer", what);
+  if (!dtype_ok(dtype)) return fail(ALPX_EINVAL, "%s: unknown dtype", what);
+  if (tokens <= 0 || q_heads < 0 || kv_heads <= 0 || head_dim <= 0 || value_dim <= 0)
+    return fail(ALPX_EINVAL, "%s: sizes must be positive", what);
+  if (head_dim > kRopeMaxDim || value_dim > kRopeMaxDim)
+    return fail(ALPX_EUNSUPPORTED, "%s: head dims above %d", what, kRopeMaxDim);
+  if (((int64_t)q_heads + 2 * (int64_t)kv_heads) * ((std::max(head_dim, value_dim) + 7) / 8) >
+      0x7fffffff - 2 * kThreads * 1024)
+    return fail(ALPX_EUNSUPPORTED, "%s: too many heads", what);
+  if (rotary_dim < 0 || rotary_dim % 2 != 0 || rotary_dim > head_dim)
+    return fail(ALPX_EINVAL, "%s: rotary_dim must be even and at most the head width", what);
+  if (style != ALPX_ROTARY_NORM && style != ALPX_ROTARY_NEOX)
+    return fail(ALPX_EINVAL, "%s: unknown rotary style", what);
+  if (rotary_dim > 0 && (!(base > 0.0) || !isfinite(base) || !(scale > 0.0) || !isfinite(scale)))
+    return fail(ALPX_EINVAL, "%s: frequency base and scale must be positive and finite", what);
+  const int64_t es = (int64_t)dtype_size(dtype), row = tokens * (int64_t)head_dim * es;
+  const int64_t turned = q_heads > 0 ? q_heads * row : 0;
+  if (q_heads == 0) query = query_out = nullptr;
+  if (meet(query_out, turned, query, turned) || meet(query_out, turned, key, kv_heads * row) ||
+      meet(query_out, turned, value, tokens * (int64_t)kv_heads * value_dim * es))
+    return fail(ALPX_EINVAL, "%s: query_out must not overlap an input", what);
+  a.q = query;
+  a.k = key;
+  a.v = value;
+  a.q_out = query_out;
+  a.kc = key_rows;
+  a.vc = value_rows;
+  a.slots = slots;
+  a.positions = positions;
+  a.Hq = q_heads;
+  a.Hkv = kv_heads;
+  a.D = head_dim;
+  a.Dv = value_dim;
+  a.R = rotary_dim / 2;
+  a.neox = style == ALPX_ROTARY_NEOX;
+  if (a.R > 0) {
+    // (64 powers take a few microseconds, more than the rest of a call)
+    static thread_local struct {
+      double base, scale;
+      int R;
+      double inv[kMaxPairs];
+    } last = {};
+    if (last.R != a.R || last.base != base || last.scale != scale) {
+      inverse_frequencies(last.inv, a.R, base, scale);
+      last.R = a.R;
+      last.base = base;
+      last.scale = scale;
+    }
+    std::copy(last.inv, last.inv + a.R, a.inv);
+  }
+  return ALPX_OK;
+}
+
+// Few tokens: a token's rows are shared out over blocks.
+dim3 rotary_grid(const RotaryArgs& a, int tokens) {
+  const int items = (a.Hq + a.Hkv) * ((a.D + 7) / 8) + a.Hkv * ((a.Dv + 7) / 8);
+  const int passes = (items + kThreads - 1) / kThreads;
+  return dim3((unsigned)tokens, (unsigned)std::max(1, std::min(passes, 1024 / tokens)));
+}
+
+}  // namespace
+}  // namespace alpx
+
+using namespace alpx;
+
+extern "C" int alpx_rotary_append_rows(const void* query, const void* key, const void* value,
+                                       void* query_out, void* key_rows, void* value_rows,
+                                       int64_t pool_rows, const int32_t* slots,
+                                       const int32_t* positions, int dtype, int tokens,
+                                       int q_heads, int kv_heads, int head_dim, int value_dim,
+                                       int rotary_dim, int style, double frequency_base,
+                                       double frequency_scale, void* stream) {
+  const char* what = "alpx_rotary_append_rows";
+  RotaryArgs a = {};
+  const int status = rotary_args(what, a, query, key, value, query_out, key_rows, value_rows,
+                                 slots, positions, dtype, tokens, q_heads, kv_heads, head_dim,
+                                 value_dim, rotary_dim, style, frequency_base, frequency_scale);
+  if (status != ALPX_OK) return status;
+  if (pool_rows <= 0) return fail(ALPX_EINVAL, "%s: sizes must be positive", what);
+  a.rows = pool_rows;
+  const uintptr_t align = (uintptr_t)query | (uintptr_t)key | (uintptr_t)value |
+                          (uintptr_t)query_out | (uintptr_t)key_rows | (uintptr_t)value_rows;
+  a.vec = head_dim % 8 == 0 && value_dim % 8 == 0 && (align & 15) == 0;
+  a.pvec = a.vec && a.R % 8 == 0;
+  const void* kernel = dtype == ALPX_F32   ? (const void*)rotary_rows_kernel<float>
+                       : dtype == ALPX_F16 ? (const void*)rotary_rows_kernel<f16_t>
+                                           : (const void*)rotary_rows_kernel<bf16_t>;
+  hipStream_t s = (hipStream_t)stream;
+  TimedRegion timed(ALPX_T_KV_APPEND, s);
+  void* args[] = {&a};
+  (void)hipLaunchKernel(kernel, rotary_grid(a, tokens), dim3(kThreads), args, 0, s);
+  return check_launch(what);
+}
+
+extern "C" int alpx_q4_append_rows(const void* query, const void* key, const void* value,
+                                   void* query_out, void* key_codes, void* key_scales,
+                                   void* value_codes, void* value_scales, int page_size,
+                                   int num_pages, const int32_t* slots, const int32_t* positions,
+                                   int dtype, int tokens, int q_heads, int kv_heads, int head_dim,
+                                   int rotary_dim, int style, double frequency_base,
+                                   double frequency_scale, void* stream) {
+  const char* what = "alpx_q4_append_rows";
+  RotaryArgs a = {};
+  const int status = rotary_args(what, a, query, key, value, query_out, key_codes, value_codes,
+                                 slots, positions, dtype, tokens, q_heads, kv_heads, head_dim,
+                                 head_dim, rotary_dim, style, frequency_base, frequency_scale);
+  if (status != ALPX_OK) return status;
+  if (!key_scales || !value_scales) return fail(ALPX_EINVAL, "%s: null buffer", what);
+  if (!q4_dim_ok(head_dim)) return fail(ALPX_EUNSUPPORTED, "%s: head width must be 64, 96, 128 or 256", what);
+  if (num_pages <= 0) return fail(ALPX_EINVAL, "%s: sizes must be positive", what);
+  if (!power_of_two(page_size) || page_size < 32)
+    return fail(ALPX_EINVAL, "page_size must be a power of two of at least 32");
+  if ((int64_t)num_pages * page_size > 0x7fffffff)
+    return fail(ALPX_EUNSUPPORTED, "%s: 2^31 rows or more", what);
+  if ((((uintptr_t)key_codes | (uintptr_t)value_codes | (uintptr_t)key_scales |
+        (uintptr_t)value_scales) & 15) != 0)
+    return fail(ALPX_EINVAL, "%s: codes and scales must be 16-byte aligned", what);
+  a.ks = (f16_t*)key_scales;
+  a.vs = (f16_t*)value_scales;
+  a.rows = (int64_t)num_pages * page_size;
+  a.page_shift = __builtin_ctz((unsigned)page_size);
+  const uintptr_t align = (uintptr_t)query | (uintptr_t)key | (uintptr_t)value | (uintptr_t)query_out;
+  a.vec = (align & 15) == 0;
+  a.pvec = a.vec && a.R % 8 == 0;
+  const void* kernel = dtype == ALPX_F32   ? (const void*)q4_append_kernel<float>
+                       : dtype == ALPX_F16 ? (const void*)q4_append_kernel<f16_t>
+                                           : (const void*)q4_append_kernel<bf16_t>;
+  hipStream_t s = (hipStream_t)stream;
+  TimedRegion timed(ALPX_T_KV_APPEND, s);
+  void* args[] = {&a};
+  (void)hipLaunchKernel(kernel, rotary_grid(a, tokens), dim3(kThreads), args, 0, s);
+  return check_launch(what);
+}
+
+extern "C" int alpx_q4_rows(const void* key_codes, const void* key_scales, const void* value_codes,
+                            const void* value_scales, int page_size, int num_pages,
+                            const int32_t* slots, int rows, int kv_heads, int head_dim,
+                            void* key_out, void* value_out, int out_dtype, void* stream) {
+  const char* what = "alpx_q4_rows";
+  if (!key_codes || !key_scales || !value_codes || !value_scales || !slots || !key_out || !value_out)
+    return fail(ALPX_EINVAL, "%s: null buffer", what);
+  if (!dtype_ok(out_dtype)) return fail(ALPX_EINVAL, "%s: unknown dtype", what);
+  if (rows <= 0 || kv_heads <= 0 || num_pages <= 0)
+    return fail(ALPX_EINVAL, "%s: sizes must be positive", what);
+  if (!q4_dim_ok(head_dim)) return fail(ALPX_EUNSUPPORTED, "%s: head width must be 64, 96, 128 or 256", what);
+  if (!power_of_two(page_size) || page_size < 32)
+    return fail(ALPX_EINVAL, "page_size must be a power of two of at least 32");
+  if ((int64_t)num_pages * page_size > 0x7fffffff)
+    return fail(ALPX_EUNSUPPORTED, "%s: 2^31 rows or more", what);
+  if ((((uintptr_t)key_codes | (uintptr_t)value_codes | (uintptr_t)key_scales |
+        (uintptr_t)value_scales | (uintptr_t)key_out | (uintptr_t)value_out) & 15) != 0)
+    return fail(ALPX_EINVAL, "%s: codes, scales and rows must be 16-byte aligned", what);
+  Q4RowsArgs a = {};
+  a.codes[0] = (const uint32_t*)key_codes;
+  a.codes[1] = (const uint32_t*)value_codes;
+  a.scales[0] = (const f16_t*)key_scales;
+  a.scales[1] = (const f16_t*)value_scales;
+  a.out[0] = key_out;
+  a.out[1] = value_out;
+  a.slots = slots;
+  a.rows = (int64_t)num_pages * page_size;
+  a.Hkv = kv_heads;
+  a.D = head_dim;
+  a.page_shift = __builtin_ctz((unsigned)page_size);
+  a.items = (int64_t)rows * kv_heads * (head_dim / 8);
+  const unsigned blocks = (unsigned)std::min<int64_t>((a.items + kThreads - 1) / kThreads, 1 << 20);
+  const void* kernel = out_dtype == ALPX_F32   ? (const void*)q4_rows_kernel<float>
+                       : out_dtype == ALPX_F16 ? (const void*)q4_rows_kernel<f16_t>
+                                               : (const void*)q4_rows_kernel<bf16_t>;
+  hipStream_t s = (hipStream_t)stream;
+  TimedRegion timed(ALPX_T_AUX, s);
+  void* args[] = {&a};
+  (void)hipLaunchKernel(kernel, dim3(blocks, 2), dim3(kThreads), args, 0, s);
+  return check_launch(what);
+}

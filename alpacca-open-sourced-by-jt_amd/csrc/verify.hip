@@ -1,0 +1,538 @@
+// Which drafted tokens stand, from given random numbers.
+//
+// Draft 0 of a sequence is the token that it holds already; draft i, a child
+// of draft parents[i], was proposed as the token behind it.  p = target[i] is
+// the target's distribution behind draft i, q = draft[i] the distribution
+// that the children of i were drawn from, one after the other and each from
+// all of q.  From draft 0 on, the children x_1, x_2, ... of a draft are tried
+// in rising order, with r_0 = p, Z_0 = 1:
+//   child j stands if u_j q(x_j) Z < r(x_j); the walk goes on from it;
+//   else r <- max(r - Z q, 0), Z <- sum r, and the next child is tried;
+// and where no child stands (or none is left), the last token is drawn from
+// r: the first x whose running sum exceeds u_0 sum r.  Tokens then follow the
+// target's distribution exactly.  Children that no distribution drew (draft
+// null) stand with probability r(x) / Z, which takes x out of p when refused:
+//   child j stands if u_j Z < r(x_j); else r(x_j) <- 0, Z <- Z - r(x_j).
+// If nothing is left of r, p itself is drawn from; if p holds nothing either,
+// the last token is -1.  Entries that are not positive and finite weigh 0.
+//
+// Sums run in float64: a running sum in float32 would be off by more than a
+// small token's weight.
+//
+// Bound by the one or two rows of the vocabulary that the last token is drawn
+// from.  One launch gathers the drafts' own entries, walks as far as it can
+// without a sum (in every block for itself: a walk is short) and leaves the
+// sums of slices of the row; a second finds the slice and the token.
+#include <math.h>
+
+#include <algorithm>
+
+#include "alpx_common.h"
+#include "timing.h"
+
+namespace alpx {
+namespace {
+
+constexpr int kMostDrafts = 1024;
+constexpr int kMostSlices = 64;  // one per lane
+constexpr int kSumThreads = 256, kDrawThreads = 512;
+
+struct Stand {  // where a walk stopped
+  int last;      // the draft that it reached
+  int from;      // the next child to try, from here on
+  int tried;     // children of `last` refused so far
+  int accepted;  // drafts that stand; 0: the sequence has no drafts
+};
+
+struct VerifyArgs {
+  const int32_t* tokens;   // [B, N]
+  const void* target;      // [B, N, V]
+  const void* draft;       // [B, N, V] or null
+  const int32_t* parents;  // [B, N] or null (chains)
+  const int32_t* counts;   // [B] or null
+  const float* uniforms;   // [B, N]
+  int32_t* paths;          // [B, N]
+  int32_t* accepted;       // [B]
+  int32_t* out;            // [B, N]
+  double* sums;            // [B, slices]
+  Stand* stands;           // [B]
+  int64_t vocab, slice;    // tokens; tokens of a slice
+  int nodes, slices;
+};
+
+__device__ __forceinline__ float weight(float x) {
+  return x > 0.f && x < __builtin_inff() ? x : 0.f;
+}
+
+// What a block knows of a sequence's drafts.
+struct Drafts {
+  int up[kMostDrafts];     // parent, -1: never reached
+  int token[kMostDrafts];
+  float p[kMostDrafts];    // the parent's distributions at the token
+  float q[kMostDrafts];
+  float u[kMostDrafts];
+  double z[kMostDrafts];   // Z of the refusals at the draft that the walk is at
+  int gone[kMostDrafts];   // tokens refused there (draft null)
+  Stand at;
+  bool more;               // a sum is wanted before the next child can be tried
+  int ngone;
+};
+
+template <typename T>
+__device__ __forceinline__ void gather(const VerifyArgs& a, int b, int count, Drafts& d) {
+  for (int i = threadIdx.x; i < count; i += blockDim.x) {
+    const int64_t at = (int64_t)b * a.nodes + i;
+    int up = a.parents != nullptr ? a.parents[at] : i - 1;
+    if (up < 0 || up >= i) up = -1;
+    const int x = a.tokens[at];
+    float p = 0.f, q = 1.f;
+    if (up >= 0) {
+      const int64_t row = ((int64_t)b * a.nodes + up) * a.vocab;
+      const bool in = x >= 0 && x < a.vocab;
+      p = in ? weight(to_f32(((const T*)a.target)[row + x])) : 0.f;
+      if (a.draft != nullptr) q = in ? weight(to_f32(((const T*)a.draft)[row + x])) : 0.f;
+    }
+    d.up[i] = up;
+    d.token[i] = x;
+    d.p[i] = p;
+    d.q[i] = q;
+    d.u[i] = a.uniforms[at];
+  }
+}
+
+// What `tried` refusals leave of p where the draft has q.
+__device__ __forceinline__ double left_of(double p, double q, const double* z, int tried) {
+  double r = p;
+  for (int j = 0; j < tried; ++j) r = fmax(r - z[j] * q, 0.0);
+  return r;
+}
+
+// Goes on from d.at until a sum is wanted (d.more) or no child is left.  One
+// wave; z[0 .. tried] are the sums known so far (z[0] = 1).  The drafts that
+// stand enter the sequence's path.
+__device__ __forceinline__ void walk(const VerifyArgs& a, int b, int count, Drafts& d) {
+  const int lane = threadIdx.x & 63;
+  int last = d.at.last, from = d.at.from, tried = d.at.tried, accepted = d.at.accepted;
+  double rem = 1.0;  // draft null: 1 less the tokens refused here
+  bool more = false;
+  while (true) {
+    int child = -1;
+    for (int i0 = from & ~63; i0 < count && child < 0; i0 += 64) {
+      const int i = i0 + lane;
+      const unsigned long long hit = __ballot(i >= from && i < count && d.up[i] == last);
+      if (hit != 0) child = i0 + __ffsll((long long)hit) - 1;
+    }
+    if (child < 0) break;
+    const int x = d.token[child];
+    const double u = (double)d.u[child];
+    double w;
+    bool stands;
+    if (a.draft != nullptr) {
+      const double q = (double)d.q[child];
+      w = left_of((double)d.p[child], q, d.z, tried);
+      stands = u * q * d.z[tried] < w;
+    } else {
+      bool again = false;  // a token that was refused here once weighs nothing
+      for (int j0 = 0; j0 < tried; j0 += 64)
+        again |= __ballot(j0 + lane < tried && d.gone[j0 + lane] == x) != 0;
+      w = again ? 0.0 : (double)d.p[child];
+      stands = u * rem < w;
+    }
+    from = child + 1;
+    if (stands) {
+      if (lane == 0 && a.paths != nullptr) {
+        a.paths[(int64_t)b * a.nodes + accepted] = child;
+        a.out[(int64_t)b * a.nodes + accepted - 1] = x;
+      }
+      ++accepted;
+      last = child;
+      tried = 0;
+      rem = 1.0;
+      continue;
+    }
+    rem -= w;
+    if (lane == 0) d.gone[tried] = x;
+    __builtin_amdgcn_wave_barrier();  // (LDS traffic of a wave runs in order)
+    ++tried;
+    if (a.draft != nullptr) {
+      more = true;
+      break;
+    }
+  }
+  if (lane == 0) {
+    d.at = Stand{last, from, tried, accepted};
+    d.more = more;
+  }
+}
+
+// A thread's share of the weights x0 <= x < x1 of a row: p where nothing was
+// refused, else what the refusals left.  d.gone[0 .. ngone) are the tokens of
+// the range that weigh nothing.
+template <typename T, bool DRAFT>
+__device__ __forceinline__ double range_sum(const T* p, const T* q, int64_t x0, int64_t x1,
+                                            const Drafts& d, int tried, int ngone, int thread,
+                                            int threads) {
+  constexpr int VN = 16 / (int)sizeof(T);
+  struct alignas(16) Unit {
+    T x[VN];
+  };
+  double sum = 0.0;
+  auto one = [&](int64_t x) __attribute__((always_inline)) {
+    float w = weight(to_f32(p[x]));
+    if constexpr (DRAFT) {
+      sum += tried == 0 ? (double)w
+                        : left_of((double)w, (double)weight(to_f32(q[x])), d.z, tried);
+    } else {
+      for (int j = 0; j < ngone; ++j)
+        if (d.gone[j] == x) w = 0.f;
+      sum += (double)w;
+    }
+  };
+  int64_t v0 = x0, v1 = x0;  // whole units
+  if (!DRAFT || (((uintptr_t)p ^ (uintptr_t)q) & 15) == 0) {
+    const int64_t head = (int64_t)((0u - (unsigned)((uintptr_t)(p + x0) & 15)) & 15) / (int)sizeof(T);
+    v0 = x0 + head < x1 ? x0 + head : x1;
+    v1 = v0 + (x1 - v0) / VN * VN;
+  }
+  for (int64_t x = x0 + thread; x < v0; x += threads) one(x);
+  for (int64_t x = v0 + (int64_t)thread * VN; x < v1; x += (int64_t)threads * VN) {
+    const Unit pu = *(const Unit*)(p + x);
+    float w[VN];
+#pragma unroll
+    for (int e = 0; e < VN; ++e) w[e] = weight(to_f32(pu.x[e]));
+    if constexpr (DRAFT) {
+      if (tried != 0) {
+        const Unit qu = *(const Unit*)(q + x);
+#pragma unroll
+        for (int e = 0; e < VN; ++e)
+          sum += left_of((double)w[e], (double)weight(to_f32(qu.x[e])), d.z, tried);
+        continue;
+      }
+    } else {
+      for (int j = 0; j < ngone; ++j) {
+#pragma unroll
+        for (int e = 0; e < VN; ++e)
+          if (d.gone[j] == x + e) w[e] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < VN; ++e) sum += (double)w[e];
+  }
+  for (int64_t x = v1 + thread; x < x1; x += threads) one(x);
+  return sum;
+}
+
+__device__ __forceinline__ double wave_sum(double x) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) x += __shfl_xor(x, off);
+  return x;
+}
+
+// The refused tokens of draft d.at.last that lie in [x0, x1), in d.gone: all
+// of its children, since none stands.
+__device__ __forceinline__ void gone_in(int count, int64_t x0, int64_t x1, Drafts& d) {
+  if (threadIdx.x == 0) d.ngone = 0;
+  __syncthreads();
+  const int last = d.at.last;
+  for (int i = threadIdx.x; i < count; i += blockDim.x)
+    if (d.up[i] == last && d.token[i] >= x0 && d.token[i] < x1)
+      d.gone[atomicAdd(&d.ngone, 1)] = d.token[i];
+  __syncthreads();
+}
+
+__device__ __forceinline__ int count_of(const VerifyArgs& a, int b) {
+  return a.counts != nullptr ? min(max(a.counts[b], 0), a.nodes) : a.nodes;
+}
+
+// Grid (slices, B).
+template <typename T, bool DRAFT>
+__global__ void __launch_bounds__(kSumThreads) verify_sums(VerifyArgs a) {
+  __shared__ Drafts d;
+  __shared__ double part[kSumThreads / 64];
+  const int b = blockIdx.y, s = blockIdx.x, tid = threadIdx.x;
+  const int count = count_of(a, b);
+  const int64_t row0 = (int64_t)b * a.nodes;
+  if (s == 0) {
+    for (int i = tid; i < a.nodes; i += kSumThreads)
+      a.paths[row0 + i] = i == 0 && count > 0 ? 0 : -1;
+    for (int i = tid; i < a.nodes; i += kSumThreads) a.out[row0 + i] = -1;
+  }
+  if (count == 0) {
+    if (s == 0 && tid == 0) a.stands[b] = Stand{0, 0, 0, 0};
+    return;
+  }
+  gather<T>(a, b, count, d);
+  if (tid == 0) {
+    d.at = Stand{0, 1, 0, 1};
+    d.z[0] = 1.0;
+    d.more = false;
+  }
+  __syncthreads();
+  if (tid < 64) {
+    VerifyArgs mine = a;
+    if (s != 0) mine.paths = nullptr;
+    walk(mine, b, count, d);
+  }
+  __syncthreads();
+  const Stand at = d.at;
+  if (s == 0 && tid == 0) a.stands[b] = at;
+  const int64_t x0 = s * a.slice, x1 = min(x0 + a.slice, a.vocab);
+  if (!DRAFT) gone_in(count, x0, x1, d);
+  const int64_t row = (row0 + at.last) * a.vocab;
+  double sum = range_sum<T, DRAFT>((const T*)a.target + row, (const T*)a.draft + row, x0, x1, d,
+                                   at.tried, DRAFT ? 0 : d.ngone, tid, kSumThreads);
+  sum = wave_sum(sum);
+  if ((tid & 63) == 0) part[tid >> 6] = sum;
+  __syncthreads();
+  if (tid == 0) a.sums[(int64_t)b * a.slices + s] = part[0] + part[1] + part[2] + part[3];
+}
+
+// Grid (B).
+template <typename T, bool DRAFT>
+__global__ void __launch_bounds__(kDrawThreads) verify_draw(VerifyArgs a) {
+  constexpr int kWaves = kDrawThreads / 64;
+  __shared__ Drafts d;
+  __shared__ double sums[kMostSlices], part[kWaves];
+  __shared__ int64_t found[kWaves];
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int count = count_of(a, b);
+  const int64_t row0 = (int64_t)b * a.nodes;
+  const Stand first = a.stands[b];
+  if (first.accepted == 0) {
+    if (tid == 0) a.accepted[b] = 0;
+    return;
+  }
+  if (tid < a.slices) sums[tid] = a.sums[(int64_t)b * a.slices + tid];
+  if (tid == 0) {
+    d.at = first;
+    d.z[0] = 1.0;
+    d.more = DRAFT && first.tried > 0;
+    d.ngone = 0;
+  }
+  if (!DRAFT) {  // the refused tokens
+    for (int i = tid; i < count; i += kDrawThreads) {
+      int up = a.parents != nullptr ? a.parents[row0 + i] : i - 1;
+      if (up < 0 || up >= i) up = -1;
+      d.up[i] = up;
+      d.token[i] = a.tokens[row0 + i];
+    }
+  }
+  __syncthreads();
+  auto total = [&] {
+    double z = 0.0;
+    for (int s = 0; s < a.slices; ++s) z += sums[s];
+    return z;
+  };
+  // the sums of all slices by this block alone, a wave a slice
+  auto sum_all = [&](int tried, int ngone) {
+    __syncthreads();
+    const int64_t row = (row0 + d.at.last) * a.vocab;
+    for (int s = wave; s < a.slices; s += kWaves) {
+      const int64_t x0 = s * a.slice, x1 = min(x0 + a.slice, a.vocab);
+      const double sum = wave_sum(range_sum<T, DRAFT>((const T*)a.target + row,
+                                                      (const T*)a.draft + row, x0, x1, d, tried,
+                                                      ngone, lane, 64));
+      if (lane == 0) sums[s] = sum;
+    }
+    __syncthreads();
+  };
+  if constexpr (DRAFT) {
+    bool gathered = false;
+    while (d.more) {
+      // the sum of what the last refusal left is there: try the next child
+      if (!gathered) {
+        gather<T>(a, b, count, d);
+        gathered = true;
+      }
+      const double z = total();
+      __syncthreads();
+      if (tid == 0) d.z[d.at.tried] = z;
+      __syncthreads();
+      const Stand before = d.at;
+      __syncthreads();
+      if (wave == 0) walk(a, b, count, d);
+      __syncthreads();
+      const bool moved = d.at.last != before.last || d.at.tried != before.tried;
+      if (!moved) break;  // no child left: the sums are of this row
+      sum_all(d.at.tried, 0);
+    }
+    __syncthreads();
+  }
+  const Stand at = d.at;
+  int tried = at.tried;
+  double z = total();
+  bool plain = false;  // draw from p itself
+  if (!(z > 0.0) && tried > 0) {
+    plain = true;
+    tried = 0;
+    sum_all(0, 0);
+    z = total();
+  }
+  int64_t token = -1;
+  if (z > 0.0) {
+    const double t = fmax((double)a.uniforms[row0] * z, 0.0);
+    // the slice: the first whose running sum exceeds t, or the last that has any
+    double before = 0.0, run = 0.0;
+    int slice = 0;
+    bool inside = false;
+    for (int s = 0; s < a.slices; ++s) {
+      const double next = run + sums[s];
+      if (sums[s] > 0.0) {
+        slice = s;
+        before = run;
+        if (next > t) {
+          inside = true;
+          break;
+        }
+      }
+      run = next;
+    }
+    const int64_t x0 = slice * a.slice, x1 = min(x0 + a.slice, a.vocab);
+    if (!DRAFT && !plain) gone_in(count, x0, x1, d);
+    const int ngone = DRAFT || plain ? 0 : d.ngone;
+    const int64_t row = (row0 + at.last) * a.vocab;
+    const T* p = (const T*)a.target + row;
+    const T* q = (const T*)a.draft + row;
+    auto left = [&](int64_t x) {
+      float w = weight(to_f32(p[x]));
+      if constexpr (DRAFT) {
+        if (tried > 0) return left_of((double)w, (double)weight(to_f32(q[x])), d.z, tried);
+      } else {
+        for (int j = 0; j < ngone; ++j)
+          if (d.gone[j] == x) w = 0.f;
+      }
+      return (double)w;
+    };
+    // neighbouring tokens to a thread, threads in order
+    const int64_t per = (x1 - x0 + kDrawThreads - 1) / kDrawThreads;
+    const int64_t m0 = min(x0 + tid * per, x1), m1 = min(m0 + per, x1);
+    double mine = 0.0;
+    int64_t some = -1;
+    for (int64_t x = m0; x < m1; ++x) {
+      const double w = left(x);
+      mine += w;
+      if (w > 0.0) some = x;
+    }
+    double upto = mine;  // inclusive, in the wave
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const double o = __shfl_up(upto, off);
+      if (lane >= off) upto += o;
+    }
+    if (lane == 63) part[wave] = upto;
+    __syncthreads();
+    double base = before;
+    for (int w = 0; w < wave; ++w) base += part[w];
+    int64_t hit = INT64_MAX;
+    double c = base + (upto - mine);
+    if (inside && base + upto > t) {
+      for (int64_t x = m0; x < m1; ++x) {
+        const double w = left(x);
+        c += w;
+        if (w > 0.0 && c > t) {
+          hit = x;
+          break;
+        }
+      }
+    }
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) {
+      const int64_t h = __shfl_xor(hit, off), l = __shfl_xor(some, off);
+      hit = h < hit ? h : hit;
+      some = l > some ? l : some;
+    }
+    if (lane == 0) found[wave] = hit;
+    __syncthreads();
+    hit = INT64_MAX;
+    for (int w = 0; w < kWaves; ++w) hit = found[w] < hit ? found[w] : hit;
+    __syncthreads();
+    if (lane == 0) found[wave] = some;
+    __syncthreads();
+    // (rounding alone, or u of 1 and more, leave t behind the last weight)
+    for (int w = 0; w < kWaves; ++w) some = found[w] > some ? found[w] : some;
+    token = hit != INT64_MAX ? hit : some;
+  }
+  if (tid == 0) {
+    a.accepted[b] = at.accepted;
+    a.out[row0 + at.accepted - 1] = (int32_t)token;
+  }
+}
+
+// Slices that give the device enough blocks, of at least 1024 tokens.
+void slicing(int batch, int64_t vocab, int64_t& slice, int& slices) {
+  const int64_t want = std::max(1, std::min(kMostSlices, 2048 / batch));
+  slice = std::max<int64_t>(1024, ((vocab + want - 1) / want + 255) / 256 * 256);
+  slices = (int)((vocab + slice - 1) / slice);
+}
+
+bool sizes_ok(int batch, int nodes, int64_t vocab) {
+  return batch > 0 && batch <= 65535 && nodes > 0 && nodes <= kMostDrafts && vocab > 0 &&
+         vocab <= 0x7fffffff;
+}
+
+template <typename T>
+void launch(const VerifyArgs& a, int batch, hipStream_t s) {
+  const dim3 grid((unsigned)a.slices, (unsigned)batch);
+  if (a.draft != nullptr) {
+    hipLaunchKernelGGL((verify_sums<T, true>), grid, dim3(kSumThreads), 0, s, a);
+    hipLaunchKernelGGL((verify_draw<T, true>), dim3((unsigned)batch), dim3(kDrawThreads), 0, s, a);
+  } else {
+    hipLaunchKernelGGL((verify_sums<T, false>), grid, dim3(kSumThreads), 0, s, a);
+    hipLaunchKernelGGL((verify_draw<T, false>), dim3((unsigned)batch), dim3(kDrawThreads), 0, s, a);
+  }
+}
+
+}  // namespace
+}  // namespace alpx
+
+using namespace alpx;
+
+extern "C" size_t alpx_verify_workspace_bytes(int batch, int nodes, int64_t vocab) {
+  if (!sizes_ok(batch, nodes, vocab)) return 0;
+  int64_t slice;
+  int slices;
+  slicing(batch, vocab, slice, slices);
+  return (size_t)batch * (sizeof(Stand) + (size_t)slices * sizeof(double));
+}
+
+extern "C" int alpx_verify_drafts(const int32_t* tokens, const void* target, const void* draft,
+                                  const int32_t* parents, const int32_t* counts,
+                                  const float* uniforms, int32_t* paths, int32_t* accepted,
+                                  int32_t* new_tokens, void* workspace, size_t workspace_bytes,
+                                  int batch, int nodes, int64_t vocab, int dtype, void* stream) {
+  const char* what = "alpx_verify_drafts";
+  if (!tokens || !target || !uniforms || !paths || !accepted || !new_tokens)
+    return fail(ALPX_EINVAL, "%s: null buffer", what);
+  if (!dtype_ok(dtype)) return fail(ALPX_EINVAL, "%s: unknown dtype", what);
+  if (batch <= 0 || nodes <= 0 || vocab <= 0)
+    return fail(ALPX_EINVAL, "%s: sizes must be positive", what);
+  if (!sizes_ok(batch, nodes, vocab))
+    return fail(ALPX_EUNSUPPORTED, "%s: at most 65535 sequences, %d drafts and 2^31 - 1 tokens",
+                what, kMostDrafts);
+  const size_t need = alpx_verify_workspace_bytes(batch, nodes, vocab);
+  if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15) != 0)
+    return fail(ALPX_EINVAL, "%s: needs %zu bytes of 16-byte aligned workspace", what, need);
+  VerifyArgs a = {};
+  a.tokens = tokens;
+  a.target = target;
+  a.draft = draft;
+  a.parents = parents;
+  a.counts = counts;
+  a.uniforms = uniforms;
+  a.paths = paths;
+  a.accepted = accepted;
+  a.out = new_tokens;
+  a.stands = (Stand*)workspace;
+  a.sums = (double*)((char*)workspace + (size_t)batch * sizeof(Stand));
+  a.vocab = vocab;
+  a.nodes = nodes;
+  slicing(batch, vocab, a.slice, a.slices);
+  hipStream_t s = (hipStream_t)stream;
+  TimedRegion timed(ALPX_T_AUX, s);
+  switch (dtype) {
+    case ALPX_F32: launch<float>(a, batch, s); break;
+    case ALPX_F16: launch<f16_t>(a, batch, s); break;
+    default: launch<bf16_t>(a, batch, s); break;
+  }
+  return check_launch(what);
+}

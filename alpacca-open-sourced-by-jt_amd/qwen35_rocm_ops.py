@@ -168,6 +168,37 @@ class RocmPagedAttentionWorkspace:
         }
 
 
+@dataclass(frozen=True)
+class RocmPagedQ4Workspace:
+    """A paged K/V pool of 4-bit codes (extension): codes ``[num_pages,
+    kv_heads, page_size, dim / 2]`` (uint8; channel c is the low half of byte
+    c / 2 for even c, else the high half) and scales ``[num_pages, kv_heads,
+    2, dim / 32, page_size]`` (float16; steps, then least values).  A channel
+    stands for least + step * code.  Block tables as for a float pool."""
+
+    key_codes: Any
+    key_scales: Any
+    value_codes: Any
+    value_scales: Any
+    page_size: int
+
+    @property
+    def arrays(self) -> tuple[Any, Any, Any, Any]:
+        """The pool as the ``paged_q4_*`` methods take it."""
+        return self.key_codes, self.key_scales, self.value_codes, self.value_scales
+
+    def descriptor(self) -> dict[str, Any]:
+        return {
+            "key_codes": _tensor_descriptor(self.key_codes),
+            "key_scales": _tensor_descriptor(self.key_scales),
+            "value_codes": _tensor_descriptor(self.value_codes),
+            "value_scales": _tensor_descriptor(self.value_scales),
+            "layout": "page,kv_head,row_in_page,channel_pair|page,kv_head,step_least,group,row_in_page",
+            "page_size": self.page_size,
+            "initialization": "deterministic-zero",
+        }
+
+
 class RocmTreeMasks(NamedTuple):
     """Draft trees (extension): visibility words ``masks [batch, nodes,
     ceil(nodes / 64)]`` (int64, bit j % 64 of word j / 64 is draft j),
@@ -190,6 +221,17 @@ class RocmPagedRows(NamedTuple):
     positions: Any
     sequences: Any
     granted: Any
+
+
+class RocmVerifiedDrafts(NamedTuple):
+    """Drafts that stand (extension): ``paths [batch, nodes]``, the
+    ``accepted [batch]`` of them in rising order and -1 behind; ``tokens
+    [batch, nodes]``, the tokens behind each, the drawn one last, and -1
+    behind.  All int32."""
+
+    paths: Any
+    accepted: Any
+    tokens: Any
 
 
 class Qwen35RocmOps:
@@ -1465,6 +1507,267 @@ class Qwen35RocmOps:
             key_pages, value_pages, slots, position_lanes, sections=section,
             frequency_base=_positive_finite("frequency_base", frequency_base),
             eps=_positive_finite("epsilon", epsilon))
+
+    def verify_drafts(self, drafts: Any, target: Any, uniforms: Any, *, parents: Any = None,
+                      draft: Any = None, counts: Any = None) -> RocmVerifiedDrafts:
+        """Which drafted tokens stand (extension), so that the tokens follow
+        the target's distribution.  ``drafts [B, N]`` (int32): draft 0 is the
+        token that the sequence holds already, draft i was proposed behind
+        draft ``parents[b, i]`` (as ``tree_masks``; None: chains, i - 1).
+        ``target [B, N, V]`` holds the target's probabilities behind each
+        draft, ``draft [B, N, V]`` (same dtype) those that its children were
+        drawn from, independently of each other; None: nothing drew them (the
+        likeliest tokens, a lookup).  ``uniforms [B, N]`` (float32, in [0,
+        1)): number i decides draft i, number 0 draws the last token.  From
+        draft 0 on the children are tried in rising order: child j stands if
+        ``uniforms[b, j] * q(x_j) * Z < r(x_j)`` with r = p, Z = 1 at first;
+        else r becomes ``max(r - Z q, 0)``, Z its sum (without ``draft``: q =
+        1 in the test, and x_j leaves r).  Where no child stands the last
+        token is drawn from r.  ``paths`` and ``accepted`` go to
+        ``tree_commit_``; drafts at or past ``counts[b]`` do not count."""
+        torch = self.torch
+        target = self._tensor(target, "target probabilities", dimensions=3)
+        batch, nodes, vocab = _shape(target)
+        if batch <= 0 or vocab <= 0 or not 0 < nodes <= 1024:
+            raise ValueError("a verification takes 1 to 1024 drafts over a vocabulary")
+        if batch > 65535 or vocab >= 2 ** 31:
+            raise ValueError("a verification takes at most 65535 sequences and 2^31 - 1 tokens")
+        if not torch.is_tensor(drafts):
+            raise TypeError("drafted tokens must be a [batch, nodes] int32 tensor")
+        drafts = self._device_ints(drafts, "drafted tokens", (batch, nodes))
+        uniforms = self._tensor(uniforms, "uniform numbers", dimensions=2)
+        if uniforms.dtype != torch.float32:
+            raise TypeError("uniform numbers must use float32")
+        if _shape(uniforms) != (batch, nodes):
+            raise ValueError(f"uniform numbers have {_shape(uniforms)}, expected {(batch, nodes)}")
+        if draft is not None:
+            draft = self._tensor(draft, "draft probabilities", dimensions=3)
+            self._same_shape(draft, target, "draft and target probability")
+            self._same_dtype("draft verification", target, draft)
+        if parents is not None:
+            if not torch.is_tensor(parents):
+                raise TypeError("draft parents must be a [batch, nodes] int32 tensor")
+            parents = self._device_ints(parents, "draft parents", (batch, nodes))
+        if counts is not None:
+            counts = self._device_ints(counts, "draft counts", (batch,), low=0, high=nodes)
+        return RocmVerifiedDrafts(*_ops.verify_drafts(drafts, target, uniforms, parents=parents,
+                                                      draft=draft, counts=counts))
+
+    # --------------------------------------------- packed rows, 4-bit pools
+
+    def _rotary_args(self, query, key, value, slots, positions, rows, rotary_dimension,
+                     frequency_base, style, frequency_scale):
+        """Checks what both rotated appends share; returns the tensors and the
+        rotation."""
+        key = self._tensor(key, "attention key", dimensions=3)
+        value = self._tensor(value, "attention value", dimensions=3)
+        tokens, kv_heads, width = _shape(key)
+        if tokens <= 0:
+            raise ValueError("the append needs at least one token")
+        if _shape(value)[:2] != (tokens, kv_heads):
+            raise ValueError("attention key/value tokens or heads differ")
+        self._same_dtype("rotary append", key, value)
+        if query is not None:
+            query = self._tensor(query, "attention query", dimensions=3)
+            if _shape(query)[0] != tokens or _shape(query)[2] != width:
+                raise ValueError("attention query does not match the key's tokens or head width")
+            if query.shape[1] <= 0 or query.shape[1] % kv_heads:
+                raise ValueError("attention query heads must be a multiple of KV heads")
+            self._same_dtype("rotary append", query, key)
+        slots = self._device_ints(slots, "slots", (tokens,), low=-1, high=rows - 1)
+        rotary = _nonnegative_integer("rotary_dimension", rotary_dimension)
+        if rotary % 2 or rotary > width:
+            raise ValueError("rotary_dimension must be even and at most the head width")
+        if style not in ("norm", "neox"):
+            raise ValueError("rotary style must be 'norm' or 'neox'")
+        if rotary:
+            if positions is None:
+                raise ValueError("a rotation needs positions")
+            frequency_base = _positive_finite("frequency_base", frequency_base)
+            frequency_scale = _positive_finite("frequency_scale", frequency_scale)
+        if positions is not None:
+            positions = self._device_ints(positions, "positions", (tokens,), low=0,
+                                          high=2 ** 31 - 1)
+        return (query, key, value), (slots, positions), dict(
+            rotary_dim=rotary, style=style, frequency_base=frequency_base,
+            frequency_scale=frequency_scale)
+
+    def paged_rotary_append_rows_(self, query: Any, key: Any, value: Any, key_pages: Any,
+                                  value_pages: Any, slots: Any, positions: Any, *,
+                                  rotary_dimension: int, frequency_base: float = 10000.0,
+                                  style: str = "norm", frequency_scale: float = 1.0) -> Any:
+        """Packed tokens of any sequences and positions into a page pool, for
+        heads without a norm of their own (extension;
+        ``paged_attention_prologue_rows_`` is the form of Qwen3.5 heads).  The
+        first ``rotary_dimension`` channels of token t of ``query [T, Hq, D]``
+        (None: keys and values alone) and ``key [T, Hkv, D]`` are turned by
+        ``positions[t]`` (int32): pairs (2 p, 2 p + 1) for ``style`` "norm",
+        (p, p + rotary_dimension / 2) for "neox", as the reference's
+        _rope_norm and _rope_neox (kernels.py:783-817).  Keys and ``value [T,
+        Hkv, Dv]`` go to pool row ``slots[t]`` (int32, page * page_size + row,
+        as ``paged_resize_`` gives them; one outside the pool writes neither;
+        no two tokens may share one).  Returns the turned query."""
+        key_pages = self._tensor(key_pages, "attention key pages", dimensions=4)
+        value_pages = self._tensor(value_pages, "attention value pages", dimensions=4)
+        pages, size, kv_heads, width = _shape(key_pages)
+        if _shape(value_pages)[:3] != (pages, size, kv_heads):
+            raise ValueError("attention K/V pages differ in count, size or heads")
+        rows, places, turn = self._rotary_args(query, key, value, slots, positions, pages * size,
+                                               rotary_dimension, frequency_base, style,
+                                               frequency_scale)
+        if _shape(rows[1])[1:] != (kv_heads, width) or rows[2].shape[2] != value_pages.shape[3]:
+            raise ValueError("attention key/value do not match the page token shape")
+        self._same_dtype("rotary append", rows[1], key_pages, value_pages)
+        return _ops.rotary_append_rows(*rows, key_pages, value_pages, *places, **turn)
+
+    def initialize_paged_q4_workspace(self, *, num_pages: int, page_size: int, kv_heads: int,
+                                      head_dimension: int) -> RocmPagedQ4Workspace:
+        """A zeroed page pool of 4-bit codes (extension): 5 bits a value, head
+        widths 64, 96, 128 and 256."""
+        pages = _positive_integer("num_pages", num_pages)
+        size = _positive_integer("page_size", page_size)
+        if size < 32 or size & (size - 1):
+            raise ValueError("page_size must be a power of two of at least 32")
+        heads = _positive_integer("kv_heads", kv_heads)
+        width = _positive_integer("head_dimension", head_dimension)
+        if width not in (64, 96, 128, 256):
+            raise ValueError("a 4-bit pool takes head widths 64, 96, 128 and 256")
+        if pages * size >= 2 ** 31:
+            raise ValueError("a 4-bit pool holds less than 2^31 rows")
+        t = self.torch
+        arrays = []
+        for _ in range(2):
+            arrays.append(t.zeros((pages, heads, size, width // 2), dtype=t.uint8,
+                                  device=self.device))
+            arrays.append(t.zeros((pages, heads, 2, width // 32, size), dtype=t.float16,
+                                  device=self.device))
+        return RocmPagedQ4Workspace(*arrays, size)
+
+    def _q4_pool(self, key_codes, key_scales, value_codes, value_scales):
+        """The pool's arrays, checked, and ``(pages, kv heads, page size, width)``."""
+        t = self.torch
+        index, shape = self.device_index, getattr(key_codes, "shape", ())
+        if len(shape) == 4:
+            pages, heads, size, half = shape
+            scales = (pages, heads, 2, half // 16, size)
+            if (key_codes.dtype == value_codes.dtype == t.uint8
+                    and key_scales.dtype == value_scales.dtype == t.float16
+                    and value_codes.shape == shape and key_scales.shape == scales
+                    and value_scales.shape == scales and key_codes.get_device() == index
+                    and key_scales.get_device() == index and value_codes.get_device() == index
+                    and value_scales.get_device() == index and key_codes.is_contiguous()
+                    and key_scales.is_contiguous() and value_codes.is_contiguous()
+                    and value_scales.is_contiguous()
+                    and half in (32, 48, 64, 128) and size >= 32 and not size & (size - 1)
+                    and pages > 0 and heads > 0 and pages * size < 2 ** 31):
+                return (key_codes, key_scales, value_codes, value_scales), (pages, heads, size,
+                                                                            2 * half)
+        for name, x, dtype in (("key codes", key_codes, t.uint8),
+                               ("key scales", key_scales, t.float16),
+                               ("value codes", value_codes, t.uint8),
+                               ("value scales", value_scales, t.float16)):
+            if not t.is_tensor(x) or x.dtype != dtype:
+                raise TypeError(f"4-bit pool {name} must be a {dtype} tensor")
+            if x.get_device() != index:
+                raise ValueError(f"4-bit pool {name} must be on device {index}")
+            if not x.is_contiguous():
+                raise ValueError(f"4-bit pool {name} must be contiguous")
+        raise ValueError(
+            "a 4-bit pool has codes [num_pages, kv_heads, page_size, dim / 2] and scales "
+            "[num_pages, kv_heads, 2, dim / 32, page_size], dim 64, 96, 128 or 256, page_size a "
+            "power of two of at least 32 and less than 2^31 rows, alike for K and V")
+
+    def paged_q4_append_rows_(self, query: Any, key: Any, value: Any, key_codes: Any,
+                              key_scales: Any, value_codes: Any, value_scales: Any, slots: Any,
+                              positions: Any, *, rotary_dimension: int,
+                              frequency_base: float = 10000.0, style: str = "norm",
+                              frequency_scale: float = 1.0) -> Any:
+        """``paged_rotary_append_rows_`` into a pool of 4-bit codes
+        (``initialize_paged_q4_workspace``; ``*pool.arrays``): of every 32
+        channels of a key (turned) and a value, least = float16(min), step =
+        float16((max - least) / 15) and the nearest code of (x - least) /
+        step.  Values past 65504 count as 65504; 32 channels that hold an
+        infinity or a NaN read as NaN.  ``rotary_dimension`` 0 (positions None)
+        stores keys that are turned already.  Returns the turned query."""
+        pool, (pages, heads, size, width) = self._q4_pool(key_codes, key_scales, value_codes,
+                                                          value_scales)
+        rows, places, turn = self._rotary_args(query, key, value, slots, positions, pages * size,
+                                               rotary_dimension, frequency_base, style,
+                                               frequency_scale)
+        if _shape(rows[1])[1:] != (heads, width) or rows[2].shape[2] != width:
+            raise ValueError("attention key/value do not match the page token shape")
+        return _ops.q4_append_rows(*rows, pool, *places, **turn)
+
+    def paged_q4_rows(self, key_codes: Any, key_scales: Any, value_codes: Any, value_scales: Any,
+                      slots: Any, *, dtype: Any = None) -> tuple[Any, Any]:
+        """Rows of a 4-bit pool as numbers (extension): ``(key, value)``, each
+        ``[T, Hkv, D]`` in ``dtype`` (float32), of pool rows ``slots [T]``
+        (int32); a slot outside the pool gives zeros.  What a prompt's chunk
+        that goes on from a stored prefix attends to, or a snapshot."""
+        pool, (pages, _, size, _) = self._q4_pool(key_codes, key_scales, value_codes,
+                                                  value_scales)
+        dtype = self.torch.float32 if dtype is None else dtype
+        if dtype not in self._float_dtypes:
+            raise TypeError("rows must be float32, float16 or bfloat16")
+        shape = _shape(slots) if self.torch.is_tensor(slots) else (len(slots),)
+        if len(shape) != 1 or shape[0] <= 0:
+            raise ValueError("slots must name at least one row")
+        slots = self._device_ints(slots, "slots", shape, low=-1, high=pages * size - 1)
+        return _ops.q4_rows(pool, slots, dtype)
+
+    def paged_q4_attention(self, query: Any, key_codes: Any, key_scales: Any, value_codes: Any,
+                           value_scales: Any, block_table: Any, *, length: int, prefix_lens: Any,
+                           counts: Any = None, scale: float | None = None, gate: Any = None,
+                           out_dtype: Any = None, out: Any = None) -> Any:
+        """Attention over a pool of 4-bit codes (extension): token i of
+        ``query [B, N, Hq, D]`` attends to rows ``0 .. prefix_lens[b] + i`` of
+        its sequence, the last of them its own (already stored).  N = 1 is a
+        decode step (``prefix_lens`` = the rows before the token), more a
+        chain of drafts or the end of a prompt; ``counts[b]`` (None: all) of
+        the N tokens count, the rest give zeros.  ``length`` bounds every
+        sequence's rows, new ones included; device lengths past it are
+        clamped, and tokens whose row lies past it give zeros.  The codes
+        enter the products as they are and the steps and least values beside
+        them, so the result is that of the numbers they stand for.  ``out``
+        must not overlap an input.  Returns ``[B, N, Hq, D]``."""
+        pool, (_, heads, size, width) = self._q4_pool(key_codes, key_scales, value_codes,
+                                                      value_scales)
+        query = self._tensor(query, "attention query", dimensions=4)
+        length = _positive_integer("attention cache length", length)
+        batch, nodes, query_heads, query_width = _shape(query)
+        if not self.torch.is_tensor(block_table) or block_table.dim() != 2:
+            raise TypeError("block table must be a [batch, max_pages] int32 tensor")
+        block_table = self._device_ints(block_table, "block table", _shape(block_table))
+        if block_table.shape[0] != batch:
+            raise ValueError("block table batch does not match the query batch")
+        if length > int(block_table.shape[1]) * size:
+            raise ValueError("attention cache length exceeds capacity")
+        if length >= 2 ** 31:
+            raise ValueError("attention cache length exceeds 2^31 rows")
+        if batch <= 0 or nodes <= 0:
+            raise ValueError("attention query must hold at least one token")
+        if query_width != width:
+            raise ValueError("attention query does not match the pool's head width")
+        if query_heads <= 0 or query_heads % heads:
+            raise ValueError("attention query heads must be a multiple of KV heads")
+        if gate is not None:
+            gate = self._tensor(gate, "sigmoid-gate logits", dimensions=4)
+            if _shape(gate) != _shape(query):
+                raise ValueError("sigmoid-gate logits must match the attention output")
+            self._same_dtype("attention gate", query, gate)
+        prefix_lens = self._device_ints(prefix_lens, "prefix_lens", (batch,), low=0, high=length)
+        if counts is not None:
+            counts = self._device_ints(counts, "token counts", (batch,), low=0, high=nodes)
+        if out_dtype is not None and out_dtype not in self._float_dtypes:
+            raise TypeError("attention output must be float32, float16 or bfloat16")
+        if out is not None:
+            self._out_buffer(out, _shape(query), query.dtype if out_dtype is None else out_dtype,
+                             "attention output")
+        scale_value = (1.0 / math.sqrt(width) if scale is None
+                       else _positive_finite("attention scale", scale))
+        return _ops.q4_attention(query, pool, block_table, length=length, prefix_lens=prefix_lens,
+                                 counts=counts, scale=scale_value, gate=gate, out_dtype=out_dtype,
+                                 out=out)
 
     # ------------------------------------------------------ chunked prefill
 

@@ -799,6 +799,123 @@ int alpx_attention_prologue_rows(const void* query_gate, const void* key, const 
                                  void* stream);
 
 /*
+ * Packed tokens into a page pool, a pool of 4-bit codes, and drafted tokens
+ * verified (extensions: the reference keeps one float cache and decodes one
+ * token per sequence).
+ *
+ * alpx_rotary_append_rows: heads without a norm of their own (llama), which
+ * the reference rotates and stores in _rope_store_batch (cuda.py:886-953).
+ * Token t of query [T, Hq, D] (null with q_heads 0: keys and values alone),
+ * key [T, Hkv, D] and value [T, Hkv, Dv] sits at positions[t]; with R =
+ * rotary_dim / 2, pair p < R of a query and a key is turned by positions[t] *
+ * frequency_scale * frequency_base^(-p / R), in float64 reduced to one turn:
+ * channels (2 p, 2 p + 1) (ALPX_ROTARY_NORM, _rope_norm, kernels.py:783-817)
+ * or (p, p + R) (ALPX_ROTARY_NEOX); the channels behind stay.  rotary_dim 0
+ * turns nothing (positions may then be null).  Queries go to query_out, keys
+ * and values to row slots[t] of key_rows [pool_rows, Hkv, D] and value_rows
+ * [pool_rows, Hkv, Dv] (a page pool, page after page); a slot outside [0,
+ * pool_rows) writes neither.  Two tokens must not share a slot.  One dtype;
+ * head dims up to 512.  query_out must not overlap an input.  One launch.
+ */
+enum alpx_rotary_style { ALPX_ROTARY_NORM = 0, ALPX_ROTARY_NEOX = 1 };
+int alpx_rotary_append_rows(const void* query, const void* key, const void* value,
+                            void* query_out, void* key_rows, void* value_rows, int64_t pool_rows,
+                            const int32_t* slots, const int32_t* positions, int dtype, int tokens,
+                            int q_heads, int kv_heads, int head_dim, int value_dim,
+                            int rotary_dim, int style, double frequency_base,
+                            double frequency_scale, void* stream);
+
+/* A pool of 4-bit codes: K and V have two arrays each, codes [num_pages,
+ * kv_heads, page_size, head_dim / 2] bytes (channel c of a row is the low
+ * half of byte c / 2 for even c, else the high half) and scales [num_pages,
+ * kv_heads, 2, head_dim / 32, page_size] float16 (steps, then least values).
+ * A channel stands for least + step * code; 32 channels of a row share step
+ * and least value: 5 bits a value.  page_size a power of two of at least 32,
+ * head_dim 64, 96, 128 or 256, pools of less than 2^31 rows, arrays 16-byte
+ * aligned.
+ *
+ * alpx_q4_append_rows: alpx_rotary_append_rows into such a pool (pool row r
+ * is row r % page_size of page r / page_size).  Of the 32 values of a group
+ * (keys after their turn), least = f16(min), step = f16((max - least) / 15),
+ * code = the nearest of (x - least) / step in 0 .. 15 (ties to even), formed
+ * in float64 and rounded to float16 through float32; values past 65504 count
+ * as 65504.  A group that holds an infinity or a NaN reads as NaN.
+ *
+ * alpx_q4_rows: rows slots[i] of the pool as numbers, step * code + least
+ * rounded once to float32 and then to out_dtype: key_out, value_out [rows,
+ * kv_heads, head_dim], 16-byte aligned.  A slot outside the pool gives zeros.
+ * One launch each. */
+int alpx_q4_append_rows(const void* query, const void* key, const void* value, void* query_out,
+                        void* key_codes, void* key_scales, void* value_codes, void* value_scales,
+                        int page_size, int num_pages, const int32_t* slots,
+                        const int32_t* positions, int dtype, int tokens, int q_heads, int kv_heads,
+                        int head_dim, int rotary_dim, int style, double frequency_base,
+                        double frequency_scale, void* stream);
+int alpx_q4_rows(const void* key_codes, const void* key_scales, const void* value_codes,
+                 const void* value_scales, int page_size, int num_pages, const int32_t* slots,
+                 int rows, int kv_heads, int head_dim, void* key_out, void* value_out,
+                 int out_dtype, void* stream);
+
+/* Attention over a pool of 4-bit codes, for one token of each sequence or a
+ * run of up to `nodes`: sequence b holds prefix_lens[b] rows and behind them
+ * one row for each of its counts[b] tokens (null: `nodes` each), and token i
+ * sees the rows up to and with its own,
+ *   out[b, i, h, :] = softmax_j(scale * q[b, i, h] . K[j, h // G]) . V[j, h // G]
+ *                     (* sigmoid(gate[b, i, h, :]) when gate != NULL), j <= prefix + i,
+ * as alpx_decode_gqa_paged does for one token (nodes 1, prefix_lens = the
+ * rows before it).  q, gate and out [batch, nodes, q_heads, head_dim],
+ * contiguous; pool as above, block_table [batch, max_pages] as
+ * alpx_decode_gqa_paged (an entry outside [0, num_pages) is clamped into the
+ * pool).  prefix_lens and counts are device int32 [batch]; rows are clamped
+ * to [0, length], and nothing behind a sequence's rows is read for its
+ * result.  A token at or past counts[b], and one whose own row lies past
+ * length, give zeros, whatever their gate holds.  NaN in rows that a token
+ * does not see stays out of its result.
+ * workspace: alpx_q4_workspace_bytes bytes (0 for sizes that the call
+ * refuses), 16-byte aligned; scratch, which calls that may overlap must not
+ * share.  out must not overlap any input. */
+size_t alpx_q4_workspace_bytes(int batch, int nodes, int q_heads, int kv_heads, int head_dim,
+                               int length, int dtype);
+int alpx_q4_attention(const void* q, const void* key_codes, const void* key_scales,
+                      const void* value_codes, const void* value_scales,
+                      const int32_t* block_table, int max_pages, int page_size, int num_pages,
+                      const int32_t* prefix_lens, const int32_t* counts, int length,
+                      const void* gate, void* out, void* workspace, size_t workspace_bytes,
+                      int batch, int nodes, int q_heads, int kv_heads, int head_dim, float scale,
+                      int dtype, int out_dtype, void* stream);
+
+/* Which drafted tokens stand, from given random numbers, so that the tokens
+ * follow the target's distribution.  Draft 0 of a sequence is the token that
+ * it holds already; draft i > 0 was proposed behind draft parents[b, i]
+ * (device int32 [batch, nodes]; null: i - 1; outside [0, i): it is never
+ * reached).  target[b, i] and draft[b, i] [batch, nodes, vocab] (`dtype`,
+ * probabilities; entries that are not positive and finite count as 0) are
+ * the distributions of the target and of the proposer behind draft i.  From
+ * draft 0 on, the children of a draft are tried in rising order.  With p, q
+ * its rows, r = p and Z = 1:
+ *   child j stands if uniforms[b, j] * q(x_j) * Z < r(x_j); else r becomes
+ *   max(r - Z q, 0), Z its sum, and the next child is tried;
+ * draft null: the proposals are no draws (the likeliest tokens, a lookup),
+ *   child j stands if uniforms[b, j] * Z < r(x_j); else r(x_j) leaves r and Z.
+ * Children of one draft are taken as independent draws from q.  The walk
+ * goes on from the child that stands; where none does, the last token is the
+ * first x whose running sum of r exceeds uniforms[b, 0] times r's sum (p for
+ * r, if nothing is left of r; -1, if p holds nothing).  All of it in float64.
+ * paths [batch, nodes]: the accepted[b] drafts that stand, draft 0 first, in
+ * rising order (what alpx_tree_commit takes), then -1; new_tokens [batch,
+ * nodes]: the tokens behind each of them, the drawn one last, then -1.
+ * counts[b] drafts of a sequence count (null: all); none: nothing stands and
+ * nothing is drawn.  Tokens outside [0, vocab) weigh 0.  Up to 1024 drafts
+ * and 65535 sequences.  workspace: alpx_verify_workspace_bytes bytes, 16-byte
+ * aligned scratch of the call.  Two launches. */
+size_t alpx_verify_workspace_bytes(int batch, int nodes, int64_t vocab);
+int alpx_verify_drafts(const int32_t* tokens, const void* target, const void* draft,
+                       const int32_t* parents, const int32_t* counts, const float* uniforms,
+                       int32_t* paths, int32_t* accepted, int32_t* new_tokens, void* workspace,
+                       size_t workspace_bytes, int batch, int nodes, int64_t vocab, int dtype,
+                       void* stream);
+
+/*
  * Kernel timing (measurement support, no reference counterpart: it serves
  * the roofline measurement of bench.py).  While enabled, each entry point
  * records a pair of HIP events on its launch stream around the kernel named

@@ -29,10 +29,11 @@ Parity pinning.  The reference ships no tests, golden vectors or fixtures
 for this path, so every oracle function is pinned by closed forms,
 invariants and special cases in ``tests/test_oracle.py`` (each test names
 the mistake it would catch); no function that the reference has a
-counterpart of is left "parity unpinned".  ``oracle.drafts`` has none there:
-``tests/test_oracle_drafts.py`` pins it by hand-written cases.
+counterpart of is left "parity unpinned".  ``oracle.drafts`` and ``oracle.q4``
+have none there: ``tests/test_oracle_drafts.py`` and ``tests/test_oracle_q4.py``
+pin them by hand-written cases.
 """
 
-from . import attention, drafts, gdn, inputs, layer, rope  # noqa: F401
+from . import attention, drafts, gdn, inputs, layer, q4, rope  # noqa: F401
 
-__all__ = ["attention", "drafts", "gdn", "inputs", "layer", "rope"]
+__all__ = ["attention", "drafts", "gdn", "inputs", "layer", "q4", "rope"]
