@@ -7,12 +7,27 @@
 //   j <= prefix + i, K and V = least + step * code,
 // times sigmoid(gate) where given.  Tokens at or past counts[b], and those
 // whose row lies past `length`, give zeros.
+//
+// The matrix products run on the codes themselves.  With g the groups of 32
+// channels, c the codes, d the steps and m the least values,
+//   q . k_j   = sum_g d_jg (q_g . c_jg) + m_jg (sum of q_g),
+//   sum_j p_j v_j = (sum_j (p_j d_jg) c_jg) + (sum_j p_j m_jg)  in group g:
+// a product of 32 channels per group, its result times a step per key; and
+// probabilities times steps against the codes, with the least values as one
+// more small product (whose next row of ones gives the sum of p).  A code is
+// the float16 number c 2^-24 as its bits stand, a subnormal that the matrix
+// unit takes at full rate, so a word of eight codes becomes an operand in
+// five instructions; codes that stay four bits up count 16-fold, which their
+// factors (q, p) take back.  Nothing is rounded but q (float32: two float16
+// parts, 22 bits; others exactly) and p d (two parts).
 #include <math.h>
 
 #include <algorithm>
 
 #include "alpx_common.h"
+#include "prefill_run.h"
 #include "q4_internal.h"
+#include "row_shares.h"
 #include "timing.h"
 
 namespace alpx {
@@ -20,103 +35,767 @@ namespace {
 
 struct Q4Args {
   const void* q;     // [B, N, Hq, D]
-  const uint32_t* kc;
-  const f16_t* ks;
-  const uint32_t* vc;
-  const f16_t* vs;
+  const char* kc;    // codes and scales of the pool
+  const char* ks;
+  const char* vc;
+  const char* vs;
   const int32_t* table;   // [B, max_pages]
   const int32_t* prefix;  // [B]
   const int32_t* counts;  // [B] or null
   const void* gate;       // null, or [B, N, Hq, D]
   void* out;              // [B, N, Hq, D]
   int page_shift, max_pages, num_pages;
-  int length, nodes, q_heads, kv_heads, group, D;
+  int length, batch, nodes, q_heads, kv_heads, group;
+  int col_tiles;      // column tiles per (sequence, kv head)
+  int slots;          // shares of the rows per (kv head, column tile)
+  float* part_o;      // segments of O, [segment, kv head, column][D]
+  float2* part_st;    // reference score and sum of P of their columns
+  int4* found;        // [batch]: first and last slot of a sequence, P, end
   float scale_log2;
   int out_dtype;
+  int vec;            // q, gate and out may be read and written in vectors
 };
 
-constexpr int kThreads = 256, kTile = 256;
+typedef f16_t f16x2 __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
-// One query head of one token per block: a tile of rows, one per thread, for
-// the scores; then a channel per thread for the weighted sum.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) q4_simple_kernel(Q4Args a) {
-  __shared__ float q[256], p[kTile], red[4];
-  const int h = blockIdx.x, i = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
-  const int kvh = h / a.group, per = a.D / 8, groups = a.D / kQ4Group, size = 1 << a.page_shift;
-  const int P = min(max(a.prefix[b], 0), a.length);
-  const int count = a.counts != nullptr ? min(max(a.counts[b], 0), a.nodes) : a.nodes;
-  const int end = i < count && P + i < a.length ? P + i + 1 : 0;
-  const int64_t at = (((int64_t)b * a.nodes + i) * a.q_heads + h) * a.D;
-  if (tid < a.D) q[tid] = to_f32(((const T*)a.q)[at + tid]) * a.scale_log2;
-  __syncthreads();
-  auto place = [&](int j, int64_t& head, int& row) {
-    int page = a.table[(int64_t)b * a.max_pages + (j >> a.page_shift)];
-    page = min(max(page, 0), a.num_pages - 1);
-    head = (int64_t)page * a.kv_heads + kvh;
-    row = j & (size - 1);
+constexpr int kRows = 32;       // rows of a tile
+constexpr int kWaves = 4;       // of a block; they take its tiles in turn
+constexpr float kLift = 12.f;   // P is formed 2^12 times as large: float16 keeps
+constexpr float kSlack = 3.f;   // more of small ones; its reference may lag by 2^3
+
+// Shape of a kernel: T of q, gate and the arithmetic's precision, G groups of
+// 32 channels, CT column tiles of 16 per wave, a ring of RING tiles per wave.
+template <typename T_, int G_, int CT_, int RING_>
+struct Q4Shape {
+  typedef T_ T;
+  static constexpr int G = G_, CT = CT_, RING = RING_, D = 32 * G_;
+  static constexpr int QP = sizeof(T_) == 4 ? 2 : 1;  // parts of q
+  // float32: codes less 8, so that the two sums that make a score or a channel
+  // of the result do not cancel (2e-5 of the result at 1500 rows, which the
+  // rounding of a 16-bit one hides).
+  static constexpr bool kCentred = QP == 2;
+  static constexpr float kUnit = kCentred ? 1.f : 0x1p24f;  // a code of 1 is 1 / kUnit
+  static constexpr float kSumUnit = 64.f / kUnit;            // of the sums of q
+  static constexpr int kCols = 16 * CT;
+  static constexpr int kCodeB = kRows * 16 * G;        // codes of K or V in a tile
+  static constexpr int kScaleB = 2 * G * kRows * 2;    // steps, then least values
+  static constexpr int kTileB = 2 * (kCodeB + kScaleB);
+  static constexpr int kCodeLoads = (kCodeB + 1023) / 1024;
+  static constexpr int kTileLoads = 2 * kCodeLoads + 2;
+  static constexpr int kMergeRow = D + 4;              // floats
+  static constexpr int kMergeB = kWaves * 16 * kMergeRow * 4 + kWaves * kCols * 16;
+  static constexpr int kRingB = kWaves * RING * kTileB;
+  static constexpr int kLds = kRingB > kMergeB ? kRingB : kMergeB;
+  static constexpr int kPerCu = 160 * 1024 / kLds < 2 ? 1 : (G == 2 && CT == 1 ? 3 : 2);
+};
+
+// Units of 16 bytes (a group's 32 codes) of row r stand at u ^ swizzle, which
+// spreads what the lanes of a read take over the banks.  K: one word each of
+// 16 rows and 4 places.  V: half a unit each of rows 4 i .. 4 i + 3 and 16 on
+// for two i at a time.  96 channels: 48-byte rows, spread as they are.
+template <int G>
+__device__ __forceinline__ int k_place(int r, int u) {
+  return G == 2 ? u ^ ((r >> 3) & 1) : G == 4 ? u ^ ((r >> 2) & 3) : G == 8 ? u ^ ((r >> 1) & 7) : u;
+}
+template <int G>
+__device__ __forceinline__ int v_place(int r, int u) {
+  return G == 2   ? u ^ ((r >> 4) & 1)
+         : G == 4 ? u ^ (((r >> 2) & 1) | ((r >> 3) & 2))
+         : G == 8 ? u ^ (((r >> 1) & 3) | ((r >> 2) & 4))
+                  : u;
+}
+
+// Eight codes as an operand: codes 0, 4, 1, 5, 2, 6, 3, 7 of the word, times
+// 2^-24, the second and fourth pair times 2^-20.
+__device__ __forceinline__ f16x8 operand(uint32_t w) {
+  u32x4 r;
+  r[0] = w & 0x000f000fu;
+  r[1] = w & 0x00f000f0u;
+  w >>= 8;
+  r[2] = w & 0x000f000fu;
+  r[3] = w & 0x00f000f0u;
+  return __builtin_bit_cast(f16x8, r);
+}
+// The same less 8, as whole numbers (the second and fourth pair times 16):
+// 1024 + c and 1024 + 16 c as their bits stand, then one exact subtraction.
+__device__ __forceinline__ f16x8 centred_operand(uint32_t w) {
+  auto pair = [](uint32_t bits, f16_t base) __attribute__((always_inline)) {
+    return __builtin_bit_cast(f16x2, bits | 0x64006400u) - (f16x2){base, base};
   };
-  float top = -__builtin_inff(), sum = 0.f, o = 0.f;
-  for (int j0 = 0; j0 < end; j0 += kTile) {
-    float s = -__builtin_inff();
-    if (j0 + tid < end) {
-      int64_t head;
-      int row;
-      place(j0 + tid, head, row);
-      s = 0.f;
-      for (int w = 0; w < per; ++w) {
-        const uint32_t c = a.kc[(head * size + row) * per + w];
-        const f16_t* sc = a.ks + (head * 2 * groups + w / 4) * size + row;
-        const float step = (float)sc[0], least = (float)sc[(int64_t)groups * size];
-        for (int e = 0; e < 8; ++e)
-          s = fmaf(q[8 * w + e], fmaf((float)((c >> (4 * e)) & 15u), step, least), s);
-      }
-    }
-    float m = s;
-    for (int off = 32; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
-    if ((tid & 63) == 0) red[tid >> 6] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), top);
-    const float base = m == -__builtin_inff() ? 0.f : m;
-    const float alpha = top == -__builtin_inff() ? 0.f : fast_exp2(top - base);
-    const float e = j0 + tid < end ? fast_exp2(s - base) : 0.f;
-    p[tid] = e;
-    float t = e;
-    for (int off = 32; off >= 1; off >>= 1) t += __shfl_xor(t, off);
-    __syncthreads();
-    if ((tid & 63) == 0) red[tid >> 6] = t;
-    __syncthreads();
-    sum = sum * alpha + (red[0] + red[1] + red[2] + red[3]);
-    top = m;
-    if (tid < a.D) {
-      o *= alpha;
-      for (int j = 0; j < min(kTile, end - j0); ++j) {
-        int64_t head;
-        int row;
-        place(j0 + j, head, row);
-        const uint32_t c = a.vc[(head * size + row) * per + tid / 8] >> (4 * (tid & 7));
-        const f16_t* sc = a.vs + (head * 2 * groups + tid / kQ4Group) * size + row;
-        const float v = fmaf((float)(c & 15u), (float)sc[0], (float)sc[(int64_t)groups * size]);
-        o = fmaf(p[j], v, o);
-      }
-    }
-    __syncthreads();
-  }
-  if (tid < a.D) {
-    float y = 0.f;
-    if (end > 0) {
-      y = o / sum;
-      if (a.gate != nullptr) y *= fast_sigmoid(to_f32(((const T*)a.gate)[at + tid]));
-    }
-    if (a.out_dtype == ALPX_F32) ((float*)a.out)[at + tid] = y;
-    else if (a.out_dtype == ALPX_F16) ((f16_t*)a.out)[at + tid] = from_f32<f16_t>(y);
-    else ((bf16_t*)a.out)[at + tid] = from_f32<bf16_t>(y);
+  const uint32_t w8 = w >> 8;
+  const f16x2 r0 = pair(w & 0x000f000fu, (f16_t)1032.f), r1 = pair(w & 0x00f000f0u, (f16_t)1152.f);
+  const f16x2 r2 = pair(w8 & 0x000f000fu, (f16_t)1032.f), r3 = pair(w8 & 0x00f000f0u, (f16_t)1152.f);
+  return (f16x8){r0[0], r0[1], r1[0], r1[1], r2[0], r2[1], r3[0], r3[1]};
+}
+constexpr int kOrder[8] = {0, 4, 1, 5, 2, 6, 3, 7};
+
+// gfx950 transposing read of 4-bit elements: lane k of 16 points at 16 of
+// them; lane j receives element j of all 16, lane k's as nibble k.
+__device__ __forceinline__ u32x2 lds_read_tr4x16(const char* p) {
+  typedef int i32x2 __attribute__((ext_vector_type(2)));
+  i32x2 v = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+      (__attribute__((address_space(3))) i32x2*)(p));
+  return __builtin_bit_cast(u32x2, v);
+}
+
+// The largest (and the sum) over the four lanes of a column.
+__device__ __forceinline__ float column_max(float x) {
+  x = fmaxf(x, __shfl_xor(x, 16));
+  return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ float column_sum(float x) {
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
+}
+
+__device__ __forceinline__ float column_weight(float m, float M) { return fast_exp2(m - M); }
+
+template <typename TO>
+__device__ __forceinline__ void store4(TO* p, f32x4 x, bool vec) {
+  typedef TO TO4 __attribute__((ext_vector_type(4)));
+  const TO4 y = {from_f32<TO>(x[0]), from_f32<TO>(x[1]), from_f32<TO>(x[2]), from_f32<TO>(x[3])};
+  if (vec) {
+    *(TO4*)p = y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = y[i];
   }
 }
 
+// Channels c .. c + 3 of a row of the output: O / l, gated; zeros where the
+// token has no row.
+template <typename T>
+__device__ __forceinline__ void write_out(const Q4Args& a, int64_t at, f32x4 o, float l, bool live) {
+  f32x4 y = {0.f, 0.f, 0.f, 0.f};
+  if (live) {
+    const float inv = 1.f / l;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = l == 0.f ? __builtin_nanf("") : o[i] * inv;
+    if (a.gate != nullptr) {
+      const T* g = (const T*)a.gate + at;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] *= fast_sigmoid(to_f32(g[i]));
+    }
+  }
+  switch (a.out_dtype) {
+    case ALPX_F32: store4((float*)a.out + at, y, a.vec); break;
+    case ALPX_F16: store4((f16_t*)a.out + at, y, a.vec); break;
+    default: store4((bf16_t*)a.out + at, y, a.vec);
+  }
+}
+
+// One block per (share of the rows, kv head, column tile): a column is one
+// query head of one token.  Each wave runs alone over its own tiles, with its
+// own ring in LDS, up to the end of a sequence, where the four meet.
+// ALONE: a share is a whole sequence, and there is nothing to join.
+template <typename S, bool ALONE>
+__global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
+  typedef typename S::T T;
+  constexpr int G = S::G, CT = S::CT, QP = S::QP, D = S::D, RING = S::RING;
+  __shared__ __attribute__((aligned(1024))) char smem[S::kLds];
+  const int tid = threadIdx.x, lane = tid & 63, hl = lane & 15, quad = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  // The column tiles of one (slot, kv head) run next to each other on one
+  // XCD, whose L2 then holds the tiles that they all read.
+  const int xcd = blockIdx.x % kXcds, place = blockIdx.x / kXcds;
+  const int ct = place % a.col_tiles;
+  const int unit = (place / a.col_tiles) * kXcds + xcd;
+  const int slot = unit / a.kv_heads, kvh = unit % a.kv_heads;
+  if (slot >= a.slots) return;
+  Share sh;
+  if constexpr (ALONE) {
+    sh = {};
+    sh.b = slot;
+    uniform_rows(a, slot, sh.P, sh.end);
+    sh.tiles = sh.nt = (sh.end + kRows - 1) / kRows;
+  } else {
+    sh = find_share<kRows>(a, slot, unit == 0 && ct == 0 && wave == 0);
+    if (sh.b < 0) return;  // fewer tiles than slots
+  }
+
+  // This lane's parts of a tile's loads: 16 bytes of codes, row L / G, and of
+  // scales, plane L / 4.
+  uint32_t kofs[S::kCodeLoads], vofs[S::kCodeLoads];
+#pragma unroll
+  for (int n = 0; n < S::kCodeLoads; ++n) {
+    const int L = 64 * n + lane, r = L / G, u = L % G;
+    kofs[n] = (uint32_t)(16 * (r * G + k_place<G>(r, u)));
+    vofs[n] = (uint32_t)(16 * (r * G + v_place<G>(r, u)));
+  }
+  const uint32_t sofs = ((uint32_t)(lane >> 2) << (a.page_shift + 1)) + 16u * (lane & 3);
+  const uint32_t plane_span = ((uint32_t)(2 * G - 1) << (a.page_shift + 1)) + 64u;
+  char* const ring = smem + wave * (RING * S::kTileB);
+  const uint32_t lring =
+      (uint32_t)(uintptr_t)(lds_void_t*)smem + (uint32_t)(wave * (RING * S::kTileB));
+
+  for (;;) {
+    const int b = sh.b, P = sh.P, end = sh.end, nt = sh.nt;
+    if (!ALONE && sh.t0 == 0 && kvh == 0 && ct == 0 && tid == 0)
+      a.found[b] = make_int4(slot, sh.s1, P, end);
+    const int32_t* table = a.table + (int64_t)b * a.max_pages;
+    const int first = sh.t0 + wave;                        // this wave's tiles
+    const int mine = (nt - wave + kWaves - 1) / kWaves;
+    auto page_of = [&](int i) __attribute__((always_inline)) {
+      return load_const(table + (((first + kWaves * i) * kRows) >> a.page_shift));
+    };
+    // Asks for tile i of this wave, of page `page`.
+    auto load_tile = [&](int i, int page, int stage) __attribute__((always_inline)) {
+      page = min(max(page, 0), a.num_pages - 1);
+      const int row = ((first + kWaves * i) * kRows) & ((1 << a.page_shift) - 1);
+      const uint64_t head = (uint64_t)((int64_t)page * a.kv_heads + kvh);
+      const uint64_t cofs = ((head << a.page_shift) + row) * (16 * G);
+      const uint64_t pofs = ((head * (2 * G) << a.page_shift) + row) * 2;
+      const uint32_t to = lring + stage * S::kTileB;
+      const i32x4 rk = rsrc_words((uint64_t)(uintptr_t)a.kc + cofs, S::kCodeB);
+      const i32x4 rv = rsrc_words((uint64_t)(uintptr_t)a.vc + cofs, S::kCodeB);
+      const i32x4 sk = rsrc_words((uint64_t)(uintptr_t)a.ks + pofs, plane_span);
+      const i32x4 sv = rsrc_words((uint64_t)(uintptr_t)a.vs + pofs, plane_span);
+      constexpr int kPart = S::kCodeB / 16 % 64;  // lanes of a last, partial load
+#pragma unroll
+      for (int n = 0; n < S::kCodeLoads; ++n)
+        if (kPart == 0 || n + 1 < S::kCodeLoads || lane < kPart)
+          lds_dma16(rk, to + n * 1024, kofs[n]);
+      if (8 * G == 64 || lane < 8 * G) lds_dma16(sk, to + 2 * S::kCodeB, sofs);
+#pragma unroll
+      for (int n = 0; n < S::kCodeLoads; ++n)
+        if (kPart == 0 || n + 1 < S::kCodeLoads || lane < kPart)
+          lds_dma16(rv, to + S::kCodeB + n * 1024, vofs[n]);
+      if (8 * G == 64 || lane < 8 * G) lds_dma16(sv, to + 2 * S::kCodeB + S::kScaleB, sofs);
+    };
+    int next_page = 0;
+#pragma unroll
+    for (int i = 0; i < RING - 1; ++i)
+      if (i < mine) load_tile(i, page_of(i), i);
+    if (RING - 1 < mine) next_page = page_of(RING - 1);
+
+    // The queries, as operands: this lane's octet of every group of its
+    // column's row, scaled by a power of two to a largest value below 2^15.
+    f16x8 q[CT][QP][G];
+    f16x8 qsum[CT];     // sums over groups, in parts: groups `quad` (and quad + 4)
+    float k1[CT];       // what a score is to be multiplied by
+    int lim[CT];        // rows that the column sees; 0: it has none
+    float m[CT];
+    uint32_t nans[CT];  // groups that a row of this column made NaN
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      const int col = ct * S::kCols + 16 * c + hl;
+      const int node = col / a.group;
+      const bool live = node < a.nodes && P + node < end;
+      lim[c] = live ? P + node + 1 : 0;
+      m[c] = -3.0e38f;
+      nans[c] = 0;
+      const int64_t row =
+          ((int64_t)b * a.nodes + (live ? node : 0)) * a.q_heads + kvh * a.group +
+          (live ? col - node * a.group : 0);
+      const T* qp = (const T*)a.q + row * D + 8 * quad;
+      float x[G][8];
+      float most = 0.f;
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        if (a.vec) {
+          typedef T T8 __attribute__((ext_vector_type(8)));
+          const T8 y = *(const T8*)(qp + 32 * g);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[g][e] = to_f32((T)y[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[g][e] = to_f32(qp[32 * g + e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[g][e]));
+      }
+      most = column_max(most);
+      int ex = 0;
+      if (most > 0.f && most < __builtin_inff()) ex = 14 - max(__builtin_amdgcn_frexp_expf(most) - 1, -90);
+      const float f = ldexpf(1.f, ex);
+      k1[c] = ldexpf(a.scale_log2, (S::kCentred ? 0 : 24) - ex);
+      u32x4 sums = {0, 0, 0, 0};
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        float s = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float y = x[g][kOrder[e]] * f;
+          const float z = (e & 2) ? y * 0.0625f : y;
+          const f16_t hi = (f16_t)z;
+          q[c][0][g][e] = hi;
+          float z1 = (float)hi;  // what the products take
+          if constexpr (QP == 2) {
+            const f16_t lo = (f16_t)(z - z1);
+            q[c][1][g][e] = lo;
+            z1 += (float)lo;
+          }
+          s += (e & 2) ? z1 * 16.f : z1;
+        }
+        // the group's sum in units that keep it below 2^14, in three parts
+        s = column_sum(s) * 0.015625f;
+        const f16_t p0 = (f16_t)s, p1 = (f16_t)(s - (float)p0);
+        const f16_t p2 = (f16_t)(s - (float)p0 - (float)p1);
+        const u32x2 w = {__builtin_bit_cast(uint32_t, (f16x2){p0, p1}),
+                         __builtin_bit_cast(uint32_t, (f16x2){p2, p0})};
+        if ((g & 3) == quad) {
+          sums[g / 4 * 2] = w[0];
+          sums[g / 4 * 2 + 1] = w[1];
+        }
+      }
+      qsum[c] = __builtin_bit_cast(f16x8, sums);
+    }
+
+    f32x4 o[CT][2 * G];  // O^T[channel 16 n + 4 quad + r][column], in units of 1 / kUnit
+    f32x4 om[CT];        // rows: the groups' sums of p m, then the sum of p
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      om[c] = (f32x4)(0.f);
+#pragma unroll
+      for (int n = 0; n < 2 * G; ++n) o[c][n] = (f32x4)(0.f);
+    }
+    // byte offsets of this lane's operands in a tile
+    const int kadr = hl * 16 * G + 4 * quad;
+    const int vk = lane & 7;  // keys 4 quad + {0, 2, -, -, 1, 3}, and 16 on: nibbles 0, 1, 4, 5 / 2, 3, 6, 7
+    const int vrow = 4 * quad + ((vk & 1) << 1) + (vk >> 2) + ((vk & 2) << 3);
+    const int vadr = S::kCodeB + vrow * 16 * G + 8 * ((lane >> 3) & 1);
+    const bool has_m = quad < G;
+
+    int stage = 0;
+    for (int i = 0; i < mine; ++i) {
+      // (the reads of the tile before, whose stage this fills, are done)
+      wait_tiles<63 & ~0>();
+      if (i + RING - 1 < mine) {
+        load_tile(i + RING - 1, next_page, stage == 0 ? RING - 1 : stage - 1);
+        next_page = page_of(min(i + RING, mine - 1));
+      }
+      const int left = mine - 1 - i;
+      if (left >= RING - 1) wait_tiles<(RING - 1) * S::kTileLoads>();
+      else if (RING > 3 && left == 2) wait_tiles<2 * S::kTileLoads>();
+      else if (RING > 2 && left == 1) wait_tiles<S::kTileLoads>();
+      else wait_tiles<0>();
+      char* const tile = ring + stage * S::kTileB;
+      const char* const sc_k = tile + 2 * S::kCodeB;
+      char* const sc_v = tile + 2 * S::kCodeB + S::kScaleB;
+      const int key0 = (first + kWaves * i) * kRows;
+      const bool tail = key0 + kRows > P + 1;  // some column does not see all of it
+      if (tail) {
+        // rows past the last: their scales count as zeros; rows that some
+        // columns do not see and that are not finite: set apart
+        uint16_t* s = (uint16_t*)sc_v;
+        bool odd = false;
+        for (int x = lane; x < 2 * G * kRows; x += 64) {
+          if (key0 + (x & (kRows - 1)) >= end) s[x] = 0;
+          odd |= (s[x] & 0x7fff) >= 0x7c00;
+        }
+        if (__ballot(odd) != 0) {
+          for (int r = 0; r < kRows && key0 + r < end; ++r) {
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+              const int sd = s[g * kRows + r] & 0x7fff, sm = s[(G + g) * kRows + r] & 0x7fff;
+              if (sd < 0x7c00 && sm < 0x7c00) continue;
+#pragma unroll
+              for (int c = 0; c < CT; ++c)
+                if (key0 + r < lim[c]) nans[c] |= 1u << g;
+              s[g * kRows + r] = 0;
+              s[(G + g) * kRows + r] = 0;
+            }
+          }
+        }
+        asm volatile("" ::: "memory");
+      }
+
+      // S^T, keys 16 kt + 4 quad + r of the tile
+      float s[CT][8];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        // least values of this lane's groups against the three parts of the
+        // sums, and what is left of least + 8 steps against the first
+        f16x8 mf = {};
+#pragma unroll
+        for (int h = 0; h < (G + 3) / 4; ++h) {
+          const char* mp = sc_k + (G + (has_m ? quad + 4 * h : 0)) * 64 + 2 * (16 * kt + hl);
+          f16_t x = *(const f16_t*)mp, rest = (f16_t)0.f;
+          if constexpr (S::kCentred) {
+            const float y = fmaf((float)*(const f16_t*)(mp - 64 * G), 8.f, (float)x);
+            x = (f16_t)y;
+            rest = (f16_t)(y - (float)x);
+          }
+          if (!has_m) x = rest = (f16_t)0.f;
+          mf[4 * h] = mf[4 * h + 1] = mf[4 * h + 2] = x;
+          mf[4 * h + 3] = rest;
+        }
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+          const f32x4 x = mfma16x16x32(mf, qsum[c], (f32x4)(0.f));
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[c][4 * kt + r] = x[r] * S::kSumUnit;
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          const int row = 16 * kt + hl;
+          const uint32_t w = *(const uint32_t*)(tile + kadr + 256 * G * kt +
+                                                16 * (k_place<G>(row, g)));
+          const f16x8 kx = S::kCentred ? centred_operand(w) : operand(w);
+          const f16x4 d = *(const f16x4*)(sc_k + 64 * g + 32 * kt + 8 * quad);
+#pragma unroll
+          for (int c = 0; c < CT; ++c) {
+            f32x4 x = mfma16x16x32(kx, q[c][0][g], (f32x4)(0.f));
+            if constexpr (QP == 2) x = mfma16x16x32(kx, q[c][1][g], x);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              s[c][4 * kt + r] = fmaf((float)d[r], x[r], s[c][4 * kt + r]);
+          }
+        }
+      }
+      if (tail) {
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (key0 + 16 * (e >> 2) + 4 * quad + (e & 3) >= lim[c]) s[c][e] = -__builtin_inff();
+      }
+
+      // The reference of the probabilities: the largest score so far, less
+      // kSlack, and as much more as V's steps pass 1, so that p d stays in
+      // float16.
+      float lift = 0.f;
+      {
+        const u32x4 x = *(const u32x4*)(sc_v + 16 * (lane < 4 * G ? lane : 0));
+        u16x2 y = __builtin_bit_cast(u16x2, x[0]);
+#pragma unroll
+        for (int e = 1; e < 4; ++e) y = __builtin_elementwise_max(y, __builtin_bit_cast(u16x2, x[e]));
+        y = __builtin_elementwise_sub_sat(y, (u16x2){0x3c00, 0x3c00});
+        if (__ballot(__builtin_bit_cast(uint32_t, y) != 0) != 0) {
+          float most = 0.f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const f16x2 h = __builtin_bit_cast(f16x2, x[e]);
+            most = fmaxf(most, fmaxf(fabsf((float)h[0]), fabsf((float)h[1])));
+          }
+#pragma unroll
+          for (int off = 1; off < 64; off <<= 1) most = fmaxf(most, __shfl_xor(most, off));
+          lift = fminf(fmaxf((float)__builtin_amdgcn_frexp_expf(most), 0.f), 16.f);
+        }
+      }
+      float top[CT];
+      bool over = false;
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        float x = fmaxf(s[c][0], s[c][1]);
+#pragma unroll
+        for (int e = 2; e < 8; ++e) x = fmaxf(x, s[c][e]);
+        top[c] = fmaf(x, k1[c], lift);
+        over |= top[c] > m[c] + kSlack;
+      }
+      if (__ballot(over) != 0) {
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+          // (a whole number: the lift and the weight of what was are exact)
+          const float M = ceilf(fmaxf(m[c], column_max(top[c])));
+          const float w = column_weight(m[c], M);
+          m[c] = M;
+          om[c] *= w;
+#pragma unroll
+          for (int n = 0; n < 2 * G; ++n) o[c][n] *= w;
+        }
+      }
+
+      // P, in float32 and as the high parts of its two; ph16 and p16: the
+      // pairs whose codes count 16-fold, a 16th
+      f16x2 ph[CT][4];
+      f16x8 pl[CT];
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        const float base = kLift - m[c];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[c][e] = fast_exp2(fmaf(s[c][e], k1[c], base));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          ph[c][e] = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(s[c][2 * e], s[c][2 * e + 1]));
+          pl[c][2 * e] = (f16_t)(s[c][2 * e] - (float)ph[c][e][0]);
+          pl[c][2 * e + 1] = (f16_t)(s[c][2 * e + 1] - (float)ph[c][e][1]);
+        }
+      }
+      {  // least values, and the sum of p
+        const char* mp = sc_v + (G + (hl < G ? hl : 0)) * 64 + 8 * quad;
+        const u32x2 m0 = *(const u32x2*)mp, m1 = *(const u32x2*)(mp + 32);
+        constexpr uint32_t kOnes = 0x3c003c00u;
+        f16x8 mf = __builtin_bit_cast(
+            f16x8, (u32x4){hl < G ? m0[0] : kOnes, hl < G ? m0[1] : kOnes, hl < G ? m1[0] : kOnes,
+                           hl < G ? m1[1] : kOnes});
+        f16x8 rest = {};  // centred codes: least + 8 steps, in two parts
+        if constexpr (S::kCentred) {
+          const char* dp = mp - 64 * G;
+          const f16x4 d0 = *(const f16x4*)dp, d1 = *(const f16x4*)(dp + 32);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float d = hl < G ? (float)(e < 4 ? d0[e & 3] : d1[e & 3]) : 0.f;
+            const float x = fmaf(d, 8.f, (float)mf[e]);
+            mf[e] = (f16_t)x;
+            rest[e] = (f16_t)(x - (float)mf[e]);
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+          f16x8 p;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) p[e] = ph[c][e >> 1][e & 1];
+          om[c] = mfma16x16x32(mf, p, om[c]);
+          om[c] = mfma16x16x32(mf, pl[c], om[c]);
+          if constexpr (S::kCentred) om[c] = mfma16x16x32(rest, p, om[c]);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+#pragma unroll
+        for (int e = 1; e < 4; e += 2) {
+          ph[c][e] *= (f16_t)0.0625f;
+          s[c][2 * e] *= 0.0625f;
+          s[c][2 * e + 1] *= 0.0625f;
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const u32x2 w = lds_read_tr4x16(tile + vadr + 16 * v_place<G>(vrow, g));
+        const f16x8 v0 = S::kCentred ? centred_operand(w[0]) : operand(w[0]);
+        const f16x8 v1 = S::kCentred ? centred_operand(w[1]) : operand(w[1]);
+        const f16x4 d0 = *(const f16x4*)(sc_v + 64 * g + 8 * quad);
+        const f16x4 d1 = *(const f16x4*)(sc_v + 64 * g + 32 + 8 * quad);
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+          f16x8 hi, lo;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const f16x4 d = e < 2 ? d0 : d1;
+            const f16x2 dd = {d[2 * (e & 1)], d[2 * (e & 1) + 1]};
+            const f16x2 h = ph[c][e] * dd;
+            hi[2 * e] = h[0];
+            hi[2 * e + 1] = h[1];
+            lo[2 * e] = (f16_t)fmaf(s[c][2 * e], (float)dd[0], -(float)h[0]);
+            lo[2 * e + 1] = (f16_t)fmaf(s[c][2 * e + 1], (float)dd[1], -(float)h[1]);
+          }
+          o[c][2 * g] = mfma16x16x32(v0, hi, o[c][2 * g]);
+          o[c][2 * g + 1] = mfma16x16x32(v1, hi, o[c][2 * g + 1]);
+          o[c][2 * g] = mfma16x16x32(v0, lo, o[c][2 * g]);
+          o[c][2 * g + 1] = mfma16x16x32(v1, lo, o[c][2 * g + 1]);
+        }
+      }
+      stage = stage + 1 == RING ? 0 : stage + 1;
+    }
+
+    // The waves meet: each leaves its reference, its sum and O, with the
+    // least values' part in it.
+    __syncthreads();  // nobody reads tiles any more
+    f32x4* const st = (f32x4*)(smem + kWaves * 16 * S::kMergeRow * 4);
+    const bool whole = ALONE || nt == sh.tiles;
+    const int64_t seg = (((int64_t)(slot + b) * a.kv_heads + kvh) * a.col_tiles + ct) * S::kCols;
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      float* const mo = (float*)smem + (wave * 16 + hl) * S::kMergeRow;
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const float pm = __shfl(om[c][g & 3], (g >> 2) * 16 + hl);
+        const float bad = (nans[c] >> g & 1) ? __builtin_nanf("") : 0.f;
+#pragma unroll
+        for (int n = 2 * g; n < 2 * g + 2; ++n) {
+          f32x4 x;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[r] = fmaf(o[c][n][r], S::kUnit, pm) + bad;
+          *(f32x4*)(mo + 16 * n + 4 * quad) = x;
+        }
+      }
+      const float l = __shfl(om[c][G & 3], (G >> 2) * 16 + hl);
+      if (quad == 0) st[(wave * CT + c) * 16 + hl] = (f32x4){m[c], l, 0.f, 0.f};
+      __syncthreads();
+      for (int x = tid; x < 16 * 8 * G; x += 64 * kWaves) {
+        const int cl = x / (8 * G), ch = 4 * (x - cl * (8 * G));
+        const int col = ct * S::kCols + 16 * c + cl, node = col / a.group;
+        if (node >= a.nodes) continue;
+        float M = -3.0e38f, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) M = fmaxf(M, st[(w * CT + c) * 16 + cl][0]);
+        f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+          const f32x4 v = st[(w * CT + c) * 16 + cl];
+          const float wt = column_weight(v[0], M);
+          sum = fmaf(v[1], wt, sum);
+          y += *(const f32x4*)((float*)smem + (w * 16 + cl) * S::kMergeRow + ch) * wt;
+        }
+        if (whole) {
+          const int64_t row = ((int64_t)b * a.nodes + node) * a.q_heads + kvh * a.group +
+                              (col - node * a.group);
+          write_out<T>(a, row * D + ch, y, sum, P + node < end);
+        } else if (P + node < end) {
+          *(f32x4*)(a.part_o + (seg + 16 * c + cl) * D + ch) = y;
+          if (ch == 0) a.part_st[seg + 16 * c + cl] = make_float2(M, sum);
+        }
+      }
+      __syncthreads();  // the space goes to the next columns, or tiles
+    }
+    if (ALONE || sh.left == 0) return;
+    // the next sequence that has rows
+    do {
+      ++sh.b;
+      uniform_rows(a, sh.b, sh.P, sh.end);
+      sh.tiles = (sh.end + kRows - 1) / kRows;
+    } while (sh.tiles == 0);
+    sh.t0 = 0;
+    sh.nt = min(sh.left, sh.tiles);
+    sh.left -= sh.nt;
+    sh.s1 = slot + (sh.tiles - sh.nt + sh.per - 1) / sh.per;
+  }
+}
+
+// Joins the segments of the sequences that more than one slot has tiles of,
+// and writes zeros for those without a row.  One block per (sequence, kv
+// head, 4 columns): 4 channels a thread, the rest of the threads share the
+// segments and meet in LDS.
+constexpr int kJoinThreads = 512, kJoinCols = 4;
+
+template <typename T, int G>
+__global__ void __launch_bounds__(kJoinThreads) q4_join(Q4Args a, int cols, int tile_cols) {
+  constexpr int D = 32 * G, kItems = kJoinCols * 8 * G, kShare = kJoinThreads / kItems, kFlight = 4;
+  __shared__ f32x4 part[kShare][kItems];
+  __shared__ float2 st[kShare][kJoinCols];
+  const int groups = (cols + kJoinCols - 1) / kJoinCols;
+  const int cg = blockIdx.x % groups;
+  const int kvh = blockIdx.x / groups % a.kv_heads, b = blockIdx.x / groups / a.kv_heads;
+  const int32_t* found = (const int32_t*)(a.found + b);
+  const int s0 = load_const(found), s1 = load_const(found + 1);
+  const int P = load_const(found + 2), end = load_const(found + 3);
+  if (s0 == s1) return;  // written by its slot
+  const int item = threadIdx.x % kItems, w = threadIdx.x / kItems;
+  const int cl = item / (8 * G), ch = 4 * (item - cl * (8 * G));
+  const int col = cg * kJoinCols + cl, node = col / a.group;
+  const bool live = node < a.nodes && P + node < end;
+  float m = -3.0e38f, l = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  if (live && w < kShare) {
+    const int ct = col / tile_cols;
+    auto at = [&](int s) __attribute__((always_inline)) {
+      return (((int64_t)(s + b) * a.kv_heads + kvh) * a.col_tiles + ct) * tile_cols +
+             (col - ct * tile_cols);
+    };
+    for (int s = s0 + w; s <= s1; s += kShare * kFlight) {
+      float2 v[kFlight];
+      f32x4 x[kFlight];
+#pragma unroll
+      for (int u = 0; u < kFlight; ++u) {
+        const int64_t row = at(min(s + kShare * u, s1));  // past the last: again, unused
+        v[u] = a.part_st[row];
+        x[u] = *(const f32x4*)(a.part_o + row * D + ch);
+      }
+      float M = m;
+#pragma unroll
+      for (int u = 0; u < kFlight; ++u)
+        if (s + kShare * u <= s1) M = fmaxf(M, v[u].x);
+      const float c = column_weight(m, M);
+      l *= c;
+      o *= c;
+#pragma unroll
+      for (int u = 0; u < kFlight; ++u) {
+        if (s + kShare * u > s1) continue;
+        const float cu = column_weight(v[u].x, M);
+        l = fmaf(v[u].y, cu, l);
+        o += x[u] * cu;
+      }
+      m = M;
+    }
+  }
+  if (w < kShare) {
+    part[w][item] = o;
+    if (ch == 0) st[w][cl] = make_float2(m, l);
+  }
+  __syncthreads();
+  if (w != 0 || node >= a.nodes) return;
+  float M = -3.0e38f, sum = 0.f;
+#pragma unroll
+  for (int v = 0; v < kShare; ++v) M = fmaxf(M, st[v][cl].x);
+  f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int v = 0; v < kShare; ++v) {
+    const float c = column_weight(st[v][cl].x, M);
+    sum = fmaf(st[v][cl].y, c, sum);
+    y += part[v][item] * c;
+  }
+  const int64_t row =
+      ((int64_t)b * a.nodes + node) * a.q_heads + kvh * a.group + (col - node * a.group);
+  write_out<T>(a, row * D + ch, y, sum, live);
+}
+
+constexpr int kCus = 256;
+
+struct Kernel {
+  const void* fn;
+  const void* alone;  // the same with a slot per sequence
+  const void* join;
+  int cols;    // columns per block
+  int per_cu;  // blocks on a CU at a time
+};
+
+template <typename S>
+Kernel make() {
+  return {(const void*)q4_kernel<S, false>, (const void*)q4_kernel<S, true>,
+          (const void*)q4_join<typename S::T, S::G>, S::kCols, S::kPerCu};
+}
+
+template <typename T>
+Kernel pick(int head_dim, int cols) {
+  const bool few = cols <= 16;
+  switch (head_dim) {
+    case 64: return few ? make<Q4Shape<T, 2, 1, 4>>() : make<Q4Shape<T, 2, 2, 4>>();
+    case 96: return few ? make<Q4Shape<T, 3, 1, 4>>() : make<Q4Shape<T, 3, 2, 4>>();
+    case 128: return few ? make<Q4Shape<T, 4, 1, 4>>() : make<Q4Shape<T, 4, 2, 4>>();
+    default: return make<Q4Shape<T, 8, 1, 2>>();
+  }
+}
+
+constexpr int64_t kAloneTiles = 32;    // of the longest sequence, for one launch
+constexpr int64_t kTilesPerSlot = 8;   // at least, beyond a block a CU
+
+struct Q4Plan {
+  Kernel kernel;
+  int col_tiles, slots;
+  bool alone;
+  size_t segments, bytes;  // columns' segments, bytes in all
+  int64_t blocks, joins;
+};
+
+Q4Plan q4_plan(int batch, int nodes, int q_heads, int kv_heads, int head_dim, int length, int dtype) {
+  Q4Plan p = {};
+  const int cols = nodes * (q_heads / kv_heads);
+  p.kernel = dtype == ALPX_F32   ? pick<float>(head_dim, cols)
+             : dtype == ALPX_F16 ? pick<f16_t>(head_dim, cols)
+                                 : pick<bf16_t>(head_dim, cols);
+  p.col_tiles = (cols + p.kernel.cols - 1) / p.kernel.cols;
+  const int64_t rows = (length + kRows - 1) / kRows;
+  const int64_t tiles = (int64_t)batch * rows;
+  const int64_t units = (int64_t)kv_heads * p.col_tiles;
+  const int64_t share = std::min(kCus * p.kernel.per_cu / units,
+                                 std::max(kCus / units, tiles / kTilesPerSlot));
+  p.slots = (int)std::min(std::max<int64_t>(share, 1), tiles);
+  p.alone = rows <= kAloneTiles;
+  if (p.alone) p.slots = batch;
+  p.blocks = ((int64_t)p.slots * kv_heads + kXcds - 1) / kXcds * kXcds * p.col_tiles;
+  if (p.alone) return p;
+  p.segments = (size_t)(p.slots + batch) * kv_heads * p.col_tiles * p.kernel.cols;
+  p.bytes = p.segments * ((size_t)head_dim * 4 + sizeof(float2)) + (size_t)batch * sizeof(int4);
+  p.joins = (int64_t)batch * kv_heads * ((cols + kJoinCols - 1) / kJoinCols);
+  return p;
+}
+
+// Sums of tiles, also rounded up to whole runs of every slot, and threads of
+// a launch stay in 31 and 32 bits.
 bool sizes_ok(int batch, int nodes, int q_heads, int kv_heads, int head_dim, int length, int dtype) {
-  return batch > 0 && nodes > 0 && q_heads > 0 && kv_heads > 0 && q_heads % kv_heads == 0 &&
-         length > 0 && q4_dim_ok(head_dim) && dtype_ok(dtype) && batch <= 65535 && nodes <= 65535;
+  if (batch <= 0 || nodes <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 ||
+      length <= 0 || !q4_dim_ok(head_dim) || !dtype_ok(dtype))
+    return false;
+  if (length > (1 << 30) || (int64_t)batch * ((int64_t)length / kRows + 1) >= ((int64_t)1 << 31) - 2048)
+    return false;
+  if ((int64_t)nodes * (q_heads / kv_heads) > (1 << 24) || batch > (1 << 24) || kv_heads > (1 << 20))
+    return false;
+  const Q4Plan p = q4_plan(batch, nodes, q_heads, kv_heads, head_dim, length, dtype);
+  return p.blocks * 64 * kWaves <= 0xffffffff && p.joins * kJoinThreads <= 0xffffffff;
 }
 
 }  // namespace
@@ -127,7 +806,7 @@ using namespace alpx;
 extern "C" size_t alpx_q4_workspace_bytes(int batch, int nodes, int q_heads, int kv_heads,
                                           int head_dim, int length, int dtype) {
   if (!sizes_ok(batch, nodes, q_heads, kv_heads, head_dim, length, dtype)) return 0;
-  return 0;
+  return q4_plan(batch, nodes, q_heads, kv_heads, head_dim, length, dtype).bytes;
 }
 
 extern "C" int alpx_q4_attention(const void* q, const void* key_codes, const void* key_scales,
@@ -153,11 +832,12 @@ extern "C" int alpx_q4_attention(const void* q, const void* key_codes, const voi
     return fail(ALPX_EINVAL, "page_size must be a power of two of at least 32");
   if ((int64_t)num_pages * page_size > 0x7fffffff || (int64_t)max_pages * page_size > 0x7fffffff)
     return fail(ALPX_EUNSUPPORTED, "%s: 2^31 rows or more", what);
+  if (page_size > 1 << 24) return fail(ALPX_EUNSUPPORTED, "%s: pages of more than 2^24 rows", what);
   if (length > (int64_t)max_pages * page_size)
     return fail(ALPX_ERANGE, "%s: length exceeds the block table", what);
   if (!(scale > 0.f) || !isfinite(scale)) return fail(ALPX_EINVAL, "scale must be positive and finite");
   if (!sizes_ok(batch, nodes, q_heads, kv_heads, head_dim, length, dtype))
-    return fail(ALPX_EUNSUPPORTED, "%s: at most 65535 sequences and tokens of one", what);
+    return fail(ALPX_EUNSUPPORTED, "%s: too many rows, tokens or sequences", what);
   if ((((uintptr_t)key_codes | (uintptr_t)value_codes | (uintptr_t)key_scales |
         (uintptr_t)value_scales) & 15) != 0)
     return fail(ALPX_EINVAL, "%s: codes and scales must be 16-byte aligned", what);
@@ -169,12 +849,13 @@ extern "C" int alpx_q4_attention(const void* q, const void* key_codes, const voi
   const size_t need = alpx_q4_workspace_bytes(batch, nodes, q_heads, kv_heads, head_dim, length, dtype);
   if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15) != 0))
     return fail(ALPX_EINVAL, "%s: needs %zu bytes of 16-byte aligned workspace", what, need);
+  const Q4Plan p = q4_plan(batch, nodes, q_heads, kv_heads, head_dim, length, dtype);
   Q4Args a = {};
   a.q = q;
-  a.kc = (const uint32_t*)key_codes;
-  a.ks = (const f16_t*)key_scales;
-  a.vc = (const uint32_t*)value_codes;
-  a.vs = (const f16_t*)value_scales;
+  a.kc = (const char*)key_codes;
+  a.ks = (const char*)key_scales;
+  a.vc = (const char*)value_codes;
+  a.vs = (const char*)value_scales;
   a.table = block_table;
   a.prefix = prefix_lens;
   a.counts = counts;
@@ -184,20 +865,30 @@ extern "C" int alpx_q4_attention(const void* q, const void* key_codes, const voi
   a.max_pages = max_pages;
   a.num_pages = num_pages;
   a.length = length;
+  a.batch = batch;
   a.nodes = nodes;
   a.q_heads = q_heads;
   a.kv_heads = kv_heads;
   a.group = q_heads / kv_heads;
-  a.D = head_dim;
+  a.col_tiles = p.col_tiles;
+  a.slots = p.slots;
   a.scale_log2 = scale * kLog2e;
   a.out_dtype = out_dtype;
+  a.vec = (((uintptr_t)q | (uintptr_t)out) & 15) == 0;
+  a.part_o = (float*)workspace;
+  a.part_st = (float2*)(a.part_o + p.segments * head_dim);
+  a.found = (int4*)(a.part_st + p.segments);
   hipStream_t s = (hipStream_t)stream;
-  TimedRegion timed(ALPX_T_DECODE, s);
-  const dim3 grid((unsigned)q_heads, (unsigned)nodes, (unsigned)batch);
-  switch (dtype) {
-    case ALPX_F32: hipLaunchKernelGGL(q4_simple_kernel<float>, grid, dim3(kThreads), 0, s, a); break;
-    case ALPX_F16: hipLaunchKernelGGL(q4_simple_kernel<f16_t>, grid, dim3(kThreads), 0, s, a); break;
-    default: hipLaunchKernelGGL(q4_simple_kernel<bf16_t>, grid, dim3(kThreads), 0, s, a);
+  {
+    TimedRegion timed(ALPX_T_DECODE, s);
+    void* args[] = {&a};
+    (void)hipLaunchKernel(p.alone ? p.kernel.alone : p.kernel.fn, dim3((unsigned)p.blocks),
+                          dim3(64 * kWaves), args, 0, s);
   }
+  if (p.alone) return check_launch(what);
+  TimedRegion timed(ALPX_T_DECODE_COMBINE, s);
+  int cols = nodes * a.group, tile_cols = p.kernel.cols;
+  void* args[] = {&a, &cols, &tile_cols};
+  (void)hipLaunchKernel(p.kernel.join, dim3((unsigned)p.joins), dim3(kJoinThreads), args, 0, s);
   return check_launch(what);
 }

@@ -110,6 +110,7 @@ def test_attention_refusals(L):
     _refused(L, name, ATTEND, "EINVAL", "multiple of KV heads", q_heads=7)
     _refused(L, name, ATTEND, "ERANGE", "block table", length=129)
     _refused(L, name, ATTEND, "EUNSUPPORTED", "2^31", max_pages=1 << 26)
+    _refused(L, name, ATTEND, "EUNSUPPORTED", "2^24", page_size=1 << 25)
     for key in ("dtype", "out_dtype"):
         for value in (-1, 3):
             _refused(L, name, ATTEND, "EINVAL", "dtype", **{key: value})
@@ -119,6 +120,27 @@ def test_attention_refusals(L):
     for at in (FAKE, FAKE + q - 2, FAKE - q + 2):
         _refused(L, name, ATTEND, "EINVAL", "overlap", out=at)
         _refused(L, name, ATTEND, "EINVAL", "overlap", q=FAR * 2, gate=FAKE, out=at)
+
+
+def test_attention_workspace(L):
+    name, size = "alpx_q4_attention", L.lib().alpx_q4_workspace_bytes
+    # sizes whose counts pass 31 bits, and no workspace that they would take
+    good = dict(batch=2, nodes=3, q_heads=8, kv_heads=2, head_dim=128, length=4000, dtype=1)
+    long = dict(ATTEND, length=4000, max_pages=1 << 20, out=1 << 60)
+    assert size(*good.values()) > 0
+    need = size(*good.values())
+    _refused(L, name, long, "EINVAL", "workspace", ws=None)
+    _refused(L, name, long, "EINVAL", "workspace", ws_bytes=need - 1)
+    _refused(L, name, long, "EINVAL", "workspace", ws=FAKE + 8)
+    for bad in (dict(batch=(1 << 24) + 1), dict(nodes=1 << 24), dict(length=2 ** 31 - 40),
+                dict(q_heads=1 << 20, nodes=60000), dict(batch=60000, length=1 << 24),
+                dict(batch=1 << 20, nodes=1 << 10, q_heads=1 << 10, kv_heads=1 << 10)):
+        _refused(L, name, dict(long, max_pages=(2 ** 31 - 32) // 32), "EUNSUPPORTED", "too many",
+                 **bad)
+        assert size(*dict(good, **bad).values()) == 0
+    for bad in (dict(batch=0), dict(nodes=-1), dict(q_heads=7), dict(kv_heads=0),
+                dict(head_dim=80), dict(length=0), dict(dtype=9)):
+        assert size(*dict(good, **bad).values()) == 0
 
 
 def test_verify_refusals(L):
