@@ -60,21 +60,23 @@ typedef f16_t f16x2 __attribute__((ext_vector_type(2)));
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
-constexpr int kRows = 32;       // rows of a tile
-constexpr int kWaves = 4;       // of a block; they take its tiles in turn
+constexpr int kRows = 32;       // rows of a tile, all of one page
+constexpr int kWaves = 4;       // of a block; they take its steps in turn
 constexpr float kLift = 12.f;   // P is formed 2^12 times as large: float16 keeps
 constexpr float kSlack = 3.f;   // more of small ones; its reference may lag by 2^3
 
 // Shape of a kernel: T of q, gate and the arithmetic's precision, G groups of
-// 32 channels, CT column tiles of 16 per wave, a ring of RING tiles per wave.
-template <typename T_, int G_, int CT_, int RING_>
+// 32 channels, CT column tiles of 16 per wave, TP tiles to a step, a ring of
+// RING steps per wave, blocks per CU.
+template <typename T_, int G_, int CT_, int TP_, int RING_, int CU_>
 struct Q4Shape {
   typedef T_ T;
-  static constexpr int G = G_, CT = CT_, RING = RING_, D = 32 * G_;
+  static constexpr int G = G_, CT = CT_, TP = TP_, RING = RING_, D = 32 * G_, kPerCu = CU_;
   static constexpr int QP = sizeof(T_) == 4 ? 2 : 1;  // parts of q
   // float32: codes less 8, so that the two sums that make a score or a channel
   // of the result do not cancel (2e-5 of the result at 1500 rows, which the
   // rounding of a 16-bit one hides).
+  static constexpr bool kOnce = CT == 1;  // one column tile: nobody reads a tile twice
   static constexpr bool kCentred = QP == 2;
   static constexpr float kUnit = kCentred ? 1.f : 0x1p24f;  // a code of 1 is 1 / kUnit
   static constexpr float kSumUnit = 64.f / kUnit;            // of the sums of q
@@ -83,12 +85,14 @@ struct Q4Shape {
   static constexpr int kScaleB = 2 * G * kRows * 2;    // steps, then least values
   static constexpr int kTileB = 2 * (kCodeB + kScaleB);
   static constexpr int kCodeLoads = (kCodeB + 1023) / 1024;
-  static constexpr int kTileLoads = 2 * kCodeLoads + 2;
+  static constexpr int kStepLoads = TP * (2 * kCodeLoads + 2);
+  static constexpr int kStepRows = TP * kRows;
+  static constexpr int kStepB = TP * kTileB;
   static constexpr int kMergeRow = D + 4;              // floats
   static constexpr int kMergeB = kWaves * 16 * kMergeRow * 4 + kWaves * kCols * 16;
-  static constexpr int kRingB = kWaves * RING * kTileB;
+  static constexpr int kRingB = kWaves * RING * kStepB;
   static constexpr int kLds = kRingB > kMergeB ? kRingB : kMergeB;
-  static constexpr int kPerCu = 160 * 1024 / kLds < 2 ? 1 : (G == 2 && CT == 1 ? 3 : 2);
+  static_assert(kLds * kPerCu <= 160 * 1024, "blocks fit a CU");
 };
 
 // Units of 16 bytes (a group's 32 codes) of row r stand at u ^ swizzle, which
@@ -138,6 +142,21 @@ __device__ __forceinline__ u32x2 lds_read_tr4x16(const char* p) {
   i32x2 v = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
       (__attribute__((address_space(3))) i32x2*)(p));
   return __builtin_bit_cast(u32x2, v);
+}
+
+// (by value: a bit cast of a vector's element in place reads its element 0)
+__device__ __forceinline__ f16x2 halves(uint32_t x) { return __builtin_bit_cast(f16x2, x); }
+__device__ __forceinline__ u16x2 bits16(uint32_t x) { return __builtin_bit_cast(u16x2, x); }
+
+__device__ __forceinline__ f16x8 four(const f16x2* x) {
+  return (f16x8){x[0][0], x[0][1], x[1][0], x[1][1], x[2][0], x[2][1], x[3][0], x[3][1]};
+}
+
+// (left to itself the compiler first makes every operand canonical)
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+  return r;
 }
 
 // The largest (and the sum) over the four lanes of a column.
@@ -193,7 +212,7 @@ __device__ __forceinline__ void write_out(const Q4Args& a, int64_t at, f32x4 o, 
 template <typename S, bool ALONE>
 __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
   typedef typename S::T T;
-  constexpr int G = S::G, CT = S::CT, QP = S::QP, D = S::D, RING = S::RING;
+  constexpr int G = S::G, CT = S::CT, TP = S::TP, QP = S::QP, D = S::D, RING = S::RING;
   __shared__ __attribute__((aligned(1024))) char smem[S::kLds];
   const int tid = threadIdx.x, lane = tid & 63, hl = lane & 15, quad = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -203,16 +222,16 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
   const int xcd = blockIdx.x % kXcds, place = blockIdx.x / kXcds;
   const int ct = place % a.col_tiles;
   const int unit = (place / a.col_tiles) * kXcds + xcd;
-  const int slot = unit / a.kv_heads, kvh = unit % a.kv_heads;
-  if (slot >= a.slots) return;
+  const int kvh = unit / a.slots, slot = unit % a.slots;
+  if (kvh >= a.kv_heads) return;
   Share sh;
   if constexpr (ALONE) {
     sh = {};
     sh.b = slot;
     uniform_rows(a, slot, sh.P, sh.end);
-    sh.tiles = sh.nt = (sh.end + kRows - 1) / kRows;
+    sh.tiles = sh.nt = (sh.end + S::kStepRows - 1) / S::kStepRows;
   } else {
-    sh = find_share<kRows>(a, slot, unit == 0 && ct == 0 && wave == 0);
+    sh = find_share<S::kStepRows>(a, slot, unit == 0 && ct == 0 && wave == 0);
     if (sh.b < 0) return;  // fewer tiles than slots
   }
 
@@ -227,49 +246,68 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
   }
   const uint32_t sofs = ((uint32_t)(lane >> 2) << (a.page_shift + 1)) + 16u * (lane & 3);
   const uint32_t plane_span = ((uint32_t)(2 * G - 1) << (a.page_shift + 1)) + 64u;
-  char* const ring = smem + wave * (RING * S::kTileB);
+  char* const ring = smem + wave * (RING * S::kStepB);
   const uint32_t lring =
-      (uint32_t)(uintptr_t)(lds_void_t*)smem + (uint32_t)(wave * (RING * S::kTileB));
+      (uint32_t)(uintptr_t)(lds_void_t*)smem + (uint32_t)(wave * (RING * S::kStepB));
 
   for (;;) {
     const int b = sh.b, P = sh.P, end = sh.end, nt = sh.nt;
     if (!ALONE && sh.t0 == 0 && kvh == 0 && ct == 0 && tid == 0)
       a.found[b] = make_int4(slot, sh.s1, P, end);
     const int32_t* table = a.table + (int64_t)b * a.max_pages;
-    const int first = sh.t0 + wave;                        // this wave's tiles
+    const int first = sh.t0 + wave;                        // this wave's steps
     const int mine = (nt - wave + kWaves - 1) / kWaves;
-    auto page_of = [&](int i) __attribute__((always_inline)) {
-      return load_const(table + (((first + kWaves * i) * kRows) >> a.page_shift));
+    const int last_row = max(end - 1, 0);
+    auto row_of = [&](int i, int u) __attribute__((always_inline)) {
+      return min((first + kWaves * i) * S::kStepRows + u * kRows, last_row & -kRows);
     };
-    // Asks for tile i of this wave, of page `page`.
-    auto load_tile = [&](int i, int page, int stage) __attribute__((always_inline)) {
-      page = min(max(page, 0), a.num_pages - 1);
-      const int row = ((first + kWaves * i) * kRows) & ((1 << a.page_shift) - 1);
-      const uint64_t head = (uint64_t)((int64_t)page * a.kv_heads + kvh);
-      const uint64_t cofs = ((head << a.page_shift) + row) * (16 * G);
-      const uint64_t pofs = ((head * (2 * G) << a.page_shift) + row) * 2;
-      const uint32_t to = lring + stage * S::kTileB;
-      const i32x4 rk = rsrc_words((uint64_t)(uintptr_t)a.kc + cofs, S::kCodeB);
-      const i32x4 rv = rsrc_words((uint64_t)(uintptr_t)a.vc + cofs, S::kCodeB);
-      const i32x4 sk = rsrc_words((uint64_t)(uintptr_t)a.ks + pofs, plane_span);
-      const i32x4 sv = rsrc_words((uint64_t)(uintptr_t)a.vs + pofs, plane_span);
-      constexpr int kPart = S::kCodeB / 16 % 64;  // lanes of a last, partial load
-#pragma unroll
-      for (int n = 0; n < S::kCodeLoads; ++n)
-        if (kPart == 0 || n + 1 < S::kCodeLoads || lane < kPart)
-          lds_dma16(rk, to + n * 1024, kofs[n]);
-      if (8 * G == 64 || lane < 8 * G) lds_dma16(sk, to + 2 * S::kCodeB, sofs);
-#pragma unroll
-      for (int n = 0; n < S::kCodeLoads; ++n)
-        if (kPart == 0 || n + 1 < S::kCodeLoads || lane < kPart)
-          lds_dma16(rv, to + S::kCodeB + n * 1024, vofs[n]);
-      if (8 * G == 64 || lane < 8 * G) lds_dma16(sv, to + 2 * S::kCodeB + S::kScaleB, sofs);
+    struct Pages {
+      int p[TP];
     };
-    int next_page = 0;
+    auto pages_of = [&](int i) __attribute__((always_inline)) {
+      Pages r;
+#pragma unroll
+      for (int u = 0; u < TP; ++u) r.p[u] = load_const(table + (row_of(i, u) >> a.page_shift));
+      return r;
+    };
+    // (the nontemporal hint on codes that no other block reads: 4 x 1 on 131072
+    // rows, 32/8 heads of 128, 153 -> 143 us; on the scales too, the same)
+    auto load = [](i32x4 r, uint32_t lds, uint32_t ofs) __attribute__((always_inline)) {
+      if constexpr (S::kOnce) lds_dma16_once(r, lds, ofs);
+      else lds_dma16(r, lds, ofs);
+    };
+    // Asks for step i of this wave; tiles behind the last row bring the last one.
+    auto load_step = [&](int i, Pages pages, int stage) __attribute__((always_inline)) {
+#pragma unroll
+      for (int u = 0; u < TP; ++u) {
+        const int page = min(max(pages.p[u], 0), a.num_pages - 1);
+        const int row = row_of(i, u) & ((1 << a.page_shift) - 1);
+        const uint64_t head = (uint64_t)((int64_t)page * a.kv_heads + kvh);
+        const uint64_t cofs = ((head << a.page_shift) + row) * (16 * G);
+        const uint64_t pofs = ((head * (2 * G) << a.page_shift) + row) * 2;
+        const uint32_t to = lring + stage * S::kStepB + u * S::kTileB;
+        const i32x4 rk = rsrc_words((uint64_t)(uintptr_t)a.kc + cofs, S::kCodeB);
+        const i32x4 rv = rsrc_words((uint64_t)(uintptr_t)a.vc + cofs, S::kCodeB);
+        const i32x4 sk = rsrc_words((uint64_t)(uintptr_t)a.ks + pofs, plane_span);
+        const i32x4 sv = rsrc_words((uint64_t)(uintptr_t)a.vs + pofs, plane_span);
+        constexpr int kPart = S::kCodeB / 16 % 64;  // lanes of a last, partial load
+#pragma unroll
+        for (int n = 0; n < S::kCodeLoads; ++n)
+          if (kPart == 0 || n + 1 < S::kCodeLoads || lane < kPart)
+            load(rk, to + n * 1024, kofs[n]);
+        if (8 * G == 64 || lane < 8 * G) lds_dma16(sk, to + 2 * S::kCodeB, sofs);
+#pragma unroll
+        for (int n = 0; n < S::kCodeLoads; ++n)
+          if (kPart == 0 || n + 1 < S::kCodeLoads || lane < kPart)
+            load(rv, to + S::kCodeB + n * 1024, vofs[n]);
+        if (8 * G == 64 || lane < 8 * G) lds_dma16(sv, to + 2 * S::kCodeB + S::kScaleB, sofs);
+      }
+    };
+    Pages next_pages = {};
 #pragma unroll
     for (int i = 0; i < RING - 1; ++i)
-      if (i < mine) load_tile(i, page_of(i), i);
-    if (RING - 1 < mine) next_page = page_of(RING - 1);
+      if (i < mine) load_step(i, pages_of(i), i);
+    if (RING - 1 < mine) next_pages = pages_of(RING - 1);
 
     // The queries, as operands: this lane's octet of every group of its
     // column's row, scaled by a power of two to a largest value below 2^15.
@@ -353,96 +391,112 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
       for (int n = 0; n < 2 * G; ++n) o[c][n] = (f32x4)(0.f);
     }
     // byte offsets of this lane's operands in a tile
-    const int kadr = hl * 16 * G + 4 * quad;
-    const int vk = lane & 7;  // keys 4 quad + {0, 2, -, -, 1, 3}, and 16 on: nibbles 0, 1, 4, 5 / 2, 3, 6, 7
+    int kadr[G], vadr[G];
+    const int vk = lane & 7;  // nibbles 0, 4 / 1, 5 / 2, 6 / 3, 7: keys 4 quad + 0 .. 3, and 16 on
     const int vrow = 4 * quad + ((vk & 1) << 1) + (vk >> 2) + ((vk & 2) << 3);
-    const int vadr = S::kCodeB + vrow * 16 * G + 8 * ((lane >> 3) & 1);
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      kadr[g] = hl * 16 * G + 16 * k_place<G>(hl, g) + 4 * quad;  // (row hl + 16: the same place)
+      vadr[g] = S::kCodeB + vrow * 16 * G + 16 * v_place<G>(vrow, g) + 8 * ((lane >> 3) & 1);
+    }
     const bool has_m = quad < G;
+    const int mk = (has_m ? quad : 0) * 64 + 2 * hl;         // least values of K, from plane G on
+    const int mv = (G + (hl < G ? hl : 0)) * 64 + 8 * quad;  // and of V
+    const int dadr = 8 * quad;                               // steps of four keys
 
-    int stage = 0;
-    for (int i = 0; i < mine; ++i) {
-      // (the reads of the tile before, whose stage this fills, are done)
-      wait_tiles<63 & ~0>();
+    // Step i, which lies in stage `stage` of the ring (a constant: offsets in
+    // the ring are then part of the LDS instructions).
+    auto step = [&](auto stage_, int i) __attribute__((always_inline)) {
+      constexpr int stage = decltype(stage_)::value;
+      // (the reads of the step before, whose stage this fills, are done)
+      wait_tiles<63>();
       if (i + RING - 1 < mine) {
-        load_tile(i + RING - 1, next_page, stage == 0 ? RING - 1 : stage - 1);
-        next_page = page_of(min(i + RING, mine - 1));
+        load_step(i + RING - 1, next_pages, (stage + RING - 1) % RING);
+        next_pages = pages_of(min(i + RING, mine - 1));
       }
       const int left = mine - 1 - i;
-      if (left >= RING - 1) wait_tiles<(RING - 1) * S::kTileLoads>();
-      else if (RING > 3 && left == 2) wait_tiles<2 * S::kTileLoads>();
-      else if (RING > 2 && left == 1) wait_tiles<S::kTileLoads>();
+      if (left >= RING - 1) wait_tiles<(RING - 1) * S::kStepLoads>();
+      else if (RING > 3 && left == 2) wait_tiles<2 * S::kStepLoads>();
+      else if (RING > 2 && left == 1) wait_tiles<S::kStepLoads>();
       else wait_tiles<0>();
-      char* const tile = ring + stage * S::kTileB;
-      const char* const sc_k = tile + 2 * S::kCodeB;
-      char* const sc_v = tile + 2 * S::kCodeB + S::kScaleB;
-      const int key0 = (first + kWaves * i) * kRows;
-      const bool tail = key0 + kRows > P + 1;  // some column does not see all of it
+      char* const tiles = ring + stage * S::kStepB;
+      const int key0 = (first + kWaves * i) * S::kStepRows;
+      const bool tail = key0 + S::kStepRows > P + 1;  // some column does not see all of it
       if (tail) {
         // rows past the last: their scales count as zeros; rows that some
         // columns do not see and that are not finite: set apart
-        uint16_t* s = (uint16_t*)sc_v;
-        bool odd = false;
-        for (int x = lane; x < 2 * G * kRows; x += 64) {
-          if (key0 + (x & (kRows - 1)) >= end) s[x] = 0;
-          odd |= (s[x] & 0x7fff) >= 0x7c00;
-        }
-        if (__ballot(odd) != 0) {
-          for (int r = 0; r < kRows && key0 + r < end; ++r) {
 #pragma unroll
-            for (int g = 0; g < G; ++g) {
-              const int sd = s[g * kRows + r] & 0x7fff, sm = s[(G + g) * kRows + r] & 0x7fff;
-              if (sd < 0x7c00 && sm < 0x7c00) continue;
+        for (int u = 0; u < TP; ++u) {
+          uint16_t* s = (uint16_t*)(tiles + u * S::kTileB + 2 * S::kCodeB + S::kScaleB);
+          const int rows = end - key0 - kRows * u;
+          bool odd = false;
+          for (int x = lane; x < 2 * G * kRows; x += 64) {
+            if ((x & (kRows - 1)) >= rows) s[x] = 0;
+            odd |= (s[x] & 0x7fff) >= 0x7c00;
+          }
+          if (__ballot(odd) != 0) {
+            for (int r = 0; r < kRows && r < rows; ++r) {
 #pragma unroll
-              for (int c = 0; c < CT; ++c)
-                if (key0 + r < lim[c]) nans[c] |= 1u << g;
-              s[g * kRows + r] = 0;
-              s[(G + g) * kRows + r] = 0;
+              for (int g = 0; g < G; ++g) {
+                const int sd = s[g * kRows + r] & 0x7fff, sm = s[(G + g) * kRows + r] & 0x7fff;
+                if (sd < 0x7c00 && sm < 0x7c00) continue;
+#pragma unroll
+                for (int c = 0; c < CT; ++c)
+                  if (key0 + kRows * u + r < lim[c]) nans[c] |= 1u << g;
+                s[g * kRows + r] = 0;
+                s[(G + g) * kRows + r] = 0;
+              }
             }
           }
         }
         asm volatile("" ::: "memory");
       }
 
-      // S^T, keys 16 kt + 4 quad + r of the tile
-      float s[CT][8];
+      // S^T: key 32 u + 16 kt + 4 quad + r of the step is value 8 u + 4 kt + r
+      float s[CT][8 * TP];
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
-        // least values of this lane's groups against the three parts of the
-        // sums, and what is left of least + 8 steps against the first
-        f16x8 mf = {};
+      for (int u = 0; u < TP; ++u) {
+        const char* const tile = tiles + u * S::kTileB;
+        const char* const sc_k = tile + 2 * S::kCodeB;
 #pragma unroll
-        for (int h = 0; h < (G + 3) / 4; ++h) {
-          const char* mp = sc_k + (G + (has_m ? quad + 4 * h : 0)) * 64 + 2 * (16 * kt + hl);
-          f16_t x = *(const f16_t*)mp, rest = (f16_t)0.f;
-          if constexpr (S::kCentred) {
-            const float y = fmaf((float)*(const f16_t*)(mp - 64 * G), 8.f, (float)x);
-            x = (f16_t)y;
-            rest = (f16_t)(y - (float)x);
+        for (int kt = 0; kt < 2; ++kt) {
+          // least values of this lane's groups against the three parts of the
+          // sums, and what is left of least + 8 steps against the first
+          f16x8 mf = {};
+#pragma unroll
+          for (int h = 0; h < (G + 3) / 4; ++h) {
+            const char* mp = sc_k + mk + (G + 4 * h) * 64 + 32 * kt;
+            f16_t x = *(const f16_t*)mp, rest = (f16_t)0.f;
+            if constexpr (S::kCentred) {
+              const float y = fmaf((float)*(const f16_t*)(mp - 64 * G), 8.f, (float)x);
+              x = (f16_t)y;
+              rest = (f16_t)(y - (float)x);
+            }
+            if (G % 4 != 0 && !has_m) x = rest = (f16_t)0.f;
+            mf[4 * h] = mf[4 * h + 1] = mf[4 * h + 2] = x;
+            mf[4 * h + 3] = rest;
           }
-          if (!has_m) x = rest = (f16_t)0.f;
-          mf[4 * h] = mf[4 * h + 1] = mf[4 * h + 2] = x;
-          mf[4 * h + 3] = rest;
-        }
-#pragma unroll
-        for (int c = 0; c < CT; ++c) {
-          const f32x4 x = mfma16x16x32(mf, qsum[c], (f32x4)(0.f));
-#pragma unroll
-          for (int r = 0; r < 4; ++r) s[c][4 * kt + r] = x[r] * S::kSumUnit;
-        }
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-          const int row = 16 * kt + hl;
-          const uint32_t w = *(const uint32_t*)(tile + kadr + 256 * G * kt +
-                                                16 * (k_place<G>(row, g)));
-          const f16x8 kx = S::kCentred ? centred_operand(w) : operand(w);
-          const f16x4 d = *(const f16x4*)(sc_k + 64 * g + 32 * kt + 8 * quad);
 #pragma unroll
           for (int c = 0; c < CT; ++c) {
-            f32x4 x = mfma16x16x32(kx, q[c][0][g], (f32x4)(0.f));
-            if constexpr (QP == 2) x = mfma16x16x32(kx, q[c][1][g], x);
+            const f32x4 x = mfma16x16x32(mf, qsum[c], (f32x4)(0.f));
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              s[c][4 * kt + r] = fmaf((float)d[r], x[r], s[c][4 * kt + r]);
+            for (int r = 0; r < 4; ++r) s[c][8 * u + 4 * kt + r] = x[r] * S::kSumUnit;
+          }
+#pragma unroll
+          for (int g = 0; g < G; ++g) {
+            const uint32_t w = *(const uint32_t*)(tile + kadr[g] + 256 * G * kt);
+            const f16x8 kx = S::kCentred ? centred_operand(w) : operand(w);
+            const f16x4 d = *(const f16x4*)(sc_k + dadr + 64 * g + 32 * kt);
+#pragma unroll
+            for (int c = 0; c < CT; ++c) {
+              f32x4 x = mfma16x16x32(kx, q[c][0][g], (f32x4)(0.f));
+              if constexpr (QP == 2) x = mfma16x16x32(kx, q[c][1][g], x);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                float& y = s[c][8 * u + 4 * kt + r];
+                y = fmaf((float)d[r], x[r], y);
+              }
+            }
           }
         }
       }
@@ -450,8 +504,9 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
 #pragma unroll
         for (int c = 0; c < CT; ++c)
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (key0 + 16 * (e >> 2) + 4 * quad + (e & 3) >= lim[c]) s[c][e] = -__builtin_inff();
+          for (int e = 0; e < 8 * TP; ++e)
+            if (key0 + 32 * (e >> 3) + 16 * (e >> 2 & 1) + 4 * quad + (e & 3) >= lim[c])
+              s[c][e] = -__builtin_inff();
       }
 
       // The reference of the probabilities: the largest score so far, less
@@ -459,16 +514,22 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
       // float16.
       float lift = 0.f;
       {
-        const u32x4 x = *(const u32x4*)(sc_v + 16 * (lane < 4 * G ? lane : 0));
-        u16x2 y = __builtin_bit_cast(u16x2, x[0]);
+        u16x2 y = {0, 0};
+        u32x4 x[TP];
 #pragma unroll
-        for (int e = 1; e < 4; ++e) y = __builtin_elementwise_max(y, __builtin_bit_cast(u16x2, x[e]));
+        for (int u = 0; u < TP; ++u) {
+          x[u] = *(const u32x4*)(tiles + u * S::kTileB + 2 * S::kCodeB + S::kScaleB +
+                                 16 * (lane < 4 * G ? lane : 0));
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            y = __builtin_elementwise_max(y, bits16(x[u][e]));
+        }
         y = __builtin_elementwise_sub_sat(y, (u16x2){0x3c00, 0x3c00});
         if (__ballot(__builtin_bit_cast(uint32_t, y) != 0) != 0) {
           float most = 0.f;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const f16x2 h = __builtin_bit_cast(f16x2, x[e]);
+          for (int e = 0; e < 4 * TP; ++e) {
+            const f16x2 h = halves(x[e / 4][e % 4]);
             most = fmaxf(most, fmaxf(fabsf((float)h[0]), fabsf((float)h[1])));
           }
 #pragma unroll
@@ -480,9 +541,10 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
       bool over = false;
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
-        float x = fmaxf(s[c][0], s[c][1]);
+        float x = max3(s[c][0], s[c][1], s[c][2]);
 #pragma unroll
-        for (int e = 2; e < 8; ++e) x = fmaxf(x, s[c][e]);
+        for (int e = 3; e + 1 < 8 * TP; e += 2) x = max3(x, s[c][e], s[c][e + 1]);
+        x = max3(x, s[c][8 * TP - 1], x);
         top[c] = fmaf(x, k1[c], lift);
         over |= top[c] > m[c] + kSlack;
       }
@@ -499,24 +561,23 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
         }
       }
 
-      // P, in float32 and as the high parts of its two; ph16 and p16: the
-      // pairs whose codes count 16-fold, a 16th
-      f16x2 ph[CT][4];
-      f16x8 pl[CT];
+      // P in two parts of float16; pairs whose codes count 16-fold then go on
+      // as a 16th
+      f16x2 ph[CT][4 * TP], pl[CT][4 * TP];
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
         const float base = kLift - m[c];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s[c][e] = fast_exp2(fmaf(s[c][e], k1[c], base));
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          ph[c][e] = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(s[c][2 * e], s[c][2 * e + 1]));
-          pl[c][2 * e] = (f16_t)(s[c][2 * e] - (float)ph[c][e][0]);
-          pl[c][2 * e + 1] = (f16_t)(s[c][2 * e + 1] - (float)ph[c][e][1]);
+        for (int e = 0; e < 4 * TP; ++e) {
+          const float x0 = fast_exp2(fmaf(s[c][2 * e], k1[c], base));
+          const float x1 = fast_exp2(fmaf(s[c][2 * e + 1], k1[c], base));
+          ph[c][e] = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x0, x1));
+          pl[c][e] = (f16x2){(f16_t)(x0 - (float)ph[c][e][0]), (f16_t)(x1 - (float)ph[c][e][1])};
         }
       }
-      {  // least values, and the sum of p
-        const char* mp = sc_v + (G + (hl < G ? hl : 0)) * 64 + 8 * quad;
+#pragma unroll
+      for (int u = 0; u < TP; ++u) {  // least values, and the sum of p
+        const char* mp = tiles + u * S::kTileB + 2 * S::kCodeB + S::kScaleB + mv;
         const u32x2 m0 = *(const u32x2*)mp, m1 = *(const u32x2*)(mp + 32);
         constexpr uint32_t kOnes = 0x3c003c00u;
         f16x8 mf = __builtin_bit_cast(
@@ -536,51 +597,54 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
         }
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
-          f16x8 p;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) p[e] = ph[c][e >> 1][e & 1];
-          om[c] = mfma16x16x32(mf, p, om[c]);
-          om[c] = mfma16x16x32(mf, pl[c], om[c]);
-          if constexpr (S::kCentred) om[c] = mfma16x16x32(rest, p, om[c]);
+          const f16x8 hi = four(ph[c] + 4 * u);
+          om[c] = mfma16x16x32(mf, hi, om[c]);
+          om[c] = mfma16x16x32(mf, four(pl[c] + 4 * u), om[c]);
+          if constexpr (S::kCentred) om[c] = mfma16x16x32(rest, hi, om[c]);
         }
       }
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
 #pragma unroll
-        for (int e = 1; e < 4; e += 2) {
+        for (int e = 1; e < 4 * TP; e += 2) {
           ph[c][e] *= (f16_t)0.0625f;
-          s[c][2 * e] *= 0.0625f;
-          s[c][2 * e + 1] *= 0.0625f;
+          pl[c][e] *= (f16_t)0.0625f;
         }
       }
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        const u32x2 w = lds_read_tr4x16(tile + vadr + 16 * v_place<G>(vrow, g));
-        const f16x8 v0 = S::kCentred ? centred_operand(w[0]) : operand(w[0]);
-        const f16x8 v1 = S::kCentred ? centred_operand(w[1]) : operand(w[1]);
-        const f16x4 d0 = *(const f16x4*)(sc_v + 64 * g + 8 * quad);
-        const f16x4 d1 = *(const f16x4*)(sc_v + 64 * g + 32 + 8 * quad);
 #pragma unroll
-        for (int c = 0; c < CT; ++c) {
-          f16x8 hi, lo;
+        for (int u = 0; u < TP; ++u) {
+          const char* const tile = tiles + u * S::kTileB;
+          const u32x2 w = lds_read_tr4x16(tile + vadr[g]);
+          const f16x8 v0 = S::kCentred ? centred_operand(w[0]) : operand(w[0]);
+          const f16x8 v1 = S::kCentred ? centred_operand(w[1]) : operand(w[1]);
+          const char* const dp = tile + 2 * S::kCodeB + S::kScaleB + dadr + 64 * g;
+          const u32x2 d01 = *(const u32x2*)dp, d23 = *(const u32x2*)(dp + 32);
+          const f16x2 d[4] = {halves(d01[0]), halves(d01[1]), halves(d23[0]), halves(d23[1])};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const f16x4 d = e < 2 ? d0 : d1;
-            const f16x2 dd = {d[2 * (e & 1)], d[2 * (e & 1) + 1]};
-            const f16x2 h = ph[c][e] * dd;
-            hi[2 * e] = h[0];
-            hi[2 * e + 1] = h[1];
-            lo[2 * e] = (f16_t)fmaf(s[c][2 * e], (float)dd[0], -(float)h[0]);
-            lo[2 * e + 1] = (f16_t)fmaf(s[c][2 * e + 1], (float)dd[1], -(float)h[1]);
+          for (int c = 0; c < CT; ++c) {
+            f16x2 hi[4], lo[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const f16x2 p = ph[c][4 * u + e];
+              hi[e] = p * d[e];
+              // what the rounding took, and the second part's share
+              lo[e] = __builtin_elementwise_fma(
+                  pl[c][4 * u + e], d[e], __builtin_elementwise_fma(p, d[e], -hi[e]));
+            }
+            o[c][2 * g] = mfma16x16x32(v0, four(hi), o[c][2 * g]);
+            o[c][2 * g + 1] = mfma16x16x32(v1, four(hi), o[c][2 * g + 1]);
+            o[c][2 * g] = mfma16x16x32(v0, four(lo), o[c][2 * g]);
+            o[c][2 * g + 1] = mfma16x16x32(v1, four(lo), o[c][2 * g + 1]);
           }
-          o[c][2 * g] = mfma16x16x32(v0, hi, o[c][2 * g]);
-          o[c][2 * g + 1] = mfma16x16x32(v1, hi, o[c][2 * g + 1]);
-          o[c][2 * g] = mfma16x16x32(v0, lo, o[c][2 * g]);
-          o[c][2 * g + 1] = mfma16x16x32(v1, lo, o[c][2 * g + 1]);
         }
       }
-      stage = stage + 1 == RING ? 0 : stage + 1;
-    }
+    };
+    for (int i = 0; i < mine; i += RING)
+      static_for<0, RING>([&](auto j) {
+        if (i + decltype(j)::value < mine) step(j, i + decltype(j)::value);
+      });
 
     // The waves meet: each leaves its reference, its sum and O, with the
     // least values' part in it.
@@ -637,7 +701,7 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
     do {
       ++sh.b;
       uniform_rows(a, sh.b, sh.P, sh.end);
-      sh.tiles = (sh.end + kRows - 1) / kRows;
+      sh.tiles = (sh.end + S::kStepRows - 1) / S::kStepRows;
     } while (sh.tiles == 0);
     sh.t0 = 0;
     sh.nt = min(sh.left, sh.tiles);
@@ -647,54 +711,54 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
 }
 
 // Joins the segments of the sequences that more than one slot has tiles of,
-// and writes zeros for those without a row.  One block per (sequence, kv
-// head, 4 columns): 4 channels a thread, the rest of the threads share the
-// segments and meet in LDS.
-constexpr int kJoinThreads = 512, kJoinCols = 4;
-
-template <typename T, int G>
-__global__ void __launch_bounds__(kJoinThreads) q4_join(Q4Args a, int cols, int tile_cols) {
-  constexpr int D = 32 * G, kItems = kJoinCols * 8 * G, kShare = kJoinThreads / kItems, kFlight = 4;
-  __shared__ f32x4 part[kShare][kItems];
-  __shared__ float2 st[kShare][kJoinCols];
-  const int groups = (cols + kJoinCols - 1) / kJoinCols;
-  const int cg = blockIdx.x % groups;
+// and writes zeros for those without a row.  One block per COLS columns:
+// 8 / COLS threads per channel quad take the segments in turn and meet in
+// LDS.  One column a block where a sequence has many segments (4 x 1 on 32768
+// rows, 32 segments of 256 channels: 4.0 us, four columns 9.5), four where
+// there are many columns (4 x 64 on 4133 rows, 8192 of them: 6.5 us, one 8.9).
+template <typename T, int G, int COLS>
+__global__ void __launch_bounds__(64 * G) q4_join(Q4Args a, int cols, int tile_cols) {
+  constexpr int D = 32 * G, kItems = 8 * G, kFlight = 4, kJoinShare = 8 / COLS;
+  __shared__ f32x4 part[kJoinShare][COLS * kItems];
+  __shared__ float2 st[kJoinShare][COLS];
+  const int groups = (cols + COLS - 1) / COLS;
+  const int cl = threadIdx.x / kItems % COLS;
+  const int col = blockIdx.x % groups * COLS + cl, node = col / a.group;
   const int kvh = blockIdx.x / groups % a.kv_heads, b = blockIdx.x / groups / a.kv_heads;
   const int32_t* found = (const int32_t*)(a.found + b);
   const int s0 = load_const(found), s1 = load_const(found + 1);
   const int P = load_const(found + 2), end = load_const(found + 3);
   if (s0 == s1) return;  // written by its slot
-  const int item = threadIdx.x % kItems, w = threadIdx.x / kItems;
-  const int cl = item / (8 * G), ch = 4 * (item - cl * (8 * G));
-  const int col = cg * kJoinCols + cl, node = col / a.group;
+  const int item = threadIdx.x % (COLS * kItems), w = threadIdx.x / (COLS * kItems);
+  const int ch = 4 * (threadIdx.x % kItems);
   const bool live = node < a.nodes && P + node < end;
   float m = -3.0e38f, l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  if (live && w < kShare) {
+  if (live) {
     const int ct = col / tile_cols;
     auto at = [&](int s) __attribute__((always_inline)) {
       return (((int64_t)(s + b) * a.kv_heads + kvh) * a.col_tiles + ct) * tile_cols +
              (col - ct * tile_cols);
     };
-    for (int s = s0 + w; s <= s1; s += kShare * kFlight) {
+    for (int s = s0 + w; s <= s1; s += kJoinShare * kFlight) {
       float2 v[kFlight];
       f32x4 x[kFlight];
 #pragma unroll
       for (int u = 0; u < kFlight; ++u) {
-        const int64_t row = at(min(s + kShare * u, s1));  // past the last: again, unused
+        const int64_t row = at(min(s + kJoinShare * u, s1));  // past the last: again, unused
         v[u] = a.part_st[row];
         x[u] = *(const f32x4*)(a.part_o + row * D + ch);
       }
       float M = m;
 #pragma unroll
       for (int u = 0; u < kFlight; ++u)
-        if (s + kShare * u <= s1) M = fmaxf(M, v[u].x);
+        if (s + kJoinShare * u <= s1) M = fmaxf(M, v[u].x);
       const float c = column_weight(m, M);
       l *= c;
       o *= c;
 #pragma unroll
       for (int u = 0; u < kFlight; ++u) {
-        if (s + kShare * u > s1) continue;
+        if (s + kJoinShare * u > s1) continue;
         const float cu = column_weight(v[u].x, M);
         l = fmaf(v[u].y, cu, l);
         o += x[u] * cu;
@@ -702,18 +766,16 @@ __global__ void __launch_bounds__(kJoinThreads) q4_join(Q4Args a, int cols, int 
       m = M;
     }
   }
-  if (w < kShare) {
-    part[w][item] = o;
-    if (ch == 0) st[w][cl] = make_float2(m, l);
-  }
+  part[w][item] = o;
+  if (ch == 0) st[w][cl] = make_float2(m, l);
   __syncthreads();
   if (w != 0 || node >= a.nodes) return;
   float M = -3.0e38f, sum = 0.f;
 #pragma unroll
-  for (int v = 0; v < kShare; ++v) M = fmaxf(M, st[v][cl].x);
+  for (int v = 0; v < kJoinShare; ++v) M = fmaxf(M, st[v][cl].x);
   f32x4 y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int v = 0; v < kShare; ++v) {
+  for (int v = 0; v < kJoinShare; ++v) {
     const float c = column_weight(st[v][cl].x, M);
     sum = fmaf(st[v][cl].y, c, sum);
     y += part[v][item] * c;
@@ -729,29 +791,32 @@ struct Kernel {
   const void* fn;
   const void* alone;  // the same with a slot per sequence
   const void* join;
+  int join_cols;
   int cols;    // columns per block
+  int rows;    // rows per step
   int per_cu;  // blocks on a CU at a time
 };
 
 template <typename S>
 Kernel make() {
   return {(const void*)q4_kernel<S, false>, (const void*)q4_kernel<S, true>,
-          (const void*)q4_join<typename S::T, S::G>, S::kCols, S::kPerCu};
+          (const void*)q4_join<typename S::T, S::G, S::CT == 1 ? 1 : 4>,
+          S::CT == 1 ? 1 : 4, S::kCols, S::kStepRows, S::kPerCu};
 }
 
 template <typename T>
 Kernel pick(int head_dim, int cols) {
   const bool few = cols <= 16;
   switch (head_dim) {
-    case 64: return few ? make<Q4Shape<T, 2, 1, 4>>() : make<Q4Shape<T, 2, 2, 4>>();
-    case 96: return few ? make<Q4Shape<T, 3, 1, 4>>() : make<Q4Shape<T, 3, 2, 4>>();
-    case 128: return few ? make<Q4Shape<T, 4, 1, 4>>() : make<Q4Shape<T, 4, 2, 4>>();
-    default: return make<Q4Shape<T, 8, 1, 2>>();
+    case 64: return few ? make<Q4Shape<T, 2, 1, 2, 2, 3>>() : make<Q4Shape<T, 2, 2, 1, 4, 2>>();
+    case 96: return few ? make<Q4Shape<T, 3, 1, 2, 2, 2>>() : make<Q4Shape<T, 3, 2, 1, 4, 2>>();
+    case 128: return few ? make<Q4Shape<T, 4, 1, 2, 2, 2>>() : make<Q4Shape<T, 4, 2, 1, 4, 2>>();
+    default: return make<Q4Shape<T, 8, 1, 1, 2, 1>>();
   }
 }
 
-constexpr int64_t kAloneTiles = 32;    // of the longest sequence, for one launch
-constexpr int64_t kTilesPerSlot = 8;   // at least, beyond a block a CU
+constexpr int64_t kAloneRows = 1024;  // of the longest sequence, for one launch
+constexpr int64_t kRowsPerSlot = 256;  // at least, beyond a block a CU
 
 struct Q4Plan {
   Kernel kernel;
@@ -768,19 +833,19 @@ Q4Plan q4_plan(int batch, int nodes, int q_heads, int kv_heads, int head_dim, in
              : dtype == ALPX_F16 ? pick<f16_t>(head_dim, cols)
                                  : pick<bf16_t>(head_dim, cols);
   p.col_tiles = (cols + p.kernel.cols - 1) / p.kernel.cols;
-  const int64_t rows = (length + kRows - 1) / kRows;
-  const int64_t tiles = (int64_t)batch * rows;
+  const int64_t steps = (length + p.kernel.rows - 1) / p.kernel.rows;
+  const int64_t tiles = (int64_t)batch * steps;
   const int64_t units = (int64_t)kv_heads * p.col_tiles;
   const int64_t share = std::min(kCus * p.kernel.per_cu / units,
-                                 std::max(kCus / units, tiles / kTilesPerSlot));
+                                 std::max(kCus / units, tiles * p.kernel.rows / kRowsPerSlot));
   p.slots = (int)std::min(std::max<int64_t>(share, 1), tiles);
-  p.alone = rows <= kAloneTiles;
+  p.alone = length <= kAloneRows;
   if (p.alone) p.slots = batch;
   p.blocks = ((int64_t)p.slots * kv_heads + kXcds - 1) / kXcds * kXcds * p.col_tiles;
   if (p.alone) return p;
   p.segments = (size_t)(p.slots + batch) * kv_heads * p.col_tiles * p.kernel.cols;
   p.bytes = p.segments * ((size_t)head_dim * 4 + sizeof(float2)) + (size_t)batch * sizeof(int4);
-  p.joins = (int64_t)batch * kv_heads * ((cols + kJoinCols - 1) / kJoinCols);
+  p.joins = (int64_t)batch * kv_heads * ((cols + p.kernel.join_cols - 1) / p.kernel.join_cols);
   return p;
 }
 
@@ -795,7 +860,7 @@ bool sizes_ok(int batch, int nodes, int q_heads, int kv_heads, int head_dim, int
   if ((int64_t)nodes * (q_heads / kv_heads) > (1 << 24) || batch > (1 << 24) || kv_heads > (1 << 20))
     return false;
   const Q4Plan p = q4_plan(batch, nodes, q_heads, kv_heads, head_dim, length, dtype);
-  return p.blocks * 64 * kWaves <= 0xffffffff && p.joins * kJoinThreads <= 0xffffffff;
+  return p.blocks * 64 * kWaves <= 0xffffffff && p.joins * 2 * head_dim <= 0xffffffff;
 }
 
 }  // namespace
@@ -889,6 +954,6 @@ extern "C" int alpx_q4_attention(const void* q, const void* key_codes, const voi
   TimedRegion timed(ALPX_T_DECODE_COMBINE, s);
   int cols = nodes * a.group, tile_cols = p.kernel.cols;
   void* args[] = {&a, &cols, &tile_cols};
-  (void)hipLaunchKernel(p.kernel.join, dim3((unsigned)p.joins), dim3(kJoinThreads), args, 0, s);
+  (void)hipLaunchKernel(p.kernel.join, dim3((unsigned)p.joins), dim3(2 * head_dim), args, 0, s);
   return check_launch(what);
 }

@@ -389,6 +389,24 @@ def test_values_of_any_size(gpu, ops, dtype, size):
     assert (np.abs(got - want) <= 1e-4 * size).all()
 
 
+@pytest.mark.parametrize("dtype,d,nodes", [("f32", 64, 1), ("f16", 128, 1), ("bf16", 256, 1),
+                                           ("f16", 96, 1), ("f16", 128, 20)])
+def test_a_row_of_large_values_anywhere(gpu, ops, dtype, d, nodes):
+    """One row whose steps a weight of float16 would overflow, alone, at every
+    place of two tiles.  A channel is the sum of its weighted steps and least
+    values, each of which may be as large as the largest value of its group of
+    32 (least + 15 steps): what float32 loses of them, 1e-4 at values of 1,
+    grows with that value, not with the channel's own."""
+    for at in range(64):
+        case = Case(gpu, 40 + at, dtype=dtype, d=d, hq=4, hkv=2, nodes=nodes, prefix=[130])
+        case.v[0, at, 0, 32 * (at % (d // 32)):][:32] *= 8000.0
+        case.store()
+        got, want = _host(case.call(ops, out_dtype=_td("f32"))), case.oracle()
+        size = np.abs(case.v[0]).max(0).reshape(2, -1, 32).max(-1).repeat(32, -1)
+        size = np.maximum(1.0, size.repeat(2, 0))
+        assert (np.abs(got - want) <= 1e-4 * size).all(), at
+
+
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 def test_queries_of_any_size(gpu, ops, dtype):
     """Large and small queries, one channel far above the rest, and zeros."""
