@@ -85,14 +85,24 @@ def get(pool, slots):
     return out
 
 
-def attend(q, k, v, prefix, length, count, scale):
+def gross(pool, slots):
+    """float64 ``|least| + step * code`` of pool rows: what the two parts of a
+    number amount to before their sum."""
+    data, scales = pool
+    out = get((data, np.abs(scales)), slots)
+    return out.astype(np.float64)
+
+
+def attend(q, k, v, prefix, length, count, scale, parts=None):
     """One sequence: ``q [N, Hq, D]`` over its rows ``k, v [R, Hkv, D]``.
     Token i < count whose row ``prefix + i`` lies below ``length`` sees the
-    rows up to and with it.  Returns ``(out, weight, spread)``: the result,
-    ``sum p |v| / sum p`` and the largest ``sum |q k| scale`` of a score."""
+    rows up to and with it.  Returns ``(out, weight)``: the result and
+    ``sum p parts / sum p`` (``parts``: ``|v|``), which bounds what roundings
+    of p do to it."""
     n, hq, d = q.shape
     hkv = k.shape[1]
-    out, weight, spread = np.zeros((n, hq, d)), np.zeros((n, hq, d)), 0.0
+    out, weight = np.zeros((n, hq, d)), np.zeros((n, hq, d))
+    parts = np.abs(v) if parts is None else parts
     prefix = min(max(prefix, 0), length)
     for i in range(n):
         if i >= count or prefix + i >= length:
@@ -104,10 +114,8 @@ def attend(q, k, v, prefix, length, count, scale):
                 s = (kk @ q[i, h].astype(np.float64)) * scale
                 p = np.exp(s - s.max())
                 p = p / p.sum()
-                out[i, h], weight[i, h] = p @ vv, p @ np.abs(vv)
-                spread = max(spread, float((np.abs(kk) @ np.abs(q[i, h].astype(np.float64))).max()
-                                           * scale))
-    return out, weight, spread
+                out[i, h], weight[i, h] = p @ vv, p @ parts[:prefix + i + 1, g]
+    return out, weight
 
 
 def verify(tokens, target, uniforms, parents=None, draft=None, count=None):

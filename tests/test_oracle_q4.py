@@ -57,6 +57,15 @@ def test_pool_puts_even_channels_low_and_steps_along_rows():
     assert np.array_equal(Q.get(pool, [37, -1])[0], x[0]) and not Q.get(pool, [96]).any()
 
 
+def test_gross_of_a_row_by_hand():
+    # a sign of the least value that is kept would make them cancel
+    pool = Q.empty_pool(1, 1, 32, 64)
+    x = np.full((1, 1, 64), -3.0)
+    x[0, 0, 0] = 12.0  # least -3, step 1: 3 + 15, the others 3
+    Q.put(pool, [4], x)
+    assert Q.gross(pool, [4])[0, 0, :2].tolist() == [18.0, 3.0]
+
+
 @pytest.mark.parametrize("rotary", [8, 6])
 def test_rotation_matches_the_llama_tables(rotary):
     # wrong pairs, sign or frequencies
@@ -74,7 +83,7 @@ def test_rotation_matches_the_llama_tables(rotary):
 def test_attention_of_the_last_token_is_decode():
     rng = np.random.default_rng(2)
     q, k, v = (rng.standard_normal(s) for s in ((2, 4, 8), (6, 2, 8), (6, 2, 8)))
-    out, weight, _ = Q.attend(q, k, v, 4, 6, 2, 8 ** -0.5)
+    out, weight = Q.attend(q, k, v, 4, 6, 2, 8 ** -0.5)
     for i in range(2):
         want = A.attention_decode_twopass(q[i], k[:5 + i], v[:5 + i], 2, 8 ** -0.5)
         assert np.allclose(out[i], want, atol=1e-6)
