@@ -22,7 +22,8 @@
 // Bound by the one or two rows of the vocabulary that the last token is drawn
 // from.  One launch gathers the drafts' own entries, walks as far as it can
 // without a sum (in every block for itself: a walk is short) and leaves the
-// sums of slices of the row; a second finds the slice and the token.
+// sums of slices of the row, a wave a slice; a second finds the slice and the
+// token.
 #include <math.h>
 
 #include <algorithm>
@@ -34,7 +35,7 @@ namespace alpx {
 namespace {
 
 constexpr int kMostDrafts = 1024;
-constexpr int kMostSlices = 64;  // one per lane
+constexpr int kMostSlices = 256;  // four per lane
 constexpr int kSumThreads = 256, kDrawThreads = 512;
 
 struct Stand {  // where a walk stopped
@@ -64,22 +65,42 @@ __device__ __forceinline__ float weight(float x) {
   return x > 0.f && x < __builtin_inff() ? x : 0.f;
 }
 
-// What a block knows of a sequence's drafts.
+// What a block knows of a sequence's drafts, in LDS as large as they are.
 struct Drafts {
-  int up[kMostDrafts];     // parent, -1: never reached
-  int token[kMostDrafts];
-  float p[kMostDrafts];    // the parent's distributions at the token
-  float q[kMostDrafts];
-  float u[kMostDrafts];
-  double z[kMostDrafts];   // Z of the refusals at the draft that the walk is at
-  int gone[kMostDrafts];   // tokens refused there (draft null)
-  Stand at;
-  bool more;               // a sum is wanted before the next child can be tried
-  int ngone;
+  double* z;   // [N] Z of the refusals at the draft that the walk is at
+  float* p;    // [N] the parent's distributions at the token
+  float* q;
+  float* u;
+  int* up;     // [N] parent, -1: never reached
+  int* token;
+  int* gone;   // [N] tokens refused there (draft null)
+  struct Shared {
+    Stand at;
+    int more;  // a sum is wanted before the next child can be tried
+    int ngone;
+  };
+  Shared* s;
 };
 
+__host__ __device__ inline size_t drafts_bytes(int nodes) {
+  return (size_t)nodes * 32 + sizeof(Drafts::Shared);
+}
+
+__device__ __forceinline__ Drafts drafts_in(char* lds, int nodes) {
+  Drafts d;
+  d.z = (double*)lds;
+  d.p = (float*)(d.z + nodes);
+  d.q = d.p + nodes;
+  d.u = d.q + nodes;
+  d.up = (int*)(d.u + nodes);
+  d.token = d.up + nodes;
+  d.gone = d.token + nodes;
+  d.s = (Drafts::Shared*)(d.gone + nodes);
+  return d;
+}
+
 template <typename T>
-__device__ __forceinline__ void gather(const VerifyArgs& a, int b, int count, Drafts& d) {
+__device__ __forceinline__ void gather(const VerifyArgs& a, int b, int count, const Drafts& d) {
   for (int i = threadIdx.x; i < count; i += blockDim.x) {
     const int64_t at = (int64_t)b * a.nodes + i;
     int up = a.parents != nullptr ? a.parents[at] : i - 1;
@@ -107,12 +128,12 @@ __device__ __forceinline__ double left_of(double p, double q, const double* z, i
   return r;
 }
 
-// Goes on from d.at until a sum is wanted (d.more) or no child is left.  One
+// Goes on from d.s->at until a sum is wanted (more) or no child is left.  One
 // wave; z[0 .. tried] are the sums known so far (z[0] = 1).  The drafts that
 // stand enter the sequence's path.
-__device__ __forceinline__ void walk(const VerifyArgs& a, int b, int count, Drafts& d) {
+__device__ __forceinline__ void walk(const VerifyArgs& a, int b, int count, const Drafts& d) {
   const int lane = threadIdx.x & 63;
-  int last = d.at.last, from = d.at.from, tried = d.at.tried, accepted = d.at.accepted;
+  int last = d.s->at.last, from = d.s->at.from, tried = d.s->at.tried, accepted = d.s->at.accepted;
   double rem = 1.0;  // draft null: 1 less the tokens refused here
   bool more = false;
   while (true) {
@@ -160,8 +181,8 @@ __device__ __forceinline__ void walk(const VerifyArgs& a, int b, int count, Draf
     }
   }
   if (lane == 0) {
-    d.at = Stand{last, from, tried, accepted};
-    d.more = more;
+    d.s->at = Stand{last, from, tried, accepted};
+    d.s->more = more;
   }
 }
 
@@ -195,28 +216,39 @@ __device__ __forceinline__ double range_sum(const T* p, const T* q, int64_t x0, 
     v1 = v0 + (x1 - v0) / VN * VN;
   }
   for (int64_t x = x0 + thread; x < v0; x += threads) one(x);
-  for (int64_t x = v0 + (int64_t)thread * VN; x < v1; x += (int64_t)threads * VN) {
-    const Unit pu = *(const Unit*)(p + x);
-    float w[VN];
+  constexpr int kFlight = 4;  // units on their way
+  for (int64_t first = v0 + (int64_t)thread * VN; first < v1; first += (int64_t)threads * VN * kFlight) {
+    Unit pu[kFlight], qu[kFlight];
 #pragma unroll
-    for (int e = 0; e < VN; ++e) w[e] = weight(to_f32(pu.x[e]));
-    if constexpr (DRAFT) {
-      if (tried != 0) {
-        const Unit qu = *(const Unit*)(q + x);
-#pragma unroll
-        for (int e = 0; e < VN; ++e)
-          sum += left_of((double)w[e], (double)weight(to_f32(qu.x[e])), d.z, tried);
-        continue;
-      }
-    } else {
-      for (int j = 0; j < ngone; ++j) {
-#pragma unroll
-        for (int e = 0; e < VN; ++e)
-          if (d.gone[j] == x + e) w[e] = 0.f;
-      }
+    for (int i = 0; i < kFlight; ++i) {
+      const int64_t x = min(first + (int64_t)i * threads * VN, v1 - VN);  // past the last: again, unused
+      pu[i] = *(const Unit*)(p + x);
+      if (DRAFT && tried != 0) qu[i] = *(const Unit*)(q + x);
     }
 #pragma unroll
-    for (int e = 0; e < VN; ++e) sum += (double)w[e];
+    for (int i = 0; i < kFlight; ++i) {
+      const int64_t x = first + (int64_t)i * threads * VN;
+      if (x >= v1) break;
+      float w[VN];
+#pragma unroll
+      for (int e = 0; e < VN; ++e) w[e] = weight(to_f32(pu[i].x[e]));
+      if constexpr (DRAFT) {
+        if (tried != 0) {
+#pragma unroll
+          for (int e = 0; e < VN; ++e)
+            sum += left_of((double)w[e], (double)weight(to_f32(qu[i].x[e])), d.z, tried);
+          continue;
+        }
+      } else {
+        for (int j = 0; j < ngone; ++j) {
+#pragma unroll
+          for (int e = 0; e < VN; ++e)
+            if (d.gone[j] == x + e) w[e] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < VN; ++e) sum += (double)w[e];
+    }
   }
   for (int64_t x = v1 + thread; x < x1; x += threads) one(x);
   return sum;
@@ -228,15 +260,15 @@ __device__ __forceinline__ double wave_sum(double x) {
   return x;
 }
 
-// The refused tokens of draft d.at.last that lie in [x0, x1), in d.gone: all
+// The refused tokens of draft d.s->at.last that lie in [x0, x1), in d.gone: all
 // of its children, since none stands.
-__device__ __forceinline__ void gone_in(int count, int64_t x0, int64_t x1, Drafts& d) {
-  if (threadIdx.x == 0) d.ngone = 0;
+__device__ __forceinline__ void gone_in(int count, int64_t x0, int64_t x1, const Drafts& d) {
+  if (threadIdx.x == 0) d.s->ngone = 0;
   __syncthreads();
-  const int last = d.at.last;
+  const int last = d.s->at.last;
   for (int i = threadIdx.x; i < count; i += blockDim.x)
     if (d.up[i] == last && d.token[i] >= x0 && d.token[i] < x1)
-      d.gone[atomicAdd(&d.ngone, 1)] = d.token[i];
+      d.gone[atomicAdd(&d.s->ngone, 1)] = d.token[i];
   __syncthreads();
 }
 
@@ -244,70 +276,111 @@ __device__ __forceinline__ int count_of(const VerifyArgs& a, int b) {
   return a.counts != nullptr ? min(max(a.counts[b], 0), a.nodes) : a.nodes;
 }
 
-// Grid (slices, B).
+__device__ __forceinline__ void slice_of(const VerifyArgs& a, int s, int64_t& x0, int64_t& x1) {
+  x0 = min(s * a.slice, a.vocab);
+  x1 = min(x0 + a.slice, a.vocab);
+}
+
+// Grid (slices / waves, B).
 template <typename T, bool DRAFT>
 __global__ void __launch_bounds__(kSumThreads) verify_sums(VerifyArgs a) {
-  __shared__ Drafts d;
-  __shared__ double part[kSumThreads / 64];
-  const int b = blockIdx.y, s = blockIdx.x, tid = threadIdx.x;
+  constexpr int kWaves = kSumThreads / 64;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const Drafts d = drafts_in(lds, a.nodes);
+  const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const bool writes = blockIdx.x == 0;
   const int count = count_of(a, b);
   const int64_t row0 = (int64_t)b * a.nodes;
-  if (s == 0) {
-    for (int i = tid; i < a.nodes; i += kSumThreads)
+  if (writes) {
+    for (int i = tid; i < a.nodes; i += kSumThreads) {
       a.paths[row0 + i] = i == 0 && count > 0 ? 0 : -1;
-    for (int i = tid; i < a.nodes; i += kSumThreads) a.out[row0 + i] = -1;
+      a.out[row0 + i] = -1;
+    }
   }
   if (count == 0) {
-    if (s == 0 && tid == 0) a.stands[b] = Stand{0, 0, 0, 0};
+    if (writes && tid == 0) a.stands[b] = Stand{0, 0, 0, 0};
     return;
   }
   gather<T>(a, b, count, d);
   if (tid == 0) {
-    d.at = Stand{0, 1, 0, 1};
+    d.s->at = Stand{0, 1, 0, 1};
     d.z[0] = 1.0;
-    d.more = false;
   }
   __syncthreads();
-  if (tid < 64) {
+  if (wave == 0) {
     VerifyArgs mine = a;
-    if (s != 0) mine.paths = nullptr;
+    if (!writes) mine.paths = nullptr;
     walk(mine, b, count, d);
   }
   __syncthreads();
-  const Stand at = d.at;
-  if (s == 0 && tid == 0) a.stands[b] = at;
-  const int64_t x0 = s * a.slice, x1 = min(x0 + a.slice, a.vocab);
-  if (!DRAFT) gone_in(count, x0, x1, d);
+  const Stand at = d.s->at;
+  if (writes && tid == 0) a.stands[b] = at;
+  const int s = blockIdx.x * kWaves + wave;
+  int64_t x0, x1;
+  slice_of(a, s, x0, x1);
+  if (!DRAFT) {  // of all the block's slices
+    int64_t y0, y1, y2, y3;
+    slice_of(a, blockIdx.x * kWaves, y0, y1);
+    slice_of(a, blockIdx.x * kWaves + kWaves - 1, y2, y3);
+    gone_in(count, y0, y3, d);
+  }
+  if (s >= a.slices) return;
   const int64_t row = (row0 + at.last) * a.vocab;
-  double sum = range_sum<T, DRAFT>((const T*)a.target + row, (const T*)a.draft + row, x0, x1, d,
-                                   at.tried, DRAFT ? 0 : d.ngone, tid, kSumThreads);
-  sum = wave_sum(sum);
-  if ((tid & 63) == 0) part[tid >> 6] = sum;
-  __syncthreads();
-  if (tid == 0) a.sums[(int64_t)b * a.slices + s] = part[0] + part[1] + part[2] + part[3];
+  const double sum = wave_sum(range_sum<T, DRAFT>((const T*)a.target + row, (const T*)a.draft + row,
+                                                  x0, x1, d, at.tried, DRAFT ? 0 : d.s->ngone, lane, 64));
+  if (lane == 0) a.sums[(int64_t)b * a.slices + s] = sum;
+}
+
+// Running sums of the slices: a lane has those of its four, of which `s` are
+// the sums; every wave for itself.  Returns the sum of all.
+__device__ __forceinline__ double slice_scan(const double* sums, int lane, double (&s)[4],
+                                             double (&upto)[4]) {
+  double run = 0.0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    s[i] = sums[4 * lane + i];
+    run += s[i];
+  }
+  double x = run;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const double o = __shfl_up(x, off);
+    if (lane >= off) x += o;
+  }
+  double before = __shfl_up(x, 1);
+  if (lane == 0) before = 0.0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    before += s[i];
+    upto[i] = before;
+  }
+  return __shfl(upto[3], 63);
 }
 
 // Grid (B).
 template <typename T, bool DRAFT>
 __global__ void __launch_bounds__(kDrawThreads) verify_draw(VerifyArgs a) {
   constexpr int kWaves = kDrawThreads / 64;
-  __shared__ Drafts d;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const Drafts d = drafts_in(lds, a.nodes);
   __shared__ double sums[kMostSlices], part[kWaves];
-  __shared__ int64_t found[kWaves];
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ int64_t found[2][kWaves];
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int count = count_of(a, b);
   const int64_t row0 = (int64_t)b * a.nodes;
   const Stand first = a.stands[b];
+  const float u0 = a.uniforms[row0];
+  if (tid < kMostSlices) sums[tid] = tid < a.slices ? a.sums[(int64_t)b * a.slices + tid] : 0.0;
   if (first.accepted == 0) {
     if (tid == 0) a.accepted[b] = 0;
     return;
   }
-  if (tid < a.slices) sums[tid] = a.sums[(int64_t)b * a.slices + tid];
   if (tid == 0) {
-    d.at = first;
+    d.s->at = first;
     d.z[0] = 1.0;
-    d.more = DRAFT && first.tried > 0;
-    d.ngone = 0;
+    d.s->more = DRAFT && first.tried > 0;
   }
   if (!DRAFT) {  // the refused tokens
     for (int i = tid; i < count; i += kDrawThreads) {
@@ -318,17 +391,14 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw(VerifyArgs a) {
     }
   }
   __syncthreads();
-  auto total = [&] {
-    double z = 0.0;
-    for (int s = 0; s < a.slices; ++s) z += sums[s];
-    return z;
-  };
+  double own[4], upto[4];  // of this lane's slices
   // the sums of all slices by this block alone, a wave a slice
-  auto sum_all = [&](int tried, int ngone) {
+  auto sum_all = [&](int tried, int ngone) __attribute__((always_inline)) {
     __syncthreads();
-    const int64_t row = (row0 + d.at.last) * a.vocab;
+    const int64_t row = (row0 + d.s->at.last) * a.vocab;
     for (int s = wave; s < a.slices; s += kWaves) {
-      const int64_t x0 = s * a.slice, x1 = min(x0 + a.slice, a.vocab);
+      int64_t x0, x1;
+      slice_of(a, s, x0, x1);
       const double sum = wave_sum(range_sum<T, DRAFT>((const T*)a.target + row,
                                                       (const T*)a.draft + row, x0, x1, d, tried,
                                                       ngone, lane, 64));
@@ -338,62 +408,65 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw(VerifyArgs a) {
   };
   if constexpr (DRAFT) {
     bool gathered = false;
-    while (d.more) {
-      // the sum of what the last refusal left is there: try the next child
-      if (!gathered) {
-        gather<T>(a, b, count, d);
-        gathered = true;
-      }
-      const double z = total();
+    // the sum of what the last refusal left is there: try the next child, if
+    // there is one
+    while (d.s->more) {
+      if (!gathered) gather<T>(a, b, count, d);
+      gathered = true;
+      const double z = slice_scan(sums, lane, own, upto);
+      const Stand before = d.s->at;
       __syncthreads();
-      if (tid == 0) d.z[d.at.tried] = z;
-      __syncthreads();
-      const Stand before = d.at;
+      if (tid == 0) d.z[before.tried] = z;
       __syncthreads();
       if (wave == 0) walk(a, b, count, d);
       __syncthreads();
-      const bool moved = d.at.last != before.last || d.at.tried != before.tried;
-      if (!moved) break;  // no child left: the sums are of this row
-      sum_all(d.at.tried, 0);
+      // no child left: the sums are of this row
+      if (d.s->at.last == before.last && d.s->at.tried == before.tried) break;
+      sum_all(d.s->at.tried, 0);
     }
     __syncthreads();
   }
-  const Stand at = d.at;
+  const Stand at = d.s->at;
   int tried = at.tried;
-  double z = total();
+  double z = slice_scan(sums, lane, own, upto);
   bool plain = false;  // draw from p itself
   if (!(z > 0.0) && tried > 0) {
     plain = true;
     tried = 0;
     sum_all(0, 0);
-    z = total();
+    z = slice_scan(sums, lane, own, upto);
   }
   int64_t token = -1;
   if (z > 0.0) {
-    const double t = fmax((double)a.uniforms[row0] * z, 0.0);
+    const double t = fmax((double)u0 * z, 0.0);
     // the slice: the first whose running sum exceeds t, or the last that has any
-    double before = 0.0, run = 0.0;
-    int slice = 0;
-    bool inside = false;
-    for (int s = 0; s < a.slices; ++s) {
-      const double next = run + sums[s];
-      if (sums[s] > 0.0) {
-        slice = s;
-        before = run;
-        if (next > t) {
-          inside = true;
-          break;
-        }
+    int mine = -1, last = -1;
+    double before = 0.0, at_last = 0.0;
+#pragma unroll
+    for (int i = 3; i >= 0; --i) {
+      if (!(own[i] > 0.0)) continue;
+      if (last < 0) {
+        last = 4 * lane + i;
+        at_last = upto[i] - own[i];
       }
-      run = next;
+      if (upto[i] > t) {
+        mine = 4 * lane + i;
+        before = upto[i] - own[i];
+      }
     }
-    const int64_t x0 = slice * a.slice, x1 = min(x0 + a.slice, a.vocab);
+    const unsigned long long over = __ballot(mine >= 0), some_at = __ballot(last >= 0);
+    const bool inside = over != 0;
+    const int from = inside ? __ffsll((long long)over) - 1 : 63 - __clzll((long long)some_at);
+    const int slice = __shfl(inside ? mine : last, from);
+    before = __shfl(inside ? before : at_last, from);
+    int64_t x0, x1;
+    slice_of(a, slice, x0, x1);
     if (!DRAFT && !plain) gone_in(count, x0, x1, d);
-    const int ngone = DRAFT || plain ? 0 : d.ngone;
+    const int ngone = DRAFT || plain ? 0 : d.s->ngone;
     const int64_t row = (row0 + at.last) * a.vocab;
     const T* p = (const T*)a.target + row;
     const T* q = (const T*)a.draft + row;
-    auto left = [&](int64_t x) {
+    auto left = [&](int64_t x) __attribute__((always_inline)) {
       float w = weight(to_f32(p[x]));
       if constexpr (DRAFT) {
         if (tried > 0) return left_of((double)w, (double)weight(to_f32(q[x])), d.z, tried);
@@ -403,29 +476,37 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw(VerifyArgs a) {
       }
       return (double)w;
     };
-    // neighbouring tokens to a thread, threads in order
+    // neighbouring tokens to a thread, threads in order; past kKept of them
+    // their weights are formed again
+    constexpr int kKept = 4;
     const int64_t per = (x1 - x0 + kDrawThreads - 1) / kDrawThreads;
     const int64_t m0 = min(x0 + tid * per, x1), m1 = min(m0 + per, x1);
-    double mine = 0.0;
+    double kept[kKept], sum = 0.0;
     int64_t some = -1;
-    for (int64_t x = m0; x < m1; ++x) {
+#pragma unroll
+    for (int i = 0; i < kKept; ++i) kept[i] = m0 + i < m1 ? left(m0 + i) : 0.0;
+#pragma unroll
+    for (int i = 0; i < kKept; ++i) {
+      sum += kept[i];
+      if (kept[i] > 0.0) some = m0 + i;
+    }
+    for (int64_t x = m0 + kKept; x < m1; ++x) {
       const double w = left(x);
-      mine += w;
+      sum += w;
       if (w > 0.0) some = x;
     }
-    double upto = mine;  // inclusive, in the wave
+    double run = sum;  // inclusive, in the wave
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
-      const double o = __shfl_up(upto, off);
-      if (lane >= off) upto += o;
+      const double o = __shfl_up(run, off);
+      if (lane >= off) run += o;
     }
-    if (lane == 63) part[wave] = upto;
+    if (lane == 63) part[wave] = run;
     __syncthreads();
-    double base = before;
-    for (int w = 0; w < wave; ++w) base += part[w];
+    for (int w = 0; w < wave; ++w) before += part[w];
     int64_t hit = INT64_MAX;
-    double c = base + (upto - mine);
-    if (inside && base + upto > t) {
+    if (inside && before + run > t) {
+      double c = before + (run - sum);
       for (int64_t x = m0; x < m1; ++x) {
         const double w = left(x);
         c += w;
@@ -441,15 +522,16 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw(VerifyArgs a) {
       hit = h < hit ? h : hit;
       some = l > some ? l : some;
     }
-    if (lane == 0) found[wave] = hit;
-    __syncthreads();
-    hit = INT64_MAX;
-    for (int w = 0; w < kWaves; ++w) hit = found[w] < hit ? found[w] : hit;
-    __syncthreads();
-    if (lane == 0) found[wave] = some;
+    if (lane == 0) {
+      found[0][wave] = hit;
+      found[1][wave] = some;
+    }
     __syncthreads();
     // (rounding alone, or u of 1 and more, leave t behind the last weight)
-    for (int w = 0; w < kWaves; ++w) some = found[w] > some ? found[w] : some;
+    for (int w = 0; w < kWaves; ++w) {
+      hit = found[0][w] < hit ? found[0][w] : hit;
+      some = found[1][w] > some ? found[1][w] : some;
+    }
     token = hit != INT64_MAX ? hit : some;
   }
   if (tid == 0) {
@@ -458,10 +540,10 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw(VerifyArgs a) {
   }
 }
 
-// Slices that give the device enough blocks, of at least 1024 tokens.
+// Slices of at least 512 tokens, enough for some 8192 waves on the device.
 void slicing(int batch, int64_t vocab, int64_t& slice, int& slices) {
-  const int64_t want = std::max(1, std::min(kMostSlices, 2048 / batch));
-  slice = std::max<int64_t>(1024, ((vocab + want - 1) / want + 255) / 256 * 256);
+  const int64_t want = std::max(4, std::min(kMostSlices, 8192 / batch));
+  slice = std::max<int64_t>(512, ((vocab + want - 1) / want + 63) / 64 * 64);
   slices = (int)((vocab + slice - 1) / slice);
 }
 
@@ -472,13 +554,14 @@ bool sizes_ok(int batch, int nodes, int64_t vocab) {
 
 template <typename T>
 void launch(const VerifyArgs& a, int batch, hipStream_t s) {
-  const dim3 grid((unsigned)a.slices, (unsigned)batch);
+  const dim3 grid((unsigned)((a.slices + kSumThreads / 64 - 1) / (kSumThreads / 64)), (unsigned)batch);
+  const size_t lds = drafts_bytes(a.nodes);
   if (a.draft != nullptr) {
-    hipLaunchKernelGGL((verify_sums<T, true>), grid, dim3(kSumThreads), 0, s, a);
-    hipLaunchKernelGGL((verify_draw<T, true>), dim3((unsigned)batch), dim3(kDrawThreads), 0, s, a);
+    hipLaunchKernelGGL((verify_sums<T, true>), grid, dim3(kSumThreads), lds, s, a);
+    hipLaunchKernelGGL((verify_draw<T, true>), dim3((unsigned)batch), dim3(kDrawThreads), lds, s, a);
   } else {
-    hipLaunchKernelGGL((verify_sums<T, false>), grid, dim3(kSumThreads), 0, s, a);
-    hipLaunchKernelGGL((verify_draw<T, false>), dim3((unsigned)batch), dim3(kDrawThreads), 0, s, a);
+    hipLaunchKernelGGL((verify_sums<T, false>), grid, dim3(kSumThreads), lds, s, a);
+    hipLaunchKernelGGL((verify_draw<T, false>), dim3((unsigned)batch), dim3(kDrawThreads), lds, s, a);
   }
 }
 
