@@ -43,12 +43,30 @@ struct RotaryArgs {
   double inv[kMaxPairs];
 };
 
-// theta reduced to [-pi, pi]: an fma by each of the two parts of 2 pi loses
-// nothing that counts, since theta / 2 pi stays below 2^31.
-__device__ __forceinline__ double reduced(double theta) {
-  constexpr double kTwoPi = 6.283185307179586232, kRest = 2.4492935982947064e-16;
-  const double n = rint(theta * 0.15915494309189535);
-  return fma(-n, kRest, fma(-n, kTwoPi, theta));
+// sin and cos of a theta below 2^33 in size, to some 2^-52 of 1: what whole quarter
+// turns leave (an fma by each of the two parts of pi / 2 loses nothing that
+// counts), then the powers up to where the next one is below 2^-60 at pi / 4.
+__device__ __forceinline__ double2 angle_of(double theta) {
+  constexpr double kQuarter = 1.570796326794896558, kRest = 6.123233995736766e-17;
+  const double n = rint(theta * 0.63661977236758134);
+  const double x = fma(-n, kRest, fma(-n, kQuarter, theta)), z = x * x;
+  constexpr double kSin[8] = {-1.0 / 6,          1.0 / 120,           -1.0 / 5040,
+                              1.0 / 362880,      -1.0 / 39916800,     1.0 / 6227020800.0,
+                              -1.0 / 1307674368000.0, 1.0 / 355687428096000.0};
+  constexpr double kCos[8] = {-1.0 / 2,          1.0 / 24,            -1.0 / 720,
+                              1.0 / 40320,       -1.0 / 3628800,      1.0 / 479001600,
+                              -1.0 / 87178291200.0, 1.0 / 20922789888000.0};
+  double s = kSin[7], c = kCos[7];
+#pragma unroll
+  for (int i = 6; i >= 0; --i) {
+    s = fma(s, z, kSin[i]);
+    c = fma(c, z, kCos[i]);
+  }
+  s = fma(s * z, x, x);
+  c = fma(c, z, 1.0);
+  const int turns = (int)(int64_t)n & 3;
+  const double ys = turns & 1 ? c : s, yc = turns & 1 ? s : c;
+  return make_double2(turns == 1 || turns == 2 ? -yc : yc, turns >= 2 ? -ys : ys);
 }
 
 template <typename T>
@@ -134,14 +152,6 @@ __device__ __forceinline__ void token_angles(const RotaryArgs& a, int t, float2*
     cs[p] = make_float2(c, s);
   }
 }
-__device__ __forceinline__ void token_angles(const RotaryArgs& a, int t, double2* cs) {
-  for (int p = threadIdx.x; p < a.R; p += kThreads) {
-    double c, s;
-    sincos(reduced((double)a.positions[t] * a.inv[p]), &s, &c);
-    cs[p] = make_double2(c, s);
-  }
-}
-
 // One token per grid row, eight channels per thread; grid y shares out a
 // token's rows (queries, keys, values, in this order).
 template <typename T>
@@ -180,14 +190,30 @@ __global__ void __launch_bounds__(kThreads) rotary_rows_kernel(RotaryArgs a) {
   }
 }
 
-__device__ __forceinline__ double over_group(double x, bool largest) {
-#pragma unroll
-  for (int off = 1; off <= 2; off <<= 1) {
-    const double o = __shfl_xor(x, off);
-    x = largest ? fmax(x, o) : fmin(x, o);
-  }
-  return x;
+// Over the four neighbouring threads of a group (whole rows of threads are in
+// step here, so their lanes are).
+template <int CTRL>
+__device__ __forceinline__ float quad(float x) {
+  return __builtin_bit_cast(
+      float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, false));
 }
+template <int CTRL>
+__device__ __forceinline__ double quad(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xf, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(u >> 32), CTRL, 0xf, 0xf, false);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+constexpr int kQuad1 = 0xb1, kQuad2 = 0x4e;  // lane ^ 1, lane ^ 2
+template <typename A, typename F>
+__device__ __forceinline__ A over_group(A x, F f) {
+  x = f(x, quad<kQuad1>(x));
+  return f(x, quad<kQuad2>(x));
+}
+__device__ __forceinline__ float least_of(float a, float b) { return fminf(a, b); }
+__device__ __forceinline__ double least_of(double a, double b) { return fmin(a, b); }
+__device__ __forceinline__ float most_of(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ double most_of(double a, double b) { return fmax(a, b); }
 
 // Through float32, in two roundings: left to itself the compiler makes one
 // (and a long one) of them.
@@ -198,87 +224,120 @@ __device__ __forceinline__ f16_t to_half(double x) {
 }
 
 // The codes of 8 channels, and the step and least value of the group of four
-// neighbouring threads that share them.
-__device__ __forceinline__ uint32_t codes8(const double (&x)[8], f16_t& step, f16_t& least) {
-  double lo = x[0], hi = x[0];
-  bool finite = true;
+// neighbouring threads that share them.  A: double, or float where the
+// channels are values of 32 bits or fewer as they stand.
+template <typename A>
+__device__ __forceinline__ uint32_t codes8(const A (&x)[8], f16_t& step, f16_t& least) {
+  A lo = x[0], hi = x[0], odd = x[0] * (A)0;  // odd: NaN where a channel is not finite
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    lo = fmin(lo, x[i]);
-    hi = fmax(hi, x[i]);
-    finite = finite && __builtin_isfinite(x[i]);
+  for (int i = 1; i < 8; ++i) {
+    lo = least_of(lo, x[i]);
+    hi = most_of(hi, x[i]);
+    odd += x[i] * (A)0;
   }
-  lo = over_group(lo, false);
-  hi = over_group(hi, true);
-  finite = over_group(finite ? 1.0 : 0.0, false) != 0.0;
+  lo = over_group(lo, [](A a, A b) { return least_of(a, b); });
+  hi = over_group(hi, [](A a, A b) { return most_of(a, b); });
+  odd = over_group(odd, [](A a, A b) { return a + b; });
   constexpr double kMost = 65504.0;
-  least = to_half(fmin(fmax(lo, -kMost), kMost));
-  step = to_half(fmin(fmax((hi - (double)least) / 15.0, 0.0), kMost));
-  if (!finite) {  // the whole group reads as NaN
+  least = to_half(fmin(fmax((double)lo, -kMost), kMost));
+  // a fifteenth, rounded as a division rounds: the quotient by the rounded
+  // reciprocal, set right by what it leaves
+  constexpr double kFifteenth = 1.0 / 15.0;
+  const double range = (double)hi - (double)least;
+  double fifteenth = range * kFifteenth;
+  fifteenth = fma(fma(-15.0, fifteenth, range), kFifteenth, fifteenth);
+  step = to_half(fmin(fmax(fifteenth, 0.0), kMost));
+  if (odd != odd) {  // the whole group reads as NaN
     least = (f16_t)__builtin_nanf("");
     step = (f16_t)0.f;
   }
-  const double m = (double)least, d = (double)step;
-  if (!(d > 0.0)) return 0u;
-  const float inv = 1.f / (float)d;
-  uint32_t word = 0;
+  const float d = (float)step;
+  if (!(d > 0.f)) return 0u;
+  const A m = (A)(float)least;
+  const float inv = __builtin_amdgcn_rcpf(d);
+  // Adding 2^23 rounds to whole numbers and leaves them in the low bits; the
+  // bits of 2^23 itself, shifted along, are taken off the word beforehand.
+  // The float quotient is some 1e-5 off at most (16 2^-24 for the difference,
+  // the product and the reciprocal each): nearer than 1e-4 to a border the
+  // exact one decides.
+  constexpr float kWhole = 8388608.f;
+  uint32_t word = 0u - 0xfb000000u;
+  float far = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    // the float quotient is some 1e-6 off: next to a border the exact one
-    // decides
-    float c = (float)(x[i] - m) * inv;
-    const float down = floorf(c);
-    if (fabsf(c - down - 0.5f) < 1e-4f) c = (float)rint((x[i] - m) / d);
-    c = fminf(fmaxf(rintf(c), 0.f), 15.f);
-    word |= (uint32_t)c << (4 * i);
+    const float c = fminf(fmaxf((float)(x[i] - m) * inv, 0.f), 15.f);
+    const float y = c + kWhole;
+    far = fmaxf(far, fabsf(c - (y - kWhole)));
+    word += __builtin_bit_cast(uint32_t, y) << (4 * i);
+  }
+  if (far > 0.4999f) {
+    word = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const double c = rint(((double)x[i] - (double)(float)least) / (double)d);
+      word |= (uint32_t)fmin(fmax(c, 0.0), 15.0) << (4 * i);
+    }
   }
   return word;
 }
 
-// The same with the pool's rows as codes.
+// The same with the pool's rows as codes.  A thread keeps its channels and
+// goes down the rows, the next row's on their way while it works on one.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) q4_append_kernel(RotaryArgs a) {
   __shared__ double2 cs[kMaxPairs];
+  __shared__ float2 csf[kMaxPairs];
   const int t = blockIdx.x;
   const int slot = a.slots[t];
   const bool stored = slot >= 0 && slot < a.rows;
   const int per = a.D >> 3, groups = a.D / kQ4Group, size = 1 << a.page_shift;
-  const int turned = (a.Hq + a.Hkv) * per, items = turned + a.Hkv * per;
-  token_angles(a, t, cs);
+  const int down = kThreads / per, first = threadIdx.x / per;
+  const int o = threadIdx.x - first * per, c0 = 8 * o;
+  const bool works = first < down;
+  const int q_rows = works ? a.Hq : 0, kv_rows = works && stored ? 2 * a.Hkv : 0;
+  const int stride = down * gridDim.y, row0 = blockIdx.y * down + first;
+  const int kv_row0 = (gridDim.y - 1 - blockIdx.y) * down + first;
+  for (int p = threadIdx.x; p < a.R; p += kThreads) {
+    const double2 r = angle_of((double)a.positions[t] * a.inv[p]);
+    cs[p] = r;
+    csf[p] = make_float2((float)r.x, (float)r.y);
+  }
   __syncthreads();
-  // rows are whole groups of four threads, so a group's threads stay together
-  for (int j = blockIdx.y * kThreads + threadIdx.x; j < items; j += kThreads * gridDim.y) {
-    const int row = j / per, c0 = 8 * (j - row * per);
-    if (row < a.Hq) {
-      const int64_t at = ((int64_t)t * a.Hq + row) * a.D;
-      const T* src = (const T*)a.q + at;
-      const Row8<T> raw = load8(src + c0, 8, a.vec);
-      double y[8];
-      turn8(a, src, c0, 8, raw, cs, y);
-      Row8<T> out;
+  for (int row = row0; row < q_rows; row += stride) {
+    const int64_t at = ((int64_t)t * a.Hq + row) * a.D;
+    const T* src = (const T*)a.q + at;
+    int at0 = c0;  // (or a row's angles stay in registers: 92 of them, 31 us for 28)
+    asm volatile("" : "+v"(at0));
+    float y[8];
+    turn8(a, src, at0, 8, load8(src + c0, 8, a.vec), csf, y);
+    Row8<T> out;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) out.x[i] = from_f32<T>((float)y[i]);
-      store8((T*)a.q_out + at + c0, out, 8, a.vec);
-      continue;
-    }
-    if (!stored) return;
-    const bool is_k = row < a.Hq + a.Hkv;
-    const int h = is_k ? row - a.Hq : row - a.Hq - a.Hkv;
+    for (int i = 0; i < 8; ++i) out.x[i] = from_f32<T>(y[i]);
+    store8((T*)a.q_out + at + c0, out, 8, a.vec);
+  }
+  for (int row = kv_row0; row < kv_rows; row += stride) {
+    const bool is_k = row < a.Hkv;
+    const int h = is_k ? row : row - a.Hkv;
     const T* src = (const T*)(is_k ? a.k : a.v) + ((int64_t)t * a.Hkv + h) * a.D;
     const Row8<T> raw = load8(src + c0, 8, a.vec);
-    double y[8];
-    if (is_k) {
-      turn8(a, src, c0, 8, raw, cs, y);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = (double)to_f32(raw.x[i]);
-    }
     f16_t step, least;
-    const uint32_t word = codes8(y, step, least);
+    uint32_t word;
+    if (is_k) {
+      int at0 = c0;
+      asm volatile("" : "+v"(at0));
+      double y[8];
+      turn8(a, src, at0, 8, raw, cs, y);
+      word = codes8(y, step, least);
+    } else {
+      float y[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = to_f32(raw.x[i]);
+      word = codes8(y, step, least);
+    }
     const int64_t head = (int64_t)(slot >> a.page_shift) * a.Hkv + h;
-    const int r = slot & (size - 1), g = c0 / kQ4Group;
-    ((uint32_t*)(is_k ? a.kc : a.vc))[(head * size + r) * per + (c0 >> 3)] = word;
-    if ((c0 & (kQ4Group - 1)) == 0) {
+    const int r = slot & (size - 1), g = o >> 2;
+    ((uint32_t*)(is_k ? a.kc : a.vc))[(head * size + r) * per + o] = word;
+    if ((o & 3) == 0) {
       f16_t* s = (is_k ? a.ks : a.vs) + (head * 2 * groups + g) * size + r;
       s[0] = step;
       s[(int64_t)groups * size] = least;
