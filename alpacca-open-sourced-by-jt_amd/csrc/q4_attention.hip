@@ -14,8 +14,17 @@ namespace {
 
 constexpr int kCus = 256;
 
-constexpr int64_t kAloneRows = 1024;  // of the longest sequence, for one launch
-constexpr int64_t kRowsPerSlot = 256;  // at least, beyond a block a CU
+// Up to this length of the longest sequence a block takes a whole sequence and
+// one launch is all: with few blocks, and with one for every CU.  bf16, 32/8
+// heads of 128, us whole and split:
+//   1 x 1 token on 512 rows 8.7, 10.2; on 1024 12.3, 10.6; on 2048 19.6, 10.8
+//   32 x 1      on 512 10.1, 13.1; on 2048 22.1, 24.4; on 4096 36.0, 32.1
+//   4 x 64      on 512 15.8, 23.1; on 2048 33.3, 34.5; on 8192 101, 76
+constexpr int64_t kAloneRows = 512, kAloneRowsFull = 2048;
+// Beyond a block a CU a share has this many rows at least: 32 x 1 on 512 rows,
+// split: 13.1 us with 128 and 256, 23.0 with 512; 4 x 1 on 2048: 12.9 with 128,
+// 11.0 with 256 and more.
+constexpr int64_t kRowsPerSlot = 256;
 
 struct Q4Plan {
   Q4Kernel kernel;
@@ -38,7 +47,7 @@ Q4Plan q4_plan(int batch, int nodes, int q_heads, int kv_heads, int head_dim, in
   const int64_t share = std::min(kCus * p.kernel.per_cu / units,
                                  std::max(kCus / units, tiles * p.kernel.rows / kRowsPerSlot));
   p.slots = (int)std::min(std::max<int64_t>(share, 1), tiles);
-  p.alone = length <= kAloneRows;
+  p.alone = length <= (batch * units >= kCus ? kAloneRowsFull : kAloneRows);
   if (p.alone) p.slots = batch;
   p.blocks = ((int64_t)p.slots * kv_heads + kXcds - 1) / kXcds * kXcds * p.col_tiles;
   if (p.alone) return p;

@@ -1647,7 +1647,7 @@ class Qwen35RocmOps:
         """The pool's arrays, checked, and ``(pages, kv heads, page size, width)``."""
         t = self.torch
         index, shape = self.device_index, getattr(key_codes, "shape", ())
-        if len(shape) == 4:
+        if len(shape) == 4 and all(map(t.is_tensor, (key_scales, value_codes, value_scales))):
             pages, heads, size, half = shape
             scales = (pages, heads, 2, half // 16, size)
             if (key_codes.dtype == value_codes.dtype == t.uint8

@@ -870,7 +870,8 @@ int alpx_q4_rows(const void* key_codes, const void* key_scales, const void* valu
  * to [0, length], and nothing behind a sequence's rows is read for its
  * result.  A token at or past counts[b], and one whose own row lies past
  * length, give zeros, whatever their gate holds.  NaN in rows that a token
- * does not see stays out of its result.
+ * does not see stays out of its result.  Scores are float32: a query's largest
+ * value times scale stays below 2^100.
  * workspace: alpx_q4_workspace_bytes bytes (0 for sizes that the call
  * refuses), 16-byte aligned; scratch, which calls that may overlap must not
  * share.  out must not overlap any input. */
@@ -907,7 +908,8 @@ int alpx_q4_attention(const void* q, const void* key_codes, const void* key_scal
  * counts[b] drafts of a sequence count (null: all); none: nothing stands and
  * nothing is drawn.  Tokens outside [0, vocab) weigh 0.  Up to 1024 drafts
  * and 65535 sequences.  workspace: alpx_verify_workspace_bytes bytes, 16-byte
- * aligned scratch of the call.  Two launches. */
+ * aligned scratch of the call.  Two launches, up to five for trees of drawn
+ * drafts. */
 size_t alpx_verify_workspace_bytes(int batch, int nodes, int64_t vocab);
 int alpx_verify_drafts(const int32_t* tokens, const void* target, const void* draft,
                        const int32_t* parents, const int32_t* counts, const float* uniforms,

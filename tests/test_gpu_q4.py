@@ -316,6 +316,31 @@ def test_short_sequences_in_long_tables(gpu, ops, dtype, d, nodes, batch):
          page=32, spare=3000 if batch < 9 else 300).check(ops)
 
 
+@pytest.mark.parametrize("dtype,nodes,batch", [("f32", 1, 64), ("bf16", 1, 65), ("f16", 40, 33),
+                                               ("bf16", 1, 3)])
+@pytest.mark.parametrize("longest", [511, 512, 1100, 2047, 2048])
+def test_a_block_a_sequence_or_shares_of_it(gpu, ops, dtype, nodes, batch, longest):
+    """Lengths about those up to which a block takes a whole sequence, with a
+    block for every unit of the device and with fewer."""
+    prefix = [longest - nodes] + [(97 * b) % 61 for b in range(1, batch)]
+    counts = [nodes] + [b % (nodes + 1) for b in range(1, batch)]
+    for spare in (0, 1):
+        Case(gpu, longest, dtype=dtype, d=64, hq=8, hkv=4, nodes=nodes, prefix=prefix,
+             counts=counts, page=64, spare=spare).check(ops)
+
+
+@pytest.mark.parametrize("dtype,d,hq,nodes", [("f32", 64, 8, 1), ("f16", 128, 8, 2),
+                                              ("bf16", 96, 8, 1), ("bf16", 128, 8, 20)])
+def test_a_query_that_is_not_finite_stays_alone(gpu, ops, dtype, d, hq, nodes):
+    case = Case(gpu, 21, dtype=dtype, d=d, hq=hq, hkv=2, nodes=nodes, prefix=[600, 40])
+    case.q[0, 0, 1, 5], case.q[0, nodes - 1, 5, 40], case.q[1, 0, 0, 33] = np.nan, np.inf, -np.inf
+    with np.errstate(invalid="ignore"):
+        got = case.check(ops)
+    bad = np.isnan(got)
+    assert bad[0, 0, 1].all() and bad[0, nodes - 1, 5].all() and bad[1, 0, 0].all()
+    assert bad.sum() == 3 * d
+
+
 @pytest.mark.parametrize("out_dtype", ["f32", "f16", "bf16"])
 def test_output_types_and_out_buffer(gpu, ops, out_dtype):
     import torch
@@ -589,6 +614,27 @@ def test_verify_matches_oracle(gpu, ops, dtype, batch, nodes, vocab, tree, draft
     _check_verify(gpu, ops, dtype, *case)
     counts = rng.integers(-1, nodes + 2, batch)
     _check_verify(gpu, ops, dtype, *case, counts=counts)
+
+
+@pytest.mark.parametrize("children", [1, 2, 3, 4, 5, 6, 9])
+def test_verify_refusals_one_after_another(gpu, ops, children):
+    """Nodes whose children are all refused but the last, over and over, so
+    that sequences stop at different rounds of the sums."""
+    rng = np.random.default_rng(children)
+    depth, batch, vocab = 4, 5, 1500
+    nodes = 1 + depth * children
+    tokens, target, uniforms, parents, q = _verify_case(rng, "f32", batch, nodes, vocab, True, True)
+    for i in range(1, nodes):
+        parents[:, i] = (i - 1) // children * children
+    uniforms[:, 1:] = 0.999
+    for b in range(batch):  # sequence b: the last children of so many levels stand
+        for level in range(b):
+            at = 1 + level * children + children - 1
+            if at < nodes:
+                uniforms[b, at] = 0.0
+                target[b, parents[b, at], tokens[b, at]] += 0.5
+                q[b, parents[b, at], tokens[b, at]] *= 0.01
+    _check_verify(gpu, ops, "f32", tokens, target, uniforms, parents, q)
 
 
 @pytest.mark.parametrize("draft", [False, True])

@@ -333,3 +333,13 @@ def test_facade_refuses_host_tensors(pkg):
             call()
     with pytest.raises(ValueError, match="must be on device 0"):
         o.paged_q4_rows(*pool, _i32(2))
+
+
+@pytest.mark.parametrize("which", range(4))
+def test_facade_pool_arrays_that_are_no_tensors(ops, which):
+    ops.device = "cpu"
+    arrays = list(ops.initialize_paged_q4_workspace(num_pages=2, page_size=32, kv_heads=1,
+                                                    head_dimension=64).arrays)
+    arrays[which] = None
+    with pytest.raises(TypeError, match="must be a"):
+        ops.paged_q4_rows(*arrays, _i32(3))
