@@ -144,14 +144,6 @@ __device__ __forceinline__ void turn8(const RotaryArgs& a, const T* row, int c0,
   }
 }
 
-// The token's angles, once for all of its heads.
-__device__ __forceinline__ void token_angles(const RotaryArgs& a, int t, float2* cs) {
-  for (int p = threadIdx.x; p < a.R; p += kThreads) {
-    float c, s;
-    rope_cs((double)a.positions[t], a.inv[p], c, s);
-    cs[p] = make_float2(c, s);
-  }
-}
 // One token per grid row, eight channels per thread; grid y shares out a
 // token's rows (queries, keys, values, in this order).
 template <typename T>
@@ -162,7 +154,10 @@ __global__ void __launch_bounds__(kThreads) rotary_rows_kernel(RotaryArgs a) {
   const bool stored = slot >= 0 && slot < a.rows;
   const int per = (a.D + 7) >> 3, per_v = (a.Dv + 7) >> 3;
   const int turned = (a.Hq + a.Hkv) * per, items = turned + a.Hkv * per_v;
-  token_angles(a, t, cs);
+  for (int p = threadIdx.x; p < a.R; p += kThreads) {
+    const double2 r = angle_of((double)a.positions[t] * a.inv[p]);
+    cs[p] = make_float2((float)r.x, (float)r.y);
+  }
   __syncthreads();
   for (int j = blockIdx.y * kThreads + threadIdx.x; j < items; j += kThreads * gridDim.y) {
     if (j >= turned) {
