@@ -216,6 +216,14 @@ __device__ __forceinline__ void write_out(const Q4Args& a, int64_t at, f32x4 o, 
 // query head of one token.  Each wave runs alone over its own tiles, with its
 // own ring in LDS, up to the end of a sequence, where the four meet.
 // Alone (no `found`): a share is a whole sequence, and there is nothing to join.
+//
+// Few columns are bound by memory on long contexts: 4 x 1 on 131072 rows, 32/8
+// heads of 128, fp16, 672 MB in 143 us (4.7 TB/s; the loads alone, without the
+// arithmetic, 5.2).  On shorter ones the start and the end count, some 6 us:
+// the shares, pages, queries and first tiles of a block, and its waves' meeting
+// (16 x 1 ragged 8192, 95 MB: 24 us and 4 for the join).  Many columns are bound
+// by the vector unit, which multiplies by steps, takes P apart and forms
+// operands (4 x 64 on 4133 rows: busy 60% of the time, the matrix unit 24%).
 template <typename S>
 __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
   typedef typename S::T T;
@@ -872,6 +880,13 @@ Q4Kernel make() {
           S::CT == 1 ? 1 : 4, S::kCols, S::kStepRows, S::kPerCu};
 }
 
+// Up to 16 columns one column tile, two tiles of 32 rows to a step where two
+// blocks of them fit a CU (4 x 1 on 32768 rows of 256, one: two do not); up to
+// 8 and 4 of them as queries times groups (16 x 1 ragged 8192, 4 queries a head:
+// 27.8 us, 16 plain columns 33).  Of more, two column tiles to a block: K's and
+// V's operands serve both (4 x 64 on 4133 rows: 48 us; four, which leave a wave
+// a SIMD, 62; several rounds of smaller blocks 58 to 69).  Rings of three and
+// four steps for one column tile take as long as two.
 template <typename T>
 Q4Kernel pick(int head_dim, int cols) {
   const int few = cols <= 4 ? 4 : cols <= 8 ? 8 : cols <= 16 ? 16 : 0;
