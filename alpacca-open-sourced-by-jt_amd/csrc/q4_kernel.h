@@ -77,7 +77,9 @@ struct Q4Shape {
   // costs more than that is worth: 5% (4 x 1 on 131072 rows of 128) to 20% (64).
   static constexpr bool kCentred = QP == 2;
   static constexpr float kUnit = kCentred ? 1.f : 0x1p24f;  // a code of 1 is 1 / kUnit
-  static constexpr float kSumUnit = (kPacked ? 1.f : 64.f) / kUnit;  // of the sums of q
+  static constexpr float kSumScale = kCentred ? 0x1p-9f : 0x1p-6f;  // of a group's sum of q, in parts
+  static constexpr float kSumUnit = (kPacked ? 1.f : 1.f / kSumScale) / kUnit;  // of the sums of q
+  static constexpr int kBases = (G_ + 3) / 4;
   static constexpr int kCols = CP * CT;
   static constexpr int kCodeB = kRows * 16 * G;        // codes of K or V in a tile
   static constexpr int kScaleB = 2 * G * kRows * 2;    // steps, then least values
@@ -144,6 +146,9 @@ __device__ __forceinline__ u32x2 lds_read_tr4x16(const char* p) {
 
 // (by value: a bit cast of a vector's element in place reads its element 0)
 __device__ __forceinline__ f16x2 halves(uint32_t x) { return __builtin_bit_cast(f16x2, x); }
+__device__ __forceinline__ uint32_t pair(f16_t x, f16_t y) {
+  return __builtin_bit_cast(uint32_t, (f16x2){x, y});
+}
 __device__ __forceinline__ u16x2 bits16(uint32_t x) { return __builtin_bit_cast(u16x2, x); }
 
 __device__ __forceinline__ f16x8 four(const f16x2* x) {
@@ -414,25 +419,29 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
           if (g % R == slot_of) own_sum[g / R] = s * S::kSumUnit;
           continue;
         }
-        // the group's sum in units that keep it below 2^14, in three parts
-        s = column_sum(s) * 0.015625f;
+        // the group's sum in units that keep it below 2^14: in three parts, or,
+        // where steps take 8 times it, both in two (22 bits, as q)
+        s = column_sum(s) * S::kSumScale;
         const f16_t p0 = (f16_t)s, p1 = (f16_t)(s - (float)p0);
-        const f16_t p2 = (f16_t)(s - (float)p0 - (float)p1);
-        const u32x2 w = {__builtin_bit_cast(uint32_t, (f16x2){p0, p1}),
-                         __builtin_bit_cast(uint32_t, (f16x2){p2, p0})};
+        uint32_t rest;
+        if constexpr (S::kCentred) rest = pair(p0 * (f16_t)8.f, p1 * (f16_t)8.f);
+        else rest = pair((f16_t)(s - (float)p0 - (float)p1), (f16_t)0.f);
         if ((g & 3) == quad) {
-          sums[g / 4 * 2] = w[0];
-          sums[g / 4 * 2 + 1] = w[1];
+          sums[g / 4 * 2] = pair(p0, p1);
+          sums[g / 4 * 2 + 1] = rest;
         }
       }
       qsum[c] = __builtin_bit_cast(f16x8, sums);
     }
 
     f32x4 o[CT][2 * G];  // O^T[channel 16 n + 4 quad + r][column], in units of 1 / kUnit
-    f32x4 om[CT];        // rows: the groups' sums of p m, then the sum of p
+    float om[CT][S::kBases];  // sums of p m (centred: p (m + 8 d)) of groups `quad` (and quad + 4)
+    float l[CT];              // the sum of p (G = 8: of this lane's keys)
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
-      om[c] = (f32x4)(0.f);
+      l[c] = 0.f;
+#pragma unroll
+      for (int h = 0; h < S::kBases; ++h) om[c][h] = 0.f;
 #pragma unroll
       for (int n = 0; n < 2 * G; ++n) o[c][n] = (f32x4)(0.f);
     }
@@ -446,8 +455,13 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
       vadr[g] = S::kCodeB + vrow * 16 * G + 16 * v_place<G>(vrow, g) + 8 * ((lane >> 3) & 1);
     }
     const bool has_m = quad < G;
-    const int mk = (has_m ? quad : 0) * 64 + 2 * hl;         // least values of K, from plane G on
-    const int mv = (G + (hl < G ? hl : 0)) * 64 + 8 * quad;  // and of V
+    const int mk = (has_m ? quad : 0) * 64 + 2 * hl;  // steps of K; least values from plane G on
+    // and of V: rows of an operand, whose results a lane of the group's quad gets
+    // next to each other: least values, steps, ones (G = 8: those of group quad,
+    // then of quad + 4; the sum of p without the matrix unit)
+    const int vg = G == 8 ? (hl >> 2) + 4 * ((hl >> 1) & 1) : min(hl >> 2, G - 1);
+    const int mv = (((G == 8 ? hl & 1 : hl & 3) == 0 ? G : 0) + vg) * 64 + 8 * quad;
+    const bool ones = G < 8 && (hl & 3) >= 2;
     // steps of four keys; packed: of this column's group of the first R (unused
     // columns take the last group's, for sums of zeros)
     const int dadr = 8 * quad + (S::kPacked ? 64 * min(slot_of, G - 1) : 0);
@@ -534,21 +548,17 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
             for (int r = 0; r < 4; ++r) s[0][8 * u + 4 * kt + r] = over_slots<R>(s[0][8 * u + 4 * kt + r]);
             continue;
           }
-          // least values of this lane's groups against the three parts of the
-          // sums, and what is left of least + 8 steps against the first
+          // least values of this lane's groups against the parts of the sums,
+          // steps against 8 times these
           f16x8 mf = {};
 #pragma unroll
           for (int h = 0; h < (G + 3) / 4; ++h) {
-            const char* mp = sc_k + mk + (G + 4 * h) * 64 + 32 * kt;
-            f16_t x = *(const f16_t*)mp, rest = (f16_t)0.f;
-            if constexpr (S::kCentred) {
-              const float y = fmaf((float)*(const f16_t*)(mp - 64 * G), 8.f, (float)x);
-              x = (f16_t)y;
-              rest = (f16_t)(y - (float)x);
-            }
-            if (G % 4 != 0 && !has_m) x = rest = (f16_t)0.f;
-            mf[4 * h] = mf[4 * h + 1] = mf[4 * h + 2] = x;
-            mf[4 * h + 3] = rest;
+            const char* mp = sc_k + mk + 4 * h * 64 + 32 * kt;
+            f16_t least = *(const f16_t*)(mp + G * 64), d = least;
+            if constexpr (S::kCentred) d = *(const f16_t*)mp;
+            if (G % 4 != 0 && !has_m) least = d = (f16_t)0.f;
+            mf[4 * h] = mf[4 * h + 1] = least;
+            mf[4 * h + 2] = mf[4 * h + 3] = d;
           }
 #pragma unroll
           for (int c = 0; c < CT; ++c) {
@@ -629,7 +639,9 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
           const float M = ceilf(fmaxf(m[c], column_max(top[c])));
           const float w = column_weight(m[c], M);
           m[c] = M;
-          om[c] *= w;
+          l[c] *= w;
+#pragma unroll
+          for (int h = 0; h < S::kBases; ++h) om[c][h] *= w;
 #pragma unroll
           for (int n = 0; n < 2 * G; ++n) o[c][n] *= w;
         }
@@ -645,6 +657,7 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
         for (int e = 0; e < 4 * TP; ++e) {
           const float x0 = fast_exp2(fmaf(s[c][2 * e], k1[c], base));
           const float x1 = fast_exp2(fmaf(s[c][2 * e + 1], k1[c], base));
+          if constexpr (G == 8) l[c] += x0 + x1;
           if constexpr (S::PP == 1) {
             ph[c][e] = (f16x2){(f16_t)x0, (f16_t)x1};
           } else {
@@ -654,31 +667,22 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
         }
       }
 #pragma unroll
-      for (int u = 0; u < TP; ++u) {  // least values, and the sum of p
+      for (int u = 0; u < TP; ++u) {
+        // Least values and 8 steps, as exact as they stand, and joined tile by
+        // tile: their sums over all rows would grow past what they leave.
         const char* mp = tiles + u * S::kTileB + 2 * S::kCodeB + S::kScaleB + mv;
         const u32x2 m0 = *(const u32x2*)mp, m1 = *(const u32x2*)(mp + 32);
         constexpr uint32_t kOnes = 0x3c003c00u;
-        f16x8 mf = __builtin_bit_cast(
-            f16x8, (u32x4){hl < G ? m0[0] : kOnes, hl < G ? m0[1] : kOnes, hl < G ? m1[0] : kOnes,
-                           hl < G ? m1[1] : kOnes});
-        f16x8 rest = {};  // centred codes: least + 8 steps, in two parts
-        if constexpr (S::kCentred) {
-          const char* dp = mp - 64 * G;
-          const f16x4 d0 = *(const f16x4*)dp, d1 = *(const f16x4*)(dp + 32);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float d = hl < G ? (float)(e < 4 ? d0[e & 3] : d1[e & 3]) : 0.f;
-            const float x = fmaf(d, 8.f, (float)mf[e]);
-            mf[e] = (f16_t)x;
-            rest[e] = (f16_t)(x - (float)mf[e]);
-          }
-        }
+        const f16x8 mf = __builtin_bit_cast(
+            f16x8, (u32x4){ones ? kOnes : m0[0], ones ? kOnes : m0[1], ones ? kOnes : m1[0],
+                           ones ? kOnes : m1[1]});
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
-          const f16x8 hi = four(ph[c] + 4 * u);
-          om[c] = mfma16x16x32(mf, hi, om[c]);
-          if constexpr (S::PP == 2) om[c] = mfma16x16x32(mf, four(pl[c] + 4 * u), om[c]);
-          if constexpr (S::kCentred) om[c] = mfma16x16x32(rest, hi, om[c]);
+          f32x4 x = mfma16x16x32(mf, four(ph[c] + 4 * u), (f32x4)(0.f));
+          if constexpr (S::PP == 2) x = mfma16x16x32(mf, four(pl[c] + 4 * u), x);
+          om[c][0] += S::kCentred ? fmaf(x[1], 8.f, x[0]) : x[0];
+          if constexpr (G == 8) om[c][S::kBases - 1] += S::kCentred ? fmaf(x[3], 8.f, x[2]) : x[2];
+          else l[c] += x[2];
         }
       }
 #pragma unroll
@@ -748,7 +752,7 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
       float* const mo = (float*)smem + (wave * 16 + hl % CP) * S::kMergeRow;
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        const float pm = __shfl(om[c][g & 3], (g >> 2) * 16 + hl);
+        const float pm = __shfl(om[c][g >> 2], (g & 3) * 16 + hl);
         const float bad = (nans[c] >> g & 1) ? __builtin_nanf("") : 0.f;
 #pragma unroll
         for (int n = 2 * g; n < 2 * g + 2; ++n) {
@@ -758,8 +762,8 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
           if (!S::kPacked || g % R == slot_of) *(f32x4*)(mo + 16 * n + 4 * quad) = x;
         }
       }
-      const float l = __shfl(om[c][G & 3], (G >> 2) * 16 + hl);
-      if (lane < CP) st[(wave * CT + c) * 16 + hl] = (f32x4){m[c], l, 0.f, 0.f};
+      const float sum_p = G == 8 ? column_sum(l[c]) : l[c];
+      if (lane < CP) st[(wave * CT + c) * 16 + hl] = (f32x4){m[c], sum_p, 0.f, 0.f};
       __syncthreads();
       for (int x = tid; x < CP * 8 * G; x += 64 * kWaves) {
         const int cl = x / (8 * G), ch = 4 * (x - cl * (8 * G));

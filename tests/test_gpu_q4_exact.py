@@ -1,0 +1,109 @@
+"""What the attention over 4-bit pools gives before its output's rounding
+(float32 output whatever the queries' type), against the float64 oracle.
+
+Tolerances.  A weight p is off by what its score is, and by 2^-22 for its two
+float16 parts; p times a step by 2^-22 more; scores of deviation 1 stay below 8
+in size, so that float32 forms them, and the exponential, within 2^-20 or so
+(queries of 16 bits against codes as they stand: 2^-18).  Together a row's
+share p (v - 8 steps or less) is off by less than 2^-17 of its gross p (|least|
++ step code), so a channel is by less than 2^-17 of the weighted gross; and
+since the rows' errors are independent and values have mean zero, the 2-norm of
+all channels' errors is below 2^-17 of the result's, on any number of rows."""
+
+import importlib
+
+import numpy as np
+import pytest
+
+from oracle import inputs as I
+from oracle import q4 as Q
+from tests.test_gpu_q4 import PKG, Case, _host, _td
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops(gpu):
+    return importlib.import_module(PKG + ".qwen35_rocm_ops").Qwen35RocmOps()
+
+
+def _close(case, ops, bound, extra=0.0, **kw):
+    got = _host(case.call(ops, out_dtype=_td("f32"), **kw))
+    want, weight = case.oracle(kw.get("scale"), True)
+    assert np.isfinite(got).all()
+    off = np.abs(got - want)
+    assert (off <= bound * weight + extra).all(), np.max(off / (weight + 1e-30))
+    return got, want
+
+
+def _coarse(case, step):
+    """What large steps cost: weights are formed 2^lift smaller, for a step below
+    2^lift, so that their products with it stay in float16.  The largest one is
+    then 2^(11 - lift) at least, and a row's, and its product with any step, are
+    off by 2^-25 and twice 2^-25 at most where float16 is subnormal: times |least
+    + 8 step| <= gross and |code - 8| <= 8, 2^-25 (16 + gross) a row; half of the
+    codes count 16-fold and their weights as a 16th, which rounds once more: 32-fold."""
+    lift = np.frexp(step)[1]
+    lost = np.zeros(case.q.shape)
+    for b, slots in enumerate(case.slots):
+        k, gross = Q.get(case.pool[:2], slots), Q.gross(case.pool[2:], slots)
+        for i in range(case.counts[b]):
+            n = case.prefix[b] + i + 1
+            for h in range(case.q.shape[2]):
+                kv = h // (case.q.shape[2] // k.shape[1])
+                s = (k[:n, kv].astype(np.float64) @ case.q[b, i, h]) * case.d ** -0.5
+                lost[b, i, h] = (16 + gross[:n, kv]).sum(0) / np.exp(s - s.max()).sum()
+    return 2.0 ** (lift - 31) * lost
+
+
+# Groups whose middle, least + 8 steps, float16 does not hold.
+FAR_GROUPS = [(60000.0, 80000.0), (20000.0, 120000.0)]
+FAR_SHAPES = [(64, 4, 1), (96, 6, 2), (128, 4, 1), (128, 8, 3), (128, 32, 1), (128, 8, 10),
+              (256, 4, 1), (256, 4, 6), (256, 8, 9), (64, 8, 9), (96, 8, 9)]
+
+
+@pytest.mark.parametrize("dtype", ["f32"])
+@pytest.mark.parametrize("d,hq,nodes", FAR_SHAPES)
+@pytest.mark.parametrize("span", FAR_GROUPS)
+def test_values_past_what_float16_holds(gpu, ops, dtype, d, hq, nodes, span):
+    """Some of V's groups lie about a middle past 65504."""
+    case = Case(gpu, 60, dtype=dtype, d=d, hq=hq, hkv=2, nodes=nodes, prefix=[700, 33])
+    rng = np.random.default_rng(61)
+    for row in (0, 5, 32, 33):
+        case.v[:, row, :, 32:64] = rng.uniform(*span, case.v[:, row, :, 32:64].shape)
+    case.v[0, 690:700, 1, :32] = rng.uniform(*span, (10, 32))
+    case.store()
+    _close(case, ops, 2.0 ** -17, _coarse(case, (span[1] - span[0]) / 15))
+
+
+@pytest.mark.parametrize("dtype", ["f32"])
+@pytest.mark.parametrize("d,hq", [(64, 4), (128, 8), (256, 8)])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_values_past_what_float16_holds_stay_with_the_tokens_that_see_them(gpu, ops, dtype, d, hq,
+                                                                          which):
+    """They lie in the last tokens' rows; those before see none of them."""
+    for nodes in (2, 7, 20):
+        case = Case(gpu, 62, dtype=dtype, d=d, hq=hq, hkv=2, nodes=nodes, prefix=[600, 30])
+        rng = np.random.default_rng(63)
+        x = case.k if which == "k" else case.v
+        if which == "k":  # (scores that a softmax is still one of)
+            case.q[:] = I.round_to(case.q * 2.0 ** -20, dtype)
+        for b in range(2):
+            at = case.prefix[b] + nodes - 1
+            x[b, at, :, :32] = rng.uniform(20000.0, 120000.0, x[b, at, :, :32].shape)
+        case.store()
+        _close(case, ops, 2.0 ** -17, _coarse(case, 1e5 / 15) if which == "v" else 0.0)
+
+
+@pytest.mark.parametrize("dtype", ["f32"])
+@pytest.mark.parametrize("d,hq,nodes", FAR_SHAPES)
+def test_keys_past_what_float16_holds(gpu, ops, dtype, d, hq, nodes):
+    """Terms of a score sum to less than 2^5 in size, of which a float32 sum
+    loses 2^-20 at most: 2^-15 of a weight."""
+    case = Case(gpu, 64, dtype=dtype, d=d, hq=hq, hkv=2, nodes=nodes, prefix=[700, 33])
+    rng = np.random.default_rng(65)
+    case.q[:] = I.round_to(case.q * 2.0 ** -16, dtype)
+    for row in (0, 5, 32, 33):
+        case.k[:, row, :, 32:64] = rng.uniform(60000.0, 80000.0, case.k[:, row, :, 32:64].shape)
+    case.store()
+    _close(case, ops, 2.0 ** -15)
