@@ -11,15 +11,25 @@
 // The matrix products run on the codes themselves.  With g the groups of 32
 // channels, c the codes, d the steps and m the least values,
 //   q . k_j   = sum_g d_jg (q_g . c_jg) + m_jg (sum of q_g),
-//   sum_j p_j v_j = (sum_j (p_j d_jg) c_jg) + (sum_j p_j m_jg)  in group g:
+//   sum_j p_j v_j = (sum_j (p_j d_jg) (c_jg - 8)) + (sum_j p_j (m_jg + 8 d_jg)):
 // a product of 32 channels per group, its result times a step per key; and
-// probabilities times steps against the codes, with the least values as one
-// more small product (whose next row of ones gives the sum of p).  A code is
-// the float16 number c 2^-24 as its bits stand, a subnormal that the matrix
-// unit takes at full rate, so a word of eight codes becomes an operand in
-// five instructions; codes that stay four bits up count 16-fold, which their
-// factors (q, p) take back.  Nothing is rounded but q (float32: two float16
-// parts, 22 bits; others exactly) and p d (two parts).
+// probabilities times steps against the codes, with least values and steps as
+// one more small product (whose rows of ones give the sum of p).
+//
+// A code is the float16 number c 2^-24 as its bits stand, a subnormal that the
+// matrix unit takes at full rate, so a word of eight codes becomes an operand
+// in five instructions; codes that stay four bits up count 16-fold, which q
+// takes back.  The unit's sums of such products are coarser than float32, which
+// the scores of 16-bit queries bear: fp16 results, before their own rounding,
+// are 1.7e-6 off where scores have deviation 1, 1.2e-5 at 64.  Sums over many
+// rows do not: subnormal codes of V cost 1e-5 of the result on 500 rows and
+// 1.5e-4 on 131072, with least values that cancel them only at the end 1.6e-5
+// and 1.9e-4.  So V's codes, and K's for float32 queries, are centred and made
+// normal numbers, (c - 8) 2^-9, by one more instruction a pair, and least + 8
+// step joined tile by tile: 0.7e-6 to 2e-6 in every type on any number of rows.
+// (4 x 1 on 131072 rows, 32/8 heads of 128, fp16: 139.7 us for 138.)
+// Nothing is rounded but q (float32: two float16 parts, 22 bits; others
+// exactly) and p d (two parts).
 #pragma once
 
 #include <math.h>
@@ -41,6 +51,7 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kRows = kQ4Rows;
 constexpr int kWaves = kQ4Waves;
+constexpr float kUnit = 0x1p9f;  // a centred code of 1 is 1 / kUnit as an operand
 constexpr float kLift = 12.f;   // P is formed 2^12 times as large: float16 keeps
 constexpr float kSlack = 3.f;   // more of small ones; its reference may lag by 2^3
 
@@ -69,16 +80,11 @@ struct Q4Shape {
   // (11 bits: rms 0.5e-3 of the result, whose own rounding is 1.7e-3).
   static constexpr int PP = CT_ > 1 && std::is_same<T_, bf16_t>::value ? 1 : 2;
   static constexpr bool kOnce = CT == 1;  // one column tile: nobody reads a tile twice
-  // float32: codes less 8, so that the two sums that make a score or a channel
-  // of the result do not cancel (2e-5 of the result at 1500 rows).  float16 and
-  // bf16 take them as they are: where values have mean zero, the worst case,
-  // fp16 is 2.15e-4, 2.22e-4 and 2.39e-4 off on 500, 2000 and 8192 rows (less 8:
-  // 2.10e-4, 2.10e-4, 2.13e-4, the output's own rounding), and the subtraction
-  // costs more than that is worth: 5% (4 x 1 on 131072 rows of 128) to 20% (64).
+  // float32 takes K's codes centred as well.
   static constexpr bool kCentred = QP == 2;
-  static constexpr float kUnit = kCentred ? 1.f : 0x1p24f;  // a code of 1 is 1 / kUnit
   static constexpr float kSumScale = kCentred ? 0x1p-9f : 0x1p-6f;  // of a group's sum of q, in parts
-  static constexpr float kSumUnit = (kPacked ? 1.f : 1.f / kSumScale) / kUnit;  // of the sums of q
+  static constexpr float kCodeUnit = kCentred ? kUnit : 0x1p24f;  // of K
+  static constexpr float kSumUnit = (kPacked ? 1.f : 1.f / kSumScale) / kCodeUnit;  // of the sums of q
   static constexpr int kBases = (G_ + 3) / 4;
   static constexpr int kCols = CP * CT;
   static constexpr int kCodeB = kRows * 16 * G;        // codes of K or V in a tile
@@ -122,16 +128,12 @@ __device__ __forceinline__ f16x8 operand(uint32_t w) {
   r[3] = w & 0x00f000f0u;
   return __builtin_bit_cast(f16x8, r);
 }
-// The same less 8, as whole numbers (the second and fourth pair times 16):
-// 1024 + c and 1024 + 16 c as their bits stand, then one exact subtraction.
+// The same less 8, times 2^-9 all of them, as normal numbers: one exact
+// fused multiply-add per pair.
 __device__ __forceinline__ f16x8 centred_operand(uint32_t w) {
-  auto pair = [](uint32_t bits, f16_t base) __attribute__((always_inline)) {
-    return __builtin_bit_cast(f16x2, bits | 0x64006400u) - (f16x2){base, base};
-  };
-  const uint32_t w8 = w >> 8;
-  const f16x2 r0 = pair(w & 0x000f000fu, (f16_t)1032.f), r1 = pair(w & 0x00f000f0u, (f16_t)1152.f);
-  const f16x2 r2 = pair(w8 & 0x000f000fu, (f16_t)1032.f), r3 = pair(w8 & 0x00f000f0u, (f16_t)1152.f);
-  return (f16x8){r0[0], r0[1], r1[0], r1[1], r2[0], r2[1], r3[0], r3[1]};
+  const f16_t even = (f16_t)0x1p15f, odd = (f16_t)0x1p11f, eight = (f16_t)0x1p-6f;
+  return __builtin_elementwise_fma(operand(w), (f16x8){even, even, odd, odd, even, even, odd, odd},
+                                   (f16x8){-eight, -eight, -eight, -eight, -eight, -eight, -eight, -eight});
 }
 constexpr int kOrder[8] = {0, 4, 1, 5, 2, 6, 3, 7};
 
@@ -393,7 +395,7 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
       int ex = 0;
       if (most > 0.f && most < __builtin_inff()) ex = 14 - max(__builtin_amdgcn_frexp_expf(most) - 1, -90);
       const float f = ldexpf(1.f, ex);
-      k1[c] = ldexpf(a.scale_log2, (S::kCentred ? 0 : 24) - ex);
+      k1[c] = ldexpf(a.scale_log2, (S::kCentred ? 9 : 24) - ex);
       u32x4 sums = {0, 0, 0, 0};
 #pragma unroll
       for (int g = 0; g < G; ++g) {
@@ -401,7 +403,7 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float y = x[g][kOrder[e]] * f;
-          const float z = (e & 2) ? y * 0.0625f : y;
+          const float z = !S::kCentred && (e & 2) ? y * 0.0625f : y;
           const f16_t hi = (f16_t)z;
           const bool mine = !S::kPacked || g % R == slot_of;  // this column's group
           q[c][0][g][e] = mine ? hi : (f16_t)0.f;
@@ -411,7 +413,7 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
             q[c][1][g][e] = mine ? lo : (f16_t)0.f;
             z1 += (float)lo;
           }
-          s += (e & 2) ? z1 * 16.f : z1;
+          s += !S::kCentred && (e & 2) ? z1 * 16.f : z1;
         }
         if constexpr (S::kPacked) {
           s = column_sum(s);
@@ -434,8 +436,8 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
       qsum[c] = __builtin_bit_cast(f16x8, sums);
     }
 
-    f32x4 o[CT][2 * G];  // O^T[channel 16 n + 4 quad + r][column], in units of 1 / kUnit
-    float om[CT][S::kBases];  // sums of p m (centred: p (m + 8 d)) of groups `quad` (and quad + 4)
+    f32x4 o[CT][2 * G];  // O^T[channel 16 n + 4 quad + r][column] of the codes less 8
+    float om[CT][S::kBases];  // sums of p (m + 8 d) of groups `quad` (and quad + 4)
     float l[CT];              // the sum of p (G = 8: of this lane's keys)
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
@@ -647,8 +649,7 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
         }
       }
 
-      // P in two parts of float16; pairs whose codes count 16-fold then go on
-      // as a 16th
+      // P in two parts of float16
       f16x2 ph[CT][4 * TP], pl[CT][4 * TP];
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
@@ -680,17 +681,9 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
         for (int c = 0; c < CT; ++c) {
           f32x4 x = mfma16x16x32(mf, four(ph[c] + 4 * u), (f32x4)(0.f));
           if constexpr (S::PP == 2) x = mfma16x16x32(mf, four(pl[c] + 4 * u), x);
-          om[c][0] += S::kCentred ? fmaf(x[1], 8.f, x[0]) : x[0];
-          if constexpr (G == 8) om[c][S::kBases - 1] += S::kCentred ? fmaf(x[3], 8.f, x[2]) : x[2];
+          om[c][0] += fmaf(x[1], 8.f, x[0]);
+          if constexpr (G == 8) om[c][S::kBases - 1] += fmaf(x[3], 8.f, x[2]);
           else l[c] += x[2];
-        }
-      }
-#pragma unroll
-      for (int c = 0; c < CT; ++c) {
-#pragma unroll
-        for (int e = 1; e < 4 * TP; e += 2) {
-          ph[c][e] *= (f16_t)0.0625f;
-          if constexpr (S::PP == 2) pl[c][e] *= (f16_t)0.0625f;
         }
       }
       // P times the steps at dp of tile u, in two parts
@@ -717,8 +710,7 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
         for (int u = 0; u < TP; ++u) {
           const char* const tile = tiles + u * S::kTileB;
           const u32x2 w = lds_read_tr4x16(tile + vadr[g]);
-          const f16x8 v0 = S::kCentred ? centred_operand(w[0]) : operand(w[0]);
-          const f16x8 v1 = S::kCentred ? centred_operand(w[1]) : operand(w[1]);
+          const f16x8 v0 = centred_operand(w[0]), v1 = centred_operand(w[1]);
           if (!S::kPacked || g % R == 0) {  // the groups of one accumulator share their P d
             const char* const dp = tile + 2 * S::kCodeB + S::kScaleB +
                                    (!S::kPacked || g / R + 1 < NT ? dadr + 64 * g : dlast);
@@ -758,7 +750,7 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
         for (int n = 2 * g; n < 2 * g + 2; ++n) {
           f32x4 x;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) x[r] = fmaf(o[c][n][r], S::kUnit, pm) + bad;
+          for (int r = 0; r < 4; ++r) x[r] = fmaf(o[c][n][r], kUnit, pm) + bad;
           if (!S::kPacked || g % R == slot_of) *(f32x4*)(mo + 16 * n + 4 * quad) = x;
         }
       }

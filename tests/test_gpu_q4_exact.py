@@ -41,8 +41,7 @@ def _coarse(case, step):
     2^lift, so that their products with it stay in float16.  The largest one is
     then 2^(11 - lift) at least, and a row's, and its product with any step, are
     off by 2^-25 and twice 2^-25 at most where float16 is subnormal: times |least
-    + 8 step| <= gross and |code - 8| <= 8, 2^-25 (16 + gross) a row; half of the
-    codes count 16-fold and their weights as a 16th, which rounds once more: 32-fold."""
+    + 8 step| <= gross and |code - 8| <= 8, 2^-25 (16 + gross) a row."""
     lift = np.frexp(step)[1]
     lost = np.zeros(case.q.shape)
     for b, slots in enumerate(case.slots):
@@ -53,16 +52,16 @@ def _coarse(case, step):
                 kv = h // (case.q.shape[2] // k.shape[1])
                 s = (k[:n, kv].astype(np.float64) @ case.q[b, i, h]) * case.d ** -0.5
                 lost[b, i, h] = (16 + gross[:n, kv]).sum(0) / np.exp(s - s.max()).sum()
-    return 2.0 ** (lift - 31) * lost
+    return 2.0 ** (lift - 36) * lost
 
 
 # Groups whose middle, least + 8 steps, float16 does not hold.
-FAR_GROUPS = [(60000.0, 80000.0), (20000.0, 120000.0)]
+FAR_GROUPS = [(60000.0, 80000.0), (20000.0, 120000.0), (-1000.0, 900000.0)]
 FAR_SHAPES = [(64, 4, 1), (96, 6, 2), (128, 4, 1), (128, 8, 3), (128, 32, 1), (128, 8, 10),
               (256, 4, 1), (256, 4, 6), (256, 8, 9), (64, 8, 9), (96, 8, 9)]
 
 
-@pytest.mark.parametrize("dtype", ["f32"])
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
 @pytest.mark.parametrize("d,hq,nodes", FAR_SHAPES)
 @pytest.mark.parametrize("span", FAR_GROUPS)
 def test_values_past_what_float16_holds(gpu, ops, dtype, d, hq, nodes, span):
@@ -76,7 +75,7 @@ def test_values_past_what_float16_holds(gpu, ops, dtype, d, hq, nodes, span):
     _close(case, ops, 2.0 ** -17, _coarse(case, (span[1] - span[0]) / 15))
 
 
-@pytest.mark.parametrize("dtype", ["f32"])
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
 @pytest.mark.parametrize("d,hq", [(64, 4), (128, 8), (256, 8)])
 @pytest.mark.parametrize("which", ["k", "v"])
 def test_values_past_what_float16_holds_stay_with_the_tokens_that_see_them(gpu, ops, dtype, d, hq,
@@ -107,3 +106,39 @@ def test_keys_past_what_float16_holds(gpu, ops, dtype, d, hq, nodes):
         case.k[:, row, :, 32:64] = rng.uniform(60000.0, 80000.0, case.k[:, row, :, 32:64].shape)
     case.store()
     _close(case, ops, 2.0 ** -15)
+
+
+@pytest.mark.parametrize("dtype,d,hq,hkv,nodes,rows,batch", [
+    ("f16", 128, 8, 2, 1, 500, 2), ("f16", 128, 8, 2, 1, 20000, 1), ("bf16", 128, 8, 2, 1, 131072, 1),
+    ("f16", 64, 8, 2, 1, 131072, 1), ("f32", 128, 8, 2, 1, 131072, 1), ("f16", 128, 8, 2, 1, 8192, 64),
+    ("f16", 96, 6, 2, 4, 8192, 2), ("bf16", 256, 8, 1, 1, 32768, 2), ("f32", 256, 8, 1, 2, 8192, 1),
+    ("f16", 128, 8, 2, 64, 32768, 1), ("f32", 128, 8, 2, 64, 32768, 1)])
+def test_no_more_is_lost_on_more_rows(gpu, ops, dtype, d, hq, hkv, nodes, rows, batch):
+    """Values of mean zero: what is left of their sum shrinks beside its terms
+    as rows grow.  Against float64 products here on the device."""
+    import torch
+    g = torch.Generator(device=gpu).manual_seed(rows)
+    page = 64
+    per = -(-rows // page)
+    pool = ops.initialize_paged_q4_workspace(num_pages=batch * per, page_size=page, kv_heads=hkv,
+                                             head_dimension=d).arrays
+    slots = torch.arange(batch * per * page, dtype=torch.int32, device=gpu)
+    for part in slots.split(32768):
+        k, v = (torch.randn(part.numel(), hkv, d, generator=g, device=gpu) for _ in range(2))
+        ops.paged_q4_append_rows_(None, k, v, *pool, part, None, rotary_dimension=0)
+    q = torch.randn(batch, nodes, hq, d, generator=g, device=gpu).to(_td(dtype))
+    got = ops.paged_q4_attention(
+        q, *pool, torch.arange(batch * per, dtype=torch.int32, device=gpu).view(batch, per),
+        length=rows, prefix_lens=[rows - nodes] * batch, out_dtype=torch.float32).double()
+    want = torch.empty_like(got)
+    seen = torch.arange(rows, device=gpu) <= \
+        rows - nodes + torch.arange(nodes, device=gpu).unsqueeze(1)
+    for b in range(batch):
+        k, v = ops.paged_q4_rows(*pool, slots[b * per * page:][:rows])
+        for h in range(hq):
+            kv = h // (hq // hkv)
+            kt = k[:, kv].double().t().contiguous()
+            s = (q[b, :, h].double() @ kt) * d ** -0.5
+            p = torch.softmax(s.masked_fill(~seen, float("-inf")), -1)
+            want[b, :, h] = p @ v[:, kv].double().contiguous()
+    assert (got - want).norm() <= 2.0 ** -17 * want.norm()
