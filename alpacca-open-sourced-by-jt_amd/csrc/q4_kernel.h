@@ -75,10 +75,6 @@ struct Q4Shape {
   static constexpr int NT = (G + R - 1) / R;  // accumulators that the groups' products run into
   static_assert(!kPacked || CT == 1, "one column tile");
   static constexpr int QP = sizeof(T_) == 4 ? 2 : 1;  // parts of q
-  // Parts of P and of P d.  Two keep the result as exact as its type; where many
-  // columns are bound by the products, bf16 takes them rounded once to float16
-  // (11 bits: rms 0.5e-3 of the result, whose own rounding is 1.7e-3).
-  static constexpr int PP = CT_ > 1 && std::is_same<T_, bf16_t>::value ? 1 : 2;
   static constexpr bool kOnce = CT == 1;  // one column tile: nobody reads a tile twice
   // float32 takes K's codes centred as well.
   static constexpr bool kCentred = QP == 2;
@@ -659,12 +655,8 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
           const float x0 = fast_exp2(fmaf(s[c][2 * e], k1[c], base));
           const float x1 = fast_exp2(fmaf(s[c][2 * e + 1], k1[c], base));
           if constexpr (G == 8) l[c] += x0 + x1;
-          if constexpr (S::PP == 1) {
-            ph[c][e] = (f16x2){(f16_t)x0, (f16_t)x1};
-          } else {
-            ph[c][e] = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x0, x1));
-            pl[c][e] = (f16x2){(f16_t)(x0 - (float)ph[c][e][0]), (f16_t)(x1 - (float)ph[c][e][1])};
-          }
+          ph[c][e] = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x0, x1));
+          pl[c][e] = (f16x2){(f16_t)(x0 - (float)ph[c][e][0]), (f16_t)(x1 - (float)ph[c][e][1])};
         }
       }
 #pragma unroll
@@ -680,7 +672,7 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
           f32x4 x = mfma16x16x32(mf, four(ph[c] + 4 * u), (f32x4)(0.f));
-          if constexpr (S::PP == 2) x = mfma16x16x32(mf, four(pl[c] + 4 * u), x);
+          x = mfma16x16x32(mf, four(pl[c] + 4 * u), x);
           om[c][0] += fmaf(x[1], 8.f, x[0]);
           if constexpr (G == 8) om[c][S::kBases - 1] += fmaf(x[3], 8.f, x[2]);
           else l[c] += x[2];
@@ -699,7 +691,7 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
             const f16x2 h = p * d[e];
             hi[c][u][e] = h;
             // what the rounding took, and the second part's share
-            if constexpr (S::PP == 2) lo[c][u][e] = __builtin_elementwise_fma(pl[c][4 * u + e], d[e],
+            lo[c][u][e] = __builtin_elementwise_fma(pl[c][4 * u + e], d[e],
                                                     __builtin_elementwise_fma(p, d[e], -h));
           }
         }
@@ -720,10 +712,8 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
           for (int c = 0; c < CT; ++c) {
             o[c][2 * g] = mfma16x16x32(v0, four(hi[c][u]), o[c][2 * g]);
             o[c][2 * g + 1] = mfma16x16x32(v1, four(hi[c][u]), o[c][2 * g + 1]);
-            if constexpr (S::PP == 2) {
-              o[c][2 * g] = mfma16x16x32(v0, four(lo[c][u]), o[c][2 * g]);
-              o[c][2 * g + 1] = mfma16x16x32(v1, four(lo[c][u]), o[c][2 * g + 1]);
-            }
+            o[c][2 * g] = mfma16x16x32(v0, four(lo[c][u]), o[c][2 * g]);
+            o[c][2 * g + 1] = mfma16x16x32(v1, four(lo[c][u]), o[c][2 * g + 1]);
           }
         }
       }

@@ -61,7 +61,7 @@ FAR_SHAPES = [(64, 4, 1), (96, 6, 2), (128, 4, 1), (128, 8, 3), (128, 32, 1), (1
               (256, 4, 1), (256, 4, 6), (256, 8, 9), (64, 8, 9), (96, 8, 9)]
 
 
-@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("d,hq,nodes", FAR_SHAPES)
 @pytest.mark.parametrize("span", FAR_GROUPS)
 def test_values_past_what_float16_holds(gpu, ops, dtype, d, hq, nodes, span):
@@ -75,7 +75,7 @@ def test_values_past_what_float16_holds(gpu, ops, dtype, d, hq, nodes, span):
     _close(case, ops, 2.0 ** -17, _coarse(case, (span[1] - span[0]) / 15))
 
 
-@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("d,hq", [(64, 4), (128, 8), (256, 8)])
 @pytest.mark.parametrize("which", ["k", "v"])
 def test_values_past_what_float16_holds_stay_with_the_tokens_that_see_them(gpu, ops, dtype, d, hq,
@@ -94,7 +94,7 @@ def test_values_past_what_float16_holds_stay_with_the_tokens_that_see_them(gpu, 
         _close(case, ops, 2.0 ** -17, _coarse(case, 1e5 / 15) if which == "v" else 0.0)
 
 
-@pytest.mark.parametrize("dtype", ["f32"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("d,hq,nodes", FAR_SHAPES)
 def test_keys_past_what_float16_holds(gpu, ops, dtype, d, hq, nodes):
     """Terms of a score sum to less than 2^5 in size, of which a float32 sum
@@ -112,7 +112,8 @@ def test_keys_past_what_float16_holds(gpu, ops, dtype, d, hq, nodes):
     ("f16", 128, 8, 2, 1, 500, 2), ("f16", 128, 8, 2, 1, 20000, 1), ("bf16", 128, 8, 2, 1, 131072, 1),
     ("f16", 64, 8, 2, 1, 131072, 1), ("f32", 128, 8, 2, 1, 131072, 1), ("f16", 128, 8, 2, 1, 8192, 64),
     ("f16", 96, 6, 2, 4, 8192, 2), ("bf16", 256, 8, 1, 1, 32768, 2), ("f32", 256, 8, 1, 2, 8192, 1),
-    ("f16", 128, 8, 2, 64, 32768, 1), ("f32", 128, 8, 2, 64, 32768, 1)])
+    ("f16", 128, 8, 2, 64, 32768, 1), ("bf16", 128, 8, 2, 64, 4133, 2), ("f32", 128, 8, 2, 64, 32768, 1),
+    ("bf16", 256, 8, 1, 33, 8192, 1)])
 def test_no_more_is_lost_on_more_rows(gpu, ops, dtype, d, hq, hkv, nodes, rows, batch):
     """Values of mean zero: what is left of their sum shrinks beside its terms
     as rows grow.  Against float64 products here on the device."""
@@ -142,3 +143,22 @@ def test_no_more_is_lost_on_more_rows(gpu, ops, dtype, d, hq, hkv, nodes, rows, 
             p = torch.softmax(s.masked_fill(~seen, float("-inf")), -1)
             want[b, :, h] = p @ v[:, kv].double().contiguous()
     assert (got - want).norm() <= 2.0 ** -17 * want.norm()
+
+
+# Column classes of a kv head: up to 4, up to 8, up to 16, and more (one column
+# tile of 32, and several with an end inside).
+COLUMNS = {"4": (4, 1), "3": (3, 1), "8": (4, 2), "6": (6, 1), "16": (8, 2), "10": (5, 2),
+           "27": (3, 9), "40": (8, 5)}
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+@pytest.mark.parametrize("columns", list(COLUMNS))
+def test_every_kernel_matches_the_oracle(gpu, ops, dtype, d, columns):
+    """Every type, width and class of columns, on whole sequences (one launch)
+    and on shares of them (two), with a tile and a page that end inside."""
+    group, nodes = COLUMNS[columns]
+    for prefix in ([100, 0, 33], [1301, 70]):
+        case = Case(gpu, 66, dtype=dtype, d=d, hq=2 * group, hkv=2, nodes=nodes, prefix=prefix)
+        got, want = _close(case, ops, 2.0 ** -17)
+        assert np.linalg.norm(got - want) <= 2.0 ** -17 * np.linalg.norm(want)
