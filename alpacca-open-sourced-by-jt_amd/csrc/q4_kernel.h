@@ -391,7 +391,8 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
       int ex = 0;
       if (most > 0.f && most < __builtin_inff()) ex = 14 - max(__builtin_amdgcn_frexp_expf(most) - 1, -90);
       const float f = ldexpf(1.f, ex);
-      k1[c] = ldexpf(a.scale_log2, (S::kCentred ? 9 : 24) - ex);
+      // (never 0: a masked score, -inf, has to stay one)
+      k1[c] = fmaxf(ldexpf(a.scale_log2, (S::kCentred ? 9 : 24) - ex), 0x1p-126f);
       u32x4 sums = {0, 0, 0, 0};
 #pragma unroll
       for (int g = 0; g < G; ++g) {

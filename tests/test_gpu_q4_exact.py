@@ -145,6 +145,16 @@ def test_no_more_is_lost_on_more_rows(gpu, ops, dtype, d, hq, hkv, nodes, rows, 
     assert (got - want).norm() <= 2.0 ** -17 * want.norm()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d,hq,nodes", [(64, 4, 1), (128, 8, 2), (128, 8, 9), (256, 8, 3)])
+@pytest.mark.parametrize("size,scale", [(2.0 ** -24, 1e-38), (1.0, 1e-44), (2.0 ** -20, 1e-30)])
+def test_scores_too_small_for_float32(gpu, ops, dtype, d, hq, nodes, size, scale):
+    """All scores are as good as 0: the mean of the rows that a token sees."""
+    case = Case(gpu, 67, dtype=dtype, d=d, hq=hq, hkv=2, nodes=nodes, prefix=[600, 30])
+    case.q[:] = I.round_to(case.q * size, dtype)
+    _close(case, ops, 2.0 ** -17, scale=scale)
+
+
 # Column classes of a kv head: up to 4, up to 8, up to 16, and more (one column
 # tile of 32, and several with an end inside).
 COLUMNS = {"4": (4, 1), "3": (3, 1), "8": (4, 2), "6": (6, 1), "16": (8, 2), "10": (5, 2),
