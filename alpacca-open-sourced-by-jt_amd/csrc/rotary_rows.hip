@@ -29,6 +29,8 @@ constexpr int kThreads = 256;
 template <typename T>
 constexpr int kFlight = sizeof(T) == 4 ? 1 : 2;
 
+constexpr double kMostFrequency = 4.0;  // radians a position: what angle_of covers
+
 struct RotaryArgs {
   const void* q;     // [T, Hq, D]
   const void* k;     // [T, Hkv, D]
@@ -474,6 +476,9 @@ int rotary_args(const char* what, RotaryArgs& a, const void* query, const void* 
       last.base = base;
       last.scale = scale;
     }
+    // (rising with a base below 1; positions below 2^31 make angles below 2^33)
+    if (!(std::max(last.inv[0], last.inv[a.R - 1]) <= kMostFrequency))
+      return fail(ALPX_EUNSUPPORTED, "%s: frequencies above 4", what);
     std::copy(last.inv, last.inv + a.R, a.inv);
   }
   return ALPX_OK;

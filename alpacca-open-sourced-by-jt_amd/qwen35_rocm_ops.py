@@ -1603,7 +1603,9 @@ class Qwen35RocmOps:
         (None: keys and values alone) and ``key [T, Hkv, D]`` are turned by
         ``positions[t]`` (int32): pairs (2 p, 2 p + 1) for ``style`` "norm",
         (p, p + rotary_dimension / 2) for "neox", as the reference's
-        _rope_norm and _rope_neox (kernels.py:783-817).  Keys and ``value [T,
+        _rope_norm and _rope_neox (kernels.py:783-817); no pair's frequency,
+        ``frequency_scale * frequency_base ** (-2 p / rotary_dimension)``, may
+        exceed 4.  Keys and ``value [T,
         Hkv, Dv]`` go to pool row ``slots[t]`` (int32, page * page_size + row,
         as ``paged_resize_`` gives them; one outside the pool writes neither;
         no two tokens may share one).  Returns the turned query."""

@@ -808,7 +808,8 @@ int alpx_attention_prologue_rows(const void* query_gate, const void* key, const 
  * Token t of query [T, Hq, D] (null with q_heads 0: keys and values alone),
  * key [T, Hkv, D] and value [T, Hkv, Dv] sits at positions[t]; with R =
  * rotary_dim / 2, pair p < R of a query and a key is turned by positions[t] *
- * frequency_scale * frequency_base^(-p / R), in float64 reduced to one turn:
+ * frequency_scale * frequency_base^(-p / R), in float64 reduced to one turn
+ * (frequencies above 4, a scale past it or a base below 1, are refused):
  * channels (2 p, 2 p + 1) (ALPX_ROTARY_NORM, _rope_norm, kernels.py:783-817)
  * or (p, p + R) (ALPX_ROTARY_NEOX); the channels behind stay.  rotary_dim 0
  * turns nothing (positions may then be null).  Queries go to query_out, keys

@@ -343,3 +343,18 @@ def test_facade_pool_arrays_that_are_no_tensors(ops, which):
     arrays[which] = None
     with pytest.raises(TypeError, match="must be a"):
         ops.paged_q4_rows(*arrays, _i32(3))
+
+
+@pytest.mark.parametrize("name,args", [("alpx_rotary_append_rows", ROTARY),
+                                       ("alpx_q4_append_rows", APPEND)])
+def test_append_refuses_frequencies_past_what_angles_hold(L, name, args):
+    """Angles stay below 2^33: frequencies up to 4, positions below 2^31.  A
+    base below 1 makes frequencies rise, up to base^(-126 / 128) here."""
+    for value in (4.0000001, 1e6, 1e300):
+        _refused(L, name, args, "EUNSUPPORTED", "frequencies above 4", scale=value)
+    for value in (0.24, 1e-3, 1e-300, 5e-324):
+        _refused(L, name, args, "EUNSUPPORTED", "frequencies above 4", base=value)
+    for value in (0.06, 1e-3, 1e-300, 5e-324):  # two pairs: up to base^(-1 / 2)
+        _refused(L, name, args, "EUNSUPPORTED", "frequencies above 4", base=value, rotary=4)
+    # one pair has the scale for its frequency, whatever the base
+    _refused(L, name, args, "EUNSUPPORTED", "frequencies above 4", rotary=2, scale=5.0)
