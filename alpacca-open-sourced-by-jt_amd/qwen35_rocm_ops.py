@@ -1688,8 +1688,9 @@ class Qwen35RocmOps:
         (``initialize_paged_q4_workspace``; ``*pool.arrays``): of every 32
         channels of a key (turned) and a value, least = float16(min), step =
         float16((max - least) / 15) and the nearest code of (x - least) /
-        step.  Values past 65504 count as 65504; 32 channels that hold an
-        infinity or a NaN read as NaN.  ``rotary_dimension`` 0 (positions None)
+        step.  least is cut at -65504 and 65504 and step at 65504 (values read
+        back lie in -65504 .. 16 * 65504); 32 channels that hold an infinity or
+        a NaN read as NaN.  ``rotary_dimension`` 0 (positions None)
         stores keys that are turned already.  Returns the turned query."""
         pool, (pages, heads, size, width) = self._q4_pool(key_codes, key_scales, value_codes,
                                                           value_scales)

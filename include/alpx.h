@@ -839,8 +839,9 @@ int alpx_rotary_append_rows(const void* query, const void* key, const void* valu
  * is row r % page_size of page r / page_size).  Of the 32 values of a group
  * (keys after their turn), least = f16(min), step = f16((max - least) / 15),
  * code = the nearest of (x - least) / step in 0 .. 15 (ties to even), formed
- * in float64 and rounded to float16 through float32; values past 65504 count
- * as 65504.  A group that holds an infinity or a NaN reads as NaN.
+ * in float64 and rounded to float16 through float32.  least is cut at -65504
+ * and 65504 and step at 65504, so values read back lie in -65504 .. 16 *
+ * 65504.  A group that holds an infinity or a NaN reads as NaN.
  *
  * alpx_q4_rows: rows slots[i] of the pool as numbers, step * code + least
  * rounded once to float32 and then to out_dtype: key_out, value_out [rows,

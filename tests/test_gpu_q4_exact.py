@@ -55,6 +55,26 @@ def _coarse(case, step):
     return 2.0 ** (lift - 36) * lost
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_least_and_step_are_cut_where_float16_ends(gpu, ops, dtype):
+    """The numbers of the definition, by hand, stored and read back."""
+    import torch
+    x = torch.zeros(3, 1, 64, device=gpu)
+    x[0], x[1, :, :16], x[1, :, 16:] = 3e38, 20480.0, 122880.0
+    x[2, :, ::2], x[2, :, 1::2] = -3e38, 3e38
+    pool = ops.initialize_paged_q4_workspace(num_pages=1, page_size=32, kv_heads=1,
+                                             head_dimension=64).arrays
+    x = x.to(_td(dtype))
+    ops.paged_q4_append_rows_(None, x, x, *pool, [0, 1, 2], None, rotary_dimension=0)
+    for got in ops.paged_q4_rows(*pool, [0, 1, 2]):
+        assert (got[0] == 16 * 65504).all()
+        # (102400 / 15 = 6826.7, of steps 4 apart 6828)
+        assert (got[1, :, :16] == 20480).all() and (got[1, :, 16:32] == 20480 + 15 * 6828).all()
+        # (57376 / 15 = 3825.07 above least, of steps 2 apart 3826)
+        assert (got[1, :, 32:] == 65504 + 15 * 3826).all()
+        assert (got[2, :, ::2] == -65504).all() and (got[2, :, 1::2] == 14 * 65504).all()
+
+
 # Groups whose middle, least + 8 steps, float16 does not hold.
 FAR_GROUPS = [(60000.0, 80000.0), (20000.0, 120000.0), (-1000.0, 900000.0)]
 FAR_SHAPES = [(64, 4, 1), (96, 6, 2), (128, 4, 1), (128, 8, 3), (128, 32, 1), (128, 8, 10),

@@ -131,3 +131,15 @@ def test_verified_tokens_follow_the_target():
                               None if draft is None else np.stack([q] * 4))
             seen[new[0]] += 1
         assert np.abs(seen / seen.sum() - p).max() < 0.018
+
+
+def test_least_and_step_are_cut_where_float16_ends():
+    """By hand: 3e38 is 65504 + 15 * 65504; 20000 .. 120000 has step 6668 (4
+    apart there); -3e38 .. 3e38 becomes -65504 + 15 * 65504 at most."""
+    x = np.zeros((3, 32))
+    x[0], x[1, :16], x[1, 16:] = 3e38, 20000.0, 120000.0
+    x[2, ::2], x[2, 1::2] = -3e38, 3e38
+    got = Q.decode(*Q.encode(x))
+    assert (got[0] == 16 * 65504).all()
+    assert (got[1, :16] == 20000).all() and (got[1, 16:] == 20000 + 15 * 6668).all()
+    assert (got[2, ::2] == -65504).all() and (got[2, 1::2] == 14 * 65504).all()
