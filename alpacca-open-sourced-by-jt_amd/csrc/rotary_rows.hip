@@ -437,6 +437,8 @@ int rotary_args(const char* what, RotaryArgs& a, const void* query, const void* 
   if (((int64_t)q_heads + 2 * (int64_t)kv_heads) * ((std::max(head_dim, value_dim) + 7) / 8) >
       0x7fffffff - 2 * kThreads * 1024)
     return fail(ALPX_EUNSUPPORTED, "%s: too many heads", what);
+  if ((int64_t)tokens * kThreads > 0xffffffff)  // a block a token: the threads of a launch
+    return fail(ALPX_EUNSUPPORTED, "%s: too many tokens", what);
   if (rotary_dim < 0 || rotary_dim % 2 != 0 || rotary_dim > head_dim)
     return fail(ALPX_EINVAL, "%s: rotary_dim must be even and at most the head width", what);
   if (style != ALPX_ROTARY_NORM && style != ALPX_ROTARY_NEOX)

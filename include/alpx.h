@@ -816,7 +816,8 @@ int alpx_attention_prologue_rows(const void* query_gate, const void* key, const 
  * and values to row slots[t] of key_rows [pool_rows, Hkv, D] and value_rows
  * [pool_rows, Hkv, Dv] (a page pool, page after page); a slot outside [0,
  * pool_rows) writes neither.  Two tokens must not share a slot.  One dtype;
- * head dims up to 512.  query_out must not overlap an input.  One launch.
+ * head dims up to 512, less than 2^24 tokens.  query_out must not overlap an
+ * input.  One launch.
  */
 enum alpx_rotary_style { ALPX_ROTARY_NORM = 0, ALPX_ROTARY_NEOX = 1 };
 int alpx_rotary_append_rows(const void* query, const void* key, const void* value,

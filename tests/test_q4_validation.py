@@ -358,3 +358,10 @@ def test_append_refuses_frequencies_past_what_angles_hold(L, name, args):
         _refused(L, name, args, "EUNSUPPORTED", "frequencies above 4", base=value, rotary=4)
     # one pair has the scale for its frequency, whatever the base
     _refused(L, name, args, "EUNSUPPORTED", "frequencies above 4", rotary=2, scale=5.0)
+
+
+@pytest.mark.parametrize("name,args", [("alpx_rotary_append_rows", ROTARY),
+                                       ("alpx_q4_append_rows", APPEND)])
+def test_append_refuses_more_tokens_than_a_launch_has_blocks(L, name, args):
+    for value in (1 << 24, 0x7fffffff):
+        _refused(L, name, args, "EUNSUPPORTED", "too many tokens", tokens=value)
