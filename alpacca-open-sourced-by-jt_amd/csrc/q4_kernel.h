@@ -456,10 +456,11 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
     const bool has_m = quad < G;
     const int mk = (has_m ? quad : 0) * 64 + 2 * hl;  // steps of K; least values from plane G on
     // and of V: rows of an operand, whose results a lane of the group's quad gets
-    // next to each other: least values, steps, ones (G = 8: those of group quad,
-    // then of quad + 4; the sum of p without the matrix unit)
+    // next to each other: least values, steps less than 0, ones (G = 8: those of
+    // group quad, then of quad + 4; the sum of p without the matrix unit)
     const int vg = G == 8 ? (hl >> 2) + 4 * ((hl >> 1) & 1) : min(hl >> 2, G - 1);
     const int mv = (((G == 8 ? hl & 1 : hl & 3) == 0 ? G : 0) + vg) * 64 + 8 * quad;
+    const uint32_t sign = hl & 1 ? 0x80008000u : 0u;  // of steps
     const bool ones = G < 8 && (hl & 3) >= 2;
     // steps of four keys; packed: of this column's group of the first R (unused
     // columns take the last group's, for sums of zeros)
@@ -530,8 +531,8 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
               for (int g = R * t; g < min(R * t + R, G); ++g) {
                 const uint32_t w = *(const uint32_t*)(tile + kadr[g] + 256 * G * kt);
                 const f16x8 kx = S::kCentred ? centred_operand(w) : operand(w);
-                x = mfma16x16x32(kx, q[0][0][g], x);
                 if constexpr (QP == 2) x = mfma16x16x32(kx, q[0][1][g], x);
+                x = mfma16x16x32(kx, q[0][0][g], x);
               }
               const char* const dp = sc_k + (t + 1 < NT ? dadr + 64 * R * t : dlast) + 32 * kt;
               const f16x4 d = *(const f16x4*)dp, least = *(const f16x4*)(dp + 64 * G);
@@ -572,8 +573,9 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
             const f16x4 d = *(const f16x4*)(sc_k + dadr + 64 * g + 32 * kt);
 #pragma unroll
             for (int c = 0; c < CT; ++c) {
-              f32x4 x = mfma16x16x32(kx, q[c][0][g], (f32x4)(0.f));
+              f32x4 x = {0.f, 0.f, 0.f, 0.f};
               if constexpr (QP == 2) x = mfma16x16x32(kx, q[c][1][g], x);
+              x = mfma16x16x32(kx, q[c][0][g], x);
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
                 float& y = s[c][8 * u + 4 * kt + r];
@@ -663,19 +665,23 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
 #pragma unroll
       for (int u = 0; u < TP; ++u) {
         // Least values and 8 steps, as exact as they stand, and joined tile by
-        // tile: their sums over all rows would grow past what they leave.
+        // tile: their sums over all rows would grow past what they leave.  The
+        // unit rounds its sums downwards, small ones first the least (float32, 500
+        // rows: 5e-7 of the result, large first 7e-7); of least values and negated
+        // steps, mostly of one sign, what it takes cancels (131072 rows: 6e-7; with
+        // steps as they are 1.8e-6).
         const char* mp = tiles + u * S::kTileB + 2 * S::kCodeB + S::kScaleB + mv;
         const u32x2 m0 = *(const u32x2*)mp, m1 = *(const u32x2*)(mp + 32);
         constexpr uint32_t kOnes = 0x3c003c00u;
         const f16x8 mf = __builtin_bit_cast(
-            f16x8, (u32x4){ones ? kOnes : m0[0], ones ? kOnes : m0[1], ones ? kOnes : m1[0],
-                           ones ? kOnes : m1[1]});
+            f16x8, (u32x4){ones ? kOnes : m0[0] ^ sign, ones ? kOnes : m0[1] ^ sign,
+                           ones ? kOnes : m1[0] ^ sign, ones ? kOnes : m1[1] ^ sign});
 #pragma unroll
         for (int c = 0; c < CT; ++c) {
-          f32x4 x = mfma16x16x32(mf, four(ph[c] + 4 * u), (f32x4)(0.f));
-          x = mfma16x16x32(mf, four(pl[c] + 4 * u), x);
-          om[c][0] += fmaf(x[1], 8.f, x[0]);
-          if constexpr (G == 8) om[c][S::kBases - 1] += fmaf(x[3], 8.f, x[2]);
+          f32x4 x = mfma16x16x32(mf, four(pl[c] + 4 * u), (f32x4)(0.f));
+          x = mfma16x16x32(mf, four(ph[c] + 4 * u), x);
+          om[c][0] += fmaf(x[1], -8.f, x[0]);
+          if constexpr (G == 8) om[c][S::kBases - 1] += fmaf(x[3], -8.f, x[2]);
           else l[c] += x[2];
         }
       }
