@@ -17,13 +17,13 @@ constexpr int kCus = 256;
 // Up to this length of the longest sequence a block takes a whole sequence and
 // one launch is all: with few blocks, and with one for every CU.  bf16, 32/8
 // heads of 128, us whole and split:
-//   1 x 1 token on 512 rows 8.7, 10.2; on 1024 12.3, 10.6; on 2048 19.6, 10.8
-//   32 x 1      on 512 10.1, 13.1; on 2048 22.1, 24.4; on 4096 36.0, 32.1
-//   4 x 64      on 512 15.8, 23.1; on 2048 33.3, 34.5; on 8192 101, 76
+//   1 x 1 token on 512 rows 8.8, 10.4; on 1024 12.8, 10.8; on 2048 20.7, 11.0
+//   32 x 1      on 512 10.4, 13.2; on 2048 23.3, 25.1; on 4096 38.2, 33.0
+//   4 x 64      on 512 17.4, 24.1; on 2048 41.1, 40.3; on 8192 134, 101
 constexpr int64_t kAloneRows = 512, kAloneRowsFull = 2048;
 // Beyond a block a CU a share has this many rows at least: 32 x 1 on 512 rows,
-// split: 13.1 us with 128 and 256, 23.0 with 512; 4 x 1 on 2048: 12.9 with 128,
-// 11.0 with 256 and more.
+// split: 13.2 us with 128 and 256, 23.4 with 512; 4 x 1 on 2048: 13.0 with 128,
+// 11.3 with 256 and more.
 constexpr int64_t kRowsPerSlot = 256;
 
 struct Q4Plan {

@@ -21,13 +21,15 @@
 // in five instructions; codes that stay four bits up count 16-fold, which q
 // takes back.  The unit's sums of such products are coarser than float32, which
 // the scores of 16-bit queries bear: fp16 results, before their own rounding,
-// are 1.7e-6 off where scores have deviation 1, 1.2e-5 at 64.  Sums over many
+// are 1.5e-6 off where scores have deviation 1, 1.2e-5 at 64.  Sums over many
 // rows do not: subnormal codes of V cost 1e-5 of the result on 500 rows and
 // 1.5e-4 on 131072, with least values that cancel them only at the end 1.6e-5
 // and 1.9e-4.  So V's codes, and K's for float32 queries, are centred and made
 // normal numbers, (c - 8) 2^-9, by one more instruction a pair, and least + 8
-// step joined tile by tile: 0.7e-6 to 2e-6 in every type on any number of rows.
-// (4 x 1 on 131072 rows, 32/8 heads of 128, fp16: 139.7 us for 138.)
+// step joined tile by tile: float32 results are 4e-7 to 6e-7 off on 500 to
+// 131072 rows, 1.2e-6 where a wave alone sums 2048 of them (64 x 1 on 8192).
+// Values below 1e-3 lose more (p d is subnormal): 1.6e-6 at 1e-4, 1.7e-5 at
+// 1e-5.  (4 x 1 on 131072 rows, 32/8 heads of 128, fp16: 140.5 us for 137.)
 // Nothing is rounded but q (float32: two float16 parts, 22 bits; others
 // exactly) and p d (two parts).
 #pragma once
@@ -224,12 +226,12 @@ __device__ __forceinline__ void write_out(const Q4Args& a, int64_t at, f32x4 o, 
 // Alone (no `found`): a share is a whole sequence, and there is nothing to join.
 //
 // Few columns are bound by memory on long contexts: 4 x 1 on 131072 rows, 32/8
-// heads of 128, fp16, 672 MB in 143 us (4.7 TB/s; the loads alone, without the
+// heads of 128, fp16, 672 MB in 140 us (4.8 TB/s; the loads alone, without the
 // arithmetic, 5.2).  On shorter ones the start and the end count, some 6 us:
 // the shares, pages, queries and first tiles of a block, and its waves' meeting
-// (16 x 1 ragged 8192, 95 MB: 24 us and 4 for the join).  Many columns are bound
+// (16 x 1 ragged 8192, 95 MB: 25 to 28 us and 4 for the join).  Many columns are bound
 // by the vector unit, which multiplies by steps, takes P apart and forms
-// operands (4 x 64 on 4133 rows: busy 60% of the time, the matrix unit 24%).
+// operands (4 x 64 on 4133 rows: busy 59% of the time, the matrix unit 22%).
 template <typename S>
 __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
   typedef typename S::T T;
@@ -295,7 +297,7 @@ __global__ void __launch_bounds__(64 * kWaves, S::kPerCu) q4_kernel(Q4Args a) {
       return r;
     };
     // (the nontemporal hint on codes that no other block reads: 4 x 1 on 131072
-    // rows, 32/8 heads of 128, 153 -> 143 us; on the scales too, the same)
+    // rows, 32/8 heads of 128, 150 -> 140 us; on the scales too, the same)
     auto load = [](i32x4 r, uint32_t lds, uint32_t ofs) __attribute__((always_inline)) {
       if constexpr (S::kOnce) lds_dma16_once(r, lds, ofs);
       else lds_dma16(r, lds, ofs);
@@ -879,10 +881,11 @@ Q4Kernel make() {
 // Up to 16 columns one column tile, two tiles of 32 rows to a step where two
 // blocks of them fit a CU (4 x 1 on 32768 rows of 256, one: two do not); up to
 // 8 and 4 of them as queries times groups (16 x 1 ragged 8192, 4 queries a head:
-// 27.8 us, 16 plain columns 33).  Of more, two column tiles to a block: K's and
-// V's operands serve both (4 x 64 on 4133 rows: 48 us; four, which leave a wave
-// a SIMD, 62; several rounds of smaller blocks 58 to 69).  Rings of three and
-// four steps for one column tile take as long as two.
+// 31.2 us, 16 plain columns 34.9).  Of more, two column tiles to a block: K's and
+// V's operands serve both (4 x 64 on 4133 rows: 61 us; four, which leave a wave
+// a SIMD, 68; one 69).  Rings of three and four steps for one column tile take
+// as long as two.  float32 queries of 128 channels keep 4 registers a lane of
+// theirs in scratch (4 x 64 on 4133 rows: 69 us).
 template <typename T>
 Q4Kernel pick(int head_dim, int cols) {
   const int few = cols <= 4 ? 4 : cols <= 8 ? 8 : cols <= 16 ? 16 : 0;

@@ -84,8 +84,8 @@ __device__ __forceinline__ void uniform_rows(const A& a, int b, int& P, int& end
 // Slot s leaves the partial state of its tiles of sequence b in segment
 // s + b: both rise along the runs, so no two segments share a number, and
 // there are at most slots + batch.  A run that holds a whole sequence writes
-// its output and leaves no partial state, only a mark whether that output is
-// finite.
+// its output and leaves no partial state (trees: a mark whether that output is
+// finite).
 struct Share {
   int b;       // the sequence, -1: none
   int P, end;  // its rows: [0, P) the prefix, [P, end) the drafts

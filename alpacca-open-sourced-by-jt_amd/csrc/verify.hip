@@ -501,8 +501,8 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw(VerifyArgs a) {
       }
       return (double)w;
     };
-    // neighbouring tokens to a thread, threads in order; past kKept of them
-    // their weights are formed again
+    // neighbouring tokens to a thread, threads in order; the first kKept are
+    // asked for together (whose sum passes t goes over all of its own again)
     constexpr int kKept = 4;
     const int64_t per = (x1 - x0 + kDrawThreads - 1) / kDrawThreads;
     const int64_t m0 = min(x0 + tid * per, x1), m1 = min(m0 + per, x1);
@@ -565,7 +565,6 @@ __global__ void __launch_bounds__(kDrawThreads) verify_draw(VerifyArgs a) {
   }
 }
 
-// Slices of at least 512 tokens, enough for some 8192 waves on the device.
 // About 4096 slices in all, a wave each, of 256 tokens at least (131101 tokens,
 // 64 x 6 float32 and 32 x 24 bf16: 26.6 and 15.1 us with 8192 slices, 25.8 and
 // 13.3 with 4096, 29.7 and 14.6 with 2048; 1 x 8 over 32768: 10.1 us with slices

@@ -874,7 +874,9 @@ int alpx_q4_rows(const void* key_codes, const void* key_scales, const void* valu
  * result.  A token at or past counts[b], and one whose own row lies past
  * length, give zeros, whatever their gate holds.  NaN in rows that a token
  * does not see stays out of its result.  Scores are float32: a query's largest
- * value times scale stays below 2^100.
+ * value times scale stays below 2^100.  Weights and their products with steps
+ * have 22 bits where float16 is not subnormal: values below 1e-3 lose some
+ * (1.7e-5 of the result at 1e-5).
  * workspace: alpx_q4_workspace_bytes bytes (0 for sizes that the call
  * refuses), 16-byte aligned; scratch, which calls that may overlap must not
  * share.  out must not overlap any input. */

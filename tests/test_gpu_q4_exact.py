@@ -2,13 +2,13 @@
 (float32 output whatever the queries' type), against the float64 oracle.
 
 Tolerances.  A weight p is off by what its score is, and by 2^-22 for its two
-float16 parts; p times a step by 2^-22 more; scores of deviation 1 stay below 8
+float16 parts; p times a step by 2^-22 more.  Scores of deviation 1 stay below 8
 in size, so that float32 forms them, and the exponential, within 2^-20 or so
-(queries of 16 bits against codes as they stand: 2^-18).  Together a row's
-share p (v - 8 steps or less) is off by less than 2^-17 of its gross p (|least|
-+ step code), so a channel is by less than 2^-17 of the weighted gross; and
-since the rows' errors are independent and values have mean zero, the 2-norm of
-all channels' errors is below 2^-17 of the result's, on any number of rows."""
+(queries of 16 bits against codes as they stand: 2^-18).  A row's share of a
+channel is thus off by less than 2^-17 of its gross p (|least| + step code),
+and a channel by less than 2^-17 of the weighted gross.  The rows' errors are
+independent and values have mean zero, so the 2-norm of all channels' errors
+is below 2^-17 of the result's, on any number of rows."""
 
 import importlib
 
@@ -17,7 +17,7 @@ import pytest
 
 from oracle import inputs as I
 from oracle import q4 as Q
-from tests.test_gpu_q4 import PKG, Case, _host, _td
+from tests.test_gpu_q4 import PKG, Case, _host, _td, _up
 
 pytestmark = pytest.mark.gpu
 
@@ -192,3 +192,32 @@ def test_every_kernel_matches_the_oracle(gpu, ops, dtype, d, columns):
         case = Case(gpu, 66, dtype=dtype, d=d, hq=2 * group, hkv=2, nodes=nodes, prefix=prefix)
         got, want = _close(case, ops, 2.0 ** -17)
         assert np.linalg.norm(got - want) <= 2.0 ** -17 * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("dtype,d", [("bf16", 256), ("f16", 128), ("f32", 64)])
+def test_normed_heads_reach_codes_over_a_float_pool(gpu, ops, dtype, d):
+    """Heads with a norm and a gate of their own: their prologue writes a float
+    pool of the call's rows, which are stored as they are."""
+    import torch
+    rng = np.random.default_rng(70)
+    tokens, hq, hkv, page = 21, 4, 2, 32
+    qg = _up(gpu, rng.standard_normal((tokens, hq * 2 * d)), dtype)
+    k, v = (_up(gpu, rng.standard_normal((tokens, hkv * d)), dtype) for _ in range(2))
+    weights = [_up(gpu, rng.uniform(0.5, 1.5, d).astype(np.float32)) for _ in range(2)]
+    rows = torch.zeros(2, 1, page, hkv, d, dtype=_td(dtype), device=gpu)
+    at = torch.arange(tokens, dtype=torch.int32, device=gpu)
+    lanes = torch.from_numpy(rng.integers(0, 5000, (tokens, 4))).to(gpu)
+    ops.paged_attention_prologue_rows_(qg, k, v, *weights, rows[0], rows[1], at, lanes,
+                                       sections=(8, 8, 8, 8), frequency_base=1e7, epsilon=1e-6)
+    pages = 3
+    pool = ops.initialize_paged_q4_workspace(num_pages=pages, page_size=page, kv_heads=hkv,
+                                             head_dimension=d).arrays
+    slots = rng.permutation(pages * page)[:tokens].astype(np.int32)
+    ops.paged_q4_append_rows_(None, rows[0, 0, :tokens], rows[1, 0, :tokens], *pool,
+                              _up(gpu, slots), None, rotary_dimension=0)
+    for i in range(2):
+        want = Q.empty_pool(pages, hkv, page, d)
+        Q.put(want, slots, _host(rows[i, 0, :tokens]))
+        assert np.abs(_host(rows[i, 0, :tokens])).max() > 1.0
+        assert np.array_equal(pool[2 * i].cpu().numpy(), want[0])
+        assert np.array_equal(pool[2 * i + 1].cpu().numpy(), want[1])
