@@ -315,7 +315,10 @@ __device__ __forceinline__ double slice_scan(const double* sums, int slices, int
 // trees of drawn drafts, go on from where a sum was wanted: another refusal's
 // sum by the whole device, where the draw's block alone would form it (trees of
 // 8 x 12 drafts over 131101 tokens, float32: 137 us with 1 round, 78 with 2,
-// 31 with 4, 36 with 6, and 1.2 us a round that no sequence needs).
+// 31 with 4, 36 with 6, and 1.2 us a round that no sequence needs).  Refusals of
+// one draft's children past the fourth are that block's alone, and each forms
+// all before it again: 11, 23 and 63 refused in a row over 131101 tokens, float32,
+// take 1.1, 4.4 and 30 ms.
 template <typename T, bool DRAFT>
 __global__ void __launch_bounds__(kSumThreads) verify_sums(VerifyArgs a) {
   constexpr int kWaves = kSumThreads / 64;
